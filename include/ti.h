@@ -484,6 +484,62 @@ int ti_attn_causal_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
                       const uint32_t* vq, const float* vs, float* out,
                       int T, int pos0, int nHq, int nKv, int hd);
 
+/* ---- a bounded and a shared int8 KV cache ------------------------------------------------
+ * No reference counterparts: the reference keeps the whole of one conversation in one buffer. */
+/* Attention under a sliding window with sinks: query t (position p = pos0 + t) sees the keys j <= p with
+ * j > p - window or j < sinks; window < 0 is no window (ti_attn_causal_q8's keys), window = 0 leaves the sinks
+ * alone. A query that sees nothing gives zeros. qr/out are [T][nHq][hd], the cache is the contiguous one of
+ * positions 0 .. pos0+T-1; keys that no query sees are not read. T = 1 is a decode step, any T a prompt or a
+ * chunk of one. nHq <= 64, T * nHq < 2^23; out must not overlap qr. */
+int ti_attn_window_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
+                      const uint32_t* vq, const float* vs, float* out,
+                      int T, int pos0, int nHq, int nKv, int hd, int window, int sinks);
+/* The cache in pages: a pool of `pages` pages of `page` positions each (a power of two; page * width < 2^31), every
+ * page laid out as the contiguous cache is (position, then KV head, then dim; scales alike), and a device table
+ * [B][width] of page ids: position p of sequence b is row p % page of page table[b*width + p / page]. Ids, lengths,
+ * sequence numbers and positions are read on the device, so a captured call follows them from replay to replay. */
+/* kvQuantWrite's codes and scales (ti_kv_write_q8), row t of kr and v ([T][nKv*hd], 16-byte aligned) into position
+ * pos[t] of sequence seq[t] (seq NULL: row t is sequence t, T <= B). A row whose place does not exist (pos < 0 or
+ * past the table, seq outside [0, B), a page id outside [0, pages)) is not written. Rows of one call name different
+ * places; of rows that name the same one, which codes and which scales stay is not specified. table NULL: the
+ * positions are the rows of a contiguous cache of page * pages positions, seq and B are not looked at. */
+int ti_kv_write_paged_q8(ti_ctx* ctx, const float* kr, const float* v, uint32_t* kq, float* ks,
+                         uint32_t* vq, float* vs, const int32_t* table, const int32_t* seq,
+                         const int32_t* pos, int T, int B, int nKv, int hd, int page, int pages, int width);
+/* The inverse: row t of k and v = code * (scale / 127) of position pos[t] of sequence seq[t], zeros where there is no
+ * such place. Arguments as ti_kv_write_paged_q8's (table NULL reads a contiguous cache). */
+int ti_kv_read_paged_q8(ti_ctx* ctx, const uint32_t* kq, const float* ks, const uint32_t* vq, const float* vs,
+                        const int32_t* table, const int32_t* seq, const int32_t* pos, float* k, float* v,
+                        int T, int B, int nKv, int hd, int page, int pages, int width);
+/* Attention of one new token of each of B sequences over the pages: sequence b holds lens[b] keys (the new token's own
+ * among them, at position lens[b] - 1), its query is row b of qr [B][nHq][hd]; window and sinks as
+ * ti_attn_window_q8. Pages that hold no visible key are not looked up, so their table entries may be anything; a
+ * visible position whose page id is outside [0, pages) counts as not there. lens[b] above width * page is taken
+ * as width * page, lens[b] <= 0 gives zeros. Rows of several tokens of one sequence are sequences that
+ * repeat its table row, with their own lengths. B <= 4096, nHq <= 64; out must not overlap qr. */
+int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
+                     const uint32_t* vq, const float* vs, const int32_t* table, const int32_t* lens,
+                     float* out, int B, int nHq, int nKv, int hd, int page, int pages, int width,
+                     int window, int sinks);
+/* ti_attn_causal_q8 that also adds up the attention each key receives: mass[j*nKv + h] += the softmax weights of key j
+ * summed over the T queries and the nHq/nKv query heads of KV head h. The slots pos0 .. pos0+T-1, the call's own
+ * tokens, are set instead (no earlier query saw them), so a mass buffer needs no clearing. pos0 is a slot of the
+ * cache: after an eviction, the next free one. T * nHq <= 4096, nHq <= 64, nHq * (pos0 + T) <= 2^24 for T = 1; out must not overlap qr. */
+int ti_attn_mass_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
+                    const uint32_t* vq, const float* vs, float* out, float* mass,
+                    int T, int pos0, int nHq, int nKv, int hd);
+/* Cuts a cache of n slots to `keep` per KV head, in place, to the keys of most accumulated attention. where[i*nKv + h]
+ * is the position of the token in slot i < known; the slots from `known` on hold the last n - known positions before
+ * `next` in order (a first eviction: known 0, where may be NULL, next n). Kept first: positions below `sinks` and
+ * the `recent` last before `next` (sinks + recent <= keep), then larger mass (NaN last), equal ones by the lower slot. The kept
+ * slots at `keep` and above move into the freed ones below it, the i-th into the i-th; the others stay. The cache rows
+ * from `keep` on are left as they were. mass_out / where_out [keep][nKv] receive what the slots now hold (keep
+ * at most n); they are the input buffers themselves, or do not overlap them. Keys keep the rotation of their own
+ * positions, so attention over the slots 0 .. keep-1 needs no more than their count. nKv <= 64. */
+int ti_kv_evict_q8(ti_ctx* ctx, uint32_t* kq, float* ks, uint32_t* vq, float* vs, const float* mass,
+                   const int32_t* where, float* mass_out, int32_t* where_out, int n, int known, int keep,
+                   int sinks, int recent, int next, int nKv, int hd);
+
 #ifdef __cplusplus
 }
 #endif

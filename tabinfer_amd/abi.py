@@ -106,6 +106,12 @@ SIGS = {
     "ti_qwen3_read_tokens": [_p, _p, _i, _i, _p],
     "ti_qwen3_read_tokens_async": [_p, _p, _i, _i, _p],
     "ti_attn_causal_q8": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i],
+    "ti_attn_window_q8": [_p] * 7 + [_i] * 7,
+    "ti_kv_write_paged_q8": [_p] * 10 + [_i] * 7,
+    "ti_kv_read_paged_q8": [_p] * 10 + [_i] * 7,
+    "ti_attn_paged_q8": [_p] * 9 + [_i] * 9,
+    "ti_attn_mass_q8": [_p] * 8 + [_i] * 5,
+    "ti_kv_evict_q8": [_p] * 9 + [_i] * 8,
 }
 
 

@@ -184,6 +184,27 @@ function createEngine({ device = 0 } = {}) {
     attnCausalQ8(qrBuf, kv, oBuf, T, pos0, nHq, nKv, hd) {                                                 // :2534-2577
       TI.attn_causal_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, oBuf, T, pos0, nHq, nKv, hd);
     },
+    // a bounded and a shared KV cache (no reference counterparts). kv is the cache's four arrays; a pool of pages
+    // adds {page, pages}, a table is {buf, width, B}
+    attnWindowQ8(qrBuf, kv, oBuf, T, pos0, nHq, nKv, hd, window, sinks) {
+      TI.attn_window_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, oBuf, T, pos0, nHq, nKv, hd, window, sinks | 0);
+    },
+    kvWritePagedQ8(krBuf, vBuf, kv, table, seqBuf, posBuf, T, nKv, hd) {
+      TI.kv_write_paged_q8(ctx, krBuf, vBuf, kv.kq, kv.ks, kv.vq, kv.vs, table.buf, U(seqBuf), posBuf, T, table.B, nKv, hd, kv.page, kv.pages, table.width);
+    },
+    kvReadPagedQ8(kv, table, seqBuf, posBuf, kBuf, vBuf, T, nKv, hd) {
+      TI.kv_read_paged_q8(ctx, kv.kq, kv.ks, kv.vq, kv.vs, table.buf, U(seqBuf), posBuf, kBuf, vBuf, T, table.B, nKv, hd, kv.page, kv.pages, table.width);
+    },
+    attnPagedQ8(qrBuf, kv, table, lensBuf, oBuf, nHq, nKv, hd, window = -1, sinks = 0) {
+      TI.attn_paged_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, table.buf, lensBuf, oBuf, table.B, nHq, nKv, hd, kv.page, kv.pages, table.width, window, sinks);
+    },
+    attnMassQ8(qrBuf, kv, oBuf, massBuf, T, pos0, nHq, nKv, hd) {
+      TI.attn_mass_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, oBuf, massBuf, T, pos0, nHq, nKv, hd);
+    },
+    // in place: massBuf and whereBuf are cut with the cache
+    kvEvictQ8(kv, massBuf, whereBuf, n, known, keep, sinks, recent, next, nKv, hd) {
+      TI.kv_evict_q8(ctx, kv.kq, kv.ks, kv.vq, kv.vs, massBuf, whereBuf, massBuf, whereBuf, n, known, keep, sinks, recent, next, nKv, hd);
+    },
   };
 
   // ---- ternary (native/crates/n2-kernels/src/tern.rs, cpu/kernel/src/lib.rs) --------------------

@@ -1564,6 +1564,12 @@ napi_value module_init(napi_env env, napi_value exports) {
         ENTRY("rope_qk", ti_rope_qk),
         ENTRY("kv_write_q8", ti_kv_write_q8),
         ENTRY("attn_causal_q8", ti_attn_causal_q8),
+        ENTRY("attn_window_q8", ti_attn_window_q8),
+        ENTRY("kv_write_paged_q8", ti_kv_write_paged_q8),
+        ENTRY("kv_read_paged_q8", ti_kv_read_paged_q8),
+        ENTRY("attn_paged_q8", ti_attn_paged_q8),
+        ENTRY("attn_mass_q8", ti_attn_mass_q8),
+        ENTRY("kv_evict_q8", ti_kv_evict_q8),
         // ternary
         ENTRY("tern_gemv", ti_tern_gemv),
         ENTRY("tern_gemm", ti_tern_gemm),
