@@ -5,6 +5,7 @@
 // in the running softmax, then P V with a thread a dim and half of the tile's keys.
 #include "ti_dev.h"
 #include "ti_span.h"
+#include "ti_token_attn.h"
 
 namespace {
 
@@ -113,6 +114,17 @@ __global__ __launch_bounds__(256) void k_span_mass(SpanArgs a, float* __restrict
     mass[i] = j < a.pos0 ? mass[i] + sum : sum;
 }
 
+// thread = one (slot, KV head) of a one-token call: the weights that its G heads gave the slot, from their scores
+__global__ __launch_bounds__(256) void k_token_mass(const float* __restrict__ scores, long sstride, const float* __restrict__ ml,
+                                                    float* __restrict__ mass, int pos0, int nHq, int nKv) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (pos0 + 1L) * nKv) return;
+    const int j = (int)(i / nKv), hk = (int)(i % nKv), G = nHq / nKv;
+    float sum = 0.0f;
+    for (int h = hk * G; h < (hk + 1) * G; h++) sum += __builtin_amdgcn_exp2f(scores[h * sstride + j] - ml[2 * h]) / ml[2 * h + 1];
+    mass[i] = j < pos0 ? mass[i] + sum : sum;
+}
+
 int check_attn(const char* fn, const void* qr, const void* kq, const void* ks, const void* vq, const void* vs, const void* out,
                int n, int nHq, int nKv, int hd) {
     TI_REQUIRE(qr && kq && ks && vq && vs && out, "%s: null buffer", fn);
@@ -133,6 +145,12 @@ extern "C" int ti_attn_window_q8(ti_ctx* c, const float* qr, const uint32_t* kq,
     if (rc) return rc;
     TI_REQUIRE(pos0 >= 0 && pos0 <= 0x7fffffff - T && sinks >= 0, "ti_attn_window_q8: bad positions (T=%d pos0=%d sinks=%d)", T, pos0, sinks);
     TI_REQUIRE((long)T * nHq <= 0x7fffffffL / 256, "ti_attn_window_q8: %d x %d query rows in one call", T, nHq);
+    if (T == 1 || T * (nHq / nKv) <= 16) {
+        const long keys = window < 0 ? (long)pos0 + T : min((long)pos0 + T, (long)window + sinks + T);
+        const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
+                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, keys, nullptr, 0, nullptr};
+        return ti_token_attn_launch(c, p, hd);
+    }
     SpanArgs a = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out, nullptr,
                   TiPages{nullptr, 0, 0x7fffffff, 0}, nullptr, pos0, nHq, nKv, hd, window, sinks};
     k_span_attn<<<(unsigned)(T * nHq), 256, 0, c->stream>>>(a);
@@ -151,11 +169,10 @@ extern "C" int ti_attn_paged_q8(ti_ctx* c, const float* qr, const uint32_t* kq, 
     TI_REQUIRE(ti_pow2(page) && pages > 0 && width > 0 && (long)page * width <= 0x7fffffffL,
                "ti_attn_paged_q8: bad pages (length %d, a power of two; %d of them; table width %d)", page, pages, width);
     TI_REQUIRE(sinks >= 0, "ti_attn_paged_q8: sinks = %d", sinks);
-    SpanArgs a = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out, nullptr,
-                  TiPages{table, ti_log2(page), pages, width}, lens, 0, nHq, nKv, hd, window, sinks};
-    k_span_attn<<<(unsigned)(B * nHq), 256, 0, c->stream>>>(a);
-    TI_LAUNCHED("k_span_attn");
-    return TI_OK;
+    const long all = (long)page * width, keys = window < 0 ? all : min(all, (long)window + sinks + 1);
+    const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
+                           TiPages{table, ti_log2(page), pages, width}, lens, B, 1, 0, nHq, nKv, window, sinks, keys, nullptr, 0, nullptr};
+    return ti_token_attn_launch(c, p, hd);
 }
 
 extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, const float* ks, const uint32_t* vq, const float* vs,
@@ -166,8 +183,21 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
     TI_REQUIRE(mass, "ti_attn_mass_q8: null mass");
     TI_REQUIRE(pos0 >= 0 && pos0 <= 0x7fffffff - T, "ti_attn_mass_q8: bad positions (T=%d pos0=%d)", T, pos0);
     TI_REQUIRE((long)T * nHq <= TI_ATTN_ROWS_MAX, "ti_attn_mass_q8: T*nHq = %ld > %d", (long)T * nHq, TI_ATTN_ROWS_MAX);
-    TI_REQUIRE(T > 1 || (long)nHq * (pos0 + 1L) <= MASS_SCORES, "ti_attn_mass_q8: %d heads over %d slots exceed the scratch (%ld scores)",
+    TI_REQUIRE(T > 1 || (long)nHq * ((pos0 + 32L) / 32 * 32) <= MASS_SCORES, "ti_attn_mass_q8: %d heads over %d slots exceed the scratch (%ld scores)",
                nHq, pos0 + 1, MASS_SCORES);
+    if (T == 1) {
+        // the upper half of the partials' scratch holds the scores (2048 slots of 64 heads fill the lower one), the
+        // argmax scratch each head's (max, sum)
+        const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
+                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, c->attn_po + MASS_SCORES,
+                               (pos0 + 32L) / 32 * 32, c->amax_v};
+        const int rt = ti_token_attn_launch(c, p, hd);
+        if (rt) return rt;
+        const long n = (pos0 + 1L) * nKv;
+        k_token_mass<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(p.scores, p.sstride, p.ml, mass, pos0, nHq, nKv);
+        TI_LAUNCHED("k_token_mass");
+        return TI_OK;
+    }
     SpanArgs a = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out, c->attn_ml,
                   TiPages{nullptr, 0, 0x7fffffff, 0}, nullptr, pos0, nHq, nKv, hd, -1, 0};
     k_span_attn<<<(unsigned)(T * nHq), 256, 0, c->stream>>>(a);

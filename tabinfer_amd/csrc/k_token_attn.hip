@@ -1,0 +1,518 @@
+// k_token_attn.hip — attention of few query rows a KV head over a part of the int8 KV cache: a decode step under a
+// sliding window with sinks, one token of each of B sequences over pages, and the scores that accumulated weights are
+// made of. At most 16 rows a tile (row = token x query head of the KV head), both products on the matrix cores.
+//
+//  - The visible keys are cut into blocks of 32 at multiples of 32 (a page of 32 and more covers whole blocks). The
+//    blocks of all sequences share one number of workgroups a KV head: with C = total / target blocks a workgroup, a
+//    sequence of n blocks takes ceil(n / C) of them, so that a long one among short ones is spread like the rest.
+//    Every workgroup finds its sequence by a scan over the lengths; nothing depends on them on the host.
+//  - A wave takes a block at a time, on its own: loads of the next block in flight, the codes through LDS of its own.
+//    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-25 of
+//    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
+//    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
+//    P times the V scale of (key, group) in f32, as three bf16, exactly; V through the transposing LDS read.
+//  - The waves' (m, l, O) meet in LDS; the workgroups' partials in k_token_merge.
+//  - A row that sees nothing has m = -inf; one that sees only scores of -inf has the finite floor, and gives NaN as the formula does.
+#include "ti_dev.h"
+#include "ti_span.h"
+#include "ti_token_attn.h"
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));   // the caller's q and out need not be aligned
+typedef int v2i __attribute__((ext_vector_type(2)));
+
+constexpr int BLK = 32;                      // keys of a wave's block
+constexpr int WAVES = 4;
+constexpr int CMIN = WAVES;                  // blocks of a workgroup, at least
+constexpr float FLOOR = -3.402823466e38f;
+constexpr float VSCALE = 0x1p-24f;           // of every V scale: 127 x a V scale x thousands of keys stays in f32's range
+
+struct TokArgs {
+    TiTokenAttn p;
+    float* po;                               // [slot][nKv][T G][HD] partials, (m, l) of each
+    float* pml;
+    int32_t* meta;                           // [B][2]: a sequence's first slot and their number
+    int G, R, RT, target;                    // R = T G rows a KV head in RT tiles; target: workgroups a KV head to fill
+};
+
+// Blocks that hold the keys [0, first) and [low, end): [0, sb) and [wb, sb + ... )
+struct Blocks {
+    int sb, skip, n;                         // sink blocks; blocks between them and the window; all that are visited
+    __device__ int at(int i) const { return i < sb ? i : i + skip; }
+};
+__device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
+    Blocks b;
+    b.sb = (s.first + BLK - 1) / BLK;
+    const int w = max(b.sb, s.low / BLK);
+    b.skip = w - b.sb;
+    b.n = max(0, (int)(((long)s.end + BLK - 1) / BLK) - b.skip);
+    return b;
+}
+
+template <bool PAGED>
+__device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // position of the sequence's last query
+    if (!PAGED) return a.p.pos0 + a.p.T - 1;
+    const long most = (long)a.p.pg.width << a.p.pg.shift;
+    const int n = a.p.lens[b];
+    return (int)(n < most ? n : most) - 1;
+}
+template <bool PAGED>
+__device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int last) {   // the keys that any of its queries sees
+    TiSpan s = ti_span(last - (a.p.T - 1), a.p.window, a.p.sinks);
+    s.end = last + 1;
+    return s;
+}
+template <bool PAGED>
+__device__ __forceinline__ int seq_blocks(const TokArgs& a, int b) {
+    const int last = seq_last<PAGED>(a, b);
+    return last < 0 ? 0 : blocks_of(seq_span<PAGED>(a, last)).n;
+}
+
+struct Share {
+    int b, split, ns, chunk;                 // sequence, which of its ns workgroups, blocks of each
+};
+
+// sum over the workgroup (every thread), and the sum of the threads before this one
+template <class N>
+__device__ __forceinline__ N wg_scan(N v, N* s4, N& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    N x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const N y = __shfl_up(x, o);
+        x += lane >= o ? y : 0;
+    }
+    if (lane == 63) s4[wave] = x;
+    __syncthreads();
+    N before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        const N t = s4[w];
+        before += w < wave ? t : 0;
+        all += t;
+    }
+    total = all;
+    __syncthreads();
+    return before + x - v;
+}
+
+__device__ __forceinline__ int share_chunk(long total, int target) {
+    const long c = target > 0 ? (total + target - 1) / target : 0x7fffffffL;
+    return (int)min(max(c, (long)CMIN), 0x7fffffffL);
+}
+
+// slot w of a KV head -> its share; false: there are fewer slots
+template <bool PAGED>
+__device__ bool find_share(const TokArgs& a, int w, Share& sh, long* s8, int* s_share) {
+    const int B = a.p.B, tid = threadIdx.x;
+    if (B == 1) {
+        const int n = seq_blocks<PAGED>(a, 0);
+        sh.b = 0;
+        sh.chunk = share_chunk(n, a.target);
+        sh.ns = max(1, (int)(((long)n + sh.chunk - 1) / sh.chunk));
+        sh.split = w;
+        if (w == 0 && tid == 0) {
+            a.meta[0] = 0;
+            a.meta[1] = sh.ns;
+        }
+        return w < sh.ns;
+    }
+    // a thread: the sequences [tid per, tid per + per)
+    const int per = (B + 255) / 256, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    long mine = 0, total;
+    for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
+    (void)wg_scan(mine, s8, total);
+    const int chunk = share_chunk(total, a.target);
+    int slots = 0, all;
+    for (int b = b0; b < b1; b++) slots += max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
+    int at = wg_scan(slots, reinterpret_cast<int*>(s8), all);
+    if (w >= at && w < at + slots) {
+        for (int b = b0; b < b1; b++) {
+            const int ns = max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
+            if (w < at + ns) {
+                s_share[0] = b;
+                s_share[1] = w - at;
+                s_share[2] = ns;
+                if (w == at) {
+                    a.meta[2 * b] = at;
+                    a.meta[2 * b + 1] = ns;
+                }
+                break;
+            }
+            at += ns;
+        }
+    }
+    __syncthreads();
+    sh.b = s_share[0];
+    sh.split = s_share[1];
+    sh.ns = s_share[2];
+    sh.chunk = chunk;
+    return w < all;
+}
+
+template <int HD>
+struct TokLds {
+    static constexpr int NG = HD / 32, KS = HD + 8, VS = HD + 16;      // LDS rows (bytes): operand reads without conflicts
+    struct Wave {
+        uint8_t k[BLK * KS];
+        uint8_t v[BLK * VS];
+    };
+    union {
+        Wave w[WAVES];
+        float o[WAVES][16][HD];
+    };
+    float ks[WAVES][NG][BLK], vs[WAVES][NG][BLK];
+    float m[WAVES][16], l[WAVES][16];
+    long s8[WAVES];
+    int share[4];
+};
+
+template <int HD, bool PAGED>
+__global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) {
+    constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
+    constexpr int KS = TokLds<HD>::KS, VS = TokLds<HD>::VS;
+    constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
+    __shared__ __align__(16) TokLds<HD> L;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x % a.p.nKv, rt = (blockIdx.x / a.p.nKv) % a.RT, w = blockIdx.x / (a.p.nKv * a.RT);
+    Share sh;
+    if (!find_share<PAGED>(a, w, sh, L.s8, L.share)) return;           // workgroup-uniform
+    const int last = seq_last<PAGED>(a, sh.b);
+    const TiSpan span = seq_span<PAGED>(a, last);
+    Blocks bl = blocks_of(span);
+    if (last < 0) bl.n = 0;
+    const int c0 = sh.split * sh.chunk, c1 = min(bl.n, c0 + sh.chunk);
+    const int r16 = lane & 15, j = lane >> 4;
+
+    // this lane's row
+    const int rg = min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;
+    const int pos = last - (a.p.T - 1) + t;
+    const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
+    // what every row of the tile sees: [full_low, full_end)
+    const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
+
+    // ---- a block's loads
+    uint4 kr[NL], vr[NL];
+    float ksr[SL], vsr[SL];
+    // the page of key k0 + lane % 32, where some row sees it; -1 where none does or there is none
+    auto fetch_page = [&](int i) -> int {
+        const int key = bl.at(i) * BLK + (lane & 31);
+        const bool in = key < span.end && (key >= span.low || key < span.first);
+        if constexpr (!PAGED) return in ? 0 : -1;
+        const int k = key >> a.p.pg.shift;
+        if (!in || k >= a.p.pg.width) return -1;
+        const int id = a.p.pg.table[(size_t)sh.b * a.p.pg.width + k];
+        return id >= 0 && id < a.p.pg.pages ? id : -1;
+    };
+    auto row_of = [&](int k0, int kl, int page) -> size_t {            // the row of key k0 + kl; a row that exists where there is none
+        if constexpr (!PAGED) return (size_t)min(k0 + kl, span.end - 1);
+        const int id = max(__shfl(page, kl), 0);
+        return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
+    };
+    auto load = [&](int i, int page) {
+        const int k0 = bl.at(i) * BLK;
+#pragma unroll
+        for (int p = 0; p < NL; p++) {
+            const int pc = lane + 64 * p, kl = pc / PC, c = pc % PC;
+            const size_t off = (row_of(k0, kl, page) * a.p.nKv + hk) * HD + 16 * c;
+            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + off));
+            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + off));
+        }
+#pragma unroll
+        for (int p = 0; p < SL; p++) {
+            const int e = min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
+            const size_t off = (row_of(k0, kl, page) * a.p.nKv + hk) * NG + g;
+            ksr[p] = a.p.ks[off];
+            vsr[p] = a.p.vs[off];
+        }
+    };
+    auto stage = [&]() {
+        uint8_t* kt = L.w[wave].k;
+        uint8_t* vt = L.w[wave].v;
+#pragma unroll
+        for (int p = 0; p < NL; p++) {
+            const int pc = lane + 64 * p, kl = pc / PC, c = pc % PC;
+            uint2* kd = reinterpret_cast<uint2*>(kt + kl * KS + 16 * c);
+            kd[0] = make_uint2(kr[p].x, kr[p].y);
+            kd[1] = make_uint2(kr[p].z, kr[p].w);
+            *reinterpret_cast<uint4*>(vt + kl * VS + 16 * c) = vr[p];
+        }
+#pragma unroll
+        for (int p = 0; p < SL; p++) {
+            const int e = min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
+            L.ks[wave][g][kl] = ksr[p];
+            L.vs[wave][g][kl] = vsr[p] * VSCALE;
+        }
+    };
+
+    int i = c0 + wave;
+    int page = i < c1 ? fetch_page(i) : -1, page1 = -1;
+    if (i + WAVES < c1) page1 = fetch_page(i + WAVES);
+    if (i < c1) load(i, page);
+
+    // ---- Q operand: row r16, dims 32 g + 8 j.., scaled by 2^k so that the row's largest element is below 16
+    ti_h8 qh[NG], ql[NG];
+    float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
+    {
+        const float* q = a.p.qr + ((size_t)(sh.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD + 8 * j;
+        v4f_u qv[NG][2];
+        float mx = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(qv[g][u][e]));
+            }
+        mx = fmaxf(mx, ti_xor(mx, 16));
+        mx = fmaxf(mx, ti_xor(mx, 32));
+        int ex = 4;
+        if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+        const int k = min(4 - ex, 100);
+        const float up = ldexpf(1.0f, k);
+        fr = fr * ldexpf(1.0f, -k);
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = qv[g][e / 4][e % 4] * up;
+                const _Float16 hi = (_Float16)v;
+                qh[g][e] = hi;
+                ql[g][e] = (_Float16)(v - (float)hi);
+            }
+    }
+
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f o[HD / 16];
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) o[d] = zero;
+    float m = -INFINITY, l = 0.0f;
+    // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
+    const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
+
+    for (; i < c1; i += WAVES) {
+        ti_wave_lds_fence();                               // the last block is read
+        stage();
+        ti_wave_lds_fence();
+        const int k0 = bl.at(i) * BLK;
+        const uint32_t there = (uint32_t)__ballot(page >= 0);
+        page = page1;
+        if (i + WAVES < c1) load(i + WAVES, page);
+        if (i + 2 * WAVES < c1) page1 = fetch_page(i + 2 * WAVES);
+
+        float s[8];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            v4f acc = zero;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint2 kw = *reinterpret_cast<const uint2*>(L.w[wave].k + (16 * b + r16) * KS + 32 * g + 8 * j);
+                const ti_h8 kk = ti_i8x8_h8(kw.x, kw.y);
+                const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[wave][g][16 * b + 4 * j]);
+                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[g], zero, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[g], d, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e] * fr;
+        }
+        // which of the lane's keys its row sees
+        uint32_t seen = 0xffu;
+        const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
+        if (!whole) {                                      // wave-uniform
+            seen = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int kl = 16 * (e >> 2) + 4 * j + (e & 3), key = k0 + kl;
+                const bool ok = ((there >> kl) & 1u) && key <= pos && (key >= low || key < a.p.sinks);
+                seen |= ok ? 1u << e : 0u;
+            }
+        }
+        if (a.p.scores && rt * 16 + r16 < a.R) {
+            float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
+            *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]};
+            *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]};
+        }
+        float tm = FLOOR;
+        if (!whole) {
+            tm = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen >> e & 1u ? fmaxf(s[e], FLOOR) : -INFINITY);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[e]);
+        }
+        tm = fmaxf(tm, ti_xor(tm, 16));
+        tm = fmaxf(tm, ti_xor(tm, 32));
+        // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
+        const bool bump = tm > m + 6.0f;
+        if (__any(bump)) {
+            const float mn = bump ? tm : m;
+            const float alpha = bump ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+            l = l * alpha;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) o[d] = o[d] * alpha;
+            m = mn;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float p = __builtin_amdgcn_exp2f(s[e] - m);
+            if (!whole) p = seen >> e & 1u ? p : 0.0f;
+            s[e] = p;
+            sum += p;
+        }
+        l += sum;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[wave][g][4 * j]);
+            const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[wave][g][16 + 4 * j]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = s[e] * v0[e];
+                x[4 + e] = s[4 + e] * v1[e];
+            }
+            if (!whole) {                                  // the scale of a key that the row does not see may be NaN
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
+            }
+            ti_b8 pb[3];
+            ti_bf16x3(x, pb);
+#pragma unroll
+            for (int d = 2 * g; d < 2 * g + 2; d++) {
+                const v2i vb = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) v2i*)(L.w[wave].v + vrow * VS + 8 * (r16 & 1) + 16 * d));
+                const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
+                const ti_b8 vv = __builtin_bit_cast(ti_b8, make_uint4(lo.x, lo.y, hi.x, hi.y));
+#pragma unroll
+                for (int e = 2; e >= 0; e--) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[e], o[d], 0, 0, 0);
+            }
+        }
+    }
+
+    // ---- the waves' parts into the workgroup's partial
+    l += ti_xor(l, 16);
+    l += ti_xor(l, 32);
+    __syncthreads();                                       // the tiles are read
+    if (j == 0) {
+        L.m[wave][r16] = m;
+        L.l[wave][r16] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f*>(&L.o[wave][r16][16 * d + 4 * j]) = o[d];
+    __syncthreads();
+    const int nr = min(16, a.R - rt * 16);
+    const size_t base = ((size_t)w * a.p.nKv + hk) * a.R + rt * 16;
+    for (int e = tid; e < nr * (HD / 4); e += 256) {
+        const int r = e / (HD / 4), d = e % (HD / 4);
+        float M = L.m[0][r];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) M = fmaxf(M, L.m[k][r]);
+        v4f x = zero;
+        float y = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) {
+            const float mk = L.m[k][r], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+            const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][r][4 * d]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
+            y = fmaf(L.l[k][r], f, y);
+        }
+        *reinterpret_cast<v4f*>(a.po + (base + r) * HD + 4 * d) = x;
+        if (d == 0) {
+            a.pml[2 * (base + r)] = M;
+            a.pml[2 * (base + r) + 1] = y;
+        }
+    }
+}
+
+// A wave a (sequence, token, head): its slots' partials into the output row
+template <int HD>
+__global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int rows) {
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;                               // wave-uniform
+    const int hq = row % a.p.nHq, t = (row / a.p.nHq) % a.p.T, b = row / (a.p.nHq * a.p.T);
+    const int hk = hq / a.G, r = t * a.G + hq % a.G;
+    const int s0 = a.meta[2 * b], ns = a.meta[2 * b + 1];
+    const size_t step = (size_t)a.p.nKv * a.R, base = (size_t)s0 * step + (size_t)hk * a.R + r;
+    const float* ml = a.pml + 2 * base;
+    float M = -INFINITY;
+    for (int i = lane; i < ns; i += 64) M = fmaxf(M, ml[2 * i * step]);
+    M = ti_wave_max(M);
+    const int d = lane % (HD / 2);                         // dims 2 d, 2 d + 1
+    float v0 = 0.0f, v1 = 0.0f, L = 0.0f;
+    const float* po = a.po + base * HD + 2 * d;
+    for (int i0 = 0; i0 < ns; i0 += 64) {
+        const int i = i0 + lane;
+        const float mi = i < ns ? ml[2 * i * step] : -INFINITY, li = i < ns ? ml[2 * i * step + 1] : 0.0f;
+        const float wi = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
+        L += wi * li;
+        const int n = min(64, ns - i0);
+        for (int k0 = 0; k0 < n; k0 += 8) {
+            float2 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float2*>(po + (size_t)min(i0 + k0 + k, ns - 1) * step * HD);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = k0 + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), k0 + k)) : 0.0f;
+                v0 = fmaf(x[k].x, f, v0);
+                v1 = fmaf(x[k].y, f, v1);
+            }
+        }
+    }
+    L = ti_wave_sum(L);
+    if (lane < HD / 2) {
+        const float div = 127.0f * VSCALE * L;
+        float* out = a.p.out + (size_t)row * HD + 2 * d;
+        out[0] = M == -INFINITY ? 0.0f : v0 / div;
+        out[1] = M == -INFINITY ? 0.0f : v1 / div;
+    }
+    if (a.p.ml && lane == 0) {
+        a.p.ml[2 * row] = M;
+        a.p.ml[2 * row + 1] = L;
+    }
+}
+
+template <int HD, bool PAGED>
+void launch(ti_ctx* c, const TokArgs& a, int slots) {
+    k_token_attn<HD, PAGED><<<(unsigned)((long)slots * a.RT * a.p.nKv), 256, 0, c->stream>>>(a);
+    const int rows = a.p.B * a.p.T * a.p.nHq;
+    k_token_merge<HD><<<(unsigned)((rows + 3) / 4), 256, 0, c->stream>>>(a, rows);
+}
+
+}  // namespace
+
+int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
+    TokArgs a;
+    a.p = p;
+    a.po = c->attn_po;
+    a.pml = c->attn_ml;
+    a.meta = reinterpret_cast<int32_t*>(c->tg_part);
+    a.G = p.nHq / p.nKv;
+    a.R = p.T * a.G;
+    a.RT = (a.R + 15) / 16;
+    static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
+    // two workgroups a CU, as far as the partials fit; a sequence takes a slot at least
+    const int fit = TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B;
+    int target = (2 * c->cus + p.nKv * a.RT - 1) / (p.nKv * a.RT);
+    if (target > fit) target = fit;
+    a.target = target;
+    // the slots there can be: of B = 1 the host knows the blocks' bound
+    const long most = p.max_keys / BLK + 3;                // blocks of a sequence, at most (three ragged ends)
+    long slots = p.B + (target > 0 ? target : 0);
+    const long alone = p.B * ((most + CMIN - 1) / CMIN);
+    if (slots > alone) slots = alone;
+    const bool paged = p.lens != nullptr;
+#define TOK(HD_) if (hd == HD_) { if (paged) launch<HD_, true>(c, a, (int)slots); else launch<HD_, false>(c, a, (int)slots); }
+    TOK(128) TOK(96) TOK(64) TOK(32)
+#undef TOK
+    TI_LAUNCHED("k_token_attn");
+    return TI_OK;
+}

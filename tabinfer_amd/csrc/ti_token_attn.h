@@ -1,0 +1,23 @@
+// ti_token_attn.h — the launch of k_token_attn.hip, used by the entry points of k_span_attn.hip.
+#pragma once
+#include "ti_internal.h"
+#include "ti_span.h"
+
+constexpr int TI_TOKEN_SEQS = 4096;          // sequences of one call, at most
+
+struct TiTokenAttn {
+    const float* qr;                         // [B][T][nHq][hd]
+    const uint8_t* kq;
+    const float* ks;
+    const uint8_t* vq;
+    const float* vs;
+    float* out;
+    TiPages pg;
+    const int32_t* lens;                     // keys of each sequence (pages); else the one sequence's queries are at pos0 ..
+    int B, T, pos0, nHq, nKv, window, sinks;
+    long max_keys;                           // keys that a sequence's queries can see, at most
+    float* scores;                           // [nHq][sstride] scores in log2 of a one-token call, or nullptr
+    long sstride;
+    float* ml;                               // [T nHq][2] (max in log2, sum) of each row, or nullptr
+};
+int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd);
