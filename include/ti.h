@@ -494,7 +494,7 @@ int ti_attn_causal_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
 int ti_attn_window_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
                       const uint32_t* vq, const float* vs, float* out,
                       int T, int pos0, int nHq, int nKv, int hd, int window, int sinks);
-/* The cache in pages: a pool of `pages` pages of `page` positions each (a power of two; page * width < 2^31), every
+/* The cache in pages: a pool of `pages` pages of `page` positions each (a power of two; page * width < 2^31 - 255), every
  * page laid out as the contiguous cache is (position, then KV head, then dim; scales alike), and a device table
  * [B][width] of page ids: position p of sequence b is row p % page of page table[b*width + p / page]. Ids, lengths,
  * sequence numbers and positions are read on the device, so a captured call follows them from replay to replay. */

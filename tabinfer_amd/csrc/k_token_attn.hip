@@ -45,9 +45,9 @@ struct Blocks {
 __device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
     Blocks b;
     b.sb = (s.first + BLK - 1) / BLK;
-    const int w = max(b.sb, s.low / BLK);
+    const int w = ti_max(b.sb, s.low / BLK);
     b.skip = w - b.sb;
-    b.n = max(0, (int)(((long)s.end + BLK - 1) / BLK) - b.skip);
+    b.n = ti_max(0, (int)(((long)s.end + BLK - 1) / BLK) - b.skip);
     return b;
 }
 
@@ -100,7 +100,7 @@ __device__ __forceinline__ N wg_scan(N v, N* s4, N& total) {
 
 __device__ __forceinline__ int share_chunk(long total, int target) {
     const long c = target > 0 ? (total + target - 1) / target : 0x7fffffffL;
-    return (int)min(max(c, (long)CMIN), 0x7fffffffL);
+    return (int)ti_min(ti_max(c, (long)CMIN), 0x7fffffffL);
 }
 
 // slot w of a KV head -> its share; false: there are fewer slots
@@ -111,7 +111,7 @@ __device__ bool find_share(const TokArgs& a, int w, Share& sh, long* s8, int* s_
         const int n = seq_blocks<PAGED>(a, 0);
         sh.b = 0;
         sh.chunk = share_chunk(n, a.target);
-        sh.ns = max(1, (int)(((long)n + sh.chunk - 1) / sh.chunk));
+        sh.ns = ti_max(1, (int)(((long)n + sh.chunk - 1) / sh.chunk));
         sh.split = w;
         if (w == 0 && tid == 0) {
             a.meta[0] = 0;
@@ -120,17 +120,17 @@ __device__ bool find_share(const TokArgs& a, int w, Share& sh, long* s8, int* s_
         return w < sh.ns;
     }
     // a thread: the sequences [tid per, tid per + per)
-    const int per = (B + 255) / 256, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    const int per = (B + 255) / 256, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
     for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
     (void)wg_scan(mine, s8, total);
     const int chunk = share_chunk(total, a.target);
     int slots = 0, all;
-    for (int b = b0; b < b1; b++) slots += max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
+    for (int b = b0; b < b1; b++) slots += ti_max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
     int at = wg_scan(slots, reinterpret_cast<int*>(s8), all);
     if (w >= at && w < at + slots) {
         for (int b = b0; b < b1; b++) {
-            const int ns = max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
+            const int ns = ti_max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
             if (w < at + ns) {
                 s_share[0] = b;
                 s_share[1] = w - at;
@@ -184,11 +184,11 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
     const TiSpan span = seq_span<PAGED>(a, last);
     Blocks bl = blocks_of(span);
     if (last < 0) bl.n = 0;
-    const int c0 = sh.split * sh.chunk, c1 = min(bl.n, c0 + sh.chunk);
+    const int c0 = sh.split * sh.chunk, c1 = ti_min(bl.n, c0 + sh.chunk);
     const int r16 = lane & 15, j = lane >> 4;
 
     // this lane's row
-    const int rg = min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;
+    const int rg = ti_min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;
     const int pos = last - (a.p.T - 1) + t;
     const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
     // what every row of the tile sees: [full_low, full_end)
@@ -208,8 +208,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
         return id >= 0 && id < a.p.pg.pages ? id : -1;
     };
     auto row_of = [&](int k0, int kl, int page) -> size_t {            // the row of key k0 + kl; a row that exists where there is none
-        if constexpr (!PAGED) return (size_t)min(k0 + kl, span.end - 1);
-        const int id = max(__shfl(page, kl), 0);
+        if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
+        const int id = ti_max(__shfl(page, kl), 0);
         return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
     };
     auto load = [&](int i, int page) {
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
-            const int e = min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
+            const int e = ti_min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
             const size_t off = (row_of(k0, kl, page) * a.p.nKv + hk) * NG + g;
             ksr[p] = a.p.ks[off];
             vsr[p] = a.p.vs[off];
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
-            const int e = min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
+            const int e = ti_min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
             L.ks[wave][g][kl] = ksr[p];
             L.vs[wave][g][kl] = vsr[p] * VSCALE;
         }
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
         mx = fmaxf(mx, ti_xor(mx, 32));
         int ex = 4;
         if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
-        const int k = min(4 - ex, 100);
+        const int k = ti_min(4 - ex, 100);
         const float up = ldexpf(1.0f, k);
         fr = fr * ldexpf(1.0f, -k);
 #pragma unroll
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f*>(&L.o[wave][r16][16 * d + 4 * j]) = o[d];
     __syncthreads();
-    const int nr = min(16, a.R - rt * 16);
+    const int nr = ti_min(16, a.R - rt * 16);
     const size_t base = ((size_t)w * a.p.nKv + hk) * a.R + rt * 16;
     for (int e = tid; e < nr * (HD / 4); e += 256) {
         const int r = e / (HD / 4), d = e % (HD / 4);
@@ -454,11 +454,11 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int rows) {
         const float mi = i < ns ? ml[2 * i * step] : -INFINITY, li = i < ns ? ml[2 * i * step + 1] : 0.0f;
         const float wi = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
         L += wi * li;
-        const int n = min(64, ns - i0);
+        const int n = ti_min(64, ns - i0);
         for (int k0 = 0; k0 < n; k0 += 8) {
             float2 x[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float2*>(po + (size_t)min(i0 + k0 + k, ns - 1) * step * HD);
+            for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float2*>(po + (size_t)ti_min(i0 + k0 + k, ns - 1) * step * HD);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float f = k0 + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), k0 + k)) : 0.0f;

@@ -1,0 +1,483 @@
+// k_window_attn.hip — causal attention of a prompt's tokens over the int8 KV cache under a sliding window with sinks,
+// both products on the matrix cores at f32 accuracy; and the columns' sums of its weights.
+//
+// Workgroup (4 waves): one KV head, 64 RW query rows (row = token x query head of the KV head), 16 RW a wave, and the keys
+// that any of them sees, or a range of these. Blocks of 64 keys, at multiples of 64, are staged in LDS as MFMA operands
+// (K codes f16, V codes bf16, exact), the next block's loads in flight meanwhile; a wave passes over the 32 keys that none of its
+// rows sees and masks only where an edge of the window cuts them.
+//   - S^T = K Q^T (v_mfma_f32_16x16x32_f16 per 32-dim group, q half and 16 keys; the row scaled by a power of two, q =
+//     hi + lo to 2^-25 of its largest element), each group's sum times its key's scale in f32.
+//   - O^T = V^T P^T with P times the V scale of (key, group) in f32 as three bf16, exactly; a lane's scores are the
+//     operand as they stand.
+#include "ti_dev.h"
+#include "ti_span.h"
+#include "ti_window_attn.h"
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));   // the caller's q and out need not be aligned
+
+constexpr int KB = 64;                       // keys of a staged block
+constexpr int VSTRIDE = 65;                  // 16-byte pieces of a V operand tile (1 of padding: writes of eight tiles would meet in one bank)
+constexpr float FLOOR = -3.402823466e38f;    // below it only rows that see nothing: scores of -inf give NaN as the formula does
+constexpr float VSCALE = 0x1p-24f;           // of every V scale: 127 x a V scale x thousands of keys stays in f32's range
+
+struct WinArgs {
+    TiWindowAttn p;
+    float* po;                               // [row][nsplit][HD] partials, (m, l) of each; nsplit = 1: none
+    float* pml;
+    int G, nblk, nsplit;
+};
+
+// The query row of this lane: MFMA operands of its dims 32 g + 8 j.., and the factor that scales its scores to log2 units
+template <int HD>
+__device__ __forceinline__ float query_operand(const float* q, ti_h8 (&qh)[HD / 32], ti_h8 (&ql)[HD / 32]) {
+    constexpr int NG = HD / 32;
+    v4f_u qv[NG][2];
+    float mx = 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(qv[g][u][e]));
+        }
+    mx = fmaxf(mx, ti_xor(mx, 16));
+    mx = fmaxf(mx, ti_xor(mx, 32));
+    int ex = 4;
+    if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+    const int k = ti_min(4 - ex, 100);
+    const float up = ldexpf(1.0f, k);
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float v = qv[g][e / 4][e % 4] * up;
+            const _Float16 hi = (_Float16)v;
+            qh[g][e] = hi;
+            ql[g][e] = (_Float16)(v - (float)hi);
+        }
+    return 1.44269504088896341f / (127.0f * sqrtf((float)HD)) * ldexpf(1.0f, -k);
+}
+
+// 4 x 4 bytes: in, w[r] = row r's four bytes; out, w[e] = byte e of rows 0..3
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+template <int HD>
+struct WinLds {
+    ti_h8 k[KB / 16][HD / 32][64];           // [16 keys][group][lane]: key lane % 16, dims 8 (lane / 16)..
+    ti_b8 v[KB / 32][HD / 16][VSTRIDE];      // [32 keys][16 dims][lane]: dim lane % 16, keys 4 j.., 16 + 4 j..
+    float ks[HD / 32][KB], vs[HD / 32][KB];
+};
+
+template <int HD, int RW>
+__global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a) {
+    constexpr int NG = HD / 32, PC = HD / 16;
+    constexpr int KL = (KB * PC + 255) / 256, VL = (KB * HD / 16 + 255) / 256, SL = (KB * NG + 255) / 256;
+    __shared__ WinLds<HD> L;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m16 = lane & 15, j = lane >> 4;
+    const int hk = blockIdx.x % a.p.nKv, blk = (blockIdx.x / a.p.nKv) % a.nblk, split = blockIdx.x / (a.p.nKv * a.nblk);
+    const int nrows = a.G * a.p.T, window = a.p.window, sinks = a.p.sinks, pos0 = a.p.pos0;
+    const int wg0 = blk * 64 * RW, wg1 = ti_min(wg0 + 64 * RW, nrows) - 1;
+    auto low_of = [&](int pos) { return window < 0 || window > pos ? 0 : pos + 1 - window; };
+
+    // the blocks that hold keys which some row of the workgroup sees, this range's part of them
+    const TiSpan sp = ti_span(pos0 + wg0 / a.G, window, sinks);
+    const int end = pos0 + wg1 / a.G + 1;
+    const int sb = (sp.first + KB - 1) / KB, skip = ti_max(sb, sp.low / KB) - sb;
+    const int nb = ti_max(0, (int)(((long)end + KB - 1) / KB) - skip);
+    const int per = (nb + a.nsplit - 1) / a.nsplit;
+    const int c0 = split * per, c1 = ti_min(nb, c0 + per);
+    auto block_key = [&](int i) { return (i < sb ? i : i + skip) * KB; };
+
+    const size_t code_row = (size_t)a.p.nKv * HD, scale_row = (size_t)a.p.nKv * NG;
+    const uint8_t* kp = a.p.kq + hk * HD;
+    const uint8_t* vp = a.p.vq + hk * HD;
+    const float* ksp = a.p.ks + hk * NG;
+    const float* vsp = a.p.vs + hk * NG;
+
+    uint4 kr[KL];
+    uint32_t vr[VL][4];
+    float ksr[SL], vsr[SL];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < KL; u++) {
+            const int x = ti_min(tid + 256 * u, KB * PC - 1), key = (x >> 4) / PC * 16 + (x & 15), c = (x >> 4) % PC;
+            kr[u] = *reinterpret_cast<const uint4*>(kp + (size_t)ti_min(k0 + key, end - 1) * code_row + 16 * c);
+        }
+#pragma unroll
+        for (int u = 0; u < VL; u++) {
+            const int x = ti_min(tid + 256 * u, KB * HD / 16 - 1), db = x % (HD / 4), kb = x / (HD / 4);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                vr[u][r] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ti_min(k0 + 4 * kb + r, end - 1) * code_row + 4 * db);
+        }
+#pragma unroll
+        for (int u = 0; u < SL; u++) {
+            const int x = ti_min(tid + 256 * u, KB * NG - 1);
+            const size_t s = (size_t)ti_min(k0 + x / NG, end - 1) * scale_row + x % NG;
+            ksr[u] = ksp[s];
+            vsr[u] = vsp[s];
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int u = 0; u < KL; u++) {
+            const int x = tid + 256 * u, t = (x >> 4) / PC, c = (x >> 4) % PC, m = x & 15;
+            if (KB * PC % 256 == 0 || x < KB * PC) {
+                L.k[t][c >> 1][(c & 1) * 32 + m] = ti_i8x8_h8(kr[u].x, kr[u].y);
+                L.k[t][c >> 1][(c & 1) * 32 + 16 + m] = ti_i8x8_h8(kr[u].z, kr[u].w);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < VL; u++) {
+            const int x = tid + 256 * u, db = x % (HD / 4), kb = x / (HD / 4), kk = kb & 7;
+            if (KB * HD / 16 % 256 == 0 || x < KB * HD / 16) {
+                transpose4(vr[u]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ti_b8* p = &L.v[kb >> 3][db >> 2][(kk & 3) * 16 + 4 * (db & 3) + e];
+                    reinterpret_cast<uint2*>(p)[kk >> 2] = ti_i8x4_b4(vr[u][e]);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < SL; u++) {
+            const int x = tid + 256 * u;
+            if (KB * NG % 256 == 0 || x < KB * NG) {
+                L.ks[x % NG][x / NG] = ksr[u];
+                L.vs[x % NG][x / NG] = vsr[u] * VSCALE;
+            }
+        }
+    };
+    if (c0 < c1) load(block_key(c0));
+
+    // this lane's rows (past the last: that one again), and what all rows of the wave and any of them see
+    const int row0 = wg0 + wave * 16 * RW;
+    int pos[RW], low[RW];
+    size_t orow[RW];
+    ti_h8 qh[RW][NG], ql[RW][NG];
+    float fr[RW];
+#pragma unroll
+    for (int r = 0; r < RW; r++) {
+        const int gr = ti_min(row0 + 16 * r + m16, nrows - 1), t = gr / a.G;
+        pos[r] = pos0 + t;
+        low[r] = low_of(pos[r]);
+        orow[r] = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
+        fr[r] = query_operand<HD>(a.p.qr + orow[r] * HD + 8 * j, qh[r], ql[r]);
+    }
+    const int first_pos = pos0 + ti_min(row0, nrows - 1) / a.G, last_pos = pos0 + ti_min(row0 + 16 * RW - 1, nrows - 1) / a.G;
+    const int any_low = low_of(first_pos), all_low = low_of(last_pos);
+
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f o[RW][HD / 16];
+    float mx[RW], l[RW];
+#pragma unroll
+    for (int r = 0; r < RW; r++) {
+        mx[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[r][d] = zero;
+    }
+    for (int i = c0; i < c1; i++) {
+        const int t0 = block_key(i);
+        __syncthreads();                                   // the last block is read
+        stage();
+        __syncthreads();
+        if (i + 1 < c1) load(block_key(i + 1));
+        TI_ISSUE_FENCE();
+#pragma unroll 1
+        for (int h = 0; h < KB / 32; h++) {                // 32 keys
+            const int k0 = t0 + 32 * h;
+            // wave-uniform: no row of the wave sees any of them
+            if (row0 >= nrows || k0 > last_pos || (k0 + 31 < any_low && k0 >= sinks)) continue;
+            const bool whole = k0 + 31 <= first_pos && (k0 >= all_low || k0 + 32 <= sinks);
+            float s[RW][8];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                v4f acc[RW];
+#pragma unroll
+                for (int r = 0; r < RW; r++) acc[r] = zero;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const ti_h8 kk = L.k[2 * h + b][g][lane];
+                    const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[g][32 * h + 16 * b + 4 * j]);
+#pragma unroll
+                    for (int r = 0; r < RW; r++) {
+                        v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[r][g], zero, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[r][g], d, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[r][e] = fmaf(d[e], sc[e], acc[r][e]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RW; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[r][4 * b + e] = acc[r][e] * fr[r];
+            }
+            uint32_t seen[RW];
+#pragma unroll
+            for (int r = 0; r < RW; r++) {
+                seen[r] = 0xffu;
+                float tm = FLOOR;
+                if (!whole) {
+                    tm = -INFINITY;
+                    seen[r] = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int key = k0 + 16 * (e >> 2) + 4 * j + (e & 3);
+                        const bool ok = key <= pos[r] && (key >= low[r] || key < sinks);
+                        seen[r] |= ok ? 1u << e : 0u;
+                        tm = fmaxf(tm, ok ? fmaxf(s[r][e], FLOOR) : -INFINITY);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[r][e]);
+                }
+                tm = fmaxf(tm, ti_xor(tm, 16));
+                tm = fmaxf(tm, ti_xor(tm, 32));
+                // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
+                const bool bump = tm > mx[r] + 6.0f;
+                if (__any(bump)) {
+                    const float mn = bump ? tm : mx[r];
+                    const float alpha = bump ? __builtin_amdgcn_exp2f(mx[r] - mn) : 1.0f;
+                    l[r] = l[r] * alpha;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; d++) o[r][d] = o[r][d] * alpha;
+                    mx[r] = mn;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float p = __builtin_amdgcn_exp2f(s[r][e] - mx[r]);
+                    if (!whole) p = seen[r] >> e & 1u ? p : 0.0f;
+                    s[r][e] = p;
+                }
+                l[r] += ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3])) + ((s[r][4] + s[r][5]) + (s[r][6] + s[r][7]));
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * h + 4 * j]);
+                const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * h + 16 + 4 * j]);
+                ti_b8 p[RW][3];
+#pragma unroll
+                for (int r = 0; r < RW; r++) {
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        w[e] = s[r][e] * v0[e];
+                        w[4 + e] = s[r][4 + e] * v1[e];
+                    }
+                    if (!whole) {                          // the scale of a key that the row does not see may be NaN
+#pragma unroll
+                        for (int e = 0; e < 8; e++) w[e] = seen[r] >> e & 1u ? w[e] : 0.0f;
+                    }
+                    ti_bf16x3(w, p[r]);
+                }
+#pragma unroll
+                for (int d = 2 * g; d < 2 * g + 2; d++) {
+                    const ti_b8 vv = L.v[h][d][lane];
+#pragma unroll
+                    for (int r = 0; r < RW; r++)
+#pragma unroll
+                        for (int e = 2; e >= 0; e--) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[r][e], o[r][d], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RW; r++) {
+        float lt = l[r] + ti_xor(l[r], 16);
+        lt += ti_xor(lt, 32);
+        if (row0 + 16 * r + m16 >= nrows) continue;
+        const bool direct = a.nsplit == 1;
+        const float inv = 1.0f / (127.0f * VSCALE * lt);
+        const float f = !direct ? 1.0f : mx[r] == -INFINITY ? 0.0f : inv;
+        float* dst = direct ? a.p.out + orow[r] * HD : a.po + (orow[r] * a.nsplit + split) * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f_u*>(dst + 16 * d + 4 * j) = o[r][d] * f;
+        float* ml = direct ? a.p.ml ? a.p.ml + 2 * orow[r] : nullptr : a.pml + 2 * (orow[r] * a.nsplit + split);
+        if (j == 0 && ml) {
+            ml[0] = mx[r];
+            ml[1] = lt;
+        }
+    }
+}
+
+// A wave a row: its ranges' partials (at most 64) into the output
+template <int HD>
+__global__ __launch_bounds__(256) void k_window_merge(WinArgs a, int rows) {
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;                               // wave-uniform
+    const int n = a.nsplit;
+    const float* ml = a.pml + 2 * (size_t)row * n;
+    const float mi = lane < n ? ml[2 * lane] : -INFINITY, li = lane < n ? ml[2 * lane + 1] : 0.0f;
+    const float M = ti_wave_max(mi);
+    const float wi = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
+    const float Lt = ti_wave_sum(wi * li);
+    const int d = lane % (HD / 2);
+    const float* po = a.po + (size_t)row * n * HD + 2 * d;
+    float v0 = 0.0f, v1 = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+        float2 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float2*>(po + (size_t)ti_min(i0 + k, n - 1) * HD);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float f = i0 + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), i0 + k)) : 0.0f;
+            v0 = fmaf(x[k].x, f, v0);
+            v1 = fmaf(x[k].y, f, v1);
+        }
+    }
+    if (lane < HD / 2) {
+        const float div = 127.0f * VSCALE * Lt;
+        float* out = a.p.out + (size_t)row * HD + 2 * d;
+        out[0] = M == -INFINITY ? 0.0f : v0 / div;
+        out[1] = M == -INFINITY ? 0.0f : v1 / div;
+    }
+    if (a.p.ml && lane == 0) {
+        a.p.ml[2 * row] = M;
+        a.p.ml[2 * row + 1] = Lt;
+    }
+}
+
+// Column sums of the weights: a wave holds 16 keys of a KV head as the MFMA's A operand and passes over the rows, whose operands a
+// workgroup stages 64 at a time; a lane adds up the weights that one row in 16 gives to four keys, in the rows' order.
+template <int HD>
+__global__ __launch_bounds__(256) void k_mass_columns(WinArgs a, float* __restrict__ mass) {
+    constexpr int NG = HD / 32;
+    __shared__ ti_h8 s_q[4][2][NG][64];                    // [16 rows][hi, lo][group][lane]
+    __shared__ float s_f[64], s_m[64], s_l[64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m16 = lane & 15, j = lane >> 4;
+    const int hk = blockIdx.x % a.p.nKv;
+    const long kw = (long)(blockIdx.x / a.p.nKv) * 64;     // the workgroup's first key
+    const long k0 = kw + 16 * wave, S = (long)a.p.pos0 + a.p.T;
+    const int nrows = a.G * a.p.T;
+
+    ti_h8 kk[NG];
+    float sc[NG][4];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const uint2 w = *reinterpret_cast<const uint2*>(a.p.kq + ((size_t)ti_min(k0 + m16, S - 1) * a.p.nKv + hk) * HD + 32 * g + 8 * j);
+        kk[g] = ti_i8x8_h8(w.x, w.y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[g][e] = a.p.ks[((size_t)ti_min(k0 + 4 * j + e, S - 1) * a.p.nKv + hk) * NG + g];
+    }
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // rows before the one of the workgroup's first key see none of its keys
+    const int start = (int)ti_max(0L, kw - a.p.pos0) * a.G / 64 * 64;
+    for (int r0 = start; r0 < nrows; r0 += 64) {
+        __syncthreads();
+        {
+            const int gr = ti_min(r0 + 16 * wave + m16, nrows - 1), t = gr / a.G;
+            const size_t row = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
+            ti_h8 qh[NG], ql[NG];
+            const float f = query_operand<HD>(a.p.qr + row * HD + 8 * j, qh, ql);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                s_q[wave][0][g][lane] = qh[g];
+                s_q[wave][1][g][lane] = ql[g];
+            }
+            if (j == 0) {
+                s_f[16 * wave + m16] = f;
+                s_m[16 * wave + m16] = a.p.ml[2 * row];
+                s_l[16 * wave + m16] = 1.0f / a.p.ml[2 * row + 1];
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int t = 0; t < 4 && r0 + 16 * t < nrows; t++) {
+            const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            v4f acc = zero;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g], s_q[t][0][g][lane], zero, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g], s_q[t][1][g][lane], d, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[g][e], acc[e]);
+            }
+            const int rl = 16 * t + m16, gr = r0 + rl;
+            const float f = s_f[rl], m = s_m[rl], inv = s_l[rl];
+            const long pos = gr < nrows ? a.p.pos0 + gr / a.G : -1;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p = __builtin_amdgcn_exp2f(acc[e] * f - m) * inv;
+                sum[e] += k0 + 4 * j + e <= pos ? p : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        sum[e] += ti_xor(sum[e], 1);
+        sum[e] += ti_xor(sum[e], 2);
+        sum[e] += ti_xor(sum[e], 4);
+        sum[e] += ti_xor(sum[e], 8);
+        const long key = k0 + 4 * j + e;
+        if (m16 == 0 && key < S) {
+            float* d = mass + (size_t)key * a.p.nKv + hk;
+            *d = key < a.p.pos0 ? *d + sum[e] : sum[e];
+        }
+    }
+}
+
+template <int HD>
+int launch(ti_ctx* c, const TiWindowAttn& p) {
+    const int G = p.nHq / p.nKv, nrows = G * p.T;
+    // keys that 64 rows see, at most, in blocks
+    const int tokens = (63 + G) / G + 1;
+    const long keys = p.window < 0 ? (long)p.pos0 + p.T : ti_min((long)p.pos0 + p.T, (long)p.window + p.sinks + tokens);
+    const long kb = keys / KB + 3;
+    // 32 rows a wave where that still gives every CU its workgroups
+    const bool two = (long)p.nKv * ((nrows + 127) / 128) >= c->cus;
+    const int rows = two ? 128 : 64, nblk = (nrows + rows - 1) / rows;
+    const long wg = (long)p.nKv * nblk;
+    long ns = (2L * c->cus + wg - 1) / wg;
+    if (two) ns = 1;
+    if (ns > kb / 2) ns = kb / 2;
+    if (ns > 64) ns = 64;
+    if (ns * p.T * p.nHq > TI_ATTN_ROWSPLITS) ns = TI_ATTN_ROWSPLITS / ((long)p.T * p.nHq);
+    if (ns < 1) ns = 1;
+    const WinArgs a = {p, c->attn_po, c->attn_ml, G, nblk, (int)ns};
+    const unsigned grid = (unsigned)(wg * ns);
+    if (two) k_window_attn<HD, 2><<<grid, 256, 0, c->stream>>>(a);
+    else k_window_attn<HD, 1><<<grid, 256, 0, c->stream>>>(a);
+    TI_LAUNCHED("k_window_attn");
+    if (ns > 1) {
+        const int total = p.T * p.nHq;
+        k_window_merge<HD><<<(unsigned)((total + 3) / 4), 256, 0, c->stream>>>(a, total);
+        TI_LAUNCHED("k_window_merge");
+    }
+    return TI_OK;
+}
+
+template <int HD>
+int launch_mass(ti_ctx* c, const TiWindowAttn& p, float* mass) {
+    const WinArgs a = {p, nullptr, nullptr, p.nHq / p.nKv, 0, 0};
+    const long S = (long)p.pos0 + p.T;
+    k_mass_columns<HD><<<(unsigned)((S + 63) / 64 * p.nKv), 256, 0, c->stream>>>(a, mass);
+    TI_LAUNCHED("k_mass_columns");
+    return TI_OK;
+}
+
+}  // namespace
+
+int ti_window_attn_launch(ti_ctx* c, const TiWindowAttn& p, int hd) {
+    return hd == 128 ? launch<128>(c, p) : hd == 96 ? launch<96>(c, p) : hd == 64 ? launch<64>(c, p) : launch<32>(c, p);
+}
+int ti_mass_columns_launch(ti_ctx* c, const TiWindowAttn& p, int hd, float* mass) {
+    return hd == 128 ? launch_mass<128>(c, p, mass) : hd == 96 ? launch_mass<96>(c, p, mass)
+         : hd == 64 ? launch_mass<64>(c, p, mass) : launch_mass<32>(c, p, mass);
+}

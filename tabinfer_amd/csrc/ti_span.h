@@ -9,6 +9,13 @@
 #define TI_HD
 #endif
 
+// One type on both sides: the toolkit's host min and max take int.
+template <class N> TI_HD inline N ti_min(N a, N b) { return b < a ? b : a; }
+template <class N> TI_HD inline N ti_max(N a, N b) { return a < b ? b : a; }
+
+// Positions of the attention calls end here, so that a block of keys past the last one has 32-bit positions too.
+constexpr int TI_POS_END = 0x7fffff00;
+
 // The keys a query at position p sees: [0, first) and [low, p + 1), in order; first <= low. window < 0: all of them.
 struct TiSpan {
     int first, low, end;
