@@ -516,7 +516,7 @@ int ti_kv_read_paged_q8(ti_ctx* ctx, const uint32_t* kq, const float* ks, const 
  * ti_attn_window_q8. Pages that hold no visible key are not looked up, so their table entries may be anything; a
  * visible position whose page id is outside [0, pages) counts as not there. lens[b] above width * page is taken
  * as width * page, lens[b] <= 0 gives zeros. Rows of several tokens of one sequence are sequences that
- * repeat its table row, with their own lengths. B <= 4096, nHq <= 64; out must not overlap qr. */
+ * repeat its table row, with their own lengths. B <= 2048, nHq <= 64; out must not overlap qr. */
 int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
                      const uint32_t* vq, const float* vs, const int32_t* table, const int32_t* lens,
                      float* out, int B, int nHq, int nKv, int hd, int page, int pages, int width,

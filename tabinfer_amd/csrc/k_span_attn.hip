@@ -59,7 +59,7 @@ extern "C" int ti_attn_paged_q8(ti_ctx* c, const float* qr, const uint32_t* kq, 
     const int rc = check_attn("ti_attn_paged_q8", qr, kq, ks, vq, vs, out, B, nHq, nKv, hd);
     if (rc) return rc;
     TI_REQUIRE(table && lens, "ti_attn_paged_q8: null table or lengths");
-    TI_REQUIRE(B <= 4096, "ti_attn_paged_q8: %d sequences > 4096", B);
+    TI_REQUIRE(B <= TI_TOKEN_SEQS, "ti_attn_paged_q8: %d sequences > %d", B, TI_TOKEN_SEQS);
     TI_REQUIRE(ti_pow2(page) && pages > 0 && width > 0 && (long)page * width <= TI_POS_END,
                "ti_attn_paged_q8: bad pages (length %d, a power of two; %d of them; table width %d)", page, pages, width);
     TI_REQUIRE(sinks >= 0, "ti_attn_paged_q8: sinks = %d", sinks);

@@ -3,9 +3,10 @@
 // made of. At most 16 rows a tile (row = token x query head of the KV head), both products on the matrix cores.
 //
 //  - The visible keys are cut into blocks of 32 at multiples of 32 (a page of 32 and more covers whole blocks). The
-//    blocks of all sequences share one number of workgroups a KV head: with C = total / target blocks a workgroup, a
-//    sequence of n blocks takes ceil(n / C) of them, so that a long one among short ones is spread like the rest.
-//    Every workgroup finds its sequence by a scan over the lengths; nothing depends on them on the host.
+//    blocks of all sequences, one sequence's behind the other's, are dealt out in runs of `chunk` to the workgroups of a
+//    KV head: each has the same work whatever the lengths, a run that ends one sequence begins the next, and its part of
+//    a sequence is a partial in slot (workgroup + sequence). Every workgroup finds its run by a scan over the lengths;
+//    nothing depends on them on the host.
 //  - A wave takes a block at a time, on its own: loads of the next block in flight, the codes through LDS of its own.
 //    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-25 of
 //    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
@@ -25,6 +26,7 @@ typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int BLK = 32;                      // keys of a wave's block
 constexpr int WAVES = 4;
+constexpr int XCDS = 8;
 constexpr int CMIN = WAVES;                  // blocks of a workgroup, at least
 constexpr float FLOOR = -3.402823466e38f;
 constexpr float VSCALE = 0x1p-24f;           // of every V scale: 127 x a V scale x thousands of keys stays in f32's range
@@ -34,7 +36,7 @@ struct TokArgs {
     float* po;                               // [slot][nKv][T G][HD] partials, (m, l) of each
     float* pml;
     int32_t* meta;                           // [B][2]: a sequence's first slot and their number
-    int G, R, RT, target;                    // R = T G rows a KV head in RT tiles; target: workgroups a KV head to fill
+    int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups a KV head, at most
 };
 
 // Blocks that hold the keys [0, first) and [low, end): [0, sb) and [wb, sb + ... )
@@ -42,7 +44,7 @@ struct Blocks {
     int sb, skip, n;                         // sink blocks; blocks between them and the window; all that are visited
     __device__ int at(int i) const { return i < sb ? i : i + skip; }
 };
-__device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
+__host__ __device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
     Blocks b;
     b.sb = (s.first + BLK - 1) / BLK;
     const int w = ti_max(b.sb, s.low / BLK);
@@ -64,92 +66,82 @@ __device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int last) {   // th
     s.end = last + 1;
     return s;
 }
+// blocks of a sequence; one (of nothing) where no key is visible, so that every sequence has a slot
 template <bool PAGED>
 __device__ __forceinline__ int seq_blocks(const TokArgs& a, int b) {
     const int last = seq_last<PAGED>(a, b);
-    return last < 0 ? 0 : blocks_of(seq_span<PAGED>(a, last)).n;
+    return last < 0 ? 1 : ti_max(1, blocks_of(seq_span<PAGED>(a, last)).n);
 }
 
-struct Share {
-    int b, split, ns, chunk;                 // sequence, which of its ns workgroups, blocks of each
-};
-
-// sum over the workgroup (every thread), and the sum of the threads before this one
-template <class N>
-__device__ __forceinline__ N wg_scan(N v, N* s4, N& total) {
+// sum of the threads before this one, and of all of the workgroup
+__device__ __forceinline__ long wg_scan(long v, long* s4, long& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    N x = v;
+    long x = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const N y = __shfl_up(x, o);
+        const long y = __shfl_up(x, o);
         x += lane >= o ? y : 0;
     }
     if (lane == 63) s4[wave] = x;
     __syncthreads();
-    N before = 0, all = 0;
+    long before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
-        const N t = s4[w];
+        const long t = s4[w];
         before += w < wave ? t : 0;
         all += t;
     }
     total = all;
-    __syncthreads();
     return before + x - v;
 }
 
-__device__ __forceinline__ int share_chunk(long total, int target) {
-    const long c = target > 0 ? (total + target - 1) / target : 0x7fffffffL;
-    return (int)ti_min(ti_max(c, (long)CMIN), 0x7fffffffL);
+// The run of blocks of a workgroup, in sequence b from its block `block` (at block `start` of all) on
+struct Run {
+    long chunk, left;                        // blocks of every workgroup's run; of this one, still to do
+    long start;
+    int b, block;
+};
+// blocks of a run: all workgroups', but CMIN (each wave a block) where the sequences have as many
+__host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs) {
+    return ti_max((total + wgs - 1) / wgs, ti_min((long)CMIN, (total + B - 1) / B));
 }
-
-// slot w of a KV head -> its share; false: there are fewer slots
 template <bool PAGED>
-__device__ bool find_share(const TokArgs& a, int w, Share& sh, long* s8, int* s_share) {
+__device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, int* s_b) {
     const int B = a.p.B, tid = threadIdx.x;
     if (B == 1) {
-        const int n = seq_blocks<PAGED>(a, 0);
-        sh.b = 0;
-        sh.chunk = share_chunk(n, a.target);
-        sh.ns = ti_max(1, (int)(((long)n + sh.chunk - 1) / sh.chunk));
-        sh.split = w;
-        if (w == 0 && tid == 0) {
-            a.meta[0] = 0;
-            a.meta[1] = sh.ns;
-        }
-        return w < sh.ns;
+        const long n = seq_blocks<PAGED>(a, 0);
+        r.chunk = run_chunk(n, 1, a.wgs);
+        r.b = 0;
+        r.start = 0;
+        r.block = (int)ti_min(w * r.chunk, n);
+        r.left = ti_min(r.chunk, n - r.block);
+        return r.left > 0;
     }
     // a thread: the sequences [tid per, tid per + per)
     const int per = (B + 255) / 256, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
     for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
-    (void)wg_scan(mine, s8, total);
-    const int chunk = share_chunk(total, a.target);
-    int slots = 0, all;
-    for (int b = b0; b < b1; b++) slots += ti_max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
-    int at = wg_scan(slots, reinterpret_cast<int*>(s8), all);
-    if (w >= at && w < at + slots) {
+    long at = wg_scan(mine, s4, total);
+    r.chunk = run_chunk(total, B, a.wgs);
+    const long g0 = w * r.chunk;
+    if (g0 >= at && g0 < at + mine) {
         for (int b = b0; b < b1; b++) {
-            const int ns = ti_max(1, (int)(((long)seq_blocks<PAGED>(a, b) + chunk - 1) / chunk));
-            if (w < at + ns) {
-                s_share[0] = b;
-                s_share[1] = w - at;
-                s_share[2] = ns;
-                if (w == at) {
-                    a.meta[2 * b] = at;
-                    a.meta[2 * b + 1] = ns;
-                }
+            const int n = seq_blocks<PAGED>(a, b);
+            if (g0 < at + n) {
+                *s_b = b;
+                *s_at = at;
                 break;
             }
-            at += ns;
+            at += n;
         }
     }
     __syncthreads();
-    sh.b = s_share[0];
-    sh.split = s_share[1];
-    sh.ns = s_share[2];
-    sh.chunk = chunk;
-    return w < all;
+    if (g0 >= total) return false;
+    r.left = ti_min(r.chunk, total - g0);
+    r.b = __builtin_amdgcn_readfirstlane(*s_b);
+    r.start = *s_at;
+    r.block = (int)(g0 - r.start);
+    return true;
 }
 
 template <int HD>
@@ -165,34 +157,67 @@ struct TokLds {
     };
     float ks[WAVES][NG][BLK], vs[WAVES][NG][BLK];
     float m[WAVES][16], l[WAVES][16];
-    long s8[WAVES];
-    int share[4];
+    long s4[WAVES], at;
+    int b;
 };
 
 template <int HD, bool PAGED>
-__global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) {
+__global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_attn(TokArgs a) {
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
     constexpr int KS = TokLds<HD>::KS, VS = TokLds<HD>::VS;
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     __shared__ __align__(16) TokLds<HD> L;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % a.p.nKv, rt = (blockIdx.x / a.p.nKv) % a.RT, w = blockIdx.x / (a.p.nKv * a.RT);
-    Share sh;
-    if (!find_share<PAGED>(a, w, sh, L.s8, L.share)) return;           // workgroup-uniform
-    const int last = seq_last<PAGED>(a, sh.b);
+    // the KV heads of a run on one XCD (workgroups go to the eight in turn), near each other in time: their scales, 4 NG bytes
+    // a head and position, share cache lines, and so do the codes of narrow heads
+    const int heads = a.p.nKv * a.RT, hr = (blockIdx.x / XCDS) % heads, w = blockIdx.x / (XCDS * heads) * XCDS + blockIdx.x % XCDS;
+    const int hk = hr % a.p.nKv, rt = hr / a.p.nKv;
+    Run run;
+    if (!find_run<PAGED>(a, w, run, L.s4, &L.at, &L.b)) return;        // workgroup-uniform
+    const int r16 = lane & 15, j = lane >> 4;
+
+    const int rg = ti_min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;   // this lane's row
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
+    const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
+    // a lane's loads of a block: row and byte in it
+    int pl[NL], sl[SL];
+    uint32_t po[NL], so[SL];
+#pragma unroll
+    for (int p = 0; p < NL; p++) {
+        const int pc = lane + 64 * p;
+        pl[p] = pc / PC;
+        po[p] = (uint32_t)(pl[p] * a.p.nKv) * HD + 16 * (pc % PC);
+    }
+#pragma unroll
+    for (int p = 0; p < SL; p++) {
+        const int e = ti_min(lane + 64 * p, BLK * NG - 1);
+        sl[p] = e / NG;
+        so[p] = (uint32_t)(sl[p] * a.p.nKv) * NG + e % NG;
+    }
+
+  for (;;) {
+    // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
+    const int last = seq_last<PAGED>(a, run.b);
     const TiSpan span = seq_span<PAGED>(a, last);
     Blocks bl = blocks_of(span);
     if (last < 0) bl.n = 0;
-    const int c0 = sh.split * sh.chunk, c1 = ti_min(bl.n, c0 + sh.chunk);
-    const int r16 = lane & 15, j = lane >> 4;
-
-    // this lane's row
-    const int rg = ti_min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;
+    const int nb = ti_max(1, bl.n);
+    const int c0 = run.block, part = (int)ti_min((long)(nb - c0), run.left), c1 = ti_min(bl.n, c0 + part);
     const int pos = last - (a.p.T - 1) + t;
     const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
     // what every row of the tile sees: [full_low, full_end)
     const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
+    // the query's loads before the keys': they come back first
+    v4f_u qv[NG][2];
+    {
+        const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD + 8 * j;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
+    }
 
     // ---- a block's loads
     uint4 kr[NL], vr[NL];
@@ -204,27 +229,50 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
         if constexpr (!PAGED) return in ? 0 : -1;
         const int k = key >> a.p.pg.shift;
         if (!in || k >= a.p.pg.width) return -1;
-        const int id = a.p.pg.table[(size_t)sh.b * a.p.pg.width + k];
+        const int id = a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
         return id >= 0 && id < a.p.pg.pages ? id : -1;
     };
-    auto row_of = [&](int k0, int kl, int page) -> size_t {            // the row of key k0 + kl; a row that exists where there is none
-        if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
-        const int id = ti_max(__shfl(page, kl), 0);
-        return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
-    };
+    // rows of one page, or of the contiguous cache, follow each other: one base and the lanes' fixed offsets
+    const bool runs = !PAGED || a.p.pg.shift >= 5;
     auto load = [&](int i, int page) {
         const int k0 = bl.at(i) * BLK;
+        if (runs && (PAGED || k0 + BLK <= span.end)) {
+            size_t row = (size_t)k0;
+            if constexpr (PAGED) {
+                // the id of any of the block's keys that is seen (the others carry -1); page 0 where there is none
+                const uint64_t some = __ballot(page >= 0);
+                const int id = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
+                row = ((size_t)(uint32_t)id << a.p.pg.shift) + (k0 & ((1 << a.p.pg.shift) - 1));
+            }
+            const size_t base = (row * a.p.nKv + hk) * HD, sbase = (row * a.p.nKv + hk) * NG;
+            const uint8_t *kb = a.p.kq + base, *vb = a.p.vq + base;
+            const float *ksb = a.p.ks + sbase, *vsb = a.p.vs + sbase;
+#pragma unroll
+            for (int p = 0; p < NL; p++) {
+                kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + po[p]));
+                vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
+            }
+#pragma unroll
+            for (int p = 0; p < SL; p++) {
+                ksr[p] = ksb[so[p]];
+                vsr[p] = vsb[so[p]];
+            }
+            return;
+        }
+        auto row_of = [&](int kl) -> size_t {                          // a row that exists where the key does not
+            if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
+            const int id = ti_max(__shfl(page, kl), 0);
+            return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
+        };
 #pragma unroll
         for (int p = 0; p < NL; p++) {
-            const int pc = lane + 64 * p, kl = pc / PC, c = pc % PC;
-            const size_t off = (row_of(k0, kl, page) * a.p.nKv + hk) * HD + 16 * c;
+            const size_t off = (row_of(pl[p]) * a.p.nKv + hk) * HD + 16 * ((lane + 64 * p) % PC);
             kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + off));
             vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + off));
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
-            const int e = ti_min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
-            const size_t off = (row_of(k0, kl, page) * a.p.nKv + hk) * NG + g;
+            const size_t off = (row_of(sl[p]) * a.p.nKv + hk) * NG + ti_min(lane + 64 * p, BLK * NG - 1) % NG;
             ksr[p] = a.p.ks[off];
             vsr[p] = a.p.vs[off];
         }
@@ -252,22 +300,17 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
     int page = i < c1 ? fetch_page(i) : -1, page1 = -1;
     if (i + WAVES < c1) page1 = fetch_page(i + WAVES);
     if (i < c1) load(i, page);
+    TI_ISSUE_FENCE();
 
     // ---- Q operand: row r16, dims 32 g + 8 j.., scaled by 2^k so that the row's largest element is below 16
     ti_h8 qh[NG], ql[NG];
     float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
     {
-        const float* q = a.p.qr + ((size_t)(sh.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD + 8 * j;
-        v4f_u qv[NG][2];
         float mx = 0.0f;
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(qv[g][u][e]));
-            }
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[g][e / 4][e % 4]));
         mx = fmaxf(mx, ti_xor(mx, 16));
         mx = fmaxf(mx, ti_xor(mx, 32));
         int ex = 4;
@@ -286,13 +329,10 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
             }
     }
 
-    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     v4f o[HD / 16];
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) o[d] = zero;
     float m = -INFINITY, l = 0.0f;
-    // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
-    const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
 
     for (; i < c1; i += WAVES) {
         ti_wave_lds_fence();                               // the last block is read
@@ -408,7 +448,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
     for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f*>(&L.o[wave][r16][16 * d + 4 * j]) = o[d];
     __syncthreads();
     const int nr = ti_min(16, a.R - rt * 16);
-    const size_t base = ((size_t)w * a.p.nKv + hk) * a.R + rt * 16;
+    const size_t base = ((size_t)(w + run.b) * a.p.nKv + hk) * a.R + rt * 16;
     for (int e = tid; e < nr * (HD / 4); e += 256) {
         const int r = e / (HD / 4), d = e % (HD / 4);
         float M = L.m[0][r];
@@ -430,61 +470,88 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 4) void k_token_attn(TokArgs a) 
             a.pml[2 * (base + r) + 1] = y;
         }
     }
+    if (PAGED && c0 == 0 && hk == 0 && rt == 0 && tid == 0) {          // the sequence's slots, for the merge
+        a.meta[2 * run.b] = w + run.b;
+        a.meta[2 * run.b + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
+    }
+    run.left -= part;
+    if (run.left <= 0) return;
+    run.b++;
+    run.start += nb;
+    run.block = 0;
+    __syncthreads();                                       // the parts are read
+  }
 }
 
-// A wave a (sequence, token, head): its slots' partials into the output row
+// A workgroup a (sequence, token, head): its slots' partials into the output row, each group of threads those of its own
+// slots with every load in flight at once
 template <int HD>
-__global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int rows) {
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;                               // wave-uniform
+__global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
+    constexpr int D4 = HD / 4, SG = 256 / D4, UN = 8;
+    __shared__ float s_m[SG], s_l[SG];
+    __shared__ __align__(16) float s_o[SG][HD];
+    const int tid = threadIdx.x, sg = tid / D4, d = tid % D4;
+    const int row = blockIdx.x;
     const int hq = row % a.p.nHq, t = (row / a.p.nHq) % a.p.T, b = row / (a.p.nHq * a.p.T);
     const int hk = hq / a.G, r = t * a.G + hq % a.G;
-    const int s0 = a.meta[2 * b], ns = a.meta[2 * b + 1];
+    const int s0 = ns1 ? 0 : a.meta[2 * b], ns = ns1 ? ns1 : a.meta[2 * b + 1];
     const size_t step = (size_t)a.p.nKv * a.R, base = (size_t)s0 * step + (size_t)hk * a.R + r;
-    const float* ml = a.pml + 2 * base;
-    float M = -INFINITY;
-    for (int i = lane; i < ns; i += 64) M = fmaxf(M, ml[2 * i * step]);
-    M = ti_wave_max(M);
-    const int d = lane % (HD / 2);                         // dims 2 d, 2 d + 1
-    float v0 = 0.0f, v1 = 0.0f, L = 0.0f;
-    const float* po = a.po + base * HD + 2 * d;
-    for (int i0 = 0; i0 < ns; i0 += 64) {
-        const int i = i0 + lane;
-        const float mi = i < ns ? ml[2 * i * step] : -INFINITY, li = i < ns ? ml[2 * i * step + 1] : 0.0f;
-        const float wi = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
-        L += wi * li;
-        const int n = ti_min(64, ns - i0);
-        for (int k0 = 0; k0 < n; k0 += 8) {
-            float2 x[8];
+    float m = -INFINITY, l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = sg; i0 < ns && sg < SG; i0 += UN * SG) {
+        v4f x[UN];
+        float mi[UN], li[UN];
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float2*>(po + (size_t)ti_min(i0 + k0 + k, ns - 1) * step * HD);
+        for (int k = 0; k < UN; k++) {
+            const size_t at = base + (size_t)ti_min(i0 + k * SG, ns - 1) * step;
+            mi[k] = a.pml[2 * at];
+            li[k] = a.pml[2 * at + 1];
+            x[k] = *reinterpret_cast<const v4f*>(a.po + at * HD + 4 * d);
+        }
+        float mn = m;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float f = k0 + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), k0 + k)) : 0.0f;
-                v0 = fmaf(x[k].x, f, v0);
-                v1 = fmaf(x[k].y, f, v1);
-            }
+        for (int k = 0; k < UN; k++) mn = fmaxf(mn, mi[k]);
+        if (mn == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        o = o * f;
+        m = mn;
+#pragma unroll
+        for (int k = 0; k < UN; k++) {
+            const float e = i0 + k * SG < ns && mi[k] != -INFINITY ? __builtin_amdgcn_exp2f(mi[k] - m) : 0.0f;
+            l = fmaf(li[k], e, l);
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = fmaf(x[k][c], e, o[c]);
         }
     }
-    L = ti_wave_sum(L);
-    if (lane < HD / 2) {
-        const float div = 127.0f * VSCALE * L;
-        float* out = a.p.out + (size_t)row * HD + 2 * d;
-        out[0] = M == -INFINITY ? 0.0f : v0 / div;
-        out[1] = M == -INFINITY ? 0.0f : v1 / div;
+    if (sg < SG) {
+        *reinterpret_cast<v4f*>(&s_o[sg][4 * d]) = o;
+        if (d == 0) {
+            s_m[sg] = m;
+            s_l[sg] = l;
+        }
     }
-    if (a.p.ml && lane == 0) {
+    __syncthreads();
+    if (tid >= HD) return;
+    const int n = ti_min(SG, ns);
+    float M = -INFINITY, Lt = 0.0f, v = 0.0f;
+    for (int g = 0; g < n; g++) M = fmaxf(M, s_m[g]);
+    for (int g = 0; g < n; g++) {
+        const float e = s_m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[g] - M);
+        Lt = fmaf(s_l[g], e, Lt);
+        v = fmaf(s_o[g][tid], e, v);
+    }
+    a.p.out[(size_t)row * HD + tid] = M == -INFINITY ? 0.0f : v / (127.0f * VSCALE * Lt);
+    if (a.p.ml && tid == 0) {
         a.p.ml[2 * row] = M;
-        a.p.ml[2 * row + 1] = L;
+        a.p.ml[2 * row + 1] = Lt;
     }
 }
 
 template <int HD, bool PAGED>
-void launch(ti_ctx* c, const TokArgs& a, int slots) {
-    k_token_attn<HD, PAGED><<<(unsigned)((long)slots * a.RT * a.p.nKv), 256, 0, c->stream>>>(a);
-    const int rows = a.p.B * a.p.T * a.p.nHq;
-    k_token_merge<HD><<<(unsigned)((rows + 3) / 4), 256, 0, c->stream>>>(a, rows);
+void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
+    k_token_attn<HD, PAGED><<<(unsigned)((wgs + XCDS - 1) / XCDS * XCDS * a.RT * a.p.nKv), 256, 0, c->stream>>>(a);
+    k_token_merge<HD><<<(unsigned)(a.p.B * a.p.T * a.p.nHq), 256, 0, c->stream>>>(a, ns1);
 }
 
 }  // namespace
@@ -499,18 +566,25 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     a.R = p.T * a.G;
     a.RT = (a.R + 15) / 16;
     static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
-    // two workgroups a CU, as far as the partials fit; a sequence takes a slot at least
-    const int fit = TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B;
-    int target = (2 * c->cus + p.nKv * a.RT - 1) / (p.nKv * a.RT);
-    if (target > fit) target = fit;
-    a.target = target;
-    // the slots there can be: of B = 1 the host knows the blocks' bound
-    const long most = p.max_keys / BLK + 3;                // blocks of a sequence, at most (three ragged ends)
-    long slots = p.B + (target > 0 ? target : 0);
-    const long alone = p.B * ((most + CMIN - 1) / CMIN);
-    if (slots > alone) slots = alone;
+    // two workgroups a CU; as many as there are sequences, if that is more; as far as the partials' slots (one for each
+    // workgroup and one for each sequence) fit
+    long wgs = ti_max((2L * c->cus + p.nKv * a.RT - 1) / (p.nKv * a.RT), (long)p.B);
+    wgs = ti_max(1L, ti_min(wgs, (long)TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B));
+    a.wgs = (int)wgs;
     const bool paged = p.lens != nullptr;
-#define TOK(HD_) if (hd == HD_) { if (paged) launch<HD_, true>(c, a, (int)slots); else launch<HD_, false>(c, a, (int)slots); }
+    int ns1 = 0;
+    if (!paged) {                                          // one sequence of known length: its blocks, and slots
+        const int last = p.pos0 + p.T - 1;
+        TiSpan s = ti_span(p.pos0, p.window, p.sinks);
+        s.end = last + 1;
+        const long n = ti_max(1, blocks_of(s).n), chunk = run_chunk(n, 1, a.wgs);
+        wgs = (n + chunk - 1) / chunk;
+        ns1 = (int)wgs;
+    } else {
+        const long most = p.max_keys / BLK + 3;            // blocks of a sequence, at most (three ragged ends)
+        wgs = ti_min(wgs, p.B * most);
+    }
+#define TOK(HD_) if (hd == HD_) { if (paged) launch<HD_, true>(c, a, wgs, ns1); else launch<HD_, false>(c, a, wgs, ns1); }
     TOK(128) TOK(96) TOK(64) TOK(32)
 #undef TOK
     TI_LAUNCHED("k_token_attn");

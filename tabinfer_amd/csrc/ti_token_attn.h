@@ -3,7 +3,7 @@
 #include "ti_internal.h"
 #include "ti_span.h"
 
-constexpr int TI_TOKEN_SEQS = 4096;          // sequences of one call, at most
+constexpr int TI_TOKEN_SEQS = 2048;          // sequences of one call, at most: of 64 heads, half of the partials' slots
 
 struct TiTokenAttn {
     const float* qr;                         // [B][T][nHq][hd]

@@ -23,7 +23,7 @@ EVICT = [P, P, P, P, P, P, P, P, 100, 10, 50, 2, 8, 200, 2, 64]
 REFUSED = {
     "ti_attn_window_q8": (ATTN_W, [{i: None} for i in range(6)] + [{5: P}, {1: P + 8}, {3: P + 4}, {6: 0}, {6: -1}, {7: -1}, {6: 2, 7: IMAX - 1}, {8: 0},
                                    {9: 0}, {9: 3}, {8: -4}, {9: -2}, {8: 128, 9: 64}, {10: 0}, {10: 48}, {10: 160}, {10: -32}, {12: -1}, {6: 2 ** 22}]),
-    "ti_attn_paged_q8": (ATTN_P, [{i: None} for i in range(8)] + [{7: P}, {1: P + 8}, {3: P + 4}, {8: 0}, {8: 4097}, {9: 3}, {9: 65, 10: 65}, {10: 0}, {11: 40},
+    "ti_attn_paged_q8": (ATTN_P, [{i: None} for i in range(8)] + [{7: P}, {1: P + 8}, {3: P + 4}, {8: 0}, {8: 2049}, {9: 3}, {9: 65, 10: 65}, {10: 0}, {11: 40},
                                   {12: 0}, {12: 12}, {12: -16}, {13: 0}, {13: -1}, {14: 0}, {14: 2 ** 27 + 1}, {16: -1}]),
     "ti_attn_mass_q8": (MASS, [{i: None} for i in range(7)] + [{5: P}, {1: P + 8}, {7: 0}, {7: 1025}, {8: -1}, {7: 2, 8: IMAX - 1}, {9: 3}, {10: 0}, {11: 31},
                                {11: 256}, {8: 2 ** 23}]),
