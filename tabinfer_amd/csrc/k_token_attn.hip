@@ -17,6 +17,7 @@
 #include "ti_dev.h"
 #include "ti_span.h"
 #include "ti_token_attn.h"
+#include <type_traits>
 
 namespace {
 
@@ -144,16 +145,22 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     return true;
 }
 
-template <int HD>
+// Query rows in a tile's 16 columns. COLS: a row has a column for each of its 32-dim groups (four for three groups), which
+// scales one group's dots and weights, so that a lane splits 8 weights a block instead of 8 for every group, and K goes to the
+// matrix cores as it was loaded. Else a column a row.
+constexpr int tile_slots(int hd, bool cols) { return !cols || hd == 32 ? 1 : hd == 64 ? 2 : 4; }
+constexpr int tile_rows(int hd, bool cols) { return 16 / tile_slots(hd, cols); }
+
+template <int HD, bool COLS>
 struct TokLds {
     static constexpr int NG = HD / 32, KS = HD + 8, VS = HD + 16;      // LDS rows (bytes): operand reads without conflicts
     struct Wave {
-        uint8_t k[BLK * KS];
+        uint8_t k[COLS ? 16 : BLK * KS];
         uint8_t v[BLK * VS];
     };
     union {
         Wave w[WAVES];
-        float o[WAVES][16][HD];
+        float o[WAVES][tile_rows(HD, COLS)][HD];
     };
     float ks[WAVES][NG][BLK], vs[WAVES][NG][BLK];
     float m[WAVES][16], l[WAVES][16];
@@ -161,12 +168,27 @@ struct TokLds {
     int b;
 };
 
-template <int HD, bool PAGED>
-__global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_attn(TokArgs a) {
+// v of the 16 / SLOTS columns of one row, added up in each of them
+template <int SLOTS>
+__device__ __forceinline__ float slot_sum(float v) {
+    auto ror = [](float x, auto c) {
+        const int i = __builtin_bit_cast(int, x);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, decltype(c)::value, 0xF, 0xF, true));
+    };
+    if constexpr (SLOTS >= 2) v += ror(v, std::integral_constant<int, 0x128>{});   // row_ror:8
+    if constexpr (SLOTS == 4) v += ror(v, std::integral_constant<int, 0x124>{});   // row_ror:4
+    return v;
+}
+
+template <int HD, bool PAGED, bool COLS>
+__global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) {
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
-    constexpr int KS = TokLds<HD>::KS, VS = TokLds<HD>::VS;
+    constexpr int KS = TokLds<HD, COLS>::KS, VS = TokLds<HD, COLS>::VS;
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
-    __shared__ __align__(16) TokLds<HD> L;
+    constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
+    constexpr int KU = HD > 64 ? 2 : 1, NK = COLS ? 2 * KU : NL;       // K loads: pieces j + 4 u of a lane's key, 16 keys each
+    constexpr int NQ = COLS ? 2 * KU : NG;                             // Q operands
+    __shared__ __align__(16) TokLds<HD, COLS> L;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the KV heads of a run on one XCD (workgroups go to the eight in turn), near each other in time: their scales, 4 NG bytes
@@ -177,19 +199,22 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
     if (!find_run<PAGED>(a, w, run, L.s4, &L.at, &L.b)) return;        // workgroup-uniform
     const int r16 = lane & 15, j = lane >> 4;
 
-    const int rg = ti_min(rt * 16 + r16, a.R - 1), t = rg / a.G, h = rg % a.G;   // this lane's row
+    const int slot = r16 / ROWS, grp = ti_min(slot, NG - 1), tr = r16 % ROWS;   // this lane's column: row of the tile, group
+    const int rg = ti_min(rt * ROWS + tr, a.R - 1), t = rg / a.G, h = rg % a.G;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
     const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
     // a lane's loads of a block: row and byte in it
-    int pl[NL], sl[SL];
-    uint32_t po[NL], so[SL];
+    int sl[SL];
+    uint32_t po[NL], ko[NK], so[SL];
+    auto v_key = [&](int p) { return (lane + 64 * p) / PC; };
+    auto v_byte = [&](int p) { return 16 * ((lane + 64 * p) % PC); };
+    auto k_key = [&](int p) { return COLS ? 16 * (p / KU) + r16 : v_key(p); };
+    auto k_byte = [&](int p) { return COLS ? 16 * ti_min(j + 4 * (p % KU), PC - 1) : v_byte(p); };
 #pragma unroll
-    for (int p = 0; p < NL; p++) {
-        const int pc = lane + 64 * p;
-        pl[p] = pc / PC;
-        po[p] = (uint32_t)(pl[p] * a.p.nKv) * HD + 16 * (pc % PC);
-    }
+    for (int p = 0; p < NL; p++) po[p] = (uint32_t)(v_key(p) * a.p.nKv) * HD + v_byte(p);
+#pragma unroll
+    for (int p = 0; p < NK; p++) ko[p] = (uint32_t)(k_key(p) * a.p.nKv) * HD + k_byte(p);
 #pragma unroll
     for (int p = 0; p < SL; p++) {
         const int e = ti_min(lane + 64 * p, BLK * NG - 1);
@@ -210,17 +235,18 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
     // what every row of the tile sees: [full_low, full_end)
     const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
     // the query's loads before the keys': they come back first
-    v4f_u qv[NG][2];
+    v4f_u qv[NQ][2];
+    auto q_dim = [&](int x) { return COLS ? 16 * ti_min(j + 4 * (x / 2), PC - 1) + 8 * (x % 2) : 32 * x + 8 * j; };
     {
-        const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD + 8 * j;
+        const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD;
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+        for (int x = 0; x < NQ; x++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
+            for (int u = 0; u < 2; u++) qv[x][u] = *reinterpret_cast<const v4f_u*>(q + q_dim(x) + 4 * u);
     }
 
     // ---- a block's loads
-    uint4 kr[NL], vr[NL];
+    uint4 kr[NK], vr[NL];
     float ksr[SL], vsr[SL];
     // the page of key k0 + lane % 32, where some row sees it; -1 where none does or there is none
     auto fetch_page = [&](int i) -> int {
@@ -234,24 +260,41 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
     };
     // rows of one page, or of the contiguous cache, follow each other: one base and the lanes' fixed offsets
     const bool runs = !PAGED || a.p.pg.shift >= 5;
-    auto load = [&](int i, int page) {
+    // the first row of block i
+    auto base_row = [&](int i, int page) -> size_t {
         const int k0 = bl.at(i) * BLK;
-        if (runs && (PAGED || k0 + BLK <= span.end)) {
-            size_t row = (size_t)k0;
-            if constexpr (PAGED) {
-                // the id of any of the block's keys that is seen (the others carry -1); page 0 where there is none
-                const uint64_t some = __ballot(page >= 0);
-                const int id = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
-                row = ((size_t)(uint32_t)id << a.p.pg.shift) + (k0 & ((1 << a.p.pg.shift) - 1));
-            }
-            const size_t base = (row * a.p.nKv + hk) * HD, sbase = (row * a.p.nKv + hk) * NG;
-            const uint8_t *kb = a.p.kq + base, *vb = a.p.vq + base;
-            const float *ksb = a.p.ks + sbase, *vsb = a.p.vs + sbase;
+        if constexpr (!PAGED) return (size_t)k0;
+        // the id of any of the block's keys that is seen (the others carry -1); page 0 where there is none
+        const uint64_t some = __ballot(page >= 0);
+        const int id = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
+        return ((size_t)(uint32_t)id << a.p.pg.shift) + (k0 & ((1 << a.p.pg.shift) - 1));
+    };
+    auto in_run = [&](int i) { return runs && (PAGED || bl.at(i) * BLK + BLK <= span.end); };
+    auto row_of = [&](int k0, int kl, int page) -> size_t {            // a row that exists where the key does not
+        if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
+        const int id = ti_max(__shfl(page, kl), 0);
+        return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
+    };
+    auto load_k = [&](int i, int page) {
+        const int k0 = bl.at(i) * BLK;
+        if (in_run(i)) {
+            const uint8_t* kb = a.p.kq + (base_row(i, page) * a.p.nKv + hk) * HD;
 #pragma unroll
-            for (int p = 0; p < NL; p++) {
-                kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + po[p]));
-                vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
-            }
+            for (int p = 0; p < NK; p++) kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + ko[p]));
+            return;
+        }
+#pragma unroll
+        for (int p = 0; p < NK; p++)
+            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + (row_of(k0, k_key(p), page) * a.p.nKv + hk) * HD + k_byte(p)));
+    };
+    auto load_v = [&](int i, int page) {                               // and both scales
+        const int k0 = bl.at(i) * BLK;
+        if (in_run(i)) {
+            const size_t row = base_row(i, page) * a.p.nKv + hk;
+            const uint8_t* vb = a.p.vq + row * HD;
+            const float *ksb = a.p.ks + row * NG, *vsb = a.p.vs + row * NG;
+#pragma unroll
+            for (int p = 0; p < NL; p++) vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
 #pragma unroll
             for (int p = 0; p < SL; p++) {
                 ksr[p] = ksb[so[p]];
@@ -259,34 +302,26 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
             }
             return;
         }
-        auto row_of = [&](int kl) -> size_t {                          // a row that exists where the key does not
-            if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
-            const int id = ti_max(__shfl(page, kl), 0);
-            return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
-        };
 #pragma unroll
-        for (int p = 0; p < NL; p++) {
-            const size_t off = (row_of(pl[p]) * a.p.nKv + hk) * HD + 16 * ((lane + 64 * p) % PC);
-            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + off));
-            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + off));
-        }
+        for (int p = 0; p < NL; p++)
+            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + (row_of(k0, v_key(p), page) * a.p.nKv + hk) * HD + v_byte(p)));
 #pragma unroll
         for (int p = 0; p < SL; p++) {
-            const size_t off = (row_of(sl[p]) * a.p.nKv + hk) * NG + ti_min(lane + 64 * p, BLK * NG - 1) % NG;
+            const size_t off = (row_of(k0, sl[p], page) * a.p.nKv + hk) * NG + ti_min(lane + 64 * p, BLK * NG - 1) % NG;
             ksr[p] = a.p.ks[off];
             vsr[p] = a.p.vs[off];
         }
     };
     auto stage = [&]() {
-        uint8_t* kt = L.w[wave].k;
         uint8_t* vt = L.w[wave].v;
 #pragma unroll
         for (int p = 0; p < NL; p++) {
-            const int pc = lane + 64 * p, kl = pc / PC, c = pc % PC;
-            uint2* kd = reinterpret_cast<uint2*>(kt + kl * KS + 16 * c);
-            kd[0] = make_uint2(kr[p].x, kr[p].y);
-            kd[1] = make_uint2(kr[p].z, kr[p].w);
-            *reinterpret_cast<uint4*>(vt + kl * VS + 16 * c) = vr[p];
+            if constexpr (!COLS) {
+                uint2* kd = reinterpret_cast<uint2*>(L.w[wave].k + k_key(p) * KS + k_byte(p));
+                kd[0] = make_uint2(kr[p].x, kr[p].y);
+                kd[1] = make_uint2(kr[p].z, kr[p].w);
+            }
+            *reinterpret_cast<uint4*>(vt + v_key(p) * VS + v_byte(p)) = vr[p];
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
@@ -299,18 +334,22 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
     int i = c0 + wave;
     int page = i < c1 ? fetch_page(i) : -1, page1 = -1;
     if (i + WAVES < c1) page1 = fetch_page(i + WAVES);
-    if (i < c1) load(i, page);
+    if (i < c1) {
+        load_k(i, page);
+        load_v(i, page);
+    }
     TI_ISSUE_FENCE();
 
-    // ---- Q operand: row r16, dims 32 g + 8 j.., scaled by 2^k so that the row's largest element is below 16
-    ti_h8 qh[NG], ql[NG];
+    // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: its K bytes' dims, those of other groups than the column's as
+    // zeros), scaled by 2^k so that the row's largest element is below 16
+    ti_h8 qh[NQ], ql[NQ];
     float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
     {
         float mx = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+        for (int x = 0; x < NQ; x++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[g][e / 4][e % 4]));
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[x][e / 4][e % 4]));
         mx = fmaxf(mx, ti_xor(mx, 16));
         mx = fmaxf(mx, ti_xor(mx, 32));
         int ex = 4;
@@ -319,14 +358,17 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
         const float up = ldexpf(1.0f, k);
         fr = fr * ldexpf(1.0f, -k);
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+        for (int x = 0; x < NQ; x++) {
+            const int c = j + 4 * (x / 2);
+            const bool mine = !COLS || (c < PC && (c >> 1) == slot);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = qv[g][e / 4][e % 4] * up;
+                const float v = mine ? qv[x][e / 4][e % 4] * up : 0.0f;
                 const _Float16 hi = (_Float16)v;
-                qh[g][e] = hi;
-                ql[g][e] = (_Float16)(v - (float)hi);
+                qh[x][e] = hi;
+                ql[x][e] = (_Float16)(v - (float)hi);
             }
+        }
     }
 
     v4f o[HD / 16];
@@ -341,30 +383,48 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
         const int k0 = bl.at(i) * BLK;
         const uint32_t there = (uint32_t)__ballot(page >= 0);
         page = page1;
-        if (i + WAVES < c1) load(i + WAVES, page);
+        if (i + WAVES < c1) {
+            if constexpr (!COLS) load_k(i + WAVES, page);
+            load_v(i + WAVES, page);
+        }
         if (i + 2 * WAVES < c1) page1 = fetch_page(i + 2 * WAVES);
 
         float s[8];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             v4f acc = zero;
+            if constexpr (COLS) {
+#pragma unroll
+                for (int x = 0; x < NQ; x++) {
+                    const uint4 kw = kr[KU * b + x / 2];
+                    const ti_h8 kf = x % 2 ? ti_i8x8_h8(kw.z, kw.w) : ti_i8x8_h8(kw.x, kw.y);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], acc, 0, 0, 0);
+                }
+                const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[wave][grp][16 * b + 4 * j]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] = slot_sum<SLOTS>(acc[e] * sc[e]);
+            } else
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 const uint2 kw = *reinterpret_cast<const uint2*>(L.w[wave].k + (16 * b + r16) * KS + 32 * g + 8 * j);
-                const ti_h8 kk = ti_i8x8_h8(kw.x, kw.y);
+                const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
                 const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[wave][g][16 * b + 4 * j]);
-                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[g], zero, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[g], d, 0, 0, 0);
+                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e] * fr;
         }
+        if constexpr (COLS)
+            if (i + WAVES < c1) load_k(i + WAVES, page);
         // which of the lane's keys its row sees
         uint32_t seen = 0xffu;
         const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
         if (!whole) {                                      // wave-uniform
+            asm volatile("");                              // a branch: not computed where every key is seen
             seen = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -373,7 +433,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
                 seen |= ok ? 1u << e : 0u;
             }
         }
-        if (a.p.scores && rt * 16 + r16 < a.R) {
+        if (a.p.scores && slot == 0 && rt * ROWS + tr < a.R) {
             float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
             *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]};
             *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]};
@@ -408,24 +468,26 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
             sum += p;
         }
         l += sum;
+        ti_b8 pb[3];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[wave][g][4 * j]);
-            const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[wave][g][16 + 4 * j]);
-            float x[8];
+            if (!COLS || g == 0) {
+                const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[wave][COLS ? grp : g][4 * j]);
+                const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[wave][COLS ? grp : g][16 + 4 * j]);
+                float x[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[e] = s[e] * v0[e];
-                x[4 + e] = s[4 + e] * v1[e];
+                for (int e = 0; e < 4; e++) {
+                    x[e] = s[e] * v0[e];
+                    x[4 + e] = s[4 + e] * v1[e];
+                }
+                if (!whole) {                              // the scale of a key that the row does not see may be NaN
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
+                }
+                ti_bf16x3(x, pb);
             }
-            if (!whole) {                                  // the scale of a key that the row does not see may be NaN
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
-            }
-            ti_b8 pb[3];
-            ti_bf16x3(x, pb);
-#pragma unroll
-            for (int d = 2 * g; d < 2 * g + 2; d++) {
+            for (int d = 2 * g; d < 2 * g + 2; d++) {      // COLS: of these 16 dims, the columns of group g hold the output
                 const v2i vb = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (__attribute__((address_space(3))) v2i*)(L.w[wave].v + vrow * VS + 8 * (r16 & 1) + 16 * d));
                 const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
@@ -440,15 +502,16 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : HD == 64 ? 3 : 4) void k_token_a
     l += ti_xor(l, 16);
     l += ti_xor(l, 32);
     __syncthreads();                                       // the tiles are read
-    if (j == 0) {
-        L.m[wave][r16] = m;
-        L.l[wave][r16] = l;
+    if (j == 0 && slot == 0) {
+        L.m[wave][tr] = m;
+        L.l[wave][tr] = l;
     }
 #pragma unroll
-    for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f*>(&L.o[wave][r16][16 * d + 4 * j]) = o[d];
+    for (int d = 0; d < HD / 16; d++)
+        if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
     __syncthreads();
-    const int nr = ti_min(16, a.R - rt * 16);
-    const size_t base = ((size_t)(w + run.b) * a.p.nKv + hk) * a.R + rt * 16;
+    const int nr = ti_min(ROWS, a.R - rt * ROWS);
+    const size_t base = ((size_t)(w + run.b) * a.p.nKv + hk) * a.R + rt * ROWS;
     for (int e = tid; e < nr * (HD / 4); e += 256) {
         const int r = e / (HD / 4), d = e % (HD / 4);
         float M = L.m[0][r];
@@ -550,7 +613,9 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
 
 template <int HD, bool PAGED>
 void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
-    k_token_attn<HD, PAGED><<<(unsigned)((wgs + XCDS - 1) / XCDS * XCDS * a.RT * a.p.nKv), 256, 0, c->stream>>>(a);
+    const unsigned grid = (unsigned)((wgs + XCDS - 1) / XCDS * XCDS * a.RT * a.p.nKv);
+    if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, 256, 0, c->stream>>>(a);
+    else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, 256, 0, c->stream>>>(a);
     k_token_merge<HD><<<(unsigned)(a.p.B * a.p.T * a.p.nHq), 256, 0, c->stream>>>(a, ns1);
 }
 
@@ -564,7 +629,8 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     a.meta = reinterpret_cast<int32_t*>(c->tg_part);
     a.G = p.nHq / p.nKv;
     a.R = p.T * a.G;
-    a.RT = (a.R + 15) / 16;
+    const int rows = tile_rows(hd, true) >= a.R ? tile_rows(hd, true) : 16;
+    a.RT = (a.R + rows - 1) / rows;
     static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
     // two workgroups a CU; as many as there are sequences, if that is more; as far as the partials' slots (one for each
     // workgroup and one for each sequence) fit
