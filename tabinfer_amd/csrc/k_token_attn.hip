@@ -26,9 +26,7 @@ typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));   // the ca
 typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int BLK = 32;                      // keys of a wave's block
-constexpr int WAVES = 4;
-constexpr int XCDS = 8;
-constexpr int CMIN = WAVES;                  // blocks of a workgroup, at least
+constexpr int WAVES = 8, THREADS = 64 * WAVES;
 constexpr float FLOOR = -3.402823466e38f;
 constexpr float VSCALE = 0x1p-24f;           // of every V scale: 127 x a V scale x thousands of keys stays in f32's range
 
@@ -37,7 +35,8 @@ struct TokArgs {
     float* po;                               // [slot][nKv][T G][HD] partials, (m, l) of each
     float* pml;
     int32_t* meta;                           // [B][2]: a sequence's first slot and their number
-    int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups a KV head, at most
+    int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups of HW KV heads, at most
+    int HW, BW;                              // a workgroup's waves: HW KV heads x BW blocks
 };
 
 // Blocks that hold the keys [0, first) and [low, end): [0, sb) and [wb, sb + ... )
@@ -102,16 +101,16 @@ struct Run {
     long start;
     int b, block;
 };
-// blocks of a run: all workgroups', but CMIN (each wave a block) where the sequences have as many
-__host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs) {
-    return ti_max((total + wgs - 1) / wgs, ti_min((long)CMIN, (total + B - 1) / B));
+// blocks of a run: an equal share, but a block for each of the BW waves of a head where the sequences have as many
+__host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs, int BW) {
+    return ti_max((total + wgs - 1) / wgs, ti_min((long)BW, (total + B - 1) / B));
 }
 template <bool PAGED>
 __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, int* s_b) {
     const int B = a.p.B, tid = threadIdx.x;
     if (B == 1) {
         const long n = seq_blocks<PAGED>(a, 0);
-        r.chunk = run_chunk(n, 1, a.wgs);
+        r.chunk = run_chunk(n, 1, a.wgs, a.BW);
         r.b = 0;
         r.start = 0;
         r.block = (int)ti_min(w * r.chunk, n);
@@ -119,11 +118,11 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
         return r.left > 0;
     }
     // a thread: the sequences [tid per, tid per + per)
-    const int per = (B + 255) / 256, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
+    const int per = (B + THREADS - 1) / THREADS, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
     for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
     long at = wg_scan(mine, s4, total);
-    r.chunk = run_chunk(total, B, a.wgs);
+    r.chunk = run_chunk(total, B, a.wgs, a.BW);
     const long g0 = w * r.chunk;
     if (g0 >= at && g0 < at + mine) {
         for (int b = b0; b < b1; b++) {
@@ -146,16 +145,16 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
 }
 
 // Query rows in a tile's 16 columns. COLS: a row has a column for each of its 32-dim groups (four for three groups), which
-// scales one group's dots and weights, so that a lane splits 8 weights a block instead of 8 for every group, and K goes to the
-// matrix cores as it was loaded. Else a column a row.
+// scales one group's dots and weights, so that a lane splits 8 weights a block instead of 8 for every group. Else a column a
+// row.
 constexpr int tile_slots(int hd, bool cols) { return !cols || hd == 32 ? 1 : hd == 64 ? 2 : 4; }
 constexpr int tile_rows(int hd, bool cols) { return 16 / tile_slots(hd, cols); }
 
 template <int HD, bool COLS>
 struct TokLds {
-    static constexpr int NG = HD / 32, KS = HD + 8, VS = HD + 16;      // LDS rows (bytes): operand reads without conflicts
+    static constexpr int NG = HD / 32, KS = COLS ? HD + 16 : HD + 8, VS = HD + 16;   // LDS rows (bytes): operand reads without conflicts
     struct Wave {
-        uint8_t k[COLS ? 16 : BLK * KS];
+        uint8_t k[BLK * KS];
         uint8_t v[BLK * VS];
     };
     union {
@@ -181,20 +180,18 @@ __device__ __forceinline__ float slot_sum(float v) {
 }
 
 template <int HD, bool PAGED, bool COLS>
-__global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) {
+__global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
     constexpr int KS = TokLds<HD, COLS>::KS, VS = TokLds<HD, COLS>::VS;
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
-    constexpr int KU = HD > 64 ? 2 : 1, NK = COLS ? 2 * KU : NL;       // K loads: pieces j + 4 u of a lane's key, 16 keys each
-    constexpr int NQ = COLS ? 2 * KU : NG;                             // Q operands
+    constexpr int NQ = COLS ? HD > 64 ? 4 : 2 : NG;                    // Q operands
     __shared__ __align__(16) TokLds<HD, COLS> L;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the KV heads of a run on one XCD (workgroups go to the eight in turn), near each other in time: their scales, 4 NG bytes
-    // a head and position, share cache lines, and so do the codes of narrow heads
-    const int heads = a.p.nKv * a.RT, hr = (blockIdx.x / XCDS) % heads, w = blockIdx.x / (XCDS * heads) * XCDS + blockIdx.x % XCDS;
-    const int hk = hr % a.p.nKv, rt = hr / a.p.nKv;
+    // the waves of a workgroup read HW heads of the same positions together: rows of a position lie side by side
+    const int groups = a.p.nKv / a.HW, hr = blockIdx.x % (groups * a.RT), w = blockIdx.x / (groups * a.RT);
+    const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs, rt = hr / groups;
     Run run;
     if (!find_run<PAGED>(a, w, run, L.s4, &L.at, &L.b)) return;        // workgroup-uniform
     const int r16 = lane & 15, j = lane >> 4;
@@ -206,15 +203,11 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
     const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
     // a lane's loads of a block: row and byte in it
     int sl[SL];
-    uint32_t po[NL], ko[NK], so[SL];
-    auto v_key = [&](int p) { return (lane + 64 * p) / PC; };
-    auto v_byte = [&](int p) { return 16 * ((lane + 64 * p) % PC); };
-    auto k_key = [&](int p) { return COLS ? 16 * (p / KU) + r16 : v_key(p); };
-    auto k_byte = [&](int p) { return COLS ? 16 * ti_min(j + 4 * (p % KU), PC - 1) : v_byte(p); };
+    uint32_t po[NL], so[SL];
+    auto l_key = [&](int p) { return (lane + 64 * p) / PC; };
+    auto l_byte = [&](int p) { return 16 * ((lane + 64 * p) % PC); };
 #pragma unroll
-    for (int p = 0; p < NL; p++) po[p] = (uint32_t)(v_key(p) * a.p.nKv) * HD + v_byte(p);
-#pragma unroll
-    for (int p = 0; p < NK; p++) ko[p] = (uint32_t)(k_key(p) * a.p.nKv) * HD + k_byte(p);
+    for (int p = 0; p < NL; p++) po[p] = (uint32_t)(l_key(p) * a.p.nKv) * HD + l_byte(p);
 #pragma unroll
     for (int p = 0; p < SL; p++) {
         const int e = ti_min(lane + 64 * p, BLK * NG - 1);
@@ -246,7 +239,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
     }
 
     // ---- a block's loads
-    uint4 kr[NK], vr[NL];
+    uint4 kr[NL], vr[NL];
     float ksr[SL], vsr[SL];
     // the page of key k0 + lane % 32, where some row sees it; -1 where none does or there is none
     auto fetch_page = [&](int i) -> int {
@@ -275,26 +268,17 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
         const int id = ti_max(__shfl(page, kl), 0);
         return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
     };
-    auto load_k = [&](int i, int page) {
-        const int k0 = bl.at(i) * BLK;
-        if (in_run(i)) {
-            const uint8_t* kb = a.p.kq + (base_row(i, page) * a.p.nKv + hk) * HD;
-#pragma unroll
-            for (int p = 0; p < NK; p++) kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + ko[p]));
-            return;
-        }
-#pragma unroll
-        for (int p = 0; p < NK; p++)
-            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + (row_of(k0, k_key(p), page) * a.p.nKv + hk) * HD + k_byte(p)));
-    };
-    auto load_v = [&](int i, int page) {                               // and both scales
+    auto load = [&](int i, int page) {
         const int k0 = bl.at(i) * BLK;
         if (in_run(i)) {
             const size_t row = base_row(i, page) * a.p.nKv + hk;
-            const uint8_t* vb = a.p.vq + row * HD;
+            const uint8_t *kb = a.p.kq + row * HD, *vb = a.p.vq + row * HD;
             const float *ksb = a.p.ks + row * NG, *vsb = a.p.vs + row * NG;
 #pragma unroll
-            for (int p = 0; p < NL; p++) vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
+            for (int p = 0; p < NL; p++) {
+                kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + po[p]));
+                vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
+            }
 #pragma unroll
             for (int p = 0; p < SL; p++) {
                 ksr[p] = ksb[so[p]];
@@ -303,8 +287,11 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
             return;
         }
 #pragma unroll
-        for (int p = 0; p < NL; p++)
-            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + (row_of(k0, v_key(p), page) * a.p.nKv + hk) * HD + v_byte(p)));
+        for (int p = 0; p < NL; p++) {
+            const size_t off = (row_of(k0, l_key(p), page) * a.p.nKv + hk) * HD + l_byte(p);
+            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + off));
+            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + off));
+        }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
             const size_t off = (row_of(k0, sl[p], page) * a.p.nKv + hk) * NG + ti_min(lane + 64 * p, BLK * NG - 1) % NG;
@@ -316,12 +303,14 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
         uint8_t* vt = L.w[wave].v;
 #pragma unroll
         for (int p = 0; p < NL; p++) {
-            if constexpr (!COLS) {
-                uint2* kd = reinterpret_cast<uint2*>(L.w[wave].k + k_key(p) * KS + k_byte(p));
-                kd[0] = make_uint2(kr[p].x, kr[p].y);
-                kd[1] = make_uint2(kr[p].z, kr[p].w);
+            uint8_t* kd = L.w[wave].k + l_key(p) * KS + l_byte(p);
+            if constexpr (COLS) {
+                *reinterpret_cast<uint4*>(kd) = kr[p];
+            } else {                                       // 8-byte rows
+                reinterpret_cast<uint2*>(kd)[0] = make_uint2(kr[p].x, kr[p].y);
+                reinterpret_cast<uint2*>(kd)[1] = make_uint2(kr[p].z, kr[p].w);
             }
-            *reinterpret_cast<uint4*>(vt + v_key(p) * VS + v_byte(p)) = vr[p];
+            *reinterpret_cast<uint4*>(vt + l_key(p) * VS + l_byte(p)) = vr[p];
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
@@ -331,17 +320,14 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
         }
     };
 
-    int i = c0 + wave;
+    int i = c0 + bw;
     int page = i < c1 ? fetch_page(i) : -1, page1 = -1;
-    if (i + WAVES < c1) page1 = fetch_page(i + WAVES);
-    if (i < c1) {
-        load_k(i, page);
-        load_v(i, page);
-    }
+    if (i + a.BW < c1) page1 = fetch_page(i + a.BW);
+    if (i < c1) load(i, page);
     TI_ISSUE_FENCE();
 
-    // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: its K bytes' dims, those of other groups than the column's as
-    // zeros), scaled by 2^k so that the row's largest element is below 16
+    // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: dims 16 j.. of 64, those of other groups than the column's
+    // as zeros), scaled by 2^k so that the row's largest element is below 16
     ti_h8 qh[NQ], ql[NQ];
     float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
     {
@@ -376,18 +362,15 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
     for (int d = 0; d < HD / 16; d++) o[d] = zero;
     float m = -INFINITY, l = 0.0f;
 
-    for (; i < c1; i += WAVES) {
+    for (; i < c1; i += a.BW) {
         ti_wave_lds_fence();                               // the last block is read
         stage();
         ti_wave_lds_fence();
         const int k0 = bl.at(i) * BLK;
         const uint32_t there = (uint32_t)__ballot(page >= 0);
         page = page1;
-        if (i + WAVES < c1) {
-            if constexpr (!COLS) load_k(i + WAVES, page);
-            load_v(i + WAVES, page);
-        }
-        if (i + 2 * WAVES < c1) page1 = fetch_page(i + 2 * WAVES);
+        if (i + a.BW < c1) load(i + a.BW, page);
+        if (i + 2 * a.BW < c1) page1 = fetch_page(i + 2 * a.BW);
 
         float s[8];
 #pragma unroll
@@ -396,8 +379,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
             if constexpr (COLS) {
 #pragma unroll
                 for (int x = 0; x < NQ; x++) {
-                    const uint4 kw = kr[KU * b + x / 2];
-                    const ti_h8 kf = x % 2 ? ti_i8x8_h8(kw.z, kw.w) : ti_i8x8_h8(kw.x, kw.y);
+                    const uint2 kw = *reinterpret_cast<const uint2*>(L.w[wave].k + (16 * b + r16) * KS + q_dim(x));
+                    const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], acc, 0, 0, 0);
                 }
@@ -418,8 +401,6 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
 #pragma unroll
             for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e] * fr;
         }
-        if constexpr (COLS)
-            if (i + WAVES < c1) load_k(i + WAVES, page);
         // which of the lane's keys its row sees
         uint32_t seen = 0xffu;
         const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
@@ -511,29 +492,27 @@ __global__ __launch_bounds__(256, HD > 64 ? 2 : 3) void k_token_attn(TokArgs a) 
         if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
     __syncthreads();
     const int nr = ti_min(ROWS, a.R - rt * ROWS);
-    const size_t base = ((size_t)(w + run.b) * a.p.nKv + hk) * a.R + rt * ROWS;
-    for (int e = tid; e < nr * (HD / 4); e += 256) {
-        const int r = e / (HD / 4), d = e % (HD / 4);
-        float M = L.m[0][r];
-#pragma unroll
-        for (int k = 1; k < WAVES; k++) M = fmaxf(M, L.m[k][r]);
+    for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
+        const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, r = q % nr;
+        float M = L.m[hh][r];
+        for (int k = hh + a.HW; k < WAVES; k += a.HW) M = fmaxf(M, L.m[k][r]);
         v4f x = zero;
         float y = 0.0f;
-#pragma unroll
-        for (int k = 0; k < WAVES; k++) {
+        for (int k = hh; k < WAVES; k += a.HW) {
             const float mk = L.m[k][r], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
             const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][r][4 * d]);
 #pragma unroll
             for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
             y = fmaf(L.l[k][r], f, y);
         }
-        *reinterpret_cast<v4f*>(a.po + (base + r) * HD + 4 * d) = x;
+        const size_t at = ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
+        *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
         if (d == 0) {
-            a.pml[2 * (base + r)] = M;
-            a.pml[2 * (base + r) + 1] = y;
+            a.pml[2 * at] = M;
+            a.pml[2 * at + 1] = y;
         }
     }
-    if (PAGED && c0 == 0 && hk == 0 && rt == 0 && tid == 0) {          // the sequence's slots, for the merge
+    if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
         a.meta[2 * run.b] = w + run.b;
         a.meta[2 * run.b + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
     }
@@ -613,9 +592,9 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
 
 template <int HD, bool PAGED>
 void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
-    const unsigned grid = (unsigned)((wgs + XCDS - 1) / XCDS * XCDS * a.RT * a.p.nKv);
-    if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, 256, 0, c->stream>>>(a);
-    else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, 256, 0, c->stream>>>(a);
+    const unsigned grid = (unsigned)(wgs * a.RT * (a.p.nKv / a.HW));
+    if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, THREADS, 0, c->stream>>>(a);
+    else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, THREADS, 0, c->stream>>>(a);
     k_token_merge<HD><<<(unsigned)(a.p.B * a.p.T * a.p.nHq), 256, 0, c->stream>>>(a, ns1);
 }
 
@@ -632,9 +611,12 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     const int rows = tile_rows(hd, true) >= a.R ? tile_rows(hd, true) : 16;
     a.RT = (a.R + rows - 1) / rows;
     static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
-    // two workgroups a CU; as many as there are sequences, if that is more; as far as the partials' slots (one for each
+    a.HW = p.nKv % 8 == 0 ? 8 : p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
+    a.BW = WAVES / a.HW;
+    // a workgroup a CU; as many as there are sequences, if that is more; as far as the partials' slots (one for each
     // workgroup and one for each sequence) fit
-    long wgs = ti_max((2L * c->cus + p.nKv * a.RT - 1) / (p.nKv * a.RT), (long)p.B);
+    const int groups = p.nKv / a.HW * a.RT;
+    long wgs = ti_max(((long)c->cus + groups - 1) / groups, (long)p.B);
     wgs = ti_max(1L, ti_min(wgs, (long)TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B));
     a.wgs = (int)wgs;
     const bool paged = p.lens != nullptr;
@@ -643,7 +625,7 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
         const int last = p.pos0 + p.T - 1;
         TiSpan s = ti_span(p.pos0, p.window, p.sinks);
         s.end = last + 1;
-        const long n = ti_max(1, blocks_of(s).n), chunk = run_chunk(n, 1, a.wgs);
+        const long n = ti_max(1, blocks_of(s).n), chunk = run_chunk(n, 1, a.wgs, a.BW);
         wgs = (n + chunk - 1) / chunk;
         ns1 = (int)wgs;
     } else {
