@@ -7,7 +7,7 @@
 //    KV head: each has the same work whatever the lengths, a run that ends one sequence begins the next, and its part of
 //    a sequence is a partial in slot (workgroup + sequence). Every workgroup finds its run by a scan over the lengths;
 //    nothing depends on them on the host.
-//  - A wave takes a block at a time, on its own: loads of the next block in flight, the codes through LDS of its own.
+//  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 16 waves a CU cover each other's loads.
 //    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-25 of
 //    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
@@ -26,9 +26,9 @@ typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));   // the ca
 typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int BLK = 32;                      // keys of a wave's block
-constexpr int WAVES = 8, THREADS = 64 * WAVES;
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr float FLOOR = -3.402823466e38f;
-constexpr float VSCALE = 0x1p-24f;           // of every V scale: 127 x a V scale x thousands of keys stays in f32's range
+constexpr float PSCALE = 0x1p-24f;           // of every weight in P V: 127 x a V scale x thousands of keys stays in f32's range
 
 struct TokArgs {
     TiTokenAttn p;
@@ -95,6 +95,12 @@ __device__ __forceinline__ long wg_scan(long v, long* s4, long& total) {
     return before + x - v;
 }
 
+// a value that all lanes hold, in scalar registers
+__device__ __forceinline__ long uniform(long v) {
+    const int lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (long)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
 // The run of blocks of a workgroup, in sequence b from its block `block` (at block `start` of all) on
 struct Run {
     long chunk, left;                        // blocks of every workgroup's run; of this one, still to do
@@ -122,6 +128,7 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     long mine = 0, total;
     for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
     long at = wg_scan(mine, s4, total);
+    total = uniform(total);
     r.chunk = run_chunk(total, B, a.wgs, a.BW);
     const long g0 = w * r.chunk;
     if (g0 >= at && g0 < at + mine) {
@@ -139,7 +146,7 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     if (g0 >= total) return false;
     r.left = ti_min(r.chunk, total - g0);
     r.b = __builtin_amdgcn_readfirstlane(*s_b);
-    r.start = *s_at;
+    r.start = uniform(*s_at);
     r.block = (int)(g0 - r.start);
     return true;
 }
@@ -152,20 +159,42 @@ constexpr int tile_rows(int hd, bool cols) { return 16 / tile_slots(hd, cols); }
 
 template <int HD, bool COLS>
 struct TokLds {
-    static constexpr int NG = HD / 32, KS = COLS ? HD + 16 : HD + 8, VS = HD + 16;   // LDS rows (bytes): operand reads without conflicts
+    static constexpr int NG = HD / 32;
+    // a block as its loads write it: rows of HD bytes one behind the other, their 16-byte pieces permuted (piece_slot)
     struct Wave {
-        uint8_t k[BLK * KS];
-        uint8_t v[BLK * VS];
+        uint8_t k[BLK * HD], v[BLK * HD];
+        float ks[(NG * BLK + 63) / 64 * 64], vs[(NG * BLK + 63) / 64 * 64];       // [group][key]
     };
     union {
         Wave w[WAVES];
         float o[WAVES][tile_rows(HD, COLS)][HD];
     };
-    float ks[WAVES][NG][BLK], vs[WAVES][NG][BLK];
     float m[WAVES][16], l[WAVES][16];
     long s4[WAVES], at;
     int b;
 };
+
+// Where piece c of a key's row lies: both operand reads, 16 keys' piece and 8 keys' 16 bytes, without bank conflicts (rows of
+// 32 and 96 bytes are so as they are)
+template <int HD>
+__device__ __forceinline__ int piece_slot(int key, int c) {
+    return HD == 128 ? c ^ ((key >> 1) & 7) : HD == 64 ? c ^ ((key >> 2) & 3) : c;
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* glb_ptr;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
+}
+// a lane's 16 bytes (streamed) or 4 (scales: neighbouring heads share their cache lines) to LDS, lane after lane
+__device__ __forceinline__ void run_to_lds16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t lane_off, int off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, lane_off, off, 0, 2);
+}
+__device__ __forceinline__ void run_to_lds4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t lane_off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 4, lane_off, 0, 0, 0);
+}
+__device__ __forceinline__ void to_lds16(const void* p, void* lds) { __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)lds, 16, 0, 2); }
+__device__ __forceinline__ void to_lds4(const void* p, void* lds) { __builtin_amdgcn_global_load_lds((glb_ptr)p, (lds_ptr)lds, 4, 0, 0); }
 
 // v of the 16 / SLOTS columns of one row, added up in each of them
 template <int SLOTS>
@@ -180,12 +209,11 @@ __device__ __forceinline__ float slot_sum(float v) {
 }
 
 template <int HD, bool PAGED, bool COLS>
-__global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
+__global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a) {
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
-    constexpr int KS = TokLds<HD, COLS>::KS, VS = TokLds<HD, COLS>::VS;
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
-    constexpr int NQ = COLS ? HD > 64 ? 4 : 2 : NG;                    // Q operands
+    constexpr int NQ = COLS ? 2 : NG, NU = HD > 64 ? 2 : 1;            // Q operands; COLS: of NU x 64 dims, a column's own
     __shared__ __align__(16) TokLds<HD, COLS> L;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -202,18 +230,17 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
     // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
     const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
     // a lane's loads of a block: row and byte in it
-    int sl[SL];
-    uint32_t po[NL], so[SL];
+    // (of 64 and 128 dims the loads p and p + PF are a fixed distance apart)
+    constexpr int PF = HD == 96 ? NL : HD == 128 ? 2 : 1;
+    uint32_t po[PF];
     auto l_key = [&](int p) { return (lane + 64 * p) / PC; };
-    auto l_byte = [&](int p) { return 16 * ((lane + 64 * p) % PC); };
+    auto l_byte = [&](int p) { return 16 * piece_slot<HD>(l_key(p), (lane + 64 * p) % PC); };
+    auto s_key = [&](int p) { return lane % BLK; };
+    auto s_grp = [&](int p) { return ti_min(2 * p + lane / BLK, NG - 1); };
 #pragma unroll
-    for (int p = 0; p < NL; p++) po[p] = (uint32_t)(l_key(p) * a.p.nKv) * HD + l_byte(p);
-#pragma unroll
-    for (int p = 0; p < SL; p++) {
-        const int e = ti_min(lane + 64 * p, BLK * NG - 1);
-        sl[p] = e / NG;
-        so[p] = (uint32_t)(sl[p] * a.p.nKv) * NG + e % NG;
-    }
+    for (int p = 0; p < PF; p++) po[p] = (uint32_t)(l_key(p) * a.p.nKv) * HD + l_byte(p);
+    const uint32_t so = 4 * ((uint32_t)(s_key(0) * a.p.nKv) * NG + s_grp(0));
+    const int far = 64 / PC * PF * a.p.nKv * HD;
 
   for (;;) {
     // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
@@ -229,7 +256,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
     const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
     // the query's loads before the keys': they come back first
     v4f_u qv[NQ][2];
-    auto q_dim = [&](int x) { return COLS ? 16 * ti_min(j + 4 * (x / 2), PC - 1) + 8 * (x % 2) : 32 * x + 8 * j; };
+    const int qc = j + 4 * (slot / 2);                     // COLS: the lane's 16 dims of the 64 that its column's group is in
+    auto q_dim = [&](int x) { return COLS ? 16 * ti_min(qc, PC - 1) + 8 * x : 32 * x + 8 * j; };
     {
         const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD;
 #pragma unroll
@@ -238,18 +266,19 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
             for (int u = 0; u < 2; u++) qv[x][u] = *reinterpret_cast<const v4f_u*>(q + q_dim(x) + 4 * u);
     }
 
-    // ---- a block's loads
-    uint4 kr[NL], vr[NL];
-    float ksr[SL], vsr[SL];
-    // the page of key k0 + lane % 32, where some row sees it; -1 where none does or there is none
+    // ---- a block's loads, straight to the wave's LDS
+    // the table's entry for key k0 + lane % 32 of block i; and, once it is there, the page of that key: -1 where no row sees
+    // the key or there is no such page. Apart, so that nothing waits where the entry is asked for
     auto fetch_page = [&](int i) -> int {
+        if constexpr (!PAGED) return 0;
+        const int k = ti_min((bl.at(i) * BLK + (lane & 31)) >> a.p.pg.shift, a.p.pg.width - 1);
+        return a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
+    };
+    auto check_page = [&](int i, int id) -> int {
         const int key = bl.at(i) * BLK + (lane & 31);
         const bool in = key < span.end && (key >= span.low || key < span.first);
         if constexpr (!PAGED) return in ? 0 : -1;
-        const int k = key >> a.p.pg.shift;
-        if (!in || k >= a.p.pg.width) return -1;
-        const int id = a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
-        return id >= 0 && id < a.p.pg.pages ? id : -1;
+        return in && (key >> a.p.pg.shift) < a.p.pg.width && id >= 0 && id < a.p.pg.pages ? id : -1;
     };
     // rows of one page, or of the contiguous cache, follow each other: one base and the lanes' fixed offsets
     const bool runs = !PAGED || a.p.pg.shift >= 5;
@@ -268,62 +297,49 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
         const int id = ti_max(__shfl(page, kl), 0);
         return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
     };
+    auto& W = L.w[wave];
     auto load = [&](int i, int page) {
         const int k0 = bl.at(i) * BLK;
         if (in_run(i)) {
+            // scalar bases and the lanes' 32-bit offsets
             const size_t row = base_row(i, page) * a.p.nKv + hk;
-            const uint8_t *kb = a.p.kq + row * HD, *vb = a.p.vq + row * HD;
-            const float *ksb = a.p.ks + row * NG, *vsb = a.p.vs + row * NG;
+            const int codes = BLK * a.p.nKv * HD, scales = BLK * a.p.nKv * NG * 4;
+            const __amdgpu_buffer_rsrc_t rk = resource(a.p.kq + row * HD, codes), rv = resource(a.p.vq + row * HD, codes);
+            const __amdgpu_buffer_rsrc_t rks = resource(a.p.ks + row * NG, scales), rvs = resource(a.p.vs + row * NG, scales);
 #pragma unroll
             for (int p = 0; p < NL; p++) {
-                kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(kb + po[p]));
-                vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(vb + po[p]));
+                run_to_lds16(rk, &W.k[1024 * p], po[p % PF], p / PF * far);
+                run_to_lds16(rv, &W.v[1024 * p], po[p % PF], p / PF * far);
             }
 #pragma unroll
             for (int p = 0; p < SL; p++) {
-                ksr[p] = ksb[so[p]];
-                vsr[p] = vsb[so[p]];
+                const uint32_t o = so + 4 * (s_grp(p) - s_grp(0));
+                run_to_lds4(rks, &W.ks[64 * p], o);
+                run_to_lds4(rvs, &W.vs[64 * p], o);
             }
             return;
         }
 #pragma unroll
         for (int p = 0; p < NL; p++) {
             const size_t off = (row_of(k0, l_key(p), page) * a.p.nKv + hk) * HD + l_byte(p);
-            kr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.kq + off));
-            vr[p] = ti_ld_nt(reinterpret_cast<const uint4*>(a.p.vq + off));
+            to_lds16(a.p.kq + off, &W.k[1024 * p]);
+            to_lds16(a.p.vq + off, &W.v[1024 * p]);
         }
 #pragma unroll
         for (int p = 0; p < SL; p++) {
-            const size_t off = (row_of(k0, sl[p], page) * a.p.nKv + hk) * NG + ti_min(lane + 64 * p, BLK * NG - 1) % NG;
-            ksr[p] = a.p.ks[off];
-            vsr[p] = a.p.vs[off];
-        }
-    };
-    auto stage = [&]() {
-        uint8_t* vt = L.w[wave].v;
-#pragma unroll
-        for (int p = 0; p < NL; p++) {
-            uint8_t* kd = L.w[wave].k + l_key(p) * KS + l_byte(p);
-            if constexpr (COLS) {
-                *reinterpret_cast<uint4*>(kd) = kr[p];
-            } else {                                       // 8-byte rows
-                reinterpret_cast<uint2*>(kd)[0] = make_uint2(kr[p].x, kr[p].y);
-                reinterpret_cast<uint2*>(kd)[1] = make_uint2(kr[p].z, kr[p].w);
-            }
-            *reinterpret_cast<uint4*>(vt + l_key(p) * VS + l_byte(p)) = vr[p];
-        }
-#pragma unroll
-        for (int p = 0; p < SL; p++) {
-            const int e = ti_min(lane + 64 * p, BLK * NG - 1), kl = e / NG, g = e % NG;
-            L.ks[wave][g][kl] = ksr[p];
-            L.vs[wave][g][kl] = vsr[p] * VSCALE;
+            const size_t off = (row_of(k0, s_key(p), page) * a.p.nKv + hk) * NG + s_grp(p);
+            to_lds4(a.p.ks + off, &W.ks[64 * p]);
+            to_lds4(a.p.vs + off, &W.vs[64 * p]);
         }
     };
 
     int i = c0 + bw;
-    int page = i < c1 ? fetch_page(i) : -1, page1 = -1;
-    if (i + a.BW < c1) page1 = fetch_page(i + a.BW);
-    if (i < c1) load(i, page);
+    int page = -1, entry = 0;
+    if (i < c1) {
+        page = check_page(i, fetch_page(i));
+        if (i + a.BW < c1) entry = fetch_page(i + a.BW);
+        load(i, page);
+    }
     TI_ISSUE_FENCE();
 
     // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: dims 16 j.. of 64, those of other groups than the column's
@@ -338,6 +354,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[x][e / 4][e % 4]));
         mx = fmaxf(mx, ti_xor(mx, 16));
         mx = fmaxf(mx, ti_xor(mx, 32));
+        if (COLS && NU == 2) mx = fmaxf(mx, ti_xor(mx, 8));            // the row's other 64 dims
         int ex = 4;
         if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
         const int k = ti_min(4 - ex, 100);
@@ -345,8 +362,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
         fr = fr * ldexpf(1.0f, -k);
 #pragma unroll
         for (int x = 0; x < NQ; x++) {
-            const int c = j + 4 * (x / 2);
-            const bool mine = !COLS || (c < PC && (c >> 1) == slot);
+            const bool mine = !COLS || (qc < PC && qc / 2 == slot);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = mine ? qv[x][e / 4][e % 4] * up : 0.0f;
@@ -363,14 +379,10 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
     float m = -INFINITY, l = 0.0f;
 
     for (; i < c1; i += a.BW) {
-        ti_wave_lds_fence();                               // the last block is read
-        stage();
+        __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): the block is there
         ti_wave_lds_fence();
         const int k0 = bl.at(i) * BLK;
         const uint32_t there = (uint32_t)__ballot(page >= 0);
-        page = page1;
-        if (i + a.BW < c1) load(i + a.BW, page);
-        if (i + 2 * a.BW < c1) page1 = fetch_page(i + 2 * a.BW);
 
         float s[8];
 #pragma unroll
@@ -378,21 +390,27 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
             v4f acc = zero;
             if constexpr (COLS) {
 #pragma unroll
-                for (int x = 0; x < NQ; x++) {
-                    const uint2 kw = *reinterpret_cast<const uint2*>(L.w[wave].k + (16 * b + r16) * KS + q_dim(x));
-                    const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], acc, 0, 0, 0);
+                for (int u = 0; u < NU; u++) {
+                    const int key = 16 * b + r16;
+                    const uint4 kw = *reinterpret_cast<const uint4*>(&W.k[key * HD + 16 * piece_slot<HD>(key, ti_min(j + 4 * u, PC - 1))]);
+                    const ti_h8 k0f = ti_i8x8_h8(kw.x, kw.y), k1f = ti_i8x8_h8(kw.z, kw.w);
+                    v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, qh[0], zero, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, ql[0], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, qh[1], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, ql[1], d, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[e] = u == 0 || slot / 2 == u ? d[e] : acc[e];
                 }
-                const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[wave][grp][16 * b + 4 * j]);
+                const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * grp + 16 * b + 4 * j]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[e] = slot_sum<SLOTS>(acc[e] * sc[e]);
             } else
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const uint2 kw = *reinterpret_cast<const uint2*>(L.w[wave].k + (16 * b + r16) * KS + 32 * g + 8 * j);
+                const int key = 16 * b + r16;
+                const uint2 kw = *reinterpret_cast<const uint2*>(&W.k[key * HD + 16 * piece_slot<HD>(key, 2 * g + j / 2) + 8 * (j & 1)]);
                 const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
-                const v4f sc = *reinterpret_cast<const v4f*>(&L.ks[wave][g][16 * b + 4 * j]);
+                const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * g + 16 * b + 4 * j]);
                 v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
 #pragma unroll
@@ -445,16 +463,17 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
         for (int e = 0; e < 8; e++) {
             float p = __builtin_amdgcn_exp2f(s[e] - m);
             if (!whole) p = seen >> e & 1u ? p : 0.0f;
-            s[e] = p;
             sum += p;
+            s[e] = p * PSCALE;
         }
         l += sum;
         ti_b8 pb[3];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
+            if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for four waves a SIMD
             if (!COLS || g == 0) {
-                const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[wave][COLS ? grp : g][4 * j]);
-                const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[wave][COLS ? grp : g][16 + 4 * j]);
+                const v4f v0 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 4 * j]);
+                const v4f v1 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 16 + 4 * j]);
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -470,12 +489,20 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
 #pragma unroll
             for (int d = 2 * g; d < 2 * g + 2; d++) {      // COLS: of these 16 dims, the columns of group g hold the output
                 const v2i vb = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) v2i*)(L.w[wave].v + vrow * VS + 8 * (r16 & 1) + 16 * d));
+                    (__attribute__((address_space(3))) v2i*)&W.v[vrow * HD + 16 * piece_slot<HD>(vrow, d) + 8 * (r16 & 1)]);
                 const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
                 const ti_b8 vv = __builtin_bit_cast(ti_b8, make_uint4(lo.x, lo.y, hi.x, hi.y));
 #pragma unroll
                 for (int e = 2; e >= 0; e--) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[e], o[d], 0, 0, 0);
             }
+        }
+        // the next block into the place of this one, which has been read
+        if (i + a.BW < c1) {
+            ti_wave_lds_fence();
+            __builtin_amdgcn_s_waitcnt(0xC07F);            // lgkmcnt(0)
+            page = check_page(i + a.BW, entry);
+            if (i + 2 * a.BW < c1) entry = fetch_page(i + 2 * a.BW);
+            load(i + a.BW, page);
         }
     }
 
@@ -525,22 +552,22 @@ __global__ __launch_bounds__(THREADS, 2) void k_token_attn(TokArgs a) {
   }
 }
 
-// A workgroup a (sequence, token, head): its slots' partials into the output row, each group of threads those of its own
-// slots with every load in flight at once
-template <int HD>
+// A workgroup a (sequence, token, head) and DW of its dims: the slots' partials into the output row, each group of threads
+// those of its own slots with every load in flight at once. DW = 32 where that is what it takes to fill the CUs
+template <int HD, int DW>
 __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
-    constexpr int D4 = HD / 4, SG = 256 / D4, UN = 8;
+    constexpr int D4 = DW / 4, SG = 256 / D4, UN = 8;
     __shared__ float s_m[SG], s_l[SG];
-    __shared__ __align__(16) float s_o[SG][HD];
+    __shared__ __align__(16) float s_o[SG][4 * D4];
     const int tid = threadIdx.x, sg = tid / D4, d = tid % D4;
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, d0 = DW * blockIdx.y;
     const int hq = row % a.p.nHq, t = (row / a.p.nHq) % a.p.T, b = row / (a.p.nHq * a.p.T);
     const int hk = hq / a.G, r = t * a.G + hq % a.G;
     const int s0 = ns1 ? 0 : a.meta[2 * b], ns = ns1 ? ns1 : a.meta[2 * b + 1];
     const size_t step = (size_t)a.p.nKv * a.R, base = (size_t)s0 * step + (size_t)hk * a.R + r;
     float m = -INFINITY, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i0 = sg; i0 < ns && sg < SG; i0 += UN * SG) {
+    for (int i0 = sg; i0 < ns && (256 % D4 == 0 || sg < SG); i0 += UN * SG) {
         v4f x[UN];
         float mi[UN], li[UN];
 #pragma unroll
@@ -548,7 +575,7 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
             const size_t at = base + (size_t)ti_min(i0 + k * SG, ns - 1) * step;
             mi[k] = a.pml[2 * at];
             li[k] = a.pml[2 * at + 1];
-            x[k] = *reinterpret_cast<const v4f*>(a.po + at * HD + 4 * d);
+            x[k] = *reinterpret_cast<const v4f*>(a.po + at * HD + d0 + 4 * d);
         }
         float mn = m;
 #pragma unroll
@@ -566,7 +593,7 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
             for (int c = 0; c < 4; c++) o[c] = fmaf(x[k][c], e, o[c]);
         }
     }
-    if (sg < SG) {
+    if (256 % D4 == 0 || sg < SG) {
         *reinterpret_cast<v4f*>(&s_o[sg][4 * d]) = o;
         if (d == 0) {
             s_m[sg] = m;
@@ -574,7 +601,7 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
         }
     }
     __syncthreads();
-    if (tid >= HD) return;
+    if (tid >= DW) return;
     const int n = ti_min(SG, ns);
     float M = -INFINITY, Lt = 0.0f, v = 0.0f;
     for (int g = 0; g < n; g++) M = fmaxf(M, s_m[g]);
@@ -583,8 +610,8 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
         Lt = fmaf(s_l[g], e, Lt);
         v = fmaf(s_o[g][tid], e, v);
     }
-    a.p.out[(size_t)row * HD + tid] = M == -INFINITY ? 0.0f : v / (127.0f * VSCALE * Lt);
-    if (a.p.ml && tid == 0) {
+    a.p.out[(size_t)row * HD + d0 + tid] = M == -INFINITY ? 0.0f : v / (127.0f * PSCALE * Lt);
+    if (a.p.ml && tid == 0 && d0 == 0) {
         a.p.ml[2 * row] = M;
         a.p.ml[2 * row + 1] = Lt;
     }
@@ -595,7 +622,9 @@ void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
     const unsigned grid = (unsigned)(wgs * a.RT * (a.p.nKv / a.HW));
     if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, THREADS, 0, c->stream>>>(a);
     else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, THREADS, 0, c->stream>>>(a);
-    k_token_merge<HD><<<(unsigned)(a.p.B * a.p.T * a.p.nHq), 256, 0, c->stream>>>(a, ns1);
+    const int rows = a.p.B * a.p.T * a.p.nHq;
+    if (HD == 32 || rows >= c->cus) k_token_merge<HD, HD><<<rows, 256, 0, c->stream>>>(a, ns1);
+    else if constexpr (HD > 32) k_token_merge<HD, 32><<<dim3(rows, HD / 32), 256, 0, c->stream>>>(a, ns1);
 }
 
 }  // namespace
@@ -611,12 +640,14 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     const int rows = tile_rows(hd, true) >= a.R ? tile_rows(hd, true) : 16;
     a.RT = (a.R + rows - 1) / rows;
     static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
-    a.HW = p.nKv % 8 == 0 ? 8 : p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
+    // four heads of a position together where their number allows it: more of each 1 KB row at a time (32 ragged sequences of
+    // 8 heads, 211 MB, one head a wave of 1 / 2 / 4: 72 / 61 / 56 us)
+    a.HW = p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
     a.BW = WAVES / a.HW;
-    // a workgroup a CU; as many as there are sequences, if that is more; as far as the partials' slots (one for each
-    // workgroup and one for each sequence) fit
-    const int groups = p.nKv / a.HW * a.RT;
-    long wgs = ti_max(((long)c->cus + groups - 1) / groups, (long)p.B);
+    // the workgroups that the CUs hold at once (four; two of those with a column a row); as many as there are sequences,
+    // if that is more; as far as the partials' slots (one for each workgroup and one for each sequence) fit
+    const int groups = p.nKv / a.HW * a.RT, held = a.R <= tile_rows(hd, true) ? 4 : 2;
+    long wgs = ti_max(((long)held * c->cus + groups - 1) / groups, (long)p.B);
     wgs = ti_max(1L, ti_min(wgs, (long)TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B));
     a.wgs = (int)wgs;
     const bool paged = p.lens != nullptr;
