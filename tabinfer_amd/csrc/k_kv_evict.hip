@@ -1,7 +1,7 @@
 // k_kv_evict.hip — an int8 KV cache cut, per KV head, to the slots whose keys received the most attention.
 //
-// A slot's key is an unsigned word that orders as (protected, mass): the k-th largest is found by a radix select, eight
-// bits a pass, by one workgroup a head; ties go to the lower slot. The kept slots at and above `keep` then move into the
+// A slot's key is an unsigned word that orders as (protected, mass): the keep-th largest is found by a radix select, by one
+// workgroup a head; ties go to the lower slot. The kept slots at and above `keep` then move into the
 // freed ones below it, the i-th into the i-th: no slot is both read and written, so the moves run in any order, a cache
 // that frees one slot moves one row, and what stays below `keep` stays where it is.
 #include "ti_dev.h"
@@ -22,7 +22,10 @@ struct EvictArgs {
     int32_t* where_out;
     int32_t* moves;          // [nKv][room][2]: (from, to)
     int32_t* count;          // [nKv]
-    int n, known, keep, sinks, late, next, nKv, hd, room;   // late: positions from here on are protected
+    uint32_t* keys;          // [nKv][n]: the slots' keys head by head, or nullptr: up to 8192 slots a head's
+                             // workgroup forms its own
+    uint64_t* stays;         // [nKv][words]: a bit a slot below keep that stays
+    int n, known, keep, sinks, late, next, nKv, hd, room, words;   // late: positions from here on are protected
 };
 
 // the position of a slot: as `where` says, or of the last tokens in order
@@ -30,106 +33,221 @@ __device__ __forceinline__ int slot_pos(const EvictArgs& a, int i, int h) {
     return i < a.known ? a.where[(size_t)i * a.nKv + h] : a.next - (a.n - i);
 }
 // larger: kept sooner. NaN below everything, -0 equal to 0
-__device__ __forceinline__ uint32_t slot_key(const EvictArgs& a, int i, int h) {
-    const int p = slot_pos(a, i, h);
-    if (p < a.sinks || p >= a.late) return 0xffffffffu;
-    const float m = a.mass[(size_t)i * a.nKv + h] + 0.0f;
+__device__ __forceinline__ uint32_t order_key(const EvictArgs& a, int p, float mass) {
+    const float m = mass + 0.0f;
     const uint32_t b = __builtin_bit_cast(uint32_t, m);
-    return m != m ? 0u : (b >> 31 ? ~b : b | 0x80000000u);
+    return p < a.sinks || p >= a.late ? 0xffffffffu : m != m ? 0u : (b >> 31 ? ~b : b | 0x80000000u);
+}
+// the bookkeeping of a slot that stays (nothing to do where it is in place already), and of a move
+__device__ __forceinline__ void stay(const EvictArgs& a, int i, int h) {
+    const size_t at = (size_t)i * a.nKv + h;
+    if (a.mass_out != a.mass) a.mass_out[at] = a.mass[at];
+    if (a.where_out != a.where || i >= a.known) a.where_out[at] = slot_pos(a, i, h);
+}
+__device__ __forceinline__ void moved(const EvictArgs& a, int from, int to, int h) {
+    a.mass_out[(size_t)to * a.nKv + h] = a.mass[(size_t)from * a.nKv + h];
+    a.where_out[(size_t)to * a.nKv + h] = slot_pos(a, from, h);
 }
 
-// exclusive count of the flags of the lanes and waves before this thread, and the total, over 1024 threads
-__device__ __forceinline__ int flag_scan(bool f, int* s16, int& total) {
+// nothing to evict: every slot stays
+__global__ __launch_bounds__(256) void k_evict_none(EvictArgs a) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < (long)a.n * a.nKv) stay(a, (int)(i / a.nKv), (int)(i % a.nKv));
+}
+
+// The keys of many slots, head by head: rows of all heads are read in whole lines here, where a head's one workgroup would
+// take a 4-byte piece of each (16384 slots of 8 heads: 9 us against 5.5 with this launch)
+__global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
+    const long x = (long)blockIdx.x * 256 + threadIdx.x;
+    if (x >= (long)a.n * a.nKv) return;
+    const int i = (int)(x / a.nKv), h = (int)(x % a.nKv);
+    a.keys[(size_t)h * a.n + i] = order_key(a, slot_pos(a, i, h), a.mass[x]);
+}
+
+// A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 32 every key stays in a register, more slots
+// go through in chunks. The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
+// up from the top, and only the keys with the digits so far go on. Lanes of a wave that all have one digit count as one, so
+// that equal masses do not queue for their bin.
+constexpr int BINS = 2048;
+template <int KPT>
+struct SelLds {
+    uint32_t hist[BINS];
+    uint32_t digit, need;
+    int part[KPT * (SEL / 64)], tot[SEL / 64];
+};
+
+// sum over the threads before this one
+__device__ __forceinline__ int thread_scan(int v, int* tot) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t b = __ballot(f);
-    if (lane == 0) s16[wave] = __popcll(b);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < SEL / 64; w++) {
-        const int v = s16[w];
-        before += w < wave ? v : 0;
-        all += v;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        x += lane >= o ? y : 0;
     }
-    total = all;
+    if (lane == 63) tot[wave] = x;
     __syncthreads();
-    return before + __popcll(b & ((1ull << lane) - 1));
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < SEL / 64; w++) before += w < wave ? tot[w] : 0;
+    return before + x - v;
 }
 
-__global__ __launch_bounds__(SEL) void k_evict_select(EvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_prefix, s_need;
-    __shared__ int s16[SEL / 64];
-    const int tid = threadIdx.x, h = blockIdx.x;
-    uint32_t prefix = 0, need = (uint32_t)a.keep;        // the need-th largest among the keys that share the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+// exclusive sums of part[0 .. KPT waves) in place; its total
+template <int KPT>
+__device__ __forceinline__ int part_scan(SelLds<KPT>& L) {
+    constexpr int N = KPT * (SEL / 64);
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const int v = tid < N ? L.part[tid] : 0;
+    const int before = thread_scan(v, L.tot);
+    if (tid < N) L.part[tid] = before;
+    __syncthreads();
+    int sum = L.tot[0];
+#pragma unroll
+    for (int w = 1; w < SEL / 64; w++) sum += L.tot[w];
+    return sum;
+}
+
+template <int KPT>
+__global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
+    constexpr int W = SEL / 64;
+    static_assert(KPT * W <= SEL && KPT * SEL <= 32768, "counts of 16 bits");
+    __shared__ SelLds<KPT> L;
+    const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t key[KPT];                                     // 0 behind the last slot
+    auto load = [&](int i0) {
+        if constexpr (KPT > 8) {                           // k_evict_keys formed them
+#pragma unroll
+            for (int k = 0; k < KPT; k++) key[k] = a.keys[(size_t)h * a.n + ti_min(i0 + k * SEL + tid, a.n - 1)];
+#pragma unroll
+            for (int k = 0; k < KPT; k++) key[k] = i0 + k * SEL + tid < a.n ? key[k] : 0u;
+        } else {
+#pragma unroll
+        for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
+        int at[KPT];                                       // every load in flight at once
+#pragma unroll
+        for (int k = 0; k < KPT; k++) at[k] = a.known ? a.where[(size_t)ti_min(i0 + k * SEL + tid, a.known - 1) * a.nKv + h] : 0;
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const int i = i0 + k * SEL + tid;
+            if (i >= a.known) at[k] = a.next - (a.n - i);
+            key[k] = i < a.n ? order_key(a, at[k], __builtin_bit_cast(float, key[k])) : 0u;
+        }
+        }
+    };
+    constexpr int CHUNK = KPT * SEL;
+    const bool one = a.n <= CHUNK;
+    if (one) load(0);
+    uint32_t top = 0;                                      // the keep-th largest key, its digits so far
+    int need = a.keep;                                     // which of the keys with those digits, from the largest
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        L.hist[tid] = 0;
+        L.hist[tid + SEL] = 0;
         __syncthreads();
-        for (int i = tid; i < a.n; i += SEL) {
-            const uint32_t k = slot_key(a, i, h);
-            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+        for (int i0 = 0; i0 < a.n; i0 += CHUNK) {
+        if (!one) load(i0);
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const bool on = i0 + k * SEL + tid < a.n && (pass == 0 || key[k] >> (shift + bits) == top);
+            const uint64_t b = __ballot(on);
+            if (b == 0) continue;                          // wave-uniform
+            const uint32_t d = key[k] >> shift & ((1u << bits) - 1);
+            const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(b));
+            if (__ballot(on && d == d0) == b) {
+                if (lane == __builtin_ctzll(b)) atomicAdd(&L.hist[d0], (uint32_t)__popcll(b));
+            } else if (on) {
+                atomicAdd(&L.hist[d], 1u);
+            }
+        }
         }
         __syncthreads();
-        if (tid == 0) {
-            uint32_t left = need;
-            int d = 255;
-            for (; d > 0 && hist[d] < left; d--) left -= hist[d];
-            s_prefix = (prefix << 8) | (uint32_t)d;
-            s_need = left;
+        const int h0 = (int)L.hist[BINS - 1 - 2 * tid], h1 = (int)L.hist[BINS - 2 - 2 * tid];
+        const int before = thread_scan(h0 + h1, L.tot);
+        if (before < need && need <= before + h0 + h1) {   // one thread
+            const bool second = need > before + h0;
+            L.digit = (uint32_t)(BINS - 1 - 2 * tid - (second ? 1 : 0));
+            L.need = (uint32_t)(need - before - (second ? h0 : 0));
         }
         __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
+        top = top << bits | L.digit;
+        need = (int)L.need;
     }
-    // kept: above the threshold, and the first `need` slots at it
-    int ties = 0, holes = 0, tails = 0;
-    for (int i0 = 0; i0 < a.n; i0 += SEL) {
-        const int i = i0 + tid;
-        const uint32_t k = i < a.n ? slot_key(a, i, h) : 0u;
-        const bool tie = i < a.n && k == prefix;
-        int all;
-        const int rank = ties + flag_scan(tie, s16, all);
-        ties += all;
-        const bool kept = i < a.n && (k > prefix || (tie && rank < (int)need));
-        const bool hole = i < a.keep && !kept, tail = i >= a.keep && kept;
-        const int hr = holes + flag_scan(hole, s16, all);
-        holes += all;
-        const int tr = tails + flag_scan(tail, s16, all);
-        tails += all;
-        int32_t* mv = a.moves + (size_t)h * a.room * 2;
-        if (hole) mv[2 * hr + 1] = i;
-        if (tail) mv[2 * tr] = i;
+    // kept: the keys above it, and of those equal to it the first `need` slots
+    const uint64_t below = (1ull << lane) - 1;
+    int32_t* mv = a.moves + (size_t)h * a.room * 2;
+    int ties = 0, holes = 0, tails = 0;                    // of the chunks before
+    for (int i0 = 0; i0 < a.n; i0 += CHUNK) {
+        if (!one) load(i0);
+        auto is_tie = [&](int k) { return key[k] == top && i0 + k * SEL + tid < a.n; };
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const uint64_t b = __ballot(is_tie(k));
+            if (lane == 0) L.part[k * W + wave] = __popcll(b);
+        }
+        const int chunk_ties = part_scan<KPT>(L);
+        uint32_t kept = 0;                                 // a bit a slot
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const uint64_t b = __ballot(is_tie(k));
+            const int rank = ties + L.part[k * W + wave] + __popcll(b & below);
+            const bool st = key[k] > top || (is_tie(k) && rank < need);
+            kept |= st ? 1u << k : 0u;
+            const uint64_t stays = __ballot(st);           // for the launch that follows
+            const int w0 = i0 + k * SEL + 64 * wave;
+            if (lane == 0 && w0 < a.keep) a.stays[(size_t)h * a.words + w0 / 64] = stays;
+        }
+        ties += chunk_ties;
+        __syncthreads();
+        // ranks of the freed slots below keep and of the kept ones above: counts side by side in a word
+        auto moves = [&](int k) { return (i0 + k * SEL + tid < a.keep) != (bool)(kept >> k & 1u); };
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const uint64_t b = __ballot(moves(k)), low = __ballot(i0 + k * SEL + tid < a.keep);
+            if (lane == 0) L.part[k * W + wave] = __popcll(b & low) | __popcll(b & ~low) << 16;
+        }
+        const int total = part_scan<KPT>(L);
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const int i = i0 + k * SEL + tid;
+            const uint64_t b = __ballot(moves(k)), low = __ballot(i < a.keep);
+            const uint32_t base = (uint32_t)L.part[k * W + wave];
+            if (moves(k)) {
+                if (i < a.keep) mv[2 * (holes + (int)(base & 0xffff) + __popcll(b & low & below)) + 1] = i;
+                else mv[2 * (tails + (int)(base >> 16) + __popcll(b & ~low & below))] = i;
+            }
+        }
+        holes += total & 0xffff;
+        tails += (int)((uint32_t)total >> 16);
+        __syncthreads();                                   // the parts are read
     }
     if (tid == 0) a.count[h] = holes;
 }
 
-// The bookkeeping of the slots that stay where they are, then the moves: a wave a (move, KV head)
-__global__ __launch_bounds__(256) void k_evict_stay(EvictArgs a) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long)a.keep * a.nKv) return;
-    a.mass_out[i] = a.mass[i];
-    a.where_out[i] = slot_pos(a, (int)(i / a.nKv), (int)(i % a.nKv));
-}
-__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
-    const int h = blockIdx.y, lane = threadIdx.x & 63;
-    const int count = a.count[h];
-    for (int m = blockIdx.x * 4 + (threadIdx.x >> 6); m < count; m += gridDim.x * 4) {
-        const int32_t* mv = a.moves + ((size_t)h * a.room + m) * 2;
-        const int from = mv[0], to = mv[1];
-        const size_t src = (size_t)from * a.nKv + h, dst = (size_t)to * a.nKv + h;
-        const int w4 = a.hd / 16, ng = a.hd / 32;
-        if (lane < w4) {
-            reinterpret_cast<uint4*>(a.kq)[dst * w4 + lane] = reinterpret_cast<const uint4*>(a.kq)[src * w4 + lane];
-            reinterpret_cast<uint4*>(a.vq)[dst * w4 + lane] = reinterpret_cast<const uint4*>(a.vq)[src * w4 + lane];
-        }
-        if (lane < ng) {
-            a.ks[dst * ng + lane] = a.ks[src * ng + lane];
-            a.vs[dst * ng + lane] = a.vs[src * ng + lane];
-        }
-        if (lane == 0) {
-            a.mass_out[dst] = a.mass[src];
-            a.where_out[dst] = slot_pos(a, from, h);
-        }
+// The moves, 16 lanes each: K's and V's pieces and scales, and what the slot holds (read above keep, written below). Behind
+// them (blocks from mblocks on) the bookkeeping of the slots that stay, along the rows of all heads
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int mblocks, int per_head) {
+    if ((int)blockIdx.x >= mblocks) {
+        const long x = (long)(blockIdx.x - mblocks) * 256 + threadIdx.x;
+        const int i = (int)(x / a.nKv), h = (int)(x % a.nKv);
+        if (i < a.keep && (a.stays[(size_t)h * a.words + i / 64] >> (i & 63) & 1)) stay(a, i, h);
+        return;
     }
+    const int h = blockIdx.x / per_head, l = threadIdx.x & 15, m = blockIdx.x % per_head * 16 + (threadIdx.x >> 4);
+    if (m >= a.count[h]) return;
+    const int32_t* mv = a.moves + ((size_t)h * a.room + m) * 2;
+    const int from = mv[0], to = mv[1];
+    const size_t src = (size_t)from * a.nKv + h, dst = (size_t)to * a.nKv + h;
+    const int w4 = a.hd / 16, ng = a.hd / 32, p = l & 7;
+    const uint4* cs = reinterpret_cast<const uint4*>(l < 8 ? a.kq : a.vq);
+    uint4* cd = reinterpret_cast<uint4*>(l < 8 ? a.kq : a.vq);
+    float* sc = l < 8 ? a.ks : a.vs;
+    if (p < w4) cd[dst * w4 + p] = cs[src * w4 + p];
+    if (p < ng) sc[dst * ng + p] = sc[src * ng + p];
+    if (l == 0) moved(a, from, to, h);
 }
 
 }  // namespace
@@ -148,20 +266,33 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     TI_REQUIRE(next >= n - known, "ti_kv_evict_q8: %d slots without a known position before position %d", n - known, next);
     const int kept = keep < n ? keep : n;
     const int room = kept < n - kept ? kept : n - kept;      // moves of a head, at most
-    TI_REQUIRE((long)nKv * room * 2 + nKv <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "ti_kv_evict_q8: %d moves a head exceed the scratch", room);
+    const int words = (kept + 63) / 64;
+    // scratch: the slots that stay, the moves' counts, the moves, the keys of many slots
+    const bool many = n > 8 * SEL;
+    const long need = 2L * nKv * words + nKv + 2L * nKv * room + (many ? (long)nKv * n : 0);
+    TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX && (long)nKv * room <= 0x7fffffffL, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch",
+               n, room);
+    uint64_t* stays = reinterpret_cast<uint64_t*>(c->attn_po);
+    int32_t* count = reinterpret_cast<int32_t*>(stays + (size_t)nKv * words);
     EvictArgs a = {reinterpret_cast<uint8_t*>(kq), ks, reinterpret_cast<uint8_t*>(vq), vs, mass, where, mass_out, where_out,
-                   reinterpret_cast<int32_t*>(c->attn_po) + nKv, reinterpret_cast<int32_t*>(c->attn_po), n, known, kept, sinks,
-                   recent > next ? 0 : next - recent, next, nKv, hd, room};
-    if (room > 0) {
-        k_evict_select<<<nKv, SEL, 0, c->stream>>>(a);
-        TI_LAUNCHED("k_evict_select");
+                   count + nKv, count, many ? reinterpret_cast<uint32_t*>(count + nKv + 2 * (size_t)nKv * room) : nullptr, stays, n, known, kept, sinks, recent > next ? 0 : next - recent, next, nKv, hd, room, words};
+    if (room == 0) {
+        k_evict_none<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
+        TI_LAUNCHED("k_evict_none");
+        return TI_OK;
     }
-    k_evict_stay<<<(unsigned)(((long)kept * nKv + 255) / 256), 256, 0, c->stream>>>(a);
-    TI_LAUNCHED("k_evict_stay");
-    if (room > 0) {
-        const int blocks = (room + 3) / 4 < 256 ? (room + 3) / 4 : 256;
-        k_evict_move<<<dim3(blocks, nKv), 256, 0, c->stream>>>(a);
-        TI_LAUNCHED("k_evict_move");
+    if (a.keys) {
+        k_evict_keys<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
+        TI_LAUNCHED("k_evict_keys");
     }
+    if (n <= 8 * SEL) k_evict_pick<8><<<nKv, SEL, 0, c->stream>>>(a);
+    else if (n <= 16 * SEL) k_evict_pick<16><<<nKv, SEL, 0, c->stream>>>(a);
+    else k_evict_pick<32><<<nKv, SEL, 0, c->stream>>>(a);
+    TI_LAUNCHED("k_evict_pick");
+    // in place, the slots that stay already hold what they held
+    const bool placed = mass_out == mass && where_out == where && known >= kept;
+    const int per_head = (room + 15) / 16, sblocks = placed ? 0 : (int)(((long)kept * nKv + 255) / 256);
+    k_evict_move<<<(unsigned)(per_head * nKv + sblocks), 256, 0, c->stream>>>(a, per_head * nKv, per_head);
+    TI_LAUNCHED("k_evict_move");
     return TI_OK;
 }

@@ -22,53 +22,81 @@ __device__ __forceinline__ long place_row(const PlaceArgs& a, int t) {
     return a.pg.row(s, a.pos[t]);
 }
 
-// thread = one 32-group of K, then of V
+// A thread takes four elements (a word of codes) at a time, a workgroup WORDS words of K or V, row behind row, so that both
+// sides are read and written in whole lines; eight neighbouring lanes share a 32-group. Bound by the launch below a few
+// hundred rows, by the floats' traffic above.
+constexpr int WORDS = 1024;
+
+// word x of the workgroup -> row t and word of it; false: behind the last
+struct WordAt {
+    int t, w;
+    __device__ WordAt(const PlaceArgs& a, int x) {
+        const int rw = a.rowg * 8;
+        const long base = (long)blockIdx.x * WORDS;
+        const long t0 = base / rw;                         // workgroup-uniform
+        const unsigned l = (unsigned)(base - t0 * rw) + x;
+        t = (int)(t0 + l / (unsigned)rw);
+        w = (int)(l % (unsigned)rw);
+    }
+};
+
 __global__ __launch_bounds__(256) void k_kv_write_paged(PlaceArgs a, const float* __restrict__ k, const float* __restrict__ v,
                                                         uint32_t* __restrict__ kq, float* __restrict__ ks,
                                                         uint32_t* __restrict__ vq, float* __restrict__ vs) {
-    const long nG = (long)a.T * a.rowg;
-    const long idx = (long)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= 2 * nG) return;
-    const bool isv = idx >= nG;
-    const long g = isv ? idx - nG : idx;
-    const long row = place_row(a, (int)(g / a.rowg));
-    if (row < 0) return;
-    float x[32];
-    load32((isv ? v : k) + g * 32, x);
-    float mx = 1e-12f;
+    const bool isv = blockIdx.y;
+    const float4* src = reinterpret_cast<const float4*>(isv ? v : k);
+    float4 x[WORDS / 256];
+    long row[WORDS / 256];
+    int w[WORDS / 256];
 #pragma unroll
-    for (int j = 0; j < 32; j++) mx = fmaxf(mx, fabsf(x[j]));
-    const long at = row * a.rowg + g % a.rowg;
-    (isv ? vs : ks)[at] = mx;
-    uint32_t w[8];
+    for (int u = 0; u < WORDS / 256; u++) {
+        const WordAt at(a, threadIdx.x + 256 * u);
+        const bool in = at.t < a.T;
+        x[u] = in ? src[(size_t)at.t * a.rowg * 8 + at.w] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        row[u] = in ? place_row(a, at.t) : -1;
+        w[u] = at.w;
+    }
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        w[j] = snorm_code(x[4 * j], mx) | (snorm_code(x[4 * j + 1], mx) << 8) | (snorm_code(x[4 * j + 2], mx) << 16) |
-               (snorm_code(x[4 * j + 3], mx) << 24);
-    uint4* o = reinterpret_cast<uint4*>(isv ? vq : kq) + at * 2;
-    o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    for (int u = 0; u < WORDS / 256; u++) {
+        const float4 f = x[u];
+        const float mx = fmaxf(group_max_contig<4>(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)))), 1e-12f);
+        if (row[u] < 0) continue;
+        const size_t at = (size_t)row[u] * a.rowg * 8 + w[u];
+        (isv ? vq : kq)[at] = snorm_code(f.x, mx) | (snorm_code(f.y, mx) << 8) | (snorm_code(f.z, mx) << 16) | (snorm_code(f.w, mx) << 24);
+        if ((w[u] & 7) == 0) (isv ? vs : ks)[at / 8] = mx;
+    }
 }
 
 __global__ __launch_bounds__(256) void k_kv_read_paged(PlaceArgs a, const uint32_t* __restrict__ kq, const float* __restrict__ ks,
                                                        const uint32_t* __restrict__ vq, const float* __restrict__ vs,
                                                        float* __restrict__ k, float* __restrict__ v) {
-    const long nG = (long)a.T * a.rowg;
-    const long idx = (long)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= 2 * nG) return;
-    const bool isv = idx >= nG;
-    const long g = isv ? idx - nG : idx;
-    const long row = place_row(a, (int)(g / a.rowg));
-    float* out = (isv ? v : k) + g * 32;
-    const long at = row * a.rowg + g % a.rowg;
-    const float s = row < 0 ? 0.0f : (isv ? vs : ks)[at] / 127.0f;
+    const bool isv = blockIdx.y;
+    const uint32_t* codes = isv ? vq : kq;
+    const float* scales = isv ? vs : ks;
+    float4* out = reinterpret_cast<float4*>(isv ? v : k);
+    uint32_t c[WORDS / 256];
+    float s[WORDS / 256];
+    long dst[WORDS / 256];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t w = row < 0 ? 0u : (isv ? vq : kq)[at * 8 + j];
+    for (int u = 0; u < WORDS / 256; u++) {
+        const WordAt at(a, threadIdx.x + 256 * u);
+        const bool in = at.t < a.T;
+        const long row = in ? place_row(a, at.t) : -1;
+        const size_t g = (size_t)(row < 0 ? 0 : row) * a.rowg * 8 + at.w;
+        c[u] = row < 0 ? 0u : codes[g];
+        s[u] = row < 0 ? 0.0f : scales[g / 8];
+        dst[u] = in ? (long)at.t * a.rowg * 8 + at.w : -1;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; e++) out[4 * j + e] = (float)(int8_t)(w >> (8 * e)) * s;
+    for (int u = 0; u < WORDS / 256; u++) {
+        if (dst[u] < 0) continue;
+        const float f = s[u] / 127.0f;
+        out[dst[u]] = make_float4((float)(int8_t)c[u] * f, (float)(int8_t)(c[u] >> 8) * f, (float)(int8_t)(c[u] >> 16) * f,
+                                  (float)(int8_t)(c[u] >> 24) * f);
     }
 }
+
+dim3 word_grid(const PlaceArgs& a) { return dim3((unsigned)(((long)a.T * a.rowg * 8 + WORDS - 1) / WORDS), 2); }
 
 int place_args(PlaceArgs& a, const char* fn, const int32_t* table, const int32_t* seq, const int32_t* pos, int T, int B,
                int nKv, int hd, int page, int pages, int width) {
@@ -100,8 +128,7 @@ extern "C" int ti_kv_write_paged_q8(ti_ctx* c, const float* kr, const float* v, 
     PlaceArgs a;
     const int rc = place_args(a, "ti_kv_write_paged_q8", table, seq, pos, T, B, nKv, hd, page, pages, width);
     if (rc) return rc;
-    const long threads = 2L * T * a.rowg;
-    k_kv_write_paged<<<(unsigned)((threads + 255) / 256), 256, 0, c->stream>>>(a, kr, v, kq, ks, vq, vs);
+    k_kv_write_paged<<<word_grid(a), 256, 0, c->stream>>>(a, kr, v, kq, ks, vq, vs);
     TI_LAUNCHED("k_kv_write_paged");
     return TI_OK;
 }
@@ -115,8 +142,7 @@ extern "C" int ti_kv_read_paged_q8(ti_ctx* c, const uint32_t* kq, const float* k
     PlaceArgs a;
     const int rc = place_args(a, "ti_kv_read_paged_q8", table, seq, pos, T, B, nKv, hd, page, pages, width);
     if (rc) return rc;
-    const long threads = 2L * T * a.rowg;
-    k_kv_read_paged<<<(unsigned)((threads + 255) / 256), 256, 0, c->stream>>>(a, kq, ks, vq, vs, k, v);
+    k_kv_read_paged<<<word_grid(a), 256, 0, c->stream>>>(a, kq, ks, vq, vs, k, v);
     TI_LAUNCHED("k_kv_read_paged");
     return TI_OK;
 }
