@@ -417,7 +417,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a)
                 for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e] * fr;
+            for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e];
         }
         // which of the lane's keys its row sees
         uint32_t seen = 0xffu;
@@ -434,8 +434,8 @@ __global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a)
         }
         if (a.p.scores && slot == 0 && rt * ROWS + tr < a.R) {
             float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
-            *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]};
-            *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]};
+            *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
+            *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
         }
         float tm = FLOOR;
         if (!whole) {
@@ -448,6 +448,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a)
         }
         tm = fmaxf(tm, ti_xor(tm, 16));
         tm = fmaxf(tm, ti_xor(tm, 32));
+        tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;       // in log2 units from here on
         // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
         const bool bump = tm > m + 6.0f;
         if (__any(bump)) {
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a)
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            float p = __builtin_amdgcn_exp2f(s[e] - m);
+            float p = __builtin_amdgcn_exp2f(fmaf(s[e], fr, -m));
             if (!whole) p = seen >> e & 1u ? p : 0.0f;
             sum += p;
             s[e] = p * PSCALE;

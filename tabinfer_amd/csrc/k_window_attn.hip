@@ -30,20 +30,22 @@ struct WinArgs {
     int G, nblk, nsplit;
 };
 
-// The query row of this lane: MFMA operands of its dims 32 g + 8 j.., and the factor that scales its scores to log2 units
+// The query row of this lane, its dims 32 g + 8 j..; as MFMA operands, and the factor that scales its scores to log2 units
 template <int HD>
-__device__ __forceinline__ float query_operand(const float* q, ti_h8 (&qh)[HD / 32], ti_h8 (&ql)[HD / 32]) {
+__device__ __forceinline__ void query_load(const float* q, v4f_u (&qv)[HD / 32][2]) {
+#pragma unroll
+    for (int g = 0; g < HD / 32; g++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
+}
+template <int HD>
+__device__ __forceinline__ float query_operand(const v4f_u (&qv)[HD / 32][2], ti_h8 (&qh)[HD / 32], ti_h8 (&ql)[HD / 32]) {
     constexpr int NG = HD / 32;
-    v4f_u qv[NG][2];
     float mx = 0.0f;
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            qv[g][u] = *reinterpret_cast<const v4f_u*>(q + 32 * g + 4 * u);
-#pragma unroll
-            for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(qv[g][u][e]));
-        }
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[g][e / 4][e % 4]));
     mx = fmaxf(mx, ti_xor(mx, 16));
     mx = fmaxf(mx, ti_xor(mx, 32));
     int ex = 4;
@@ -101,34 +103,51 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
     const int c0 = split * per, c1 = ti_min(nb, c0 + per);
     auto block_key = [&](int i) { return (i < sb ? i : i + skip) * KB; };
 
-    const size_t code_row = (size_t)a.p.nKv * HD, scale_row = (size_t)a.p.nKv * NG;
-    const uint8_t* kp = a.p.kq + hk * HD;
-    const uint8_t* vp = a.p.vq + hk * HD;
-    const float* ksp = a.p.ks + hk * NG;
-    const float* vsp = a.p.vs + hk * NG;
-
+    // a thread's loads of a block: K, 16 codes of a key; V, 4 dims of 4 keys; scales. Bytes from the block's first row on
     uint4 kr[KL];
     uint32_t vr[VL][4];
     float ksr[SL], vsr[SL];
+    const uint32_t code_row = (uint32_t)a.p.nKv * HD, scale_row = (uint32_t)a.p.nKv * NG;
+    auto k_at = [&](int u) { const int x = ti_min(tid + 256 * u, KB * PC - 1); return make_int2((x >> 4) / PC * 16 + (x & 15), 16 * ((x >> 4) % PC)); };
+    auto v_at = [&](int u) { const int x = ti_min(tid + 256 * u, KB * HD / 16 - 1); return make_int2(4 * (x / (HD / 4)), 4 * (x % (HD / 4))); };
+    auto s_at = [&](int u) { const int x = ti_min(tid + 256 * u, KB * NG - 1); return make_int2(x / NG, x % NG); };
+    uint32_t ko[KL], vo[VL], so[SL];
+#pragma unroll
+    for (int u = 0; u < KL; u++) ko[u] = k_at(u).x * code_row + k_at(u).y;
+#pragma unroll
+    for (int u = 0; u < VL; u++) vo[u] = v_at(u).x * code_row + v_at(u).y;
+#pragma unroll
+    for (int u = 0; u < SL; u++) so[u] = s_at(u).x * scale_row + s_at(u).y;
     auto load = [&](int k0) {
+        const size_t row = (size_t)k0 * a.p.nKv + hk;
+        const uint8_t *kb = a.p.kq + row * HD, *vb = a.p.vq + row * HD;
+        const float *ksb = a.p.ks + row * NG, *vsb = a.p.vs + row * NG;
+        if (k0 + KB <= end) {
 #pragma unroll
-        for (int u = 0; u < KL; u++) {
-            const int x = ti_min(tid + 256 * u, KB * PC - 1), key = (x >> 4) / PC * 16 + (x & 15), c = (x >> 4) % PC;
-            kr[u] = *reinterpret_cast<const uint4*>(kp + (size_t)ti_min(k0 + key, end - 1) * code_row + 16 * c);
+            for (int u = 0; u < KL; u++) kr[u] = *reinterpret_cast<const uint4*>(kb + ko[u]);
+#pragma unroll
+            for (int u = 0; u < VL; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) vr[u][r] = *reinterpret_cast<const uint32_t*>(vb + (size_t)r * code_row + vo[u]);
+#pragma unroll
+            for (int u = 0; u < SL; u++) {
+                ksr[u] = ksb[so[u]];
+                vsr[u] = vsb[so[u]];
+            }
+            return;
         }
+        const int top = end - 1 - k0;                      // the last row there is
 #pragma unroll
-        for (int u = 0; u < VL; u++) {
-            const int x = ti_min(tid + 256 * u, KB * HD / 16 - 1), db = x % (HD / 4), kb = x / (HD / 4);
+        for (int u = 0; u < KL; u++) kr[u] = *reinterpret_cast<const uint4*>(kb + ti_min(k_at(u).x, top) * code_row + k_at(u).y);
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                vr[u][r] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ti_min(k0 + 4 * kb + r, end - 1) * code_row + 4 * db);
-        }
+        for (int u = 0; u < VL; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) vr[u][r] = *reinterpret_cast<const uint32_t*>(vb + ti_min(v_at(u).x + r, top) * code_row + v_at(u).y);
 #pragma unroll
         for (int u = 0; u < SL; u++) {
-            const int x = ti_min(tid + 256 * u, KB * NG - 1);
-            const size_t s = (size_t)ti_min(k0 + x / NG, end - 1) * scale_row + x % NG;
-            ksr[u] = ksp[s];
-            vsr[u] = vsp[s];
+            const uint32_t o = ti_min(s_at(u).x, top) * scale_row + s_at(u).y;
+            ksr[u] = ksb[o];
+            vsr[u] = vsb[o];
         }
     };
     auto stage = [&]() {
@@ -161,7 +180,9 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
             }
         }
     };
-    if (c0 < c1) load(block_key(c0));
+    // 32 rows a wave leave no registers for a block ahead: their two workgroups a CU load and compute in turn
+    constexpr bool AHEAD = RW == 1;
+    if (AHEAD && c0 < c1) load(block_key(c0));
 
     // this lane's rows (past the last: that one again), and what all rows of the wave and any of them see
     const int row0 = wg0 + wave * 16 * RW;
@@ -175,7 +196,9 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
         pos[r] = pos0 + t;
         low[r] = low_of(pos[r]);
         orow[r] = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
-        fr[r] = query_operand<HD>(a.p.qr + orow[r] * HD + 8 * j, qh[r], ql[r]);
+        v4f_u qv[NG][2];
+        query_load<HD>(a.p.qr + orow[r] * HD + 8 * j, qv);
+        fr[r] = query_operand<HD>(qv, qh[r], ql[r]);
     }
     const int first_pos = pos0 + ti_min(row0, nrows - 1) / a.G, last_pos = pos0 + ti_min(row0 + 16 * RW - 1, nrows - 1) / a.G;
     const int any_low = low_of(first_pos), all_low = low_of(last_pos);
@@ -192,10 +215,11 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
     }
     for (int i = c0; i < c1; i++) {
         const int t0 = block_key(i);
+        if (!AHEAD) load(t0);
         __syncthreads();                                   // the last block is read
         stage();
         __syncthreads();
-        if (i + 1 < c1) load(block_key(i + 1));
+        if (AHEAD && i + 1 < c1) load(block_key(i + 1));
         TI_ISSUE_FENCE();
 #pragma unroll 1
         for (int h = 0; h < KB / 32; h++) {                // 32 keys
@@ -224,15 +248,15 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
 #pragma unroll
                 for (int r = 0; r < RW; r++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[r][4 * b + e] = acc[r][e] * fr[r];
+                    for (int e = 0; e < 4; e++) s[r][4 * b + e] = acc[r][e];
             }
             uint32_t seen[RW];
 #pragma unroll
             for (int r = 0; r < RW; r++) {
                 seen[r] = 0xffu;
-                float tm = FLOOR;
+                float tm = -INFINITY;
                 if (!whole) {
-                    tm = -INFINITY;
+                    asm volatile("");                      // a branch: not computed where every key is seen
                     seen[r] = 0;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -244,9 +268,11 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[r][e]);
+                    tm = fmaxf(tm, FLOOR);
                 }
                 tm = fmaxf(tm, ti_xor(tm, 16));
                 tm = fmaxf(tm, ti_xor(tm, 32));
+                tm = tm > -INFINITY ? fmaxf(tm * fr[r], FLOOR) : -INFINITY;   // in log2 units from here on
                 // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
                 const bool bump = tm > mx[r] + 6.0f;
                 if (__any(bump)) {
@@ -259,7 +285,7 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
                 }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    float p = __builtin_amdgcn_exp2f(s[r][e] - mx[r]);
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[r][e], fr[r], -mx[r]));
                     if (!whole) p = seen[r] >> e & 1u ? p : 0.0f;
                     s[r][e] = p;
                 }
@@ -379,13 +405,21 @@ __global__ __launch_bounds__(256) void k_mass_columns(WinArgs a, float* __restri
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     // rows before the one of the workgroup's first key see none of its keys
     const int start = (int)ti_max(0L, kw - a.p.pos0) * a.G / 64 * 64;
+    v4f_u qv[NG][2];
+    float rm, rl;
+    auto load = [&](int r0) {                              // this lane's row of 64, while the ones before are worked on
+        const int gr = ti_min(r0 + 16 * wave + m16, nrows - 1), t = gr / a.G;
+        const size_t row = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
+        query_load<HD>(a.p.qr + row * HD + 8 * j, qv);
+        rm = a.p.ml[2 * row];
+        rl = a.p.ml[2 * row + 1];
+    };
+    load(start);
     for (int r0 = start; r0 < nrows; r0 += 64) {
         __syncthreads();
         {
-            const int gr = ti_min(r0 + 16 * wave + m16, nrows - 1), t = gr / a.G;
-            const size_t row = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
             ti_h8 qh[NG], ql[NG];
-            const float f = query_operand<HD>(a.p.qr + row * HD + 8 * j, qh, ql);
+            const float f = query_operand<HD>(qv, qh, ql);
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 s_q[wave][0][g][lane] = qh[g];
@@ -393,10 +427,11 @@ __global__ __launch_bounds__(256) void k_mass_columns(WinArgs a, float* __restri
             }
             if (j == 0) {
                 s_f[16 * wave + m16] = f;
-                s_m[16 * wave + m16] = a.p.ml[2 * row];
-                s_l[16 * wave + m16] = 1.0f / a.p.ml[2 * row + 1];
+                s_m[16 * wave + m16] = rm;
+                s_l[16 * wave + m16] = 1.0f / rl;
             }
         }
+        if (r0 + 64 < nrows) load(r0 + 64);
         __syncthreads();
 #pragma unroll 1
         for (int t = 0; t < 4 && r0 + 16 * t < nrows; t++) {
@@ -409,12 +444,12 @@ __global__ __launch_bounds__(256) void k_mass_columns(WinArgs a, float* __restri
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[g][e], acc[e]);
             }
-            const int rl = 16 * t + m16, gr = r0 + rl;
-            const float f = s_f[rl], m = s_m[rl], inv = s_l[rl];
+            const int rw = 16 * t + m16, gr = r0 + rw;
+            const float f = s_f[rw], m = s_m[rw], inv = s_l[rw];
             const long pos = gr < nrows ? a.p.pos0 + gr / a.G : -1;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float p = __builtin_amdgcn_exp2f(acc[e] * f - m) * inv;
+                const float p = __builtin_amdgcn_exp2f(fmaf(acc[e], f, -m)) * inv;
                 sum[e] += k0 + 4 * j + e <= pos ? p : 0.0f;
             }
         }
