@@ -7,7 +7,8 @@
 //    KV head: each has the same work whatever the lengths, a run that ends one sequence begins the next, and its part of
 //    a sequence is a partial in slot (workgroup + sequence). Every workgroup finds its run by a scan over the lengths;
 //    nothing depends on them on the host.
-//  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 16 waves a CU cover each other's loads.
+//  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 12 waves a CU cover each other's loads (16 have too few
+//    registers: 57 us for 32 ragged sequences against 49).
 //    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-25 of
 //    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
@@ -209,7 +210,7 @@ __device__ __forceinline__ float slot_sum(float v) {
 }
 
 template <int HD, bool PAGED, bool COLS>
-__global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a) {
+__global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a) {
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 4 : 2) void k_token_attn(TokArgs a)
         ti_b8 pb[3];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for four waves a SIMD
+            if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for three waves a SIMD
             if (!COLS || g == 0) {
                 const v4f v0 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 4 * j]);
                 const v4f v1 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 16 + 4 * j]);
@@ -645,9 +646,9 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     // 8 heads, 211 MB, one head a wave of 1 / 2 / 4: 72 / 61 / 56 us)
     a.HW = p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
     a.BW = WAVES / a.HW;
-    // the workgroups that the CUs hold at once (four; two of those with a column a row); as many as there are sequences,
+    // the workgroups that the CUs hold at once (three; two of those with a column a row); as many as there are sequences,
     // if that is more; as far as the partials' slots (one for each workgroup and one for each sequence) fit
-    const int groups = p.nKv / a.HW * a.RT, held = a.R <= tile_rows(hd, true) ? 4 : 2;
+    const int groups = p.nKv / a.HW * a.RT, held = a.R <= tile_rows(hd, true) ? 3 : 2;
     long wgs = ti_max(((long)held * c->cus + groups - 1) / groups, (long)p.B);
     wgs = ti_max(1L, ti_min(wgs, (long)TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B));
     a.wgs = (int)wgs;
