@@ -1,15 +1,21 @@
 // k_kv_evict.hip — an int8 KV cache cut, per KV head, to the slots whose keys received the most attention.
 //
 // A slot's key is an unsigned word that orders as (protected, mass): the keep-th largest is found by a radix select, by one
-// workgroup a head; ties go to the lower slot. The kept slots at and above `keep` then move into the
-// freed ones below it, the i-th into the i-th: no slot is both read and written, so the moves run in any order, a cache
-// that frees one slot moves one row, and what stays below `keep` stays where it is.
+// workgroup a head; ties go to the lower slot. The kept slots at and above `keep` then move into the freed ones below it, the
+// i-th into the i-th: no slot is both read and written, so the moves run in any order, a cache that frees one slot moves one
+// row, and what stays below `keep` stays where it is.
+//
+// Bound by its launches and by the select's chain of barriers, not by bytes: 4097 slots of 8 heads to 4096 17.2 + 4.0 us
+// (select, moves), 16384 to 4096 3.0 + 22.2 + 5.6 us, where the moved rows' 13 MB are 2.7 us of a copy. A workgroup a head
+// and not more: the select's steps depend on one another, and counts across workgroups would cost a launch a digit (about
+// 5 us each). 1024 threads: 512 took 20.1 and 28.1 us, 256 29.3 and 54.3 (more keys a thread, behind one another).
 #include "ti_dev.h"
 #include "ti_span.h"
 
 namespace {
 
-constexpr int SEL = 1024;
+constexpr int SEL = 1024;       // threads of a head's workgroup
+constexpr int FORMED = 8192;    // up to so many slots it forms their keys itself, see k_evict_keys
 
 struct EvictArgs {
     uint8_t* kq;
@@ -22,8 +28,7 @@ struct EvictArgs {
     int32_t* where_out;
     int32_t* moves;          // [nKv][room][2]: (from, to)
     int32_t* count;          // [nKv]
-    uint32_t* keys;          // [nKv][n]: the slots' keys head by head, or nullptr: up to 8192 slots a head's
-                             // workgroup forms its own
+    uint32_t* keys;          // [nKv][n]: the keys of more than FORMED slots, head by head
     uint64_t* stays;         // [nKv][words]: a bit a slot below keep that stays
     int n, known, keep, sinks, late, next, nKv, hd, room, words;   // late: positions from here on are protected
 };
@@ -56,7 +61,8 @@ __global__ __launch_bounds__(256) void k_evict_none(EvictArgs a) {
 }
 
 // The keys of many slots, head by head: rows of all heads are read in whole lines here, where a head's one workgroup would
-// take a 4-byte piece of each (16384 slots of 8 heads: 9 us against 5.5 with this launch)
+// take a 4-byte piece of each (16384 slots of 8 heads: 9 us against 5.5 with this launch; up to 8192 slots the pieces cost
+// less than the launch)
 __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
     const long x = (long)blockIdx.x * 256 + threadIdx.x;
     if (x >= (long)a.n * a.nKv) return;
@@ -65,7 +71,7 @@ __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
 }
 
 // A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 32 every key stays in a register, more slots
-// go through in chunks. The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
+// go through in chunks, read again for each digit. The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
 // up from the top, and only the keys with the digits so far go on. Lanes of a wave that all have one digit count as one, so
 // that equal masses do not queue for their bin.
 constexpr int BINS = 2048;
@@ -93,10 +99,11 @@ __device__ __forceinline__ int thread_scan(int v, int* tot) {
     return before + x - v;
 }
 
-// exclusive sums of part[0 .. KPT waves) in place; its total
+// exclusive sums of part[] in place; its total
 template <int KPT>
 __device__ __forceinline__ int part_scan(SelLds<KPT>& L) {
     constexpr int N = KPT * (SEL / 64);
+    static_assert(N <= SEL, "a thread a count");
     const int tid = threadIdx.x;
     __syncthreads();
     const int v = tid < N ? L.part[tid] : 0;
@@ -109,32 +116,32 @@ __device__ __forceinline__ int part_scan(SelLds<KPT>& L) {
     return sum;
 }
 
-template <int KPT>
+template <int KPT, bool FORM>
 __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     constexpr int W = SEL / 64;
-    static_assert(KPT * W <= SEL && KPT * SEL <= 32768, "counts of 16 bits");
+    static_assert(KPT * SEL <= 32768, "counts of 16 bits");
     __shared__ SelLds<KPT> L;
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint32_t key[KPT];                                     // 0 behind the last slot
     auto load = [&](int i0) {
-        if constexpr (KPT > 8) {                           // k_evict_keys formed them
+        if constexpr (FORM) {
+#pragma unroll
+            for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
+            int at[KPT];                                   // every load in flight at once
+#pragma unroll
+            for (int k = 0; k < KPT; k++) at[k] = a.known ? a.where[(size_t)ti_min(i0 + k * SEL + tid, a.known - 1) * a.nKv + h] : 0;
+#pragma unroll
+            for (int k = 0; k < KPT; k++) {
+                const int i = i0 + k * SEL + tid;
+                if (i >= a.known) at[k] = a.next - (a.n - i);
+                key[k] = i < a.n ? order_key(a, at[k], __builtin_bit_cast(float, key[k])) : 0u;
+            }
+        } else {                                           // k_evict_keys formed them
 #pragma unroll
             for (int k = 0; k < KPT; k++) key[k] = a.keys[(size_t)h * a.n + ti_min(i0 + k * SEL + tid, a.n - 1)];
 #pragma unroll
             for (int k = 0; k < KPT; k++) key[k] = i0 + k * SEL + tid < a.n ? key[k] : 0u;
-        } else {
-#pragma unroll
-        for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
-        int at[KPT];                                       // every load in flight at once
-#pragma unroll
-        for (int k = 0; k < KPT; k++) at[k] = a.known ? a.where[(size_t)ti_min(i0 + k * SEL + tid, a.known - 1) * a.nKv + h] : 0;
-#pragma unroll
-        for (int k = 0; k < KPT; k++) {
-            const int i = i0 + k * SEL + tid;
-            if (i >= a.known) at[k] = a.next - (a.n - i);
-            key[k] = i < a.n ? order_key(a, at[k], __builtin_bit_cast(float, key[k])) : 0u;
-        }
         }
     };
     constexpr int CHUNK = KPT * SEL;
@@ -149,22 +156,24 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
         L.hist[tid + SEL] = 0;
         __syncthreads();
         for (int i0 = 0; i0 < a.n; i0 += CHUNK) {
-        if (!one) load(i0);
+            if (!one) load(i0);
 #pragma unroll
-        for (int k = 0; k < KPT; k++) {
-            const bool on = i0 + k * SEL + tid < a.n && (pass == 0 || key[k] >> (shift + bits) == top);
-            const uint64_t b = __ballot(on);
-            if (b == 0) continue;                          // wave-uniform
-            const uint32_t d = key[k] >> shift & ((1u << bits) - 1);
-            const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(b));
-            if (__ballot(on && d == d0) == b) {
-                if (lane == __builtin_ctzll(b)) atomicAdd(&L.hist[d0], (uint32_t)__popcll(b));
-            } else if (on) {
-                atomicAdd(&L.hist[d], 1u);
+            for (int k = 0; k < KPT; k++) {
+                const bool on = i0 + k * SEL + tid < a.n && (pass == 0 || key[k] >> (shift + bits) == top);
+                const uint64_t b = __ballot(on);
+                if (b == 0) continue;                      // wave-uniform
+                const uint32_t d = key[k] >> shift & ((1u << bits) - 1);
+                const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(b));
+                if (__ballot(on && d == d0) == b) {
+                    if (lane == __builtin_ctzll(b)) atomicAdd(&L.hist[d0], (uint32_t)__popcll(b));
+                } else if (on) {
+                    atomicAdd(&L.hist[d], 1u);
+                }
             }
         }
-        }
         __syncthreads();
+        // a thread: two bins, from the top
+        static_assert(BINS == 2 * SEL, "two bins a thread");
         const int h0 = (int)L.hist[BINS - 1 - 2 * tid], h1 = (int)L.hist[BINS - 2 - 2 * tid];
         const int before = thread_scan(h0 + h1, L.tot);
         if (before < need && need <= before + h0 + h1) {   // one thread
@@ -188,7 +197,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
             const uint64_t b = __ballot(is_tie(k));
             if (lane == 0) L.part[k * W + wave] = __popcll(b);
         }
-        const int chunk_ties = part_scan<KPT>(L);
+        const int chunk_ties = part_scan(L);
         uint32_t kept = 0;                                 // a bit a slot
 #pragma unroll
         for (int k = 0; k < KPT; k++) {
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
             const uint64_t b = __ballot(moves(k)), low = __ballot(i0 + k * SEL + tid < a.keep);
             if (lane == 0) L.part[k * W + wave] = __popcll(b & low) | __popcll(b & ~low) << 16;
         }
-        const int total = part_scan<KPT>(L);
+        const int total = part_scan(L);
 #pragma unroll
         for (int k = 0; k < KPT; k++) {
             const int i = i0 + k * SEL + tid;
@@ -268,26 +277,27 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     const int room = kept < n - kept ? kept : n - kept;      // moves of a head, at most
     const int words = (kept + 63) / 64;
     // scratch: the slots that stay, the moves' counts, the moves, the keys of many slots
-    const bool many = n > 8 * SEL;
+    const bool many = n > FORMED;
     const long need = 2L * nKv * words + nKv + 2L * nKv * room + (many ? (long)nKv * n : 0);
-    TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX && (long)nKv * room <= 0x7fffffffL, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch",
-               n, room);
+    TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch", n, room);
     uint64_t* stays = reinterpret_cast<uint64_t*>(c->attn_po);
     int32_t* count = reinterpret_cast<int32_t*>(stays + (size_t)nKv * words);
-    EvictArgs a = {reinterpret_cast<uint8_t*>(kq), ks, reinterpret_cast<uint8_t*>(vq), vs, mass, where, mass_out, where_out,
-                   count + nKv, count, many ? reinterpret_cast<uint32_t*>(count + nKv + 2 * (size_t)nKv * room) : nullptr, stays, n, known, kept, sinks, recent > next ? 0 : next - recent, next, nKv, hd, room, words};
+    int32_t* moves = count + nKv;
+    EvictArgs a = {reinterpret_cast<uint8_t*>(kq), ks, reinterpret_cast<uint8_t*>(vq), vs, mass, where, mass_out, where_out, moves, count,
+                   reinterpret_cast<uint32_t*>(moves + 2 * (size_t)nKv * room), stays, n, known, kept, sinks,
+                   recent > next ? 0 : next - recent, next, nKv, hd, room, words};
     if (room == 0) {
         k_evict_none<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_evict_none");
         return TI_OK;
     }
-    if (a.keys) {
+    if (many) {
         k_evict_keys<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_evict_keys");
     }
-    if (n <= 8 * SEL) k_evict_pick<8><<<nKv, SEL, 0, c->stream>>>(a);
-    else if (n <= 16 * SEL) k_evict_pick<16><<<nKv, SEL, 0, c->stream>>>(a);
-    else k_evict_pick<32><<<nKv, SEL, 0, c->stream>>>(a);
+    if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
+    else if (n <= 16 * SEL) k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
+    else k_evict_pick<32, false><<<nKv, SEL, 0, c->stream>>>(a);
     TI_LAUNCHED("k_evict_pick");
     // in place, the slots that stay already hold what they held
     const bool placed = mass_out == mass && where_out == where && known >= kept;

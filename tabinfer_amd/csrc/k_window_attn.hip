@@ -182,6 +182,7 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
     };
     // 32 rows a wave leave no registers for a block ahead: their two workgroups a CU load and compute in turn
     constexpr bool AHEAD = RW == 1;
+    constexpr int HN = RW == 1 ? 2 : 1;                    // 32-key parts whose scores are formed together
     if (AHEAD && c0 < c1) load(block_key(c0));
 
     // this lane's rows (past the last: that one again), and what all rows of the wave and any of them see
@@ -222,14 +223,14 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
         if (AHEAD && i + 1 < c1) load(block_key(i + 1));
         TI_ISSUE_FENCE();
 #pragma unroll 1
-        for (int h = 0; h < KB / 32; h++) {                // 32 keys
-            const int k0 = t0 + 32 * h;
+        for (int h = 0; h < KB / 32; h += HN) {            // 32 HN keys
+            const int k0 = t0 + 32 * h, kn = k0 + 32 * HN;
             // wave-uniform: no row of the wave sees any of them
-            if (row0 >= nrows || k0 > last_pos || (k0 + 31 < any_low && k0 >= sinks)) continue;
-            const bool whole = k0 + 31 <= first_pos && (k0 >= all_low || k0 + 32 <= sinks);
-            float s[RW][8];
+            if (row0 >= nrows || k0 > last_pos || (kn <= any_low && k0 >= sinks)) continue;
+            const bool whole = kn - 1 <= first_pos && (k0 >= all_low || kn <= sinks);
+            float s[RW][8 * HN];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < 2 * HN; b++) {
                 v4f acc[RW];
 #pragma unroll
                 for (int r = 0; r < RW; r++) acc[r] = zero;
@@ -253,13 +254,13 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
             uint32_t seen[RW];
 #pragma unroll
             for (int r = 0; r < RW; r++) {
-                seen[r] = 0xffu;
+                seen[r] = ~0u;
                 float tm = -INFINITY;
                 if (!whole) {
                     asm volatile("");                      // a branch: not computed where every key is seen
                     seen[r] = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
+                    for (int e = 0; e < 8 * HN; e++) {
                         const int key = k0 + 16 * (e >> 2) + 4 * j + (e & 3);
                         const bool ok = key <= pos[r] && (key >= low[r] || key < sinks);
                         seen[r] |= ok ? 1u << e : 0u;
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[r][e]);
+                    for (int e = 0; e < 8 * HN; e++) tm = fmaxf(tm, s[r][e]);
                     tm = fmaxf(tm, FLOOR);
                 }
                 tm = fmaxf(tm, ti_xor(tm, 16));
@@ -284,35 +285,38 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
                     mx[r] = mn;
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < 8 * HN; e++) {
                     float p = __builtin_amdgcn_exp2f(fmaf(s[r][e], fr[r], -mx[r]));
                     if (!whole) p = seen[r] >> e & 1u ? p : 0.0f;
                     s[r][e] = p;
                 }
-                l[r] += ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3])) + ((s[r][4] + s[r][5]) + (s[r][6] + s[r][7]));
+#pragma unroll
+                for (int e = 0; e < 8 * HN; e += 8)
+                    l[r] += ((s[r][e] + s[r][e + 1]) + (s[r][e + 2] + s[r][e + 3])) + ((s[r][e + 4] + s[r][e + 5]) + (s[r][e + 6] + s[r][e + 7]));
             }
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * h + 4 * j]);
-                const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * h + 16 + 4 * j]);
+            for (int x = 0; x < HN * NG; x++) {
+                const int hh = x / NG, g = x % NG;
+                const v4f v0 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * (h + hh) + 4 * j]);
+                const v4f v1 = *reinterpret_cast<const v4f*>(&L.vs[g][32 * (h + hh) + 16 + 4 * j]);
                 ti_b8 p[RW][3];
 #pragma unroll
                 for (int r = 0; r < RW; r++) {
                     float w[8];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = s[r][e] * v0[e];
-                        w[4 + e] = s[r][4 + e] * v1[e];
+                        w[e] = s[r][8 * hh + e] * v0[e];
+                        w[4 + e] = s[r][8 * hh + 4 + e] * v1[e];
                     }
                     if (!whole) {                          // the scale of a key that the row does not see may be NaN
 #pragma unroll
-                        for (int e = 0; e < 8; e++) w[e] = seen[r] >> e & 1u ? w[e] : 0.0f;
+                        for (int e = 0; e < 8; e++) w[e] = seen[r] >> (8 * hh + e) & 1u ? w[e] : 0.0f;
                     }
                     ti_bf16x3(w, p[r]);
                 }
 #pragma unroll
                 for (int d = 2 * g; d < 2 * g + 2; d++) {
-                    const ti_b8 vv = L.v[h][d][lane];
+                    const ti_b8 vv = L.v[h + hh][d][lane];
 #pragma unroll
                     for (int r = 0; r < RW; r++)
 #pragma unroll
@@ -378,94 +382,114 @@ __global__ __launch_bounds__(256) void k_window_merge(WinArgs a, int rows) {
     }
 }
 
-// Column sums of the weights: a wave holds 16 keys of a KV head as the MFMA's A operand and passes over the rows, whose operands a
-// workgroup stages 64 at a time; a lane adds up the weights that one row in 16 gives to four keys, in the rows' order.
+// ---- column sums of the weights --------------------------------------------------------------------------
+// The query rows in tiles of 16 as MFMA operands, formed once for all keys: [KV head][tile][hi, lo][group][lane], and of each
+// row its score factor, maximum, 1 / sum and position (rows behind the last: weights of 0)
+struct MassRows {
+    ti_h8* op;
+    float4* row;
+    int tiles;
+};
 template <int HD>
-__global__ __launch_bounds__(256) void k_mass_columns(WinArgs a, float* __restrict__ mass) {
+__global__ __launch_bounds__(256) void k_mass_rows(WinArgs a, MassRows mr) {
     constexpr int NG = HD / 32;
-    __shared__ ti_h8 s_q[4][2][NG][64];                    // [16 rows][hi, lo][group][lane]
-    __shared__ float s_f[64], s_m[64], s_l[64];
+    const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
+    const int u = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= mr.tiles * a.p.nKv) return;                   // wave-uniform
+    const int hk = u / mr.tiles, gr = u % mr.tiles * 16 + m16, nrows = a.G * a.p.T;
+    const int rc = ti_min(gr, nrows - 1), t = rc / a.G;
+    const size_t row = (size_t)t * a.p.nHq + hk * a.G + rc % a.G;
+    v4f_u qv[NG][2];
+    query_load<HD>(a.p.qr + row * HD + 8 * j, qv);
+    const float m = a.p.ml[2 * row], l = a.p.ml[2 * row + 1];
+    ti_h8 qh[NG], ql[NG];
+    const float f = query_operand<HD>(qv, qh, ql);
+    ti_h8* op = mr.op + (size_t)u * 2 * NG * 64 + lane;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        op[g * 64] = qh[g];
+        op[(NG + g) * 64] = ql[g];
+    }
+    if (j == 0)
+        mr.row[(size_t)u * 16 + m16] = gr < nrows ? make_float4(f, m, 1.0f / l, __builtin_bit_cast(float, a.p.pos0 + t))
+                                                  : make_float4(0.0f, 0.0f, 0.0f, __builtin_bit_cast(float, -1));
+}
+
+// A workgroup 32 keys of a KV head, in each wave the same as A operands, and each wave every fourth row tile, the next one's
+// loads in flight; a lane adds up what one row in 16 gives to four keys of each 16, in a fixed order. Bound by the operands'
+// way through L1 (64 bytes a clock): two key tiles a wave halve it.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr, float* __restrict__ mass) {
+    constexpr int NG = HD / 32;
+    __shared__ float s_sum[4][32];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m16 = lane & 15, j = lane >> 4;
     const int hk = blockIdx.x % a.p.nKv;
-    const long kw = (long)(blockIdx.x / a.p.nKv) * 64;     // the workgroup's first key
-    const long k0 = kw + 16 * wave, S = (long)a.p.pos0 + a.p.T;
-    const int nrows = a.G * a.p.T;
-
-    ti_h8 kk[NG];
-    float sc[NG][4];
+    const long k0 = (long)(blockIdx.x / a.p.nKv) * 32, S = (long)a.p.pos0 + a.p.T;
+    // row tiles before the one that holds the first query at or behind the first key see none of the keys
+    const int start = (int)(ti_max(0L, k0 - a.p.pos0) * a.G / 16);
+    const ti_h8* op = mr.op + (size_t)hk * mr.tiles * 2 * NG * 64 + lane;
+    const float4* rows = mr.row + (size_t)hk * mr.tiles * 16 + m16;
+    ti_h8 q[2 * NG], qn[2 * NG];
+    float4 r, rn;
+    auto load = [&](int t) {
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint2 w = *reinterpret_cast<const uint2*>(a.p.kq + ((size_t)ti_min(k0 + m16, S - 1) * a.p.nKv + hk) * HD + 32 * g + 8 * j);
-        kk[g] = ti_i8x8_h8(w.x, w.y);
-#pragma unroll
-        for (int e = 0; e < 4; e++) sc[g][e] = a.p.ks[((size_t)ti_min(k0 + 4 * j + e, S - 1) * a.p.nKv + hk) * NG + g];
-    }
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    // rows before the one of the workgroup's first key see none of its keys
-    const int start = (int)ti_max(0L, kw - a.p.pos0) * a.G / 64 * 64;
-    v4f_u qv[NG][2];
-    float rm, rl;
-    auto load = [&](int r0) {                              // this lane's row of 64, while the ones before are worked on
-        const int gr = ti_min(r0 + 16 * wave + m16, nrows - 1), t = gr / a.G;
-        const size_t row = (size_t)t * a.p.nHq + hk * a.G + gr % a.G;
-        query_load<HD>(a.p.qr + row * HD + 8 * j, qv);
-        rm = a.p.ml[2 * row];
-        rl = a.p.ml[2 * row + 1];
+        for (int x = 0; x < 2 * NG; x++) qn[x] = op[((size_t)t * 2 * NG + x) * 64];
+        rn = rows[(size_t)t * 16];
     };
-    load(start);
-    for (int r0 = start; r0 < nrows; r0 += 64) {
-        __syncthreads();
-        {
-            ti_h8 qh[NG], ql[NG];
-            const float f = query_operand<HD>(qv, qh, ql);
+    int t = start + wave;
+    if (t < mr.tiles) load(t);
+    ti_h8 kk[2][NG];
+    float sc[2][NG][4];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                s_q[wave][0][g][lane] = qh[g];
-                s_q[wave][1][g][lane] = ql[g];
-            }
-            if (j == 0) {
-                s_f[16 * wave + m16] = f;
-                s_m[16 * wave + m16] = rm;
-                s_l[16 * wave + m16] = 1.0f / rl;
-            }
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const uint2 w = *reinterpret_cast<const uint2*>(a.p.kq + ((size_t)ti_min(k0 + 16 * b + m16, S - 1) * a.p.nKv + hk) * HD + 32 * g + 8 * j);
+            kk[b][g] = ti_i8x8_h8(w.x, w.y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sc[b][g][e] = a.p.ks[((size_t)ti_min(k0 + 16 * b + 4 * j + e, S - 1) * a.p.nKv + hk) * NG + g];
         }
-        if (r0 + 64 < nrows) load(r0 + 64);
-        __syncthreads();
-#pragma unroll 1
-        for (int t = 0; t < 4 && r0 + 16 * t < nrows; t++) {
+    float sum[8] = {};
+    for (; t < mr.tiles; t += 4) {
+#pragma unroll
+        for (int x = 0; x < 2 * NG; x++) q[x] = qn[x];
+        r = rn;
+        if (t + 4 < mr.tiles) load(t + 4);
+        const long pos = __builtin_bit_cast(int, r.w);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
             const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
             v4f acc = zero;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g], s_q[t][0][g][lane], zero, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g], s_q[t][1][g][lane], d, 0, 0, 0);
+                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[b][g], q[g], zero, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[b][g], q[NG + g], d, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[g][e], acc[e]);
+                for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[b][g][e], acc[e]);
             }
-            const int rw = 16 * t + m16, gr = r0 + rw;
-            const float f = s_f[rw], m = s_m[rw], inv = s_l[rw];
-            const long pos = gr < nrows ? a.p.pos0 + gr / a.G : -1;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(acc[e], f, -m)) * inv;
-                sum[e] += k0 + 4 * j + e <= pos ? p : 0.0f;
+                const float p = __builtin_amdgcn_exp2f(fmaf(acc[e], r.x, -r.y)) * r.z;
+                sum[4 * b + e] += k0 + 16 * b + 4 * j + e <= pos ? p : 0.0f;
             }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < 8; e++) {
         sum[e] += ti_xor(sum[e], 1);
         sum[e] += ti_xor(sum[e], 2);
         sum[e] += ti_xor(sum[e], 4);
         sum[e] += ti_xor(sum[e], 8);
-        const long key = k0 + 4 * j + e;
-        if (m16 == 0 && key < S) {
-            float* d = mass + (size_t)key * a.p.nKv + hk;
-            *d = key < a.p.pos0 ? *d + sum[e] : sum[e];
-        }
+        if (m16 == 0) s_sum[wave][16 * (e >> 2) + 4 * j + (e & 3)] = sum[e];
     }
+    __syncthreads();
+    const long key = k0 + tid;
+    if (tid >= 32 || key >= S) return;
+    const float all = (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
+    float* d = mass + (size_t)key * a.p.nKv + hk;
+    *d = key < a.p.pos0 ? *d + all : all;
 }
 
 template <int HD>
@@ -502,7 +526,16 @@ template <int HD>
 int launch_mass(ti_ctx* c, const TiWindowAttn& p, float* mass) {
     const WinArgs a = {p, nullptr, nullptr, p.nHq / p.nKv, 0, 0};
     const long S = (long)p.pos0 + p.T;
-    k_mass_columns<HD><<<(unsigned)((S + 63) / 64 * p.nKv), 256, 0, c->stream>>>(a, mass);
+    // the operands in the partials' scratch, which the launches before have done with: each row 4 HD bytes of operand and 16 of
+    // its own, padded to whole tiles a KV head
+    static_assert((TI_ATTN_ROWS_MAX + 16 * TI_ATTN_HEADS_MAX) * (4L * TI_ATTN_HD_MAX + 16) <= 4L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX,
+                  "the rows' operands fit the scratch");
+    const int tiles = (a.G * p.T + 15) / 16;
+    ti_h8* op = reinterpret_cast<ti_h8*>(c->attn_po);
+    const MassRows mr = {op, reinterpret_cast<float4*>(op + (size_t)p.nKv * tiles * 2 * (HD / 32) * 64), tiles};
+    k_mass_rows<HD><<<(unsigned)((tiles * p.nKv + 3) / 4), 256, 0, c->stream>>>(a, mr);
+    TI_LAUNCHED("k_mass_rows");
+    k_mass_columns<HD><<<(unsigned)((S + 31) / 32 * p.nKv), 256, 0, c->stream>>>(a, mr, mass);
     TI_LAUNCHED("k_mass_columns");
     return TI_OK;
 }
