@@ -502,7 +502,7 @@ int ti_attn_window_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
  * pos[t] of sequence seq[t] (seq NULL: row t is sequence t, T <= B). A row whose place does not exist (pos < 0 or
  * past the table, seq outside [0, B), a page id outside [0, pages)) is not written. Rows of one call name different
  * places; of rows that name the same one, which codes and which scales stay is not specified. table NULL: the
- * positions are the rows of a contiguous cache of page * pages positions, seq and B are not looked at. */
+ * positions are the rows of a contiguous cache of page * pages positions, seq and B are not looked at. nKv <= 64. */
 int ti_kv_write_paged_q8(ti_ctx* ctx, const float* kr, const float* v, uint32_t* kq, float* ks,
                          uint32_t* vq, float* vs, const int32_t* table, const int32_t* seq,
                          const int32_t* pos, int T, int B, int nKv, int hd, int page, int pages, int width);
@@ -524,7 +524,8 @@ int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const flo
 /* ti_attn_causal_q8 that also adds up the attention each key receives: mass[j*nKv + h] += the softmax weights of key j
  * summed over the T queries and the nHq/nKv query heads of KV head h. The slots pos0 .. pos0+T-1, the call's own
  * tokens, are set instead (no earlier query saw them), so a mass buffer needs no clearing. pos0 is a slot of the
- * cache: after an eviction, the next free one. T * nHq <= 4096, nHq <= 64, nHq * (pos0 + T) <= 2^24 for T = 1; out must not overlap qr. */
+ * cache: after an eviction, the next free one. T * nHq <= 4096, nHq <= 64; for T = 1, nHq times pos0 + 1 rounded
+ * up to 32 is at most 2^24; out must not overlap qr. */
 int ti_attn_mass_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
                     const uint32_t* vq, const float* vs, float* out, float* mass,
                     int T, int pos0, int nHq, int nKv, int hd);

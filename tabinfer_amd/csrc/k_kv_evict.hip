@@ -5,10 +5,11 @@
 // i-th into the i-th: no slot is both read and written, so the moves run in any order, a cache that frees one slot moves one
 // row, and what stays below `keep` stays where it is.
 //
-// Bound by its launches and by the select's chain of barriers, not by bytes: 4097 slots of 8 heads to 4096 17.2 + 4.0 us
-// (select, moves), 16384 to 4096 3.0 + 22.2 + 5.6 us, where the moved rows' 13 MB are 2.7 us of a copy. A workgroup a head
-// and not more: the select's steps depend on one another, and counts across workgroups would cost a launch a digit (about
-// 5 us each). 1024 threads: 512 took 20.1 and 28.1 us, 256 29.3 and 54.3 (more keys a thread, behind one another).
+// Bound by its launches and by the select's chain of barriers, not by bytes: 4097 slots of 8 heads to 4096 8.6 + 2.9 us
+// (the one slot, the move and the bookkeeping), 16384 to 4096 2.7 + 19.2 + 5.9 us (keys, select, moves), where the moved
+// rows' 13 MB are 2.7 us of a copy. A workgroup a head and not more: the select's steps depend on one another, and counts
+// across workgroups would cost a launch a digit (about 5 us each). 1024 threads: for the two selections above 512 threads
+// took 20.1 and 28.1 us where 1024 took 17.2 and 22.2, and 256 took 29.3 and 54.3 (more keys a thread, one behind another).
 #include "ti_dev.h"
 #include "ti_span.h"
 
@@ -72,25 +73,27 @@ __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
 
 // A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 32 every key stays in a register, more slots
 // go through in chunks, read again for each digit. The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
-// up from the top, and only the keys with the digits so far go on. Lanes of a wave that all have one digit count as one, so
+// up from the top, and only the keys with the digits so far go on; done as soon
+// as all of these are kept (16384 slots of 8 heads to 4096: 22 us, all three digits' passes, to 20). Lanes of a wave that all have one digit count as one, so
 // that equal masses do not queue for their bin.
 constexpr int BINS = 2048;
 template <int KPT>
 struct SelLds {
     uint32_t hist[BINS];
-    uint32_t digit, need;
+    uint32_t digit, need, all;             // the bin that holds the keep-th key, its rank in it, the bin's count
     int part[KPT * (SEL / 64)], tot[SEL / 64];
 };
 
 // sum over the threads before this one
 __device__ __forceinline__ int thread_scan(int v, int* tot) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        x += lane >= o ? y : 0;
-    }
+    int x = v;                                             // rows of 16 lanes, then the rows before
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
     if (lane == 63) tot[wave] = x;
     __syncthreads();
     int before = 0;
@@ -116,6 +119,53 @@ __device__ __forceinline__ int part_scan(SelLds<KPT>& L) {
     return sum;
 }
 
+// the keys of slots i0 + 1024 k + tid, every load in flight at once; 0 behind the last slot
+template <int KPT>
+__device__ __forceinline__ void form_keys(const EvictArgs& a, int h, int i0, uint32_t (&key)[KPT]) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
+    int at[KPT];
+#pragma unroll
+    for (int k = 0; k < KPT; k++) at[k] = a.known ? a.where[(size_t)ti_min(i0 + k * SEL + tid, a.known - 1) * a.nKv + h] : 0;
+#pragma unroll
+    for (int k = 0; k < KPT; k++) {
+        const int i = i0 + k * SEL + tid;
+        if (i >= a.known) at[k] = a.next - (a.n - i);
+        key[k] = i < a.n ? order_key(a, at[k], __builtin_bit_cast(float, key[k])) : 0u;
+    }
+}
+
+// One slot too many, a bounded cache's every token: the last slot of the smallest key, by a minimum in place of the select
+// (4097 slots of 8 heads: 8.6 us, the select 17.2)
+__global__ __launch_bounds__(SEL) void k_evict_one(EvictArgs a) {
+    constexpr int KPT = FORMED / SEL;
+    __shared__ uint64_t s_best[SEL / 64];
+    const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x;
+    uint64_t best = ~0ull;                                 // (key, slots behind it)
+    for (int i0 = 0; i0 < a.n; i0 += KPT * SEL) {
+        uint32_t key[KPT];
+        form_keys(a, h, i0, key);
+#pragma unroll
+        for (int k = 0; k < KPT; k++) {
+            const int i = i0 + k * SEL + tid;
+            if (i < a.n) best = ti_min(best, (uint64_t)key[k] << 32 | (uint32_t)(a.n - 1 - i));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) best = ti_min(best, (uint64_t)__shfl_xor((unsigned long long)best, o));
+    if (lane == 0) s_best[tid >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SEL / 64; w++) best = ti_min(best, s_best[w]);
+    const int out = a.n - 1 - (int)(uint32_t)best;
+    for (int w = tid; w < a.words; w += SEL) a.stays[(size_t)h * a.words + w] = ~(out / 64 == w ? 1ull << (out & 63) : 0ull);
+    if (tid > 0) return;
+    a.count[h] = out < a.keep;
+    a.moves[2 * h] = a.keep;                               // the one slot behind them, and room for one move a head
+    a.moves[2 * h + 1] = out;
+}
+
 template <int KPT, bool FORM>
 __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     constexpr int W = SEL / 64;
@@ -126,17 +176,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     uint32_t key[KPT];                                     // 0 behind the last slot
     auto load = [&](int i0) {
         if constexpr (FORM) {
-#pragma unroll
-            for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
-            int at[KPT];                                   // every load in flight at once
-#pragma unroll
-            for (int k = 0; k < KPT; k++) at[k] = a.known ? a.where[(size_t)ti_min(i0 + k * SEL + tid, a.known - 1) * a.nKv + h] : 0;
-#pragma unroll
-            for (int k = 0; k < KPT; k++) {
-                const int i = i0 + k * SEL + tid;
-                if (i >= a.known) at[k] = a.next - (a.n - i);
-                key[k] = i < a.n ? order_key(a, at[k], __builtin_bit_cast(float, key[k])) : 0u;
-            }
+            form_keys(a, h, i0, key);
         } else {                                           // k_evict_keys formed them
 #pragma unroll
             for (int k = 0; k < KPT; k++) key[k] = a.keys[(size_t)h * a.n + ti_min(i0 + k * SEL + tid, a.n - 1)];
@@ -147,11 +187,13 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     constexpr int CHUNK = KPT * SEL;
     const bool one = a.n <= CHUNK;
     if (one) load(0);
-    uint32_t top = 0;                                      // the keep-th largest key, its digits so far
+    uint32_t top = 0;                                      // the keep-th largest key, its digits so far (from bit `shift` up)
+    int shift = 0;
     int need = a.keep;                                     // which of the keys with those digits, from the largest
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const int bits = pass == 2 ? 10 : 11;
         L.hist[tid] = 0;
         L.hist[tid + SEL] = 0;
         __syncthreads();
@@ -180,18 +222,20 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
             const bool second = need > before + h0;
             L.digit = (uint32_t)(BINS - 1 - 2 * tid - (second ? 1 : 0));
             L.need = (uint32_t)(need - before - (second ? h0 : 0));
+            L.all = (uint32_t)(second ? h1 : h0);
         }
         __syncthreads();
         top = top << bits | L.digit;
         need = (int)L.need;
+        if (L.need == L.all) break;                        // every key with these digits is kept: the other digits do not matter
     }
-    // kept: the keys above it, and of those equal to it the first `need` slots
+    // kept: the keys above those digits, and of those equal in them the first `need` slots
     const uint64_t below = (1ull << lane) - 1;
     int32_t* mv = a.moves + (size_t)h * a.room * 2;
     int ties = 0, holes = 0, tails = 0;                    // of the chunks before
     for (int i0 = 0; i0 < a.n; i0 += CHUNK) {
         if (!one) load(i0);
-        auto is_tie = [&](int k) { return key[k] == top && i0 + k * SEL + tid < a.n; };
+        auto is_tie = [&](int k) { return key[k] >> shift == top && i0 + k * SEL + tid < a.n; };
 #pragma unroll
         for (int k = 0; k < KPT; k++) {
             const uint64_t b = __ballot(is_tie(k));
@@ -203,7 +247,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
         for (int k = 0; k < KPT; k++) {
             const uint64_t b = __ballot(is_tie(k));
             const int rank = ties + L.part[k * W + wave] + __popcll(b & below);
-            const bool st = key[k] > top || (is_tie(k) && rank < need);
+            const bool st = key[k] >> shift > top || (is_tie(k) && rank < need);
             kept |= st ? 1u << k : 0u;
             const uint64_t stays = __ballot(st);           // for the launch that follows
             const int w0 = i0 + k * SEL + 64 * wave;
@@ -277,7 +321,7 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     const int room = kept < n - kept ? kept : n - kept;      // moves of a head, at most
     const int words = (kept + 63) / 64;
     // scratch: the slots that stay, the moves' counts, the moves, the keys of many slots
-    const bool many = n > FORMED;
+    const bool single = n - kept == 1, many = n > FORMED && !single;
     const long need = 2L * nKv * words + nKv + 2L * nKv * room + (many ? (long)nKv * n : 0);
     TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch", n, room);
     uint64_t* stays = reinterpret_cast<uint64_t*>(c->attn_po);
@@ -295,7 +339,8 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
         k_evict_keys<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_evict_keys");
     }
-    if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
+    if (single) k_evict_one<<<nKv, SEL, 0, c->stream>>>(a);
+    else if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
     else if (n <= 16 * SEL) k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
     else k_evict_pick<32, false><<<nKv, SEL, 0, c->stream>>>(a);
     TI_LAUNCHED("k_evict_pick");

@@ -100,8 +100,8 @@ dim3 word_grid(const PlaceArgs& a) { return dim3((unsigned)(((long)a.T * a.rowg 
 
 int place_args(PlaceArgs& a, const char* fn, const int32_t* table, const int32_t* seq, const int32_t* pos, int T, int B,
                int nKv, int hd, int page, int pages, int width) {
-    TI_REQUIRE(T > 0 && B > 0 && nKv > 0 && hd > 0 && hd % 32 == 0 && hd <= TI_ATTN_HD_MAX, "%s: bad shape (T=%d B=%d nKv=%d hd=%d)", fn,
-               T, B, nKv, hd);
+    TI_REQUIRE(T > 0 && (B > 0 || table == nullptr) && nKv > 0 && nKv <= TI_ATTN_HEADS_MAX && hd > 0 && hd % 32 == 0 && hd <= TI_ATTN_HD_MAX,
+               "%s: bad shape (T=%d B=%d nKv=%d hd=%d)", fn, T, B, nKv, hd);
     TI_REQUIRE(ti_pow2(page) && pages > 0, "%s: the page length must be a power of two (%d), the pool not empty (%d)", fn, page, pages);
     TI_REQUIRE(table == nullptr || width > 0, "%s: a table of width %d", fn, width);
     TI_REQUIRE((long)page * (table ? width : pages) <= 0x7fffffffL, "%s: %d pages of %d hold more than 2^31 - 1 positions", fn,
@@ -109,7 +109,7 @@ int place_args(PlaceArgs& a, const char* fn, const int32_t* table, const int32_t
     TI_REQUIRE(seq || table == nullptr || T <= B, "%s: %d rows without sequence numbers, %d sequences", fn, T, B);
     TI_REQUIRE((long)T * nKv * (hd / 32) <= 0x3fffffffL, "%s: %d rows of %d heads in one call", fn, T, nKv);
     a.pg = TiPages{table, ti_log2(page), pages, width};
-    a.seq = seq;
+    a.seq = table ? seq : nullptr;
     a.pos = pos;
     a.T = T;
     a.B = B;

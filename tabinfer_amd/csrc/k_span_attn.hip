@@ -1,6 +1,5 @@
 // k_span_attn.hip — the entry points of the attention over a part of the int8 KV cache: under a sliding window with sinks, over
-// pages, and with the weight that each key receives added up. Up to 16 query rows a KV head (and single tokens) take
-// k_token_attn.hip, more k_window_attn.hip. See ti_span.h for the visible keys and their rows.
+// pages, and with the weight that each key receives added up. See ti_span.h for the visible keys and their rows.
 #include "ti_dev.h"
 #include "ti_span.h"
 #include "ti_token_attn.h"
@@ -9,6 +8,11 @@
 namespace {
 
 constexpr long MASS_SCORES = 1L << 24;       // (query head, slot) scores of a one-token call
+
+// Single tokens and up to 8 query rows a KV head take k_token_attn.hip, more k_window_attn.hip. Tokens x query heads of 16
+// and 8 KV heads of 128 dims over 2000 keys, the two kernels with their merges: 4 tokens (8 rows) 13.9 / 15.6 us, 8 tokens
+// (16 rows) 16.5 / 15.9, over 16000 keys 30.9 / 27.4
+bool few_rows(int T, int G) { return T == 1 || T * G <= 8; }
 
 // thread = one (slot, KV head) of a one-token call: the weights that its G heads gave the slot, from their scores
 __global__ __launch_bounds__(256) void k_token_mass(const float* __restrict__ scores, long sstride, const float* __restrict__ ml,
@@ -41,7 +45,7 @@ extern "C" int ti_attn_window_q8(ti_ctx* c, const float* qr, const uint32_t* kq,
     if (rc) return rc;
     TI_REQUIRE(pos0 >= 0 && pos0 <= TI_POS_END - T && sinks >= 0, "ti_attn_window_q8: bad positions (T=%d pos0=%d sinks=%d)", T, pos0, sinks);
     TI_REQUIRE((long)T * nHq <= 0x7fffffffL / 256, "ti_attn_window_q8: %d x %d query rows in one call", T, nHq);
-    if (T == 1 || T * (nHq / nKv) <= 16) {
+    if (few_rows(T, nHq / nKv)) {
         const long keys = window < 0 ? (long)pos0 + T : ti_min((long)pos0 + T, (long)window + sinks + T);
         const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
                                TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, keys, nullptr, 0, nullptr};
@@ -84,7 +88,7 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
     float* ml = c->act_s;
     const uint8_t *k8 = reinterpret_cast<const uint8_t*>(kq), *v8 = reinterpret_cast<const uint8_t*>(vq);
     const TiWindowAttn p = {qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0, ml};
-    if (T == 1 || T * (nHq / nKv) <= 16) {
+    if (few_rows(T, nHq / nKv)) {
         // one token's scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one)
         TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, -1, 0, (long)pos0 + T, nullptr, 0, ml};
         if (T == 1) {

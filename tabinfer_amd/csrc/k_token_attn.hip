@@ -7,9 +7,9 @@
 //    KV head: each has the same work whatever the lengths, a run that ends one sequence begins the next, and its part of
 //    a sequence is a partial in slot (workgroup + sequence). Every workgroup finds its run by a scan over the lengths;
 //    nothing depends on them on the host.
-//  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 12 waves a CU cover each other's loads (16 have too few
-//    registers: 57 us for 32 ragged sequences against 49).
-//    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-25 of
+//  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 12 waves a CU cover each other's
+//    loads (16 have too few registers: 57 us for 32 ragged sequences against 49).
+//    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-22 of
 //    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
 //    P times the V scale of (key, group) in f32, as three bf16, exactly; V through the transposing LDS read.
@@ -236,322 +236,322 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
     uint32_t po[PF];
     auto l_key = [&](int p) { return (lane + 64 * p) / PC; };
     auto l_byte = [&](int p) { return 16 * piece_slot<HD>(l_key(p), (lane + 64 * p) % PC); };
-    auto s_key = [&](int p) { return lane % BLK; };
+    const int s_key = lane % BLK;
     auto s_grp = [&](int p) { return ti_min(2 * p + lane / BLK, NG - 1); };
 #pragma unroll
     for (int p = 0; p < PF; p++) po[p] = (uint32_t)(l_key(p) * a.p.nKv) * HD + l_byte(p);
-    const uint32_t so = 4 * ((uint32_t)(s_key(0) * a.p.nKv) * NG + s_grp(0));
+    const uint32_t so = 4 * ((uint32_t)(s_key * a.p.nKv) * NG + s_grp(0));
     const int far = 64 / PC * PF * a.p.nKv * HD;
 
-  for (;;) {
-    // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
-    const int last = seq_last<PAGED>(a, run.b);
-    const TiSpan span = seq_span<PAGED>(a, last);
-    Blocks bl = blocks_of(span);
-    if (last < 0) bl.n = 0;
-    const int nb = ti_max(1, bl.n);
-    const int c0 = run.block, part = (int)ti_min((long)(nb - c0), run.left), c1 = ti_min(bl.n, c0 + part);
-    const int pos = last - (a.p.T - 1) + t;
-    const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
-    // what every row of the tile sees: [full_low, full_end)
-    const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
-    // the query's loads before the keys': they come back first
-    v4f_u qv[NQ][2];
-    const int qc = j + 4 * (slot / 2);                     // COLS: the lane's 16 dims of the 64 that its column's group is in
-    auto q_dim = [&](int x) { return COLS ? 16 * ti_min(qc, PC - 1) + 8 * x : 32 * x + 8 * j; };
-    {
-        const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD;
+    for (;;) {
+        // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
+        const int last = seq_last<PAGED>(a, run.b);
+        const TiSpan span = seq_span<PAGED>(a, last);
+        Blocks bl = blocks_of(span);
+        if (last < 0) bl.n = 0;
+        const int nb = ti_max(1, bl.n);
+        const int c0 = run.block, part = (int)ti_min((long)(nb - c0), run.left), c1 = ti_min(bl.n, c0 + part);
+        const int pos = last - (a.p.T - 1) + t;
+        const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
+        // what every row of the tile sees: [full_low, full_end)
+        const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
+        // the query's loads before the keys': they come back first
+        v4f_u qv[NQ][2];
+        const int qc = j + 4 * (slot / 2);                     // COLS: the lane's 16 dims of the 64 that its column's group is in
+        auto q_dim = [&](int x) { return COLS ? 16 * ti_min(qc, PC - 1) + 8 * x : 32 * x + 8 * j; };
+        {
+            const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD;
 #pragma unroll
-        for (int x = 0; x < NQ; x++)
+            for (int x = 0; x < NQ; x++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) qv[x][u] = *reinterpret_cast<const v4f_u*>(q + q_dim(x) + 4 * u);
-    }
+                for (int u = 0; u < 2; u++) qv[x][u] = *reinterpret_cast<const v4f_u*>(q + q_dim(x) + 4 * u);
+        }
 
-    // ---- a block's loads, straight to the wave's LDS
-    // the table's entry for key k0 + lane % 32 of block i; and, once it is there, the page of that key: -1 where no row sees
-    // the key or there is no such page. Apart, so that nothing waits where the entry is asked for
-    auto fetch_page = [&](int i) -> int {
-        if constexpr (!PAGED) return 0;
-        const int k = ti_min((bl.at(i) * BLK + (lane & 31)) >> a.p.pg.shift, a.p.pg.width - 1);
-        return a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
-    };
-    auto check_page = [&](int i, int id) -> int {
-        const int key = bl.at(i) * BLK + (lane & 31);
-        const bool in = key < span.end && (key >= span.low || key < span.first);
-        if constexpr (!PAGED) return in ? 0 : -1;
-        return in && (key >> a.p.pg.shift) < a.p.pg.width && id >= 0 && id < a.p.pg.pages ? id : -1;
-    };
-    // rows of one page, or of the contiguous cache, follow each other: one base and the lanes' fixed offsets
-    const bool runs = !PAGED || a.p.pg.shift >= 5;
-    // the first row of block i
-    auto base_row = [&](int i, int page) -> size_t {
-        const int k0 = bl.at(i) * BLK;
-        if constexpr (!PAGED) return (size_t)k0;
-        // the id of any of the block's keys that is seen (the others carry -1); page 0 where there is none
-        const uint64_t some = __ballot(page >= 0);
-        const int id = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
-        return ((size_t)(uint32_t)id << a.p.pg.shift) + (k0 & ((1 << a.p.pg.shift) - 1));
-    };
-    auto in_run = [&](int i) { return runs && (PAGED || bl.at(i) * BLK + BLK <= span.end); };
-    auto row_of = [&](int k0, int kl, int page) -> size_t {            // a row that exists where the key does not
-        if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
-        const int id = ti_max(__shfl(page, kl), 0);
-        return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
-    };
-    auto& W = L.w[wave];
-    auto load = [&](int i, int page) {
-        const int k0 = bl.at(i) * BLK;
-        if (in_run(i)) {
-            // scalar bases and the lanes' 32-bit offsets
-            const size_t row = base_row(i, page) * a.p.nKv + hk;
-            const int codes = BLK * a.p.nKv * HD, scales = BLK * a.p.nKv * NG * 4;
-            const __amdgpu_buffer_rsrc_t rk = resource(a.p.kq + row * HD, codes), rv = resource(a.p.vq + row * HD, codes);
-            const __amdgpu_buffer_rsrc_t rks = resource(a.p.ks + row * NG, scales), rvs = resource(a.p.vs + row * NG, scales);
+        // ---- a block's loads, straight to the wave's LDS
+        // the table's entry for key k0 + lane % 32 of block i; and, once it is there, the page of that key: -1 where no row sees
+        // the key or there is no such page. Apart, so that nothing waits where the entry is asked for
+        auto fetch_page = [&](int i) -> int {
+            if constexpr (!PAGED) return 0;
+            const int k = ti_min((bl.at(i) * BLK + (lane & 31)) >> a.p.pg.shift, a.p.pg.width - 1);
+            return a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
+        };
+        auto check_page = [&](int i, int id) -> int {
+            const int key = bl.at(i) * BLK + (lane & 31);
+            const bool in = key < span.end && (key >= span.low || key < span.first);
+            if constexpr (!PAGED) return in ? 0 : -1;
+            return in && (key >> a.p.pg.shift) < a.p.pg.width && id >= 0 && id < a.p.pg.pages ? id : -1;
+        };
+        // rows of one page, or of the contiguous cache, follow each other: one base and the lanes' fixed offsets
+        const bool runs = !PAGED || a.p.pg.shift >= 5;
+        // the first row of block i
+        auto base_row = [&](int i, int page) -> size_t {
+            const int k0 = bl.at(i) * BLK;
+            if constexpr (!PAGED) return (size_t)k0;
+            // the id of any of the block's keys that is seen (the others carry -1); page 0 where there is none
+            const uint64_t some = __ballot(page >= 0);
+            const int id = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
+            return ((size_t)(uint32_t)id << a.p.pg.shift) + (k0 & ((1 << a.p.pg.shift) - 1));
+        };
+        auto in_run = [&](int i) { return runs && (PAGED || bl.at(i) * BLK + BLK <= span.end); };
+        auto row_of = [&](int k0, int kl, int page) -> size_t {            // a row that exists where the key does not
+            if constexpr (!PAGED) return (size_t)ti_min(k0 + kl, span.end - 1);
+            const int id = ti_max(__shfl(page, kl), 0);
+            return ((size_t)id << a.p.pg.shift) + ((k0 + kl) & ((1 << a.p.pg.shift) - 1));
+        };
+        auto& W = L.w[wave];
+        auto load = [&](int i, int page) {
+            const int k0 = bl.at(i) * BLK;
+            if (in_run(i)) {
+                // scalar bases and the lanes' 32-bit offsets
+                const size_t row = base_row(i, page) * a.p.nKv + hk;
+                const int codes = BLK * a.p.nKv * HD, scales = BLK * a.p.nKv * NG * 4;
+                const __amdgpu_buffer_rsrc_t rk = resource(a.p.kq + row * HD, codes), rv = resource(a.p.vq + row * HD, codes);
+                const __amdgpu_buffer_rsrc_t rks = resource(a.p.ks + row * NG, scales), rvs = resource(a.p.vs + row * NG, scales);
+#pragma unroll
+                for (int p = 0; p < NL; p++) {
+                    run_to_lds16(rk, &W.k[1024 * p], po[p % PF], p / PF * far);
+                    run_to_lds16(rv, &W.v[1024 * p], po[p % PF], p / PF * far);
+                }
+#pragma unroll
+                for (int p = 0; p < SL; p++) {
+                    const uint32_t o = so + 4 * (s_grp(p) - s_grp(0));
+                    run_to_lds4(rks, &W.ks[64 * p], o);
+                    run_to_lds4(rvs, &W.vs[64 * p], o);
+                }
+                return;
+            }
 #pragma unroll
             for (int p = 0; p < NL; p++) {
-                run_to_lds16(rk, &W.k[1024 * p], po[p % PF], p / PF * far);
-                run_to_lds16(rv, &W.v[1024 * p], po[p % PF], p / PF * far);
+                const size_t off = (row_of(k0, l_key(p), page) * a.p.nKv + hk) * HD + l_byte(p);
+                to_lds16(a.p.kq + off, &W.k[1024 * p]);
+                to_lds16(a.p.vq + off, &W.v[1024 * p]);
             }
 #pragma unroll
             for (int p = 0; p < SL; p++) {
-                const uint32_t o = so + 4 * (s_grp(p) - s_grp(0));
-                run_to_lds4(rks, &W.ks[64 * p], o);
-                run_to_lds4(rvs, &W.vs[64 * p], o);
+                const size_t off = (row_of(k0, s_key, page) * a.p.nKv + hk) * NG + s_grp(p);
+                to_lds4(a.p.ks + off, &W.ks[64 * p]);
+                to_lds4(a.p.vs + off, &W.vs[64 * p]);
             }
-            return;
-        }
-#pragma unroll
-        for (int p = 0; p < NL; p++) {
-            const size_t off = (row_of(k0, l_key(p), page) * a.p.nKv + hk) * HD + l_byte(p);
-            to_lds16(a.p.kq + off, &W.k[1024 * p]);
-            to_lds16(a.p.vq + off, &W.v[1024 * p]);
-        }
-#pragma unroll
-        for (int p = 0; p < SL; p++) {
-            const size_t off = (row_of(k0, s_key(p), page) * a.p.nKv + hk) * NG + s_grp(p);
-            to_lds4(a.p.ks + off, &W.ks[64 * p]);
-            to_lds4(a.p.vs + off, &W.vs[64 * p]);
-        }
-    };
+        };
 
-    int i = c0 + bw;
-    int page = -1, entry = 0;
-    if (i < c1) {
-        page = check_page(i, fetch_page(i));
-        if (i + a.BW < c1) entry = fetch_page(i + a.BW);
-        load(i, page);
-    }
-    TI_ISSUE_FENCE();
+        int i = c0 + bw;
+        int page = -1, entry = 0;
+        if (i < c1) {
+            page = check_page(i, fetch_page(i));
+            if (i + a.BW < c1) entry = fetch_page(i + a.BW);
+            load(i, page);
+        }
+        TI_ISSUE_FENCE();
 
-    // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: dims 16 j.. of 64, those of other groups than the column's
-    // as zeros), scaled by 2^k so that the row's largest element is below 16
-    ti_h8 qh[NQ], ql[NQ];
-    float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
-    {
-        float mx = 0.0f;
+        // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: dims 16 j.. of 64, those of other groups than the column's
+        // as zeros), scaled by 2^k so that the row's largest element is below 16
+        ti_h8 qh[NQ], ql[NQ];
+        float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
+        {
+            float mx = 0.0f;
 #pragma unroll
-        for (int x = 0; x < NQ; x++)
+            for (int x = 0; x < NQ; x++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[x][e / 4][e % 4]));
-        mx = fmaxf(mx, ti_xor(mx, 16));
-        mx = fmaxf(mx, ti_xor(mx, 32));
-        if (COLS && NU == 2) mx = fmaxf(mx, ti_xor(mx, 8));            // the row's other 64 dims
-        int ex = 4;
-        if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
-        const int k = ti_min(4 - ex, 100);
-        const float up = ldexpf(1.0f, k);
-        fr = fr * ldexpf(1.0f, -k);
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[x][e / 4][e % 4]));
+            mx = fmaxf(mx, ti_xor(mx, 16));
+            mx = fmaxf(mx, ti_xor(mx, 32));
+            if (COLS && NU == 2) mx = fmaxf(mx, ti_xor(mx, 8));            // the row's other 64 dims
+            int ex = 4;
+            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+            const int k = ti_min(4 - ex, 100);
+            const float up = ldexpf(1.0f, k);
+            fr = fr * ldexpf(1.0f, -k);
 #pragma unroll
-        for (int x = 0; x < NQ; x++) {
-            const bool mine = !COLS || (qc < PC && qc / 2 == slot);
+            for (int x = 0; x < NQ; x++) {
+                const bool mine = !COLS || (qc < PC && qc / 2 == slot);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float v = mine ? qv[x][e / 4][e % 4] * up : 0.0f;
+                    const _Float16 hi = (_Float16)v;
+                    qh[x][e] = hi;
+                    ql[x][e] = (_Float16)(v - (float)hi);
+                }
+            }
+        }
+
+        v4f o[HD / 16];
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[d] = zero;
+        float m = -INFINITY, l = 0.0f;
+
+        for (; i < c1; i += a.BW) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): the block is there
+            ti_wave_lds_fence();
+            const int k0 = bl.at(i) * BLK;
+            const uint32_t there = (uint32_t)__ballot(page >= 0);
+
+            float s[8];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                v4f acc = zero;
+                if constexpr (COLS) {
+#pragma unroll
+                    for (int u = 0; u < NU; u++) {
+                        const int key = 16 * b + r16;
+                        const uint4 kw = *reinterpret_cast<const uint4*>(&W.k[key * HD + 16 * piece_slot<HD>(key, ti_min(j + 4 * u, PC - 1))]);
+                        const ti_h8 k0f = ti_i8x8_h8(kw.x, kw.y), k1f = ti_i8x8_h8(kw.z, kw.w);
+                        v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, qh[0], zero, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, ql[0], d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, qh[1], d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, ql[1], d, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[e] = u == 0 || slot / 2 == u ? d[e] : acc[e];
+                    }
+                    const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * grp + 16 * b + 4 * j]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[e] = slot_sum<SLOTS>(acc[e] * sc[e]);
+                } else
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const int key = 16 * b + r16;
+                    const uint2 kw = *reinterpret_cast<const uint2*>(&W.k[key * HD + 16 * piece_slot<HD>(key, 2 * g + j / 2) + 8 * (j & 1)]);
+                    const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
+                    const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * g + 16 * b + 4 * j]);
+                    v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e];
+            }
+            // which of the lane's keys its row sees
+            uint32_t seen = 0xffu;
+            const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
+            if (!whole) {                                      // wave-uniform
+                asm volatile("");                              // a branch: not computed where every key is seen
+                seen = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int kl = 16 * (e >> 2) + 4 * j + (e & 3), key = k0 + kl;
+                    const bool ok = ((there >> kl) & 1u) & (key <= pos) & ((key >= low) | (key < a.p.sinks));
+                    seen |= ok ? 1u << e : 0u;
+                }
+            }
+            if (a.p.scores && slot == 0 && rt * ROWS + tr < a.R) {
+                float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
+                *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
+                *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
+            }
+            float tm = FLOOR;
+            if (!whole) {
+                tm = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen >> e & 1u ? fmaxf(s[e], FLOOR) : -INFINITY);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[e]);
+            }
+            tm = fmaxf(tm, ti_xor(tm, 16));
+            tm = fmaxf(tm, ti_xor(tm, 32));
+            tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;       // in log2 units from here on
+            // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
+            const bool bump = tm > m + 6.0f;
+            if (__any(bump)) {
+                const float mn = bump ? tm : m;
+                const float alpha = bump ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                l = l * alpha;
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) o[d] = o[d] * alpha;
+                m = mn;
+            }
+            float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = mine ? qv[x][e / 4][e % 4] * up : 0.0f;
-                const _Float16 hi = (_Float16)v;
-                qh[x][e] = hi;
-                ql[x][e] = (_Float16)(v - (float)hi);
+                float p = __builtin_amdgcn_exp2f(fmaf(s[e], fr, -m));
+                if (!whole) p = seen >> e & 1u ? p : 0.0f;
+                sum += p;
+                s[e] = p * PSCALE;
             }
-        }
-    }
-
-    v4f o[HD / 16];
-#pragma unroll
-    for (int d = 0; d < HD / 16; d++) o[d] = zero;
-    float m = -INFINITY, l = 0.0f;
-
-    for (; i < c1; i += a.BW) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): the block is there
-        ti_wave_lds_fence();
-        const int k0 = bl.at(i) * BLK;
-        const uint32_t there = (uint32_t)__ballot(page >= 0);
-
-        float s[8];
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            v4f acc = zero;
-            if constexpr (COLS) {
-#pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    const int key = 16 * b + r16;
-                    const uint4 kw = *reinterpret_cast<const uint4*>(&W.k[key * HD + 16 * piece_slot<HD>(key, ti_min(j + 4 * u, PC - 1))]);
-                    const ti_h8 k0f = ti_i8x8_h8(kw.x, kw.y), k1f = ti_i8x8_h8(kw.z, kw.w);
-                    v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, qh[0], zero, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0f, ql[0], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, qh[1], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1f, ql[1], d, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[e] = u == 0 || slot / 2 == u ? d[e] : acc[e];
-                }
-                const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * grp + 16 * b + 4 * j]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[e] = slot_sum<SLOTS>(acc[e] * sc[e]);
-            } else
+            l += sum;
+            ti_b8 pb[3];
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const int key = 16 * b + r16;
-                const uint2 kw = *reinterpret_cast<const uint2*>(&W.k[key * HD + 16 * piece_slot<HD>(key, 2 * g + j / 2) + 8 * (j & 1)]);
-                const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
-                const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * g + 16 * b + 4 * j]);
-                v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
+                if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for three waves a SIMD
+                if (!COLS || g == 0) {
+                    const v4f v0 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 4 * j]);
+                    const v4f v1 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 16 + 4 * j]);
+                    float x[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
-            }
+                    for (int e = 0; e < 4; e++) {
+                        x[e] = s[e] * v0[e];
+                        x[4 + e] = s[4 + e] * v1[e];
+                    }
+                    if (!whole) {                              // the scale of a key that the row does not see may be NaN
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e];
-        }
-        // which of the lane's keys its row sees
-        uint32_t seen = 0xffu;
-        const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
-        if (!whole) {                                      // wave-uniform
-            asm volatile("");                              // a branch: not computed where every key is seen
-            seen = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int kl = 16 * (e >> 2) + 4 * j + (e & 3), key = k0 + kl;
-                const bool ok = ((there >> kl) & 1u) && key <= pos && (key >= low || key < a.p.sinks);
-                seen |= ok ? 1u << e : 0u;
-            }
-        }
-        if (a.p.scores && slot == 0 && rt * ROWS + tr < a.R) {
-            float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
-            *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
-            *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
-        }
-        float tm = FLOOR;
-        if (!whole) {
-            tm = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen >> e & 1u ? fmaxf(s[e], FLOOR) : -INFINITY);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[e]);
-        }
-        tm = fmaxf(tm, ti_xor(tm, 16));
-        tm = fmaxf(tm, ti_xor(tm, 32));
-        tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;       // in log2 units from here on
-        // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
-        const bool bump = tm > m + 6.0f;
-        if (__any(bump)) {
-            const float mn = bump ? tm : m;
-            const float alpha = bump ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-            l = l * alpha;
-#pragma unroll
-            for (int d = 0; d < HD / 16; d++) o[d] = o[d] * alpha;
-            m = mn;
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[e], fr, -m));
-            if (!whole) p = seen >> e & 1u ? p : 0.0f;
-            sum += p;
-            s[e] = p * PSCALE;
-        }
-        l += sum;
-        ti_b8 pb[3];
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for three waves a SIMD
-            if (!COLS || g == 0) {
-                const v4f v0 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 4 * j]);
-                const v4f v1 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 16 + 4 * j]);
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[e] = s[e] * v0[e];
-                    x[4 + e] = s[4 + e] * v1[e];
+                        for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
+                    }
+                    ti_bf16x3(x, pb);
                 }
-                if (!whole) {                              // the scale of a key that the row does not see may be NaN
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
+                for (int d = 2 * g; d < 2 * g + 2; d++) {      // COLS: of these 16 dims, the columns of group g hold the output
+                    const v2i vb = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (__attribute__((address_space(3))) v2i*)&W.v[vrow * HD + 16 * piece_slot<HD>(vrow, d) + 8 * (r16 & 1)]);
+                    const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
+                    const ti_b8 vv = __builtin_bit_cast(ti_b8, make_uint4(lo.x, lo.y, hi.x, hi.y));
+#pragma unroll
+                    for (int e = 2; e >= 0; e--) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[e], o[d], 0, 0, 0);
                 }
-                ti_bf16x3(x, pb);
             }
-#pragma unroll
-            for (int d = 2 * g; d < 2 * g + 2; d++) {      // COLS: of these 16 dims, the columns of group g hold the output
-                const v2i vb = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) v2i*)&W.v[vrow * HD + 16 * piece_slot<HD>(vrow, d) + 8 * (r16 & 1)]);
-                const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
-                const ti_b8 vv = __builtin_bit_cast(ti_b8, make_uint4(lo.x, lo.y, hi.x, hi.y));
-#pragma unroll
-                for (int e = 2; e >= 0; e--) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[e], o[d], 0, 0, 0);
+            // the next block into the place of this one, which has been read
+            if (i + a.BW < c1) {
+                ti_wave_lds_fence();
+                __builtin_amdgcn_s_waitcnt(0xC07F);            // lgkmcnt(0)
+                page = check_page(i + a.BW, entry);
+                if (i + 2 * a.BW < c1) entry = fetch_page(i + 2 * a.BW);
+                load(i + a.BW, page);
             }
         }
-        // the next block into the place of this one, which has been read
-        if (i + a.BW < c1) {
-            ti_wave_lds_fence();
-            __builtin_amdgcn_s_waitcnt(0xC07F);            // lgkmcnt(0)
-            page = check_page(i + a.BW, entry);
-            if (i + 2 * a.BW < c1) entry = fetch_page(i + 2 * a.BW);
-            load(i + a.BW, page);
-        }
-    }
 
-    // ---- the waves' parts into the workgroup's partial
-    l += ti_xor(l, 16);
-    l += ti_xor(l, 32);
-    __syncthreads();                                       // the tiles are read
-    if (j == 0 && slot == 0) {
-        L.m[wave][tr] = m;
-        L.l[wave][tr] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < HD / 16; d++)
-        if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
-    __syncthreads();
-    const int nr = ti_min(ROWS, a.R - rt * ROWS);
-    for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
-        const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, r = q % nr;
-        float M = L.m[hh][r];
-        for (int k = hh + a.HW; k < WAVES; k += a.HW) M = fmaxf(M, L.m[k][r]);
-        v4f x = zero;
-        float y = 0.0f;
-        for (int k = hh; k < WAVES; k += a.HW) {
-            const float mk = L.m[k][r], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
-            const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][r][4 * d]);
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
-            y = fmaf(L.l[k][r], f, y);
+        // ---- the waves' parts into the workgroup's partial
+        l += ti_xor(l, 16);
+        l += ti_xor(l, 32);
+        __syncthreads();                                       // the tiles are read
+        if (j == 0 && slot == 0) {
+            L.m[wave][tr] = m;
+            L.l[wave][tr] = l;
         }
-        const size_t at = ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
-        *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
-        if (d == 0) {
-            a.pml[2 * at] = M;
-            a.pml[2 * at + 1] = y;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++)
+            if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
+        __syncthreads();
+        const int nr = ti_min(ROWS, a.R - rt * ROWS);
+        for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
+            const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, r = q % nr;
+            float M = L.m[hh][r];
+            for (int k = hh + a.HW; k < WAVES; k += a.HW) M = fmaxf(M, L.m[k][r]);
+            v4f x = zero;
+            float y = 0.0f;
+            for (int k = hh; k < WAVES; k += a.HW) {
+                const float mk = L.m[k][r], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+                const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][r][4 * d]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
+                y = fmaf(L.l[k][r], f, y);
+            }
+            const size_t at = ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
+            *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
+            if (d == 0) {
+                a.pml[2 * at] = M;
+                a.pml[2 * at + 1] = y;
+            }
         }
+        if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
+            a.meta[2 * run.b] = w + run.b;
+            a.meta[2 * run.b + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
+        }
+        run.left -= part;
+        if (run.left <= 0) return;
+        run.b++;
+        run.start += nb;
+        run.block = 0;
+        __syncthreads();                                   // the parts are read
     }
-    if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
-        a.meta[2 * run.b] = w + run.b;
-        a.meta[2 * run.b + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
-    }
-    run.left -= part;
-    if (run.left <= 0) return;
-    run.b++;
-    run.start += nb;
-    run.block = 0;
-    __syncthreads();                                       // the parts are read
-  }
 }
 
 // A workgroup a (sequence, token, head) and DW of its dims: the slots' partials into the output row, each group of threads

@@ -6,7 +6,7 @@
 // (K codes f16, V codes bf16, exact), the next block's loads in flight meanwhile; a wave passes over the 32 keys that none of its
 // rows sees and masks only where an edge of the window cuts them.
 //   - S^T = K Q^T (v_mfma_f32_16x16x32_f16 per 32-dim group, q half and 16 keys; the row scaled by a power of two, q =
-//     hi + lo to 2^-25 of its largest element), each group's sum times its key's scale in f32.
+//     hi + lo to 2^-22 of its largest element), each group's sum times its key's scale in f32.
 //   - O^T = V^T P^T with P times the V scale of (key, group) in f32 as three bf16, exactly; a lane's scores are the
 //     operand as they stand.
 #include "ti_dev.h"
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
 #pragma unroll
                     for (int e = 0; e < 8 * HN; e++) {
                         const int key = k0 + 16 * (e >> 2) + 4 * j + (e & 3);
-                        const bool ok = key <= pos[r] && (key >= low[r] || key < sinks);
+                        const bool ok = (key <= pos[r]) & ((key >= low[r]) | (key < sinks));
                         seen[r] |= ok ? 1u << e : 0u;
                         tm = fmaxf(tm, ok ? fmaxf(s[r][e], FLOOR) : -INFINITY);
                     }
@@ -385,6 +385,7 @@ __global__ __launch_bounds__(256) void k_window_merge(WinArgs a, int rows) {
 // ---- column sums of the weights --------------------------------------------------------------------------
 // The query rows in tiles of 16 as MFMA operands, formed once for all keys: [KV head][tile][hi, lo][group][lane], and of each
 // row its score factor, maximum, 1 / sum and position (rows behind the last: weights of 0)
+constexpr int MASS_GRID = 4096;              // 32-key parts a grid row: a grid's side holds less than 2^32 threads
 struct MassRows {
     ti_h8* op;
     float4* row;
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr,
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m16 = lane & 15, j = lane >> 4;
     const int hk = blockIdx.x % a.p.nKv;
-    const long k0 = (long)(blockIdx.x / a.p.nKv) * 32, S = (long)a.p.pos0 + a.p.T;
+    const long k0 = ((long)blockIdx.y * MASS_GRID + blockIdx.x / a.p.nKv) * 32, S = (long)a.p.pos0 + a.p.T;
     // row tiles before the one that holds the first query at or behind the first key see none of the keys
     const int start = (int)(ti_max(0L, k0 - a.p.pos0) * a.G / 16);
     const ti_h8* op = mr.op + (size_t)hk * mr.tiles * 2 * NG * 64 + lane;
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr,
     }
     __syncthreads();
     const long key = k0 + tid;
-    if (tid >= 32 || key >= S) return;
+    if (tid >= 32 || key >= S) return;                     // S: also behind the last key of the last grid row
     const float all = (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
     float* d = mass + (size_t)key * a.p.nKv + hk;
     *d = key < a.p.pos0 ? *d + all : all;
@@ -535,7 +536,9 @@ int launch_mass(ti_ctx* c, const TiWindowAttn& p, float* mass) {
     const MassRows mr = {op, reinterpret_cast<float4*>(op + (size_t)p.nKv * tiles * 2 * (HD / 32) * 64), tiles};
     k_mass_rows<HD><<<(unsigned)((tiles * p.nKv + 3) / 4), 256, 0, c->stream>>>(a, mr);
     TI_LAUNCHED("k_mass_rows");
-    k_mass_columns<HD><<<(unsigned)((S + 31) / 32 * p.nKv), 256, 0, c->stream>>>(a, mr, mass);
+    const long kb = (S + 31) / 32;
+    const dim3 grid((unsigned)(ti_min(kb, (long)MASS_GRID) * p.nKv), (unsigned)((kb + MASS_GRID - 1) / MASS_GRID));
+    k_mass_columns<HD><<<grid, 256, 0, c->stream>>>(a, mr, mass);
     TI_LAUNCHED("k_mass_columns");
     return TI_OK;
 }
