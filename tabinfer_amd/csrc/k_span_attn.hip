@@ -52,7 +52,7 @@ extern "C" int ti_attn_window_q8(ti_ctx* c, const float* qr, const uint32_t* kq,
         return ti_token_attn_launch(c, p, hd);
     }
     const TiWindowAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
-                            T, pos0, nHq, nKv, window, sinks, nullptr};
+                            T, pos0, nHq, nKv, window, sinks};
     return ti_window_attn_launch(c, p, hd);
 }
 
@@ -83,26 +83,17 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
     TI_REQUIRE((long)T * nHq <= TI_ATTN_ROWS_MAX, "ti_attn_mass_q8: T*nHq = %ld > %d", (long)T * nHq, TI_ATTN_ROWS_MAX);
     TI_REQUIRE(T > 1 || (long)nHq * ((pos0 + 32L) / 32 * 32) <= MASS_SCORES, "ti_attn_mass_q8: %d heads over %d slots exceed the scratch (%ld scores)",
                nHq, pos0 + 1, MASS_SCORES);
-    // each row's (max, sum) between the launches, in the quantizers' scratch
-    static_assert(2 * TI_ATTN_ROWS_MAX <= TI_ACT_CAP / 32 * TI_ACT_TMAX, "the rows' (max, sum) fit the scratch");
-    float* ml = c->act_s;
     const uint8_t *k8 = reinterpret_cast<const uint8_t*>(kq), *v8 = reinterpret_cast<const uint8_t*>(vq);
-    const TiWindowAttn p = {qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0, ml};
-    if (few_rows(T, nHq / nKv)) {
-        // one token's scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one)
-        TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, -1, 0, (long)pos0 + T, nullptr, 0, ml};
-        if (T == 1) {
-            t.scores = c->attn_po + MASS_SCORES;
-            t.sstride = (pos0 + 32L) / 32 * 32;
-        }
-        const int rc1 = ti_token_attn_launch(c, t, hd);
-        if (rc1) return rc1;
-        if (T > 1) return ti_mass_columns_launch(c, p, hd, mass);
-        const long n = (pos0 + 1L) * nKv;
-        k_token_mass<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(t.scores, t.sstride, ml, mass, pos0, nHq, nKv);
-        TI_LAUNCHED("k_token_mass");
-        return TI_OK;
-    }
-    const int rw = ti_window_attn_launch(c, p, hd);
-    return rw ? rw : ti_mass_columns_launch(c, p, hd, mass);
+    if (T > 1) return ti_mass_attn_launch(c, TiWindowAttn{qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0}, hd, mass);
+    // one token's scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one), each
+    // head's (max, sum) to the quantizers' scratch
+    static_assert(2 * TI_ATTN_HEADS_MAX <= TI_ACT_CAP / 32 * TI_ACT_TMAX, "the heads' (max, sum) fit the scratch");
+    float *ml = c->act_s, *scores = c->attn_po + MASS_SCORES;
+    const long sstride = (pos0 + 32L) / 32 * 32, n = (pos0 + 1L) * nKv;
+    const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, scores, sstride, ml};
+    const int rc1 = ti_token_attn_launch(c, t, hd);
+    if (rc1) return rc1;
+    k_token_mass<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(scores, sstride, ml, mass, pos0, nHq, nKv);
+    TI_LAUNCHED("k_token_mass");
+    return TI_OK;
 }

@@ -28,6 +28,7 @@ struct WinArgs {
     float* po;                               // [row][nsplit][HD] partials, (m, l) of each; nsplit = 1: none
     float* pml;
     int G, nblk, nsplit;
+    TiMassRows mr;
 };
 
 // The query row of this lane, its dims 32 g + 8 j..; as MFMA operands, and the factor that scales its scores to log2 units
@@ -62,6 +63,13 @@ __device__ __forceinline__ float query_operand(const v4f_u (&qv)[HD / 32][2], ti
             ql[g][e] = (_Float16)(v - (float)hi);
         }
     return 1.44269504088896341f / (127.0f * sqrtf((float)HD)) * ldexpf(1.0f, -k);
+}
+
+// what became of row gr of KV head hk, for the columns' sums
+__device__ __forceinline__ void mass_row(const WinArgs& a, int hk, int gr, float m, float l) {
+    float* rec = reinterpret_cast<float*>(a.mr.row + (size_t)hk * a.mr.tiles * 16 + gr);
+    rec[1] = m;
+    rec[2] = 1.0f / l;
 }
 
 // 4 x 4 bytes: in, w[r] = row r's four bytes; out, w[e] = byte e of rows 0..3
@@ -200,6 +208,22 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
         v4f_u qv[NG][2];
         query_load<HD>(a.p.qr + orow[r] * HD + 8 * j, qv);
         fr[r] = query_operand<HD>(qv, qh[r], ql[r]);
+        if (RW == 1 && a.mr.op && split == 0 && row0 < 16 * a.mr.tiles) {
+            const size_t u = (size_t)hk * a.mr.tiles + row0 / 16;
+            ti_h8* op = a.mr.op + u * 2 * NG * 64 + lane;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                op[g * 64] = qh[r][g];
+                op[(NG + g) * 64] = ql[r][g];
+            }
+            const bool in = row0 + m16 < nrows;
+            float* rec = reinterpret_cast<float*>(a.mr.row + u * 16 + m16);
+            if (j == 0) {
+                rec[0] = in ? fr[r] : 0.0f;
+                rec[3] = __builtin_bit_cast(float, in ? pos[r] : -1);
+                if (!in) rec[1] = rec[2] = 0.0f;           // the others': at the end, or in the merge
+            }
+        }
     }
     const int first_pos = pos0 + ti_min(row0, nrows - 1) / a.G, last_pos = pos0 + ti_min(row0 + 16 * RW - 1, nrows - 1) / a.G;
     const int any_low = low_of(first_pos), all_low = low_of(last_pos);
@@ -336,11 +360,12 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
         float* dst = direct ? a.p.out + orow[r] * HD : a.po + (orow[r] * a.nsplit + split) * HD;
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) *reinterpret_cast<v4f_u*>(dst + 16 * d + 4 * j) = o[r][d] * f;
-        float* ml = direct ? a.p.ml ? a.p.ml + 2 * orow[r] : nullptr : a.pml + 2 * (orow[r] * a.nsplit + split);
-        if (j == 0 && ml) {
+        if (j == 0 && !direct) {
+            float* ml = a.pml + 2 * (orow[r] * a.nsplit + split);
             ml[0] = mx[r];
             ml[1] = lt;
         }
+        if (j == 0 && direct && a.mr.op) mass_row(a, hk, row0 + 16 * r + m16, mx[r], lt);
     }
 }
 
@@ -376,62 +401,33 @@ __global__ __launch_bounds__(256) void k_window_merge(WinArgs a, int rows) {
         out[0] = M == -INFINITY ? 0.0f : v0 / div;
         out[1] = M == -INFINITY ? 0.0f : v1 / div;
     }
-    if (a.p.ml && lane == 0) {
-        a.p.ml[2 * row] = M;
-        a.p.ml[2 * row + 1] = Lt;
+    if (a.mr.op && lane == 0) {
+        const int hq = row % a.p.nHq;
+        mass_row(a, hq / a.G, row / a.p.nHq * a.G + hq % a.G, M, Lt);
     }
 }
 
 // ---- column sums of the weights --------------------------------------------------------------------------
-// The query rows in tiles of 16 as MFMA operands, formed once for all keys: [KV head][tile][hi, lo][group][lane], and of each
-// row its score factor, maximum, 1 / sum and position (rows behind the last: weights of 0)
-constexpr int MASS_GRID = 4096;              // 32-key parts a grid row: a grid's side holds less than 2^32 threads
-struct MassRows {
-    ti_h8* op;
-    float4* row;
-    int tiles;
-};
-template <int HD>
-__global__ __launch_bounds__(256) void k_mass_rows(WinArgs a, MassRows mr) {
-    constexpr int NG = HD / 32;
-    const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
-    const int u = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= mr.tiles * a.p.nKv) return;                   // wave-uniform
-    const int hk = u / mr.tiles, gr = u % mr.tiles * 16 + m16, nrows = a.G * a.p.T;
-    const int rc = ti_min(gr, nrows - 1), t = rc / a.G;
-    const size_t row = (size_t)t * a.p.nHq + hk * a.G + rc % a.G;
-    v4f_u qv[NG][2];
-    query_load<HD>(a.p.qr + row * HD + 8 * j, qv);
-    const float m = a.p.ml[2 * row], l = a.p.ml[2 * row + 1];
-    ti_h8 qh[NG], ql[NG];
-    const float f = query_operand<HD>(qv, qh, ql);
-    ti_h8* op = mr.op + (size_t)u * 2 * NG * 64 + lane;
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        op[g * 64] = qh[g];
-        op[(NG + g) * 64] = ql[g];
-    }
-    if (j == 0)
-        mr.row[(size_t)u * 16 + m16] = gr < nrows ? make_float4(f, m, 1.0f / l, __builtin_bit_cast(float, a.p.pos0 + t))
-                                                  : make_float4(0.0f, 0.0f, 0.0f, __builtin_bit_cast(float, -1));
-}
+constexpr int KT = 2;                        // 16-key tiles of a workgroup
+constexpr int MASS_GRID = 4096;              // key parts a grid row: a grid's side holds less than 2^32 threads
 
-// A workgroup 32 keys of a KV head, in each wave the same as A operands, and each wave every fourth row tile, the next one's
-// loads in flight; a lane adds up what one row in 16 gives to four keys of each 16, in a fixed order. Bound by the operands'
-// way through L1 (64 bytes a clock): two key tiles a wave halve it.
+// A workgroup 16 KT keys of a KV head, in each wave the same as A operands, and each wave every fourth row tile, the next
+// one's loads in flight; a lane adds up what one row in 16 gives to four keys of each 16, in a fixed order. Bound by the
+// operands' way out of L2 and by each wave's start, its keys' operands and scales (256 rows of 16 heads over 2048 keys of 8:
+// 11.8 us; with 3 and 4 key tiles, too few workgroups, 14.7 and 17.0)
 template <int HD>
-__global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr, float* __restrict__ mass) {
+__global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, float* __restrict__ mass) {
     constexpr int NG = HD / 32;
-    __shared__ float s_sum[4][32];
+    __shared__ float s_sum[4][16 * KT];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m16 = lane & 15, j = lane >> 4;
-    const int hk = blockIdx.x % a.p.nKv;
-    const long k0 = ((long)blockIdx.y * MASS_GRID + blockIdx.x / a.p.nKv) * 32, S = (long)a.p.pos0 + a.p.T;
+    const int hk = blockIdx.x % a.p.nKv, tiles = a.mr.tiles;
+    const long k0 = ((long)blockIdx.y * MASS_GRID + blockIdx.x / a.p.nKv) * 16 * KT, S = (long)a.p.pos0 + a.p.T;
     // row tiles before the one that holds the first query at or behind the first key see none of the keys
     const int start = (int)(ti_max(0L, k0 - a.p.pos0) * a.G / 16);
-    const ti_h8* op = mr.op + (size_t)hk * mr.tiles * 2 * NG * 64 + lane;
-    const float4* rows = mr.row + (size_t)hk * mr.tiles * 16 + m16;
+    const ti_h8* op = a.mr.op + (size_t)hk * tiles * 2 * NG * 64 + lane;
+    const float4* rows = a.mr.row + (size_t)hk * tiles * 16 + m16;
     ti_h8 q[2 * NG], qn[2 * NG];
     float4 r, rn;
     auto load = [&](int t) {
@@ -440,27 +436,33 @@ __global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr,
         rn = rows[(size_t)t * 16];
     };
     int t = start + wave;
-    if (t < mr.tiles) load(t);
-    ti_h8 kk[2][NG];
-    float sc[2][NG][4];
+    if (t < tiles) load(t);
+    ti_h8 kk[KT][NG];
+    float sc[KT][NG][4];
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+    for (int b = 0; b < KT; b++) {
+        const uint8_t* kr = a.p.kq + ((size_t)ti_min(k0 + 16 * b + m16, S - 1) * a.p.nKv + hk) * HD + 8 * j;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const uint2 w = *reinterpret_cast<const uint2*>(a.p.kq + ((size_t)ti_min(k0 + 16 * b + m16, S - 1) * a.p.nKv + hk) * HD + 32 * g + 8 * j);
+            const uint2 w = *reinterpret_cast<const uint2*>(kr + 32 * g);
             kk[b][g] = ti_i8x8_h8(w.x, w.y);
-#pragma unroll
-            for (int e = 0; e < 4; e++) sc[b][g][e] = a.p.ks[((size_t)ti_min(k0 + 16 * b + 4 * j + e, S - 1) * a.p.nKv + hk) * NG + g];
         }
-    float sum[8] = {};
-    for (; t < mr.tiles; t += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float* sr = a.p.ks + ((size_t)ti_min(k0 + 16 * b + 4 * j + e, S - 1) * a.p.nKv + hk) * NG;
+#pragma unroll
+            for (int g = 0; g < NG; g++) sc[b][g][e] = sr[g];
+        }
+    }
+    float sum[4 * KT] = {};
+    for (; t < tiles; t += 4) {
 #pragma unroll
         for (int x = 0; x < 2 * NG; x++) q[x] = qn[x];
         r = rn;
-        if (t + 4 < mr.tiles) load(t + 4);
+        if (t + 4 < tiles) load(t + 4);
         const long pos = __builtin_bit_cast(int, r.w);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < KT; b++) {
             const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
             v4f acc = zero;
 #pragma unroll
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr,
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < 4 * KT; e++) {
         sum[e] += ti_xor(sum[e], 1);
         sum[e] += ti_xor(sum[e], 2);
         sum[e] += ti_xor(sum[e], 4);
@@ -487,30 +489,31 @@ __global__ __launch_bounds__(256, 2) void k_mass_columns(WinArgs a, MassRows mr,
     }
     __syncthreads();
     const long key = k0 + tid;
-    if (tid >= 32 || key >= S) return;                     // S: also behind the last key of the last grid row
+    if (tid >= 16 * KT || key >= S) return;                // k0 too may lie behind the last key, in the last grid row
     const float all = (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
     float* d = mass + (size_t)key * a.p.nKv + hk;
     *d = key < a.p.pos0 ? *d + all : all;
 }
 
 template <int HD>
-int launch(ti_ctx* c, const TiWindowAttn& p) {
+int launch(ti_ctx* c, const TiWindowAttn& p, const TiMassRows& mr, long slots) {
     const int G = p.nHq / p.nKv, nrows = G * p.T;
     // keys that 64 rows see, at most, in blocks
     const int tokens = (63 + G) / G + 1;
     const long keys = p.window < 0 ? (long)p.pos0 + p.T : ti_min((long)p.pos0 + p.T, (long)p.window + p.sinks + tokens);
     const long kb = keys / KB + 3;
-    // 32 rows a wave where that still gives every CU its workgroups
-    const bool two = (long)p.nKv * ((nrows + 127) / 128) >= c->cus;
+    // 32 rows a wave where that still gives every CU its workgroups (4096 tokens of 16 heads: 159 us, 16 rows 169); columns'
+    // sums, of few rows, take 16
+    const bool two = !mr.op && (long)p.nKv * ((nrows + 127) / 128) >= c->cus;
     const int rows = two ? 128 : 64, nblk = (nrows + rows - 1) / rows;
     const long wg = (long)p.nKv * nblk;
     long ns = (2L * c->cus + wg - 1) / wg;
     if (two) ns = 1;
     if (ns > kb / 2) ns = kb / 2;
     if (ns > 64) ns = 64;
-    if (ns * p.T * p.nHq > TI_ATTN_ROWSPLITS) ns = TI_ATTN_ROWSPLITS / ((long)p.T * p.nHq);
+    ns = ti_min(ns, slots / ((long)p.T * p.nHq));
     if (ns < 1) ns = 1;
-    const WinArgs a = {p, c->attn_po, c->attn_ml, G, nblk, (int)ns};
+    const WinArgs a = {p, c->attn_po, c->attn_ml, G, nblk, (int)ns, mr};
     const unsigned grid = (unsigned)(wg * ns);
     if (two) k_window_attn<HD, 2><<<grid, 256, 0, c->stream>>>(a);
     else k_window_attn<HD, 1><<<grid, 256, 0, c->stream>>>(a);
@@ -523,22 +526,21 @@ int launch(ti_ctx* c, const TiWindowAttn& p) {
     return TI_OK;
 }
 
+// Attention that leaves the rows' operands behind, in the upper half of the partials' scratch, and the columns' sums
 template <int HD>
 int launch_mass(ti_ctx* c, const TiWindowAttn& p, float* mass) {
-    const WinArgs a = {p, nullptr, nullptr, p.nHq / p.nKv, 0, 0};
-    const long S = (long)p.pos0 + p.T;
-    // the operands in the partials' scratch, which the launches before have done with: each row 4 HD bytes of operand and 16 of
-    // its own, padded to whole tiles a KV head
-    static_assert((TI_ATTN_ROWS_MAX + 16 * TI_ATTN_HEADS_MAX) * (4L * TI_ATTN_HD_MAX + 16) <= 4L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX,
-                  "the rows' operands fit the scratch");
-    const int tiles = (a.G * p.T + 15) / 16;
-    ti_h8* op = reinterpret_cast<ti_h8*>(c->attn_po);
-    const MassRows mr = {op, reinterpret_cast<float4*>(op + (size_t)p.nKv * tiles * 2 * (HD / 32) * 64), tiles};
-    k_mass_rows<HD><<<(unsigned)((tiles * p.nKv + 3) / 4), 256, 0, c->stream>>>(a, mr);
-    TI_LAUNCHED("k_mass_rows");
-    const long kb = (S + 31) / 32;
+    // each row 4 HD bytes of operand and 16 of its own, padded to whole tiles a KV head
+    static_assert((TI_ATTN_ROWS_MAX + 15 * TI_ATTN_HEADS_MAX) * (4L * TI_ATTN_HD_MAX + 16) <= 2L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX,
+                  "the rows' operands fit half of the scratch");
+    const int G = p.nHq / p.nKv, tiles = (G * p.T + 15) / 16;
+    ti_h8* op = reinterpret_cast<ti_h8*>(c->attn_po + TI_ATTN_ROWSPLITS / 2 * (size_t)TI_ATTN_HD_MAX);
+    const TiMassRows mr = {op, reinterpret_cast<float4*>(op + (size_t)p.nKv * tiles * 2 * (HD / 32) * 64), tiles};
+    const int rc = launch<HD>(c, p, mr, TI_ATTN_ROWSPLITS / 2);
+    if (rc) return rc;
+    const WinArgs a = {p, nullptr, nullptr, G, 0, 0, mr};
+    const long kb = ((long)p.pos0 + p.T + 16 * KT - 1) / (16 * KT);
     const dim3 grid((unsigned)(ti_min(kb, (long)MASS_GRID) * p.nKv), (unsigned)((kb + MASS_GRID - 1) / MASS_GRID));
-    k_mass_columns<HD><<<grid, 256, 0, c->stream>>>(a, mr, mass);
+    k_mass_columns<HD><<<grid, 256, 0, c->stream>>>(a, mass);
     TI_LAUNCHED("k_mass_columns");
     return TI_OK;
 }
@@ -546,9 +548,12 @@ int launch_mass(ti_ctx* c, const TiWindowAttn& p, float* mass) {
 }  // namespace
 
 int ti_window_attn_launch(ti_ctx* c, const TiWindowAttn& p, int hd) {
-    return hd == 128 ? launch<128>(c, p) : hd == 96 ? launch<96>(c, p) : hd == 64 ? launch<64>(c, p) : launch<32>(c, p);
+    const TiMassRows none = {nullptr, nullptr, 0};
+    const long slots = TI_ATTN_ROWSPLITS;
+    return hd == 128 ? launch<128>(c, p, none, slots) : hd == 96 ? launch<96>(c, p, none, slots)
+         : hd == 64 ? launch<64>(c, p, none, slots) : launch<32>(c, p, none, slots);
 }
-int ti_mass_columns_launch(ti_ctx* c, const TiWindowAttn& p, int hd, float* mass) {
+int ti_mass_attn_launch(ti_ctx* c, const TiWindowAttn& p, int hd, float* mass) {
     return hd == 128 ? launch_mass<128>(c, p, mass) : hd == 96 ? launch_mass<96>(c, p, mass)
          : hd == 64 ? launch_mass<64>(c, p, mass) : launch_mass<32>(c, p, mass);
 }

@@ -2,6 +2,14 @@
 #pragma once
 #include "ti_internal.h"
 
+// What the columns' sums of a call's weights need of its query rows, in tiles of 16 rows of a KV head: the MFMA operands
+// [KV head][tile][hi, lo][group][lane] and of each row its score factor, maximum in log2, 1 / sum and position (rows behind
+// the last: weights of 0). op = nullptr: not kept
+struct TiMassRows {
+    ti_h8* op;
+    float4* row;
+    int tiles;
+};
 struct TiWindowAttn {
     const float* qr;                         // [T][nHq][hd], query t at position pos0 + t
     const uint8_t* kq;
@@ -10,8 +18,7 @@ struct TiWindowAttn {
     const float* vs;
     float* out;
     int T, pos0, nHq, nKv, window, sinks;
-    float* ml;                               // [T nHq][2] (max in log2, sum) of each row, or nullptr
 };
 int ti_window_attn_launch(ti_ctx* c, const TiWindowAttn& p, int hd);
-// mass[j nKv + h] (+)= the weights of key j over the rows, given each row's (max, sum) in p.ml; causal
-int ti_mass_columns_launch(ti_ctx* c, const TiWindowAttn& p, int hd, float* mass);
+// causal attention, and mass[j nKv + h] (+)= the weights of key j over the rows; T nHq <= TI_ATTN_ROWS_MAX
+int ti_mass_attn_launch(ti_ctx* c, const TiWindowAttn& p, int hd, float* mass);
