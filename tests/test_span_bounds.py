@@ -107,3 +107,24 @@ def test_page_rows_against_brute_force(host):
             assert host.page_row(None, page, pages, 0, 0, pos) == (pos if 0 <= pos < pages * page else -1)
     big = np.array([2 ** 20], np.int32)               # a pool of more than 2^31 positions: the row number is 64-bit
     assert host.page_row(big.ctypes.data_as(C.c_void_p), 4096, 2 ** 21, 1, 0, 5) == 2 ** 32 + 5
+
+
+@pytest.mark.parametrize("name,heads", [("ti_kv_write_paged_q8", 11), ("ti_kv_read_paged_q8", 11)])
+def test_paged_rows_of_too_many_heads_are_refused(name, heads):
+    ctx = C.addressof(C.create_string_buffer(1 << 16))
+    for n in (65, 2 ** 27, IMAX):                       # 2^27 heads of 64: their product passes 32 bits
+        args = list(WRITE)
+        args[9], args[heads] = 1, n
+        assert getattr(abi.lib(), name)(ctx, *args) == abi.TI_ERR_INVALID, n
+        assert name.encode() in abi.lib().ti_last_error(), n
+
+
+def test_blocks_loaded_into_a_waves_lds_are_fenced():
+    """k_token_attn.hip: a wave's block is waited for and fenced before it is read, its reads are waited for and fenced
+    before the next block's loads overwrite it."""
+    src = open(os.path.join(ROOT, "tabinfer_amd", "csrc", "k_token_attn.hip")).read()
+    i = src.index("for (; i < c1; i += a.BW) {")
+    read, nxt = src.index("W.k[", i), src.index("load(i + a.BW, page);", i)
+    assert "s_waitcnt(0x0F70)" in src[i:read] and "ti_wave_lds_fence();" in src[i:read]
+    last = src.rindex("W.v[", i, nxt)
+    assert "s_waitcnt(0xC07F)" in src[last:nxt] and "ti_wave_lds_fence();" in src[last:nxt]
