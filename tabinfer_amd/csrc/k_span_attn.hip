@@ -14,17 +14,6 @@ constexpr long MASS_SCORES = 1L << 24;       // (query head, slot) scores of a o
 // (16 rows) 16.5 / 15.9, over 16000 keys 30.9 / 27.4
 bool few_rows(int T, int G) { return T == 1 || T * G <= 8; }
 
-// thread = one (slot, KV head) of a one-token call: the weights that its G heads gave the slot, from their scores
-__global__ __launch_bounds__(256) void k_token_mass(const float* __restrict__ scores, long sstride, const float* __restrict__ ml,
-                                                    float* __restrict__ mass, int pos0, int nHq, int nKv) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (pos0 + 1L) * nKv) return;
-    const int j = (int)(i / nKv), hk = (int)(i % nKv), G = nHq / nKv;
-    float sum = 0.0f;
-    for (int h = hk * G; h < (hk + 1) * G; h++) sum += __builtin_amdgcn_exp2f(scores[h * sstride + j] - ml[2 * h]) / ml[2 * h + 1];
-    mass[i] = j < pos0 ? mass[i] + sum : sum;
-}
-
 int check_attn(const char* fn, const void* qr, const void* kq, const void* ks, const void* vq, const void* vs, const void* out,
                int n, int nHq, int nKv, int hd) {
     TI_REQUIRE(qr && kq && ks && vq && vs && out, "%s: null buffer", fn);
@@ -48,7 +37,7 @@ extern "C" int ti_attn_window_q8(ti_ctx* c, const float* qr, const uint32_t* kq,
     if (few_rows(T, nHq / nKv)) {
         const long keys = window < 0 ? (long)pos0 + T : ti_min((long)pos0 + T, (long)window + sinks + T);
         const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
-                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, keys, nullptr, 0, nullptr};
+                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, keys, nullptr, nullptr, 0};
         return ti_token_attn_launch(c, p, hd);
     }
     const TiWindowAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
@@ -69,7 +58,7 @@ extern "C" int ti_attn_paged_q8(ti_ctx* c, const float* qr, const uint32_t* kq, 
     TI_REQUIRE(sinks >= 0, "ti_attn_paged_q8: sinks = %d", sinks);
     const long all = (long)page * width, keys = window < 0 ? all : ti_min(all, (long)window + sinks + 1);
     const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
-                           TiPages{table, ti_log2(page), pages, width}, lens, B, 1, 0, nHq, nKv, window, sinks, keys, nullptr, 0, nullptr};
+                           TiPages{table, ti_log2(page), pages, width}, lens, B, 1, 0, nHq, nKv, window, sinks, keys, nullptr, nullptr, 0};
     return ti_token_attn_launch(c, p, hd);
 }
 
@@ -85,15 +74,8 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
                nHq, pos0 + 1, MASS_SCORES);
     const uint8_t *k8 = reinterpret_cast<const uint8_t*>(kq), *v8 = reinterpret_cast<const uint8_t*>(vq);
     if (T > 1) return ti_mass_attn_launch(c, TiWindowAttn{qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0}, hd, mass);
-    // one token's scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one), each
-    // head's (max, sum) to the quantizers' scratch
-    static_assert(2 * TI_ATTN_HEADS_MAX <= TI_ACT_CAP / 32 * TI_ACT_TMAX, "the heads' (max, sum) fit the scratch");
-    float *ml = c->act_s, *scores = c->attn_po + MASS_SCORES;
-    const long sstride = (pos0 + 32L) / 32 * 32, n = (pos0 + 1L) * nKv;
-    const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, scores, sstride, ml};
-    const int rc1 = ti_token_attn_launch(c, t, hd);
-    if (rc1) return rc1;
-    k_token_mass<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(scores, sstride, ml, mass, pos0, nHq, nKv);
-    TI_LAUNCHED("k_token_mass");
-    return TI_OK;
+    // the scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one)
+    const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, mass,
+                           c->attn_po + MASS_SCORES, (pos0 + 32L) / 32 * 32};
+    return ti_token_attn_launch(c, t, hd);
 }

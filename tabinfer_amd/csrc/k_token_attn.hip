@@ -433,7 +433,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                     seen |= ok ? 1u << e : 0u;
                 }
             }
-            if (a.p.scores && slot == 0 && rt * ROWS + tr < a.R) {
+            if (a.p.mass && slot == 0 && rt * ROWS + tr < a.R) {
                 float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
                 *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
                 *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
@@ -554,6 +554,37 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
     }
 }
 
+// The weights that each key received, by the merge's workgroups behind the rows' own (part of parts): every head's (max, sum)
+// from the slots', then a thread a (key, KV head). In the merge's launch and not behind it: 4096 slots of 8 heads
+// MASS_FIGURES
+__device__ __forceinline__ void token_mass(const TokArgs& a, int ns, int part, int parts) {
+    __shared__ float2 s_ml[TI_ATTN_HEADS_MAX];
+    const int lane = threadIdx.x & 63, heads = a.p.nHq, G = a.G;
+    for (int h = threadIdx.x >> 6; h < heads; h += 4) {
+        float m = -INFINITY, l = 0.0f;
+        for (int s = lane; s < ns; s += 64) {
+            const float2 x = *reinterpret_cast<const float2*>(a.pml + 2 * ((size_t)s * heads + h));
+            const float mn = fmaxf(m, x.x);
+            if (mn == -INFINITY) continue;
+            l = fmaf(l, __builtin_amdgcn_exp2f(m - mn), x.y * __builtin_amdgcn_exp2f(x.x - mn));
+            m = mn;
+        }
+        const float M = ti_wave_max(m);
+        const float L = ti_wave_sum(m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - M));
+        if (lane == 0) s_ml[h] = make_float2(M, L);
+    }
+    __syncthreads();
+    const long n = (a.p.pos0 + 1L) * a.p.nKv;
+    for (long i = (long)part * 256 + threadIdx.x; i < n; i += (long)parts * 256) {
+        const long j = i / a.p.nKv;
+        const int hk = (int)(i % a.p.nKv);
+        float sum = 0.0f;
+        for (int h = hk * G; h < (hk + 1) * G; h++)
+            sum += __builtin_amdgcn_exp2f(a.p.scores[h * a.p.sstride + j] - s_ml[h].x) / s_ml[h].y;
+        a.p.mass[i] = j < a.p.pos0 ? a.p.mass[i] + sum : sum;
+    }
+}
+
 // A workgroup a (sequence, token, head) and DW of its dims: the slots' partials into the output row, each group of threads
 // those of its own slots with every load in flight at once. DW = 32 where that is what it takes to fill the CUs
 template <int HD, int DW>
@@ -562,7 +593,8 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
     __shared__ float s_m[SG], s_l[SG];
     __shared__ __align__(16) float s_o[SG][4 * D4];
     const int tid = threadIdx.x, sg = tid / D4, d = tid % D4;
-    const int row = blockIdx.x, d0 = DW * blockIdx.y;
+    const int rows = a.p.B * a.p.T * a.p.nHq, row = blockIdx.x, d0 = DW * blockIdx.y;
+    if (row >= rows) return token_mass(a, ns1, (row - rows) * gridDim.y + blockIdx.y, (gridDim.x - rows) * gridDim.y);
     const int hq = row % a.p.nHq, t = (row / a.p.nHq) % a.p.T, b = row / (a.p.nHq * a.p.T);
     const int hk = hq / a.G, r = t * a.G + hq % a.G;
     const int s0 = ns1 ? 0 : a.meta[2 * b], ns = ns1 ? ns1 : a.meta[2 * b + 1];
@@ -613,10 +645,6 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
         v = fmaf(s_o[g][tid], e, v);
     }
     a.p.out[(size_t)row * HD + d0 + tid] = M == -INFINITY ? 0.0f : v / (127.0f * PSCALE * Lt);
-    if (a.p.ml && tid == 0 && d0 == 0) {
-        a.p.ml[2 * row] = M;
-        a.p.ml[2 * row + 1] = Lt;
-    }
 }
 
 template <int HD, bool PAGED>
@@ -625,8 +653,10 @@ void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
     if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, THREADS, 0, c->stream>>>(a);
     else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, THREADS, 0, c->stream>>>(a);
     const int rows = a.p.B * a.p.T * a.p.nHq;
-    if (HD == 32 || rows >= c->cus) k_token_merge<HD, HD><<<rows, 256, 0, c->stream>>>(a, ns1);
-    else if constexpr (HD > 32) k_token_merge<HD, 32><<<dim3(rows, HD / 32), 256, 0, c->stream>>>(a, ns1);
+    // the weights' workgroups: two a CU at most, since each forms every head's sum
+    const long n = a.p.mass ? ti_min(((a.p.pos0 + 1L) * a.p.nKv + 255) / 256, 2L * c->cus) : 0;
+    if (HD == 32 || rows >= c->cus) k_token_merge<HD, HD><<<rows + n, 256, 0, c->stream>>>(a, ns1);
+    else if constexpr (HD > 32) k_token_merge<HD, 32><<<dim3(rows + (n + HD / 32 - 1) / (HD / 32), HD / 32), 256, 0, c->stream>>>(a, ns1);
 }
 
 }  // namespace

@@ -16,8 +16,8 @@ struct TiTokenAttn {
     const int32_t* lens;                     // keys of each sequence (pages); else the one sequence's queries are at pos0 ..
     int B, T, pos0, nHq, nKv, window, sinks;
     long max_keys;                           // keys that a sequence's queries can see, at most
-    float* scores;                           // [nHq][sstride] scores in log2 of a one-token call, or nullptr
+    float* mass;                             // of one token of one sequence: mass[j nKv + h] (+)= the weights of key j, or nullptr
+    float* scores;                           // [nHq][sstride] room for its scores in log2
     long sstride;
-    float* ml;                               // [T nHq][2] (max in log2, sum) of each row, or nullptr
 };
 int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd);
