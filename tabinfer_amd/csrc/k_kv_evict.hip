@@ -44,15 +44,26 @@ __device__ __forceinline__ uint32_t order_key(const EvictArgs& a, int p, float m
     const uint32_t b = __builtin_bit_cast(uint32_t, m);
     return p < a.sinks || p >= a.late ? 0xffffffffu : m != m ? 0u : (b >> 31 ? ~b : b | 0x80000000u);
 }
-// the bookkeeping of a slot that stays (nothing to do where it is in place already), and of a move
+// the bookkeeping of a slot that stays (nothing to do where it is in place already)
 __device__ __forceinline__ void stay(const EvictArgs& a, int i, int h) {
     const size_t at = (size_t)i * a.nKv + h;
     if (a.mass_out != a.mass) a.mass_out[at] = a.mass[at];
     if (a.where_out != a.where || i >= a.known) a.where_out[at] = slot_pos(a, i, h);
 }
-__device__ __forceinline__ void moved(const EvictArgs& a, int from, int to, int h) {
-    a.mass_out[(size_t)to * a.nKv + h] = a.mass[(size_t)from * a.nKv + h];
-    a.where_out[(size_t)to * a.nKv + h] = slot_pos(a, from, h);
+
+// a move, 16 lanes: K's and V's pieces and scales, and what the slot holds (read above keep, written below)
+__device__ __forceinline__ void move_slot(const EvictArgs& a, int from, int to, int h, int l) {
+    const size_t src = (size_t)from * a.nKv + h, dst = (size_t)to * a.nKv + h;
+    const int w4 = a.hd / 16, ng = a.hd / 32, p = l & 7;
+    const uint4* cs = reinterpret_cast<const uint4*>(l < 8 ? a.kq : a.vq);
+    uint4* cd = reinterpret_cast<uint4*>(l < 8 ? a.kq : a.vq);
+    float* sc = l < 8 ? a.ks : a.vs;
+    if (p < w4) cd[dst * w4 + p] = cs[src * w4 + p];
+    if (p < ng) sc[dst * ng + p] = sc[src * ng + p];
+    if (l == 0) {
+        a.mass_out[dst] = a.mass[src];
+        a.where_out[dst] = slot_pos(a, from, h);
+    }
 }
 
 // nothing to evict: every slot stays
@@ -119,10 +130,17 @@ __device__ __forceinline__ int part_scan(SelLds<KPT>& L) {
     return sum;
 }
 
-// the keys of slots i0 + 1024 k + tid, every load in flight at once; 0 behind the last slot
-template <int KPT>
-__device__ __forceinline__ void form_keys(const EvictArgs& a, int h, int i0, uint32_t (&key)[KPT]) {
+// the keys of slots i0 + 1024 k + tid, every load in flight at once; 0 behind the last slot. FORM: else k_evict_keys did
+template <int KPT, bool FORM>
+__device__ __forceinline__ void load_keys(const EvictArgs& a, int h, int i0, uint32_t (&key)[KPT]) {
     const int tid = threadIdx.x;
+    if constexpr (!FORM) {
+#pragma unroll
+        for (int k = 0; k < KPT; k++) key[k] = a.keys[(size_t)h * a.n + ti_min(i0 + k * SEL + tid, a.n - 1)];
+#pragma unroll
+        for (int k = 0; k < KPT; k++) key[k] = i0 + k * SEL + tid < a.n ? key[k] : 0u;
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < KPT; k++) key[k] = __builtin_bit_cast(uint32_t, a.mass[(size_t)ti_min(i0 + k * SEL + tid, a.n - 1) * a.nKv + h]);
     int at[KPT];
@@ -137,15 +155,18 @@ __device__ __forceinline__ void form_keys(const EvictArgs& a, int h, int i0, uin
 }
 
 // One slot too many, a bounded cache's every token: the last slot of the smallest key, by a minimum in place of the select
-// (4097 slots of 8 heads: 8.6 us, the select 17.2)
-__global__ __launch_bounds__(SEL) void k_evict_one(EvictArgs a) {
+// (4097 slots of 8 heads: 8.4 us, the select 17.2). In place it moves the one slot too, and nothing follows (8.2 us, with a
+// launch for the move 8.3 + 2.8); elsewhere k_evict_move writes what the other slots hold along the rows of all heads (2.9 us;
+// from here, a 4-byte piece of each row at a time, 5)
+template <bool FORM>
+__global__ __launch_bounds__(SEL) void k_evict_one(EvictArgs a, bool placed) {
     constexpr int KPT = FORMED / SEL;
     __shared__ uint64_t s_best[SEL / 64];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x;
     uint64_t best = ~0ull;                                 // (key, slots behind it)
     for (int i0 = 0; i0 < a.n; i0 += KPT * SEL) {
         uint32_t key[KPT];
-        form_keys(a, h, i0, key);
+        load_keys<KPT, FORM>(a, h, i0, key);
 #pragma unroll
         for (int k = 0; k < KPT; k++) {
             const int i = i0 + k * SEL + tid;
@@ -159,6 +180,10 @@ __global__ __launch_bounds__(SEL) void k_evict_one(EvictArgs a) {
 #pragma unroll
     for (int w = 0; w < SEL / 64; w++) best = ti_min(best, s_best[w]);
     const int out = a.n - 1 - (int)(uint32_t)best;
+    if (placed) {
+        if (tid < 16 && out < a.keep) move_slot(a, a.keep, out, h, tid);
+        return;
+    }
     for (int w = tid; w < a.words; w += SEL) a.stays[(size_t)h * a.words + w] = ~(out / 64 == w ? 1ull << (out & 63) : 0ull);
     if (tid > 0) return;
     a.count[h] = out < a.keep;
@@ -174,16 +199,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint32_t key[KPT];                                     // 0 behind the last slot
-    auto load = [&](int i0) {
-        if constexpr (FORM) {
-            form_keys(a, h, i0, key);
-        } else {                                           // k_evict_keys formed them
-#pragma unroll
-            for (int k = 0; k < KPT; k++) key[k] = a.keys[(size_t)h * a.n + ti_min(i0 + k * SEL + tid, a.n - 1)];
-#pragma unroll
-            for (int k = 0; k < KPT; k++) key[k] = i0 + k * SEL + tid < a.n ? key[k] : 0u;
-        }
-    };
+    auto load = [&](int i0) { load_keys<KPT, FORM>(a, h, i0, key); };
     constexpr int CHUNK = KPT * SEL;
     const bool one = a.n <= CHUNK;
     if (one) load(0);
@@ -280,8 +296,7 @@ __global__ __launch_bounds__(SEL) void k_evict_pick(EvictArgs a) {
     if (tid == 0) a.count[h] = holes;
 }
 
-// The moves, 16 lanes each: K's and V's pieces and scales, and what the slot holds (read above keep, written below). Behind
-// them (blocks from mblocks on) the bookkeeping of the slots that stay, along the rows of all heads
+// The moves, 16 lanes each. Behind them (blocks from mblocks on) the bookkeeping of the slots that stay, along the rows of all heads
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int mblocks, int per_head) {
     if ((int)blockIdx.x >= mblocks) {
         const long x = (long)(blockIdx.x - mblocks) * 256 + threadIdx.x;
@@ -292,15 +307,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int mblocks, in
     const int h = blockIdx.x / per_head, l = threadIdx.x & 15, m = blockIdx.x % per_head * 16 + (threadIdx.x >> 4);
     if (m >= a.count[h]) return;
     const int32_t* mv = a.moves + ((size_t)h * a.room + m) * 2;
-    const int from = mv[0], to = mv[1];
-    const size_t src = (size_t)from * a.nKv + h, dst = (size_t)to * a.nKv + h;
-    const int w4 = a.hd / 16, ng = a.hd / 32, p = l & 7;
-    const uint4* cs = reinterpret_cast<const uint4*>(l < 8 ? a.kq : a.vq);
-    uint4* cd = reinterpret_cast<uint4*>(l < 8 ? a.kq : a.vq);
-    float* sc = l < 8 ? a.ks : a.vs;
-    if (p < w4) cd[dst * w4 + p] = cs[src * w4 + p];
-    if (p < ng) sc[dst * ng + p] = sc[src * ng + p];
-    if (l == 0) moved(a, from, to, h);
+    move_slot(a, mv[0], mv[1], h, l);
 }
 
 }  // namespace
@@ -321,7 +328,7 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     const int room = kept < n - kept ? kept : n - kept;      // moves of a head, at most
     const int words = (kept + 63) / 64;
     // scratch: the slots that stay, the moves' counts, the moves, the keys of many slots
-    const bool single = n - kept == 1, many = n > FORMED && !single;
+    const bool single = n - kept == 1, many = n > FORMED;
     const long need = 2L * nKv * words + nKv + 2L * nKv * room + (many ? (long)nKv * n : 0);
     TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch", n, room);
     uint64_t* stays = reinterpret_cast<uint64_t*>(c->attn_po);
@@ -335,17 +342,19 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
         TI_LAUNCHED("k_evict_none");
         return TI_OK;
     }
+    // in place, the slots that stay already hold what they held
+    const bool placed = mass_out == mass && where_out == where && known >= kept;
     if (many) {
         k_evict_keys<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_evict_keys");
     }
-    if (single) k_evict_one<<<nKv, SEL, 0, c->stream>>>(a);
+    if (single && many) k_evict_one<false><<<nKv, SEL, 0, c->stream>>>(a, placed);
+    else if (single) k_evict_one<true><<<nKv, SEL, 0, c->stream>>>(a, placed);
     else if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
     else if (n <= 16 * SEL) k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
     else k_evict_pick<32, false><<<nKv, SEL, 0, c->stream>>>(a);
     TI_LAUNCHED("k_evict_pick");
-    // in place, the slots that stay already hold what they held
-    const bool placed = mass_out == mass && where_out == where && known >= kept;
+    if (single && placed) return TI_OK;
     const int per_head = (room + 15) / 16, sblocks = placed ? 0 : (int)(((long)kept * nKv + 255) / 256);
     k_evict_move<<<(unsigned)(per_head * nKv + sblocks), 256, 0, c->stream>>>(a, per_head * nKv, per_head);
     TI_LAUNCHED("k_evict_move");
