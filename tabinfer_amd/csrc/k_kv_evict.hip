@@ -5,18 +5,18 @@
 // i-th into the i-th: no slot is both read and written, so the moves run in any order, a cache that frees one slot moves one
 // row, and what stays below `keep` stays where it is.
 //
-// Bound by its launches and by the select's chain of barriers, not by bytes: 4097 slots of 8 heads to 4096 8.6 + 2.9 us
-// (the one slot, the move and the bookkeeping), 16384 to 4096 2.7 + 19.2 + 5.9 us (keys, select, moves), where the moved
+// Bound by its launches and by the select's chain of barriers, not by bytes: 4097 slots of 8 heads to 4096
+// 2.7 + 5.1 + 2.7 us (keys, the one slot, the move and the bookkeeping), 16384 to 4096 2.7 + 19.2 + 5.9 us (keys, select, moves), where the moved
 // rows' 13 MB are 2.7 us of a copy. A workgroup a head and not more: the select's steps depend on one another, and counts
-// across workgroups would cost a launch a digit (about 5 us each). 1024 threads: for the two selections above 512 threads
-// took 20.1 and 28.1 us where 1024 took 17.2 and 22.2, and 256 took 29.3 and 54.3 (more keys a thread, one behind another).
+// across workgroups would cost a launch a digit (about 5 us each). 1024 threads: of an earlier version for 4097 and
+// 16384 slots 512 took 20.1 and 28.1 us where 1024 took 17.2 and 22.2, and 256 29.3 and 54.3 (more keys a thread, in turn).
 #include "ti_dev.h"
 #include "ti_span.h"
 
 namespace {
 
 constexpr int SEL = 1024;       // threads of a head's workgroup
-constexpr int FORMED = 8192;    // up to so many slots it forms their keys itself, see k_evict_keys
+constexpr int FORMED = 2048;    // up to so many slots it forms their keys itself, see k_evict_keys
 
 struct EvictArgs {
     uint8_t* kq;
@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256) void k_evict_none(EvictArgs a) {
 }
 
 // The keys of many slots, head by head: rows of all heads are read in whole lines here, where a head's one workgroup would
-// take a 4-byte piece of each (16384 slots of 8 heads: 9 us against 5.5 with this launch; up to 8192 slots the pieces cost
-// less than the launch)
+// take a 4-byte piece of each (8 heads: 16384 slots 9 us against 5.5 with this launch, 4097 slots to all but 99 of them 16.1
+// with the select against 14.5; up to 2048 slots the pieces cost less than the launch, 9.7 against 13.1)
 __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
     const long x = (long)blockIdx.x * 256 + threadIdx.x;
     if (x >= (long)a.n * a.nKv) return;
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
 }
 
 // A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 32 every key stays in a register, more slots
-// go through in chunks, read again for each digit. The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
+// go through in chunks, read again for each digit; no more registers than the slots need (4097 slots 11.6 us with 8, 15.2
+// with 16). The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
 // up from the top, and only the keys with the digits so far go on; done as soon
 // as all of these are kept (16384 slots of 8 heads to 4096: 22 us, all three digits' passes, to 20). Lanes of a wave that all have one digit count as one, so
 // that equal masses do not queue for their bin.
@@ -155,9 +156,9 @@ __device__ __forceinline__ void load_keys(const EvictArgs& a, int h, int i0, uin
 }
 
 // One slot too many, a bounded cache's every token: the last slot of the smallest key, by a minimum in place of the select
-// (4097 slots of 8 heads: 8.4 us, the select 17.2). In place it moves the one slot too, and nothing follows (8.2 us, with a
-// launch for the move 8.3 + 2.8); elsewhere k_evict_move writes what the other slots hold along the rows of all heads (2.9 us;
-// from here, a 4-byte piece of each row at a time, 5)
+// (4097 slots of 8 heads: 5.1 us, the select 11.6). In place it moves the one slot too, and nothing follows (with a launch for
+// the move 2.8 us more); elsewhere k_evict_move writes what the other slots hold along the rows of all heads (2.9 us; from
+// here, a 4-byte piece of each row at a time, 5)
 template <bool FORM>
 __global__ __launch_bounds__(SEL) void k_evict_one(EvictArgs a, bool placed) {
     constexpr int KPT = FORMED / SEL;
@@ -351,6 +352,7 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     if (single && many) k_evict_one<false><<<nKv, SEL, 0, c->stream>>>(a, placed);
     else if (single) k_evict_one<true><<<nKv, SEL, 0, c->stream>>>(a, placed);
     else if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
+    else if (n <= 8 * SEL) k_evict_pick<8, false><<<nKv, SEL, 0, c->stream>>>(a);
     else if (n <= 16 * SEL) k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
     else k_evict_pick<32, false><<<nKv, SEL, 0, c->stream>>>(a);
     TI_LAUNCHED("k_evict_pick");
