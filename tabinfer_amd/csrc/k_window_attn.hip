@@ -9,6 +9,9 @@
 //     hi + lo to 2^-22 of its largest element), each group's sum times its key's scale in f32.
 //   - O^T = V^T P^T with P times the V scale of (key, group) in f32 as three bf16, exactly; a lane's scores are the
 //     operand as they stand.
+// Bound by VALU work, most of it the weights': 4096 tokens of 16 heads of 128 dims under a window of 1024 in 140 us (210
+// TFLOP/s), of which the three bf16 and their products took 50, q's lower half 14, the staging 10. Chunks are split into
+// ranges of keys until two workgroups a CU are there: 250 tokens of 32 heads of 64 dims under a window of 2000 in 29 + 5 us.
 #include "ti_dev.h"
 #include "ti_span.h"
 #include "ti_window_attn.h"
