@@ -441,21 +441,23 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                 *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
                 *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
             }
+            // the largest of the lane's scores, in log2; what a row sees is never below the floor
             float tm = FLOOR;
             if (!whole) {
                 tm = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen >> e & 1u ? fmaxf(s[e], FLOOR) : -INFINITY);
+                tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[e]);
+                tm = fmaxf(tm * fr, FLOOR);
             }
-            tm = fmaxf(tm, ti_xor(tm, 16));
-            tm = fmaxf(tm, ti_xor(tm, 32));
-            tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;       // in log2 units from here on
             // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
-            const bool bump = tm > m + 6.0f;
-            if (__any(bump)) {
+            if (__any(tm > m + 6.0f)) {
+                tm = fmaxf(tm, ti_xor(tm, 16));
+                tm = fmaxf(tm, ti_xor(tm, 32));
+                const bool bump = tm > m + 6.0f;
                 const float mn = bump ? tm : m;
                 const float alpha = bump ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
                 l = l * alpha;

@@ -9,7 +9,7 @@
 //     hi + lo to 2^-22 of its largest element), each group's sum times its key's scale in f32.
 //   - O^T = V^T P^T with P times the V scale of (key, group) in f32 as three bf16, exactly; a lane's scores are the
 //     operand as they stand.
-// Bound by VALU work, most of it the weights': 4096 tokens of 16 heads of 128 dims under a window of 1024 in 140 us (210
+// Bound by VALU work, most of it the weights': 4096 tokens of 16 heads of 128 dims under a window of 1024 in 137 us (220
 // TFLOP/s), of which the three bf16 and their products took 50, q's lower half 14, the staging 10. Chunks are split into
 // ranges of keys until two workgroups a CU are there: 250 tokens of 32 heads of 64 dims under a window of 2000 in 29 + 5 us.
 #include "ti_dev.h"
@@ -278,44 +278,54 @@ __global__ __launch_bounds__(256, RW == 2 ? 2 : 3) void k_window_attn(WinArgs a)
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[r][4 * b + e] = acc[r][e];
             }
+            // the largest of the lane's scores of each row, in log2; what a row sees is never below the floor
             uint32_t seen[RW];
+            float tm[RW];
+            bool bump = false;
 #pragma unroll
             for (int r = 0; r < RW; r++) {
-                seen[r] = ~0u;
-                float tm = -INFINITY;
                 if (!whole) {
                     asm volatile("");                      // a branch: not computed where every key is seen
                     seen[r] = 0;
+                    tm[r] = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 8 * HN; e++) {
                         const int key = k0 + 16 * (e >> 2) + 4 * j + (e & 3);
                         const bool ok = (key <= pos[r]) & ((key >= low[r]) | (key < sinks));
                         seen[r] |= ok ? 1u << e : 0u;
-                        tm = fmaxf(tm, ok ? fmaxf(s[r][e], FLOOR) : -INFINITY);
+                        tm[r] = fmaxf(tm[r], ok ? fmaxf(s[r][e], FLOOR) : -INFINITY);
                     }
+                    tm[r] = tm[r] > -INFINITY ? fmaxf(tm[r] * fr[r], FLOOR) : -INFINITY;
                 } else {
+                    seen[r] = ~0u;
+                    tm[r] = FLOOR;
 #pragma unroll
-                    for (int e = 0; e < 8 * HN; e++) tm = fmaxf(tm, s[r][e]);
-                    tm = fmaxf(tm, FLOOR);
+                    for (int e = 0; e < 8 * HN; e++) tm[r] = fmaxf(tm[r], s[r][e]);
+                    tm[r] = fmaxf(tm[r] * fr[r], FLOOR);
                 }
-                tm = fmaxf(tm, ti_xor(tm, 16));
-                tm = fmaxf(tm, ti_xor(tm, 32));
-                tm = tm > -INFINITY ? fmaxf(tm * fr[r], FLOOR) : -INFINITY;   // in log2 units from here on
-                // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
-                const bool bump = tm > mx[r] + 6.0f;
-                if (__any(bump)) {
-                    const float mn = bump ? tm : mx[r];
-                    const float alpha = bump ? __builtin_amdgcn_exp2f(mx[r] - mn) : 1.0f;
+                bump |= tm[r] > mx[r] + 6.0f;
+            }
+            // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
+            if (__any(bump)) {
+#pragma unroll
+                for (int r = 0; r < RW; r++) {
+                    tm[r] = fmaxf(tm[r], ti_xor(tm[r], 16));
+                    tm[r] = fmaxf(tm[r], ti_xor(tm[r], 32));
+                    const bool up = tm[r] > mx[r] + 6.0f;
+                    const float mn = up ? tm[r] : mx[r];
+                    const float alpha = up ? __builtin_amdgcn_exp2f(mx[r] - mn) : 1.0f;
                     l[r] = l[r] * alpha;
 #pragma unroll
                     for (int d = 0; d < HD / 16; d++) o[r][d] = o[r][d] * alpha;
                     mx[r] = mn;
                 }
+            }
+#pragma unroll
+            for (int r = 0; r < RW; r++) {
 #pragma unroll
                 for (int e = 0; e < 8 * HN; e++) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[r][e], fr[r], -mx[r]));
-                    if (!whole) p = seen[r] >> e & 1u ? p : 0.0f;
-                    s[r][e] = p;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[r][e], fr[r], -mx[r]));
+                    s[r][e] = whole || (seen[r] >> e & 1u) ? p : 0.0f;
                 }
 #pragma unroll
                 for (int e = 0; e < 8 * HN; e += 8)
