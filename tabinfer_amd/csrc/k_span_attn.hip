@@ -7,7 +7,8 @@
 
 namespace {
 
-constexpr long MASS_SCORES = 1L << 24;       // (query head, slot) scores of a one-token call
+constexpr long MASS_SCORES = 1L << 24;       // (query head, slot) scores of a one-token call: half of the partials' scratch
+static_assert(2 * MASS_SCORES <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "the scores fit");
 
 // Single tokens and up to 8 query rows a KV head take k_token_attn.hip, more k_window_attn.hip. Tokens x query heads of 16
 // and 8 KV heads of 128 dims over 2000 keys, the two kernels with their merges: 4 tokens (8 rows) 13.9 / 15.6 us, 8 tokens
@@ -74,7 +75,7 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
                nHq, pos0 + 1, MASS_SCORES);
     const uint8_t *k8 = reinterpret_cast<const uint8_t*>(kq), *v8 = reinterpret_cast<const uint8_t*>(vq);
     if (T > 1) return ti_mass_attn_launch(c, TiWindowAttn{qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0}, hd, mass);
-    // the scores go to the upper half of the partials' scratch (2048 slots of 64 heads fill the lower one)
+    // the scores go to the upper half of the partials' scratch
     const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, mass,
                            c->attn_po + MASS_SCORES, (pos0 + 32L) / 32 * 32};
     return ti_token_attn_launch(c, t, hd);

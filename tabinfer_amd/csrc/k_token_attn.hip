@@ -683,10 +683,11 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     a.HW = p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
     a.BW = WAVES / a.HW;
     // the workgroups that the CUs hold at once (three; two of those with a column a row); as many as there are sequences,
-    // if that is more; as far as the partials' slots (one for each workgroup and one for each sequence) fit
+    // if that is more; as far as the partials' slots (one for each workgroup and one for each sequence) fit: half of the
+    // scratch where the other half holds scores
     const int groups = p.nKv / a.HW * a.RT, held = a.R <= tile_rows(hd, true) ? 3 : 2;
     long wgs = ti_max(((long)held * c->cus + groups - 1) / groups, (long)p.B);
-    wgs = ti_max(1L, ti_min(wgs, (long)TI_ATTN_ROWSPLITS / (p.T * p.nHq) - p.B));
+    wgs = ti_max(1L, ti_min(wgs, (p.mass ? TI_ATTN_ROWSPLITS / 2L : (long)TI_ATTN_ROWSPLITS) / (p.T * p.nHq) - p.B));
     a.wgs = (int)wgs;
     const bool paged = p.lens != nullptr;
     int ns1 = 0;

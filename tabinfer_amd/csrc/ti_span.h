@@ -20,8 +20,6 @@ constexpr int TI_POS_END = 0x7fffff00;
 struct TiSpan {
     int first, low, end;
     TI_HD int count() const { return first + (end - low); }
-    // the i-th visible position
-    TI_HD int at(int i) const { return i < first ? i : low + (i - first); }
 };
 TI_HD inline TiSpan ti_span(int p, int window, int sinks) {
     TiSpan s;

@@ -239,6 +239,73 @@ def test_a_cache_without_a_table_needs_no_sequences(ctx):
         b.free()
 
 
+@pytest.mark.parametrize("T", [1, 3, 12, 150])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_rows_query_is_its_own(ctx, T, bad):
+    """A query that is not finite (a padded row's) leaves the other heads and tokens as they are."""
+    rng = np.random.default_rng(T)
+    nHq, nKv, hd, pos0, window, sinks = 8, 4, 64, 300, 100, 2
+    S = pos0 + T
+    q, (kc, ks, vc, vs) = queries(rng, T, nHq, hd), ref.cache(rng, S, nKv, hd)
+    dirty = q.copy()
+    dirty[T // 2, 3, 5:9] = bad
+    o = ctx.zeros(q.nbytes)
+    dev = [ctx.upload(a) for a in (dirty, kc, ks, vc, vs)]
+    ctx.call("ti_attn_window_q8", *dev, o, T, pos0, nHq, nKv, hd, window, sinks)
+    got = ctx.download(o, np.float32, q.size).reshape(q.shape)
+    want, tol, _, _ = ref.attend(q, ref.values(kc, ks), ref.values(vc, vs), ref.visible(pos0 + np.arange(T), np.arange(S), window, sinks))
+    ok = np.ones((T, nHq), bool)
+    ok[T // 2, 3] = False
+    assert np.all((np.abs(got - want) <= tol)[ok]) and np.all(np.isnan(got[T // 2, 3]))
+    for x in dev + [o]:
+        x.free()
+
+
+def test_padded_rows_of_a_batch(ctx):
+    """Rows without a sequence (length 0, garbage in the query and the table) give zeros, the others their own results."""
+    rng = np.random.default_rng(2)
+    B, nHq, nKv, hd, page, pages, width = 5, 16, 8, 128, 16, 30, 6
+    lens = np.array([90, 0, 17, -3, 40], np.int32)
+    table = np.stack([rng.permutation(pages)[:width] for _ in range(B)]).astype(np.int32)
+    q, (kc, ks, vc, vs) = queries(rng, B, nHq, hd), ref.cache(rng, pages * page, nKv, hd)
+    q[1], q[3] = np.nan, np.inf
+    table[1], table[3] = 2 ** 31 - 1, -2 ** 31
+    dev = [ctx.upload(a) for a in (q, kc, ks, vc, vs, table, lens)]
+    o = ctx.upload(np.full(q.size, np.nan, np.float32))
+    ctx.call("ti_attn_paged_q8", *dev, o, B, nHq, nKv, hd, page, pages, width, -1, 0)
+    got = ctx.download(o, np.float32, q.size).reshape(q.shape)
+    assert np.all(got[[1, 3]] == 0)
+    for b in (0, 2, 4):
+        j = np.arange(lens[b])
+        rows = table[b, j // page].astype(np.int64) * page + j % page
+        want, tol, _, _ = ref.attend(q[b:b + 1], ref.values(kc[rows], ks[rows]), ref.values(vc[rows], vs[rows]), ref.visible([lens[b] - 1], j, -1, 0))
+        assert np.all(np.abs(got[b] - want[0]) <= tol[0]), b
+    for x in dev + [o]:
+        x.free()
+
+
+@pytest.mark.parametrize("n,keep", [(300, 299), (300, 120), (5000, 4000)])
+@pytest.mark.parametrize("mass_in_place", [True, False])
+def test_one_of_the_slots_buffers_in_place(ctx, n, keep, mass_in_place):
+    """Masses cut in place and positions elsewhere, or the other way round."""
+    rng = np.random.default_rng(n)
+    nKv, hd, known, nxt = 3, 32, n - 7, n + 50
+    mass = rng.uniform(0, 1, (n, nKv)).astype(np.float32)
+    where = np.stack([rng.permutation(nxt - 7)[:known] for _ in range(nKv)], 1).astype(np.int32)
+    kc, ks, vc, vs = ref.cache(rng, n, nKv, hd)
+    dev = [ctx.upload(a) for a in (kc, ks, vc, vs, mass, np.concatenate([where, np.full((7, nKv), -77, np.int32)]))]
+    mo = dev[4] if mass_in_place else ctx.zeros(keep * nKv * 4)
+    wo = ctx.zeros(keep * nKv * 4) if mass_in_place else dev[5]
+    ctx.call("ti_kv_evict_q8", *dev, mo, wo, n, known, keep, 3, 20, nxt, nKv, hd)
+    src, pos = ref.evict(mass, where, n, known, keep, 3, 20, nxt)
+    h = np.arange(nKv)[None]
+    assert np.array_equal(ctx.download(wo, np.int32, keep * nKv).reshape(keep, nKv), pos)
+    assert np.array_equal(ctx.download(mo, np.float32, keep * nKv).reshape(keep, nKv), mass[src, h])
+    assert np.array_equal(ctx.download(dev[0], np.int8, kc.size).reshape(kc.shape)[:keep], kc[src, h])
+    for x in dev + [mo, wo]:
+        x.free()
+
+
 @pytest.mark.skipif(NODE is None, reason="node is not installed")
 def test_javascript_launchers(tmp_path):
     """The host's six launchers: a paged prompt and token, a window, weights added up, an eviction and what it leaves."""
