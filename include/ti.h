@@ -502,7 +502,8 @@ int ti_attn_window_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
  * pos[t] of sequence seq[t] (seq NULL: row t is sequence t, T <= B). A row whose place does not exist (pos < 0 or
  * past the table, seq outside [0, B), a page id outside [0, pages)) is not written. Rows of one call name different
  * places; of rows that name the same one, which codes and which scales stay is not specified. table NULL: the
- * positions are the rows of a contiguous cache of page * pages positions, seq and B are not looked at. nKv <= 64. */
+ * positions are the rows of a contiguous cache of page * pages positions, seq and B are not looked at. nKv <= 64,
+ * T * nKv * hd < 2^33. */
 int ti_kv_write_paged_q8(ti_ctx* ctx, const float* kr, const float* v, uint32_t* kq, float* ks,
                          uint32_t* vq, float* vs, const int32_t* table, const int32_t* seq,
                          const int32_t* pos, int T, int B, int nKv, int hd, int page, int pages, int width);

@@ -9,6 +9,8 @@
 
 namespace {
 
+typedef float v4f __attribute__((ext_vector_type(4)));
+
 struct PlaceArgs {
     TiPages pg;
     const int32_t* seq;     // nullptr: row t is sequence t
@@ -22,22 +24,17 @@ __device__ __forceinline__ long place_row(const PlaceArgs& a, int t) {
     return a.pg.row(s, a.pos[t]);
 }
 
-// A thread takes four elements (a word of codes) at a time, a workgroup WORDS words of K or V, row behind row, so that both
-// sides are read and written in whole lines; eight neighbouring lanes share a 32-group. Bound by the launch below a few
-// hundred rows (256 rows of 8 heads of 128 dims written in 5.3 us, read in 4.7), by the floats' traffic above (4096 rows, 42
-// MB, read in 10 us: 4.2 TB/s).
-constexpr int WORDS = 1024;
-
-// word x of the workgroup -> row t and word of it; false: behind the last
+// A thread takes four elements (a word of codes) of K or V, row behind row, so that both sides are read and written in whole
+// lines; eight neighbouring lanes share a 32-group. Bound by the launch below a few hundred rows (256 rows of 8 heads of 128
+// dims written in 3.3 us, read in 3.0; two and four words a thread 3.7 and 5.2, 3.6 and 4.5), by the floats' traffic above (4096
+// rows, 42 MB, read in 8.8 us: 4.8 TB/s; with stores that stay in the caches 10.2).
 struct WordAt {
-    int t, w;
-    __device__ WordAt(const PlaceArgs& a, int x) {
-        const int rw = a.rowg * 8;
-        const long base = (long)blockIdx.x * WORDS;
-        const long t0 = base / rw;                         // workgroup-uniform
-        const unsigned l = (unsigned)(base - t0 * rw) + x;
-        t = (int)(t0 + l / (unsigned)rw);
-        w = (int)(l % (unsigned)rw);
+    int t;
+    unsigned w;                                            // word x of all: row t, word w of it
+    __device__ explicit WordAt(const PlaceArgs& a) {
+        const unsigned x = blockIdx.x * 256 + threadIdx.x, rw = a.rowg * 8;
+        t = (int)(x / rw);
+        w = x % rw;
     }
 };
 
@@ -45,59 +42,35 @@ __global__ __launch_bounds__(256) void k_kv_write_paged(PlaceArgs a, const float
                                                         uint32_t* __restrict__ kq, float* __restrict__ ks,
                                                         uint32_t* __restrict__ vq, float* __restrict__ vs) {
     const bool isv = blockIdx.y;
-    const float4* src = reinterpret_cast<const float4*>(isv ? v : k);
-    float4 x[WORDS / 256];
-    long row[WORDS / 256];
-    int w[WORDS / 256];
-#pragma unroll
-    for (int u = 0; u < WORDS / 256; u++) {
-        const WordAt at(a, threadIdx.x + 256 * u);
-        const bool in = at.t < a.T;
-        x[u] = in ? src[(size_t)at.t * a.rowg * 8 + at.w] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        row[u] = in ? place_row(a, at.t) : -1;
-        w[u] = at.w;
-    }
-#pragma unroll
-    for (int u = 0; u < WORDS / 256; u++) {
-        const float4 f = x[u];
-        const float mx = fmaxf(group_max_contig<4>(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)))), 1e-12f);
-        if (row[u] < 0) continue;
-        const size_t at = (size_t)row[u] * a.rowg * 8 + w[u];
-        (isv ? vq : kq)[at] = snorm_code(f.x, mx) | (snorm_code(f.y, mx) << 8) | (snorm_code(f.z, mx) << 16) | (snorm_code(f.w, mx) << 24);
-        if ((w[u] & 7) == 0) (isv ? vs : ks)[at / 8] = mx;
-    }
+    const WordAt at(a);
+    if (at.t >= a.T) return;                               // whole groups of eight lanes
+    const float4 f = reinterpret_cast<const float4*>(isv ? v : k)[(size_t)at.t * a.rowg * 8 + at.w];
+    const long row = place_row(a, at.t);
+    const float mx = fmaxf(group_max_contig<4>(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)))), 1e-12f);
+    if (row < 0) return;
+    const size_t to = (size_t)row * a.rowg * 8 + at.w;
+    (isv ? vq : kq)[to] = snorm_code(f.x, mx) | (snorm_code(f.y, mx) << 8) | (snorm_code(f.z, mx) << 16) | (snorm_code(f.w, mx) << 24);
+    if ((at.w & 7) == 0) (isv ? vs : ks)[to / 8] = mx;
 }
 
 __global__ __launch_bounds__(256) void k_kv_read_paged(PlaceArgs a, const uint32_t* __restrict__ kq, const float* __restrict__ ks,
                                                        const uint32_t* __restrict__ vq, const float* __restrict__ vs,
                                                        float* __restrict__ k, float* __restrict__ v) {
     const bool isv = blockIdx.y;
-    const uint32_t* codes = isv ? vq : kq;
-    const float* scales = isv ? vs : ks;
-    float4* out = reinterpret_cast<float4*>(isv ? v : k);
-    uint32_t c[WORDS / 256];
-    float s[WORDS / 256];
-    long dst[WORDS / 256];
-#pragma unroll
-    for (int u = 0; u < WORDS / 256; u++) {
-        const WordAt at(a, threadIdx.x + 256 * u);
-        const bool in = at.t < a.T;
-        const long row = in ? place_row(a, at.t) : -1;
-        const size_t g = (size_t)(row < 0 ? 0 : row) * a.rowg * 8 + at.w;
-        c[u] = row < 0 ? 0u : codes[g];
-        s[u] = row < 0 ? 0.0f : scales[g / 8];
-        dst[u] = in ? (long)at.t * a.rowg * 8 + at.w : -1;
+    const WordAt at(a);
+    if (at.t >= a.T) return;
+    const long row = place_row(a, at.t);
+    v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row >= 0) {
+        const size_t from = (size_t)row * a.rowg * 8 + at.w;
+        const uint32_t c = (isv ? vq : kq)[from];
+        const float f = (isv ? vs : ks)[from / 8] / 127.0f;
+        x = v4f{(float)(int8_t)c * f, (float)(int8_t)(c >> 8) * f, (float)(int8_t)(c >> 16) * f, (float)(int8_t)(c >> 24) * f};
     }
-#pragma unroll
-    for (int u = 0; u < WORDS / 256; u++) {
-        if (dst[u] < 0) continue;
-        const float f = s[u] / 127.0f;
-        out[dst[u]] = make_float4((float)(int8_t)c[u] * f, (float)(int8_t)(c[u] >> 8) * f, (float)(int8_t)(c[u] >> 16) * f,
-                                  (float)(int8_t)(c[u] >> 24) * f);
-    }
+    __builtin_nontemporal_store(x, reinterpret_cast<v4f*>(isv ? v : k) + (size_t)at.t * a.rowg * 8 + at.w);
 }
 
-dim3 word_grid(const PlaceArgs& a) { return dim3((unsigned)(((long)a.T * a.rowg * 8 + WORDS - 1) / WORDS), 2); }
+dim3 word_grid(const PlaceArgs& a) { return dim3((unsigned)(((long)a.T * a.rowg * 8 + 255) / 256), 2); }
 
 int place_args(PlaceArgs& a, const char* fn, const int32_t* table, const int32_t* seq, const int32_t* pos, int T, int B,
                int nKv, int hd, int page, int pages, int width) {
@@ -108,7 +81,7 @@ int place_args(PlaceArgs& a, const char* fn, const int32_t* table, const int32_t
     TI_REQUIRE((long)page * (table ? width : pages) <= 0x7fffffffL, "%s: %d pages of %d hold more than 2^31 - 1 positions", fn,
                table ? width : pages, page);
     TI_REQUIRE(seq || table == nullptr || T <= B, "%s: %d rows without sequence numbers, %d sequences", fn, T, B);
-    TI_REQUIRE((long)T * nKv * (hd / 32) <= 0x3fffffffL, "%s: %d rows of %d heads in one call", fn, T, nKv);
+    TI_REQUIRE((long)T * nKv * (hd / 32) <= 0x0fffffffL, "%s: %d rows of %d heads in one call", fn, T, nKv);
     a.pg = TiPages{table, ti_log2(page), pages, width};
     a.seq = table ? seq : nullptr;
     a.pos = pos;
