@@ -9,8 +9,10 @@
 //    nothing depends on them on the host.
 //  - A wave takes a block at a time, on its own, loaded straight into LDS of its own; 12 waves a CU cover each other's
 //    loads (16 have too few registers: 57 us for 32 ragged sequences against 49).
-//    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16 to 2^-22 of
-//    the row's largest element, the row scaled by a power of two), each group's sum times its key's scale in f32. A
+//    S^T = K Q^T, one v_mfma_f32_16x16x32_f16 per 32-dim group, 16 keys and q half (q = hi + lo in f16, the
+//    row scaled by a power of two: an element is off by 2^-22 of itself or 2^-28 of the row's largest, which the f32 sum of
+//    hd products loses anyway unless a key's scales make up for a group 2^10 below it; three bf16 would be exact for half as
+//    many products again), each group's sum times its key's scale in f32. A
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
 //    P times the V scale of (key, group) in f32, as three bf16, exactly; V through the transposing LDS read.
 //  - The waves' (m, l, O) meet in LDS; the workgroups' partials in k_token_merge.

@@ -6,7 +6,8 @@
 // (K codes f16, V codes bf16, exact), the next block's loads in flight meanwhile; a wave passes over the 32 keys that none of its
 // rows sees and masks only where an edge of the window cuts them.
 //   - S^T = K Q^T (v_mfma_f32_16x16x32_f16 per 32-dim group, q half and 16 keys; the row scaled by a power of two, q =
-//     hi + lo to 2^-22 of its largest element), each group's sum times its key's scale in f32.
+//     hi + lo to 2^-22 of each element or 2^-28 of the row's largest, see k_token_attn.hip), each group's sum times its key's
+//     scale in f32.
 //   - O^T = V^T P^T with P times the V scale of (key, group) in f32 as three bf16, exactly; a lane's scores are the
 //     operand as they stand.
 // Bound by VALU work, most of it the weights': 4096 tokens of 16 heads of 128 dims under a window of 1024 in 137 us (220
