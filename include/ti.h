@@ -489,8 +489,9 @@ int ti_attn_causal_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
 /* Attention under a sliding window with sinks: query t (position p = pos0 + t) sees the keys j <= p with
  * j > p - window or j < sinks; window < 0 is no window (ti_attn_causal_q8's keys), window = 0 leaves the sinks
  * alone. A query that sees nothing gives zeros. qr/out are [T][nHq][hd], the cache is the contiguous one of
- * positions 0 .. pos0+T-1; keys that no query sees are not read. T = 1 is a decode step, any T a prompt or a
- * chunk of one. nHq <= 64, T * nHq < 2^23; out must not overlap qr. */
+ * positions 0 .. pos0+T-1, and what it holds where no query sees it does not matter. T = 1 is a decode step, any T a
+ * prompt or a chunk of one. In these calls hd is a multiple of 32 up to 128, kq and vq 16-byte aligned. nHq <= 64,
+ * T * nHq < 2^23; out must not overlap qr. */
 int ti_attn_window_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks,
                       const uint32_t* vq, const float* vs, float* out,
                       int T, int pos0, int nHq, int nKv, int hd, int window, int sinks);
@@ -537,7 +538,7 @@ int ti_attn_mass_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const floa
  * slots at `keep` and above move into the freed ones below it, the i-th into the i-th; the others stay. The cache rows
  * from `keep` on are left as they were. mass_out / where_out [keep][nKv] receive what the slots now hold (keep
  * at most n); they are the input buffers themselves, or do not overlap them. Keys keep the rotation of their own
- * positions, so attention over the slots 0 .. keep-1 needs no more than their count. nKv <= 64. */
+ * positions, so attention over the slots 0 .. keep-1 needs no more than their count. nKv <= 64, n * nKv <= 16000000. */
 int ti_kv_evict_q8(ti_ctx* ctx, uint32_t* kq, float* ks, uint32_t* vq, float* vs, const float* mass,
                    const int32_t* where, float* mass_out, int32_t* where_out, int n, int known, int keep,
                    int sinks, int recent, int next, int nKv, int hd);

@@ -223,6 +223,25 @@ def test_one_slot_too_many(ctx, n, known, nKv, kind):
         b.free()
 
 
+def test_half_of_a_million_slots(ctx):
+    """A head's slots go through the select in many chunks, equal masses among them."""
+    rng = np.random.default_rng(6)
+    n, keep, nKv, hd = 1_000_000, 500_000, 1, 32
+    mass = rng.integers(0, 3000, (n, nKv)).astype(np.float32)
+    kc, ks, vc, vs = ref.cache(rng, n, nKv, hd)
+    dev = [ctx.upload(a) for a in (kc, ks, vc, vs, mass)]
+    mo, wo = ctx.zeros(keep * 4), ctx.zeros(keep * 4)
+    ctx.call("ti_kv_evict_q8", *dev, None, mo, wo, n, 0, keep, 4, 1000, n, nKv, hd)
+    src, pos = ref.evict(mass, None, n, 0, keep, 4, 1000, n)
+    h = np.arange(nKv)[None]
+    assert np.array_equal(ctx.download(wo, np.int32, keep).reshape(keep, 1), pos)
+    for d, a in zip(dev[:4] + [mo], (kc, ks, vc, vs, mass)):
+        got = ctx.download(d, a.dtype, keep * a[0].size).reshape((keep,) + a.shape[1:])
+        assert np.array_equal(got, a[src, h])
+    for x in dev + [mo, wo]:
+        x.free()
+
+
 def test_a_cache_without_a_table_needs_no_sequences(ctx):
     rng = np.random.default_rng(1)
     T, nKv, hd = 4, 2, 64

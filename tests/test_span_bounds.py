@@ -128,3 +128,16 @@ def test_blocks_loaded_into_a_waves_lds_are_fenced():
     assert "s_waitcnt(0x0F70)" in src[i:read] and "ti_wave_lds_fence();" in src[i:read]
     last = src.rindex("W.v[", i, nxt)
     assert "s_waitcnt(0xC07F)" in src[last:nxt] and "ti_wave_lds_fence();" in src[last:nxt]
+
+
+def test_an_eviction_beyond_the_scratch_is_refused():
+    """What the header promises fits (n * nKv up to 16 million, half of the slots moved) is half of a call that does not."""
+    ctx = C.addressof(C.create_string_buffer(1 << 16))
+    for n, nKv in ((4_200_000, 8), (525_000, 64), (33_600_000, 1)):
+        args = [P] * 8 + [n, 0, n // 2, 2, 8, n, nKv, 64]
+        assert abi.lib().ti_kv_evict_q8(ctx, *args) == abi.TI_ERR_INVALID
+        assert b"exceed the scratch" in abi.lib().ti_last_error()
+    for n, nKv in ((16_000_000, 1), (2_000_000, 8), (250_000, 64)):
+        keep = n // 2
+        words = 2 * nKv * ((keep + 63) // 64) + nKv + 2 * nKv * keep + nKv * n
+        assert words <= 512 * 512 * 128
