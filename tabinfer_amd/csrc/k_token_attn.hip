@@ -62,9 +62,7 @@ __host__ __device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
 template <bool PAGED>
 __device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // position of the sequence's last query
     if (!PAGED) return a.p.pos0 + a.p.T - 1;
-    const long most = (long)a.p.pg.width << a.p.pg.shift;
-    const int n = a.p.lens[b];
-    return (int)(n < most ? n : most) - 1;
+    return ti_last_pos(a.p.lens[b], (long)a.p.pg.width << a.p.pg.shift);
 }
 template <bool PAGED>
 __device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int last) {   // the keys that any of its queries sees

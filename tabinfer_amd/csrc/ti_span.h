@@ -43,6 +43,8 @@ struct TiPages {
         return id >= 0 && id < pages ? ((long)id << shift) + (pos & ((1 << shift) - 1)) : -1;
     }
 };
+// Position of a sequence's last query: of `len` keys, taken as at most `most` of them; -1 where there is none, whatever the length
+TI_HD inline int ti_last_pos(int len, long most) { return len <= 0 ? -1 : (int)ti_min((long)len, most) - 1; }
 inline bool ti_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
 inline int ti_log2(int v) { return 31 - __builtin_clz((unsigned)v); }
 static inline bool ti_al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
