@@ -319,6 +319,8 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     TI_CHECK_CTX(c);
     TI_REQUIRE(kq && ks && vq && vs && mass && mass_out && where_out, "ti_kv_evict_q8: null buffer");
     TI_REQUIRE(ti_al16(kq) && ti_al16(vq), "ti_kv_evict_q8: kq/vq must be 16-byte aligned");
+    TI_REQUIRE_DENSE("ti_kv_evict_q8", kq);
+    TI_REQUIRE_DENSE("ti_kv_evict_q8", vq);
     TI_REQUIRE(n > 0 && keep > 0 && nKv > 0 && nKv <= TI_ATTN_HEADS_MAX && hd > 0 && hd % 32 == 0 && hd <= TI_ATTN_HD_MAX,
                "ti_kv_evict_q8: bad shape (n=%d keep=%d nKv=%d hd=%d)", n, keep, nKv, hd);
     TI_REQUIRE(known >= 0 && known <= n && (where || known == 0), "ti_kv_evict_q8: %d slots with a known position of %d", known, n);

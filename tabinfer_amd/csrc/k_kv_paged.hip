@@ -99,6 +99,8 @@ extern "C" int ti_kv_write_paged_q8(ti_ctx* c, const float* kr, const float* v, 
     TI_CHECK_CTX(c);
     TI_REQUIRE(kr && v && kq && ks && vq && vs && pos, "ti_kv_write_paged_q8: null buffer");
     TI_REQUIRE(ti_al16(kr) && ti_al16(v) && ti_al16(kq) && ti_al16(vq), "ti_kv_write_paged_q8: kr, v, kq and vq must be 16-byte aligned");
+    TI_REQUIRE_DENSE("ti_kv_write_paged_q8", kq);
+    TI_REQUIRE_DENSE("ti_kv_write_paged_q8", vq);
     PlaceArgs a;
     const int rc = place_args(a, "ti_kv_write_paged_q8", table, seq, pos, T, B, nKv, hd, page, pages, width);
     if (rc) return rc;
@@ -113,6 +115,8 @@ extern "C" int ti_kv_read_paged_q8(ti_ctx* c, const uint32_t* kq, const float* k
     TI_CHECK_CTX(c);
     TI_REQUIRE(kq && ks && vq && vs && pos && k && v, "ti_kv_read_paged_q8: null buffer");
     TI_REQUIRE(ti_al16(kq) && ti_al16(vq) && ti_al16(k) && ti_al16(v), "ti_kv_read_paged_q8: kq, vq, k and v must be 16-byte aligned");
+    TI_REQUIRE_DENSE("ti_kv_read_paged_q8", kq);
+    TI_REQUIRE_DENSE("ti_kv_read_paged_q8", vq);
     PlaceArgs a;
     const int rc = place_args(a, "ti_kv_read_paged_q8", table, seq, pos, T, B, nKv, hd, page, pages, width);
     if (rc) return rc;

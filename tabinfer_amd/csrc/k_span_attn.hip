@@ -23,6 +23,8 @@ int check_attn(const char* fn, const void* qr, const void* kq, const void* ks, c
                fn, n, nHq, nKv);
     TI_REQUIRE(hd > 0 && hd % 32 == 0 && hd <= TI_ATTN_HD_MAX, "%s: hd must be a multiple of 32 and <= %d", fn, TI_ATTN_HD_MAX);
     TI_REQUIRE(ti_al16(kq) && ti_al16(vq), "%s: kq/vq must be 16-byte aligned", fn);
+    TI_REQUIRE_DENSE(fn, kq);
+    TI_REQUIRE_DENSE(fn, vq);
     return TI_OK;
 }
 

@@ -73,6 +73,12 @@ struct ti_graph {
 #define TI_SYNC_ATTN_EPOCH 1      // word of a KV head's counter line: the epoch of its q/k/v hand-off
 #define TI_QKV_PUB_WORDS 16384    // KV heads x (query heads per KV head + 2) x head_dim, at most
 
+// Code slots of a cached position where p points into a decoder's K or V codes that have a spare one (ti_qwen3_kv_layout),
+// else 0. Calls that take codes of n KV heads a position refuse such a buffer: they would read other rows, silently
+int ti_padded_codes(const void* p);
+#define TI_REQUIRE_DENSE(fn, codes) do { const int _s = ti_padded_codes(codes); \
+    TI_REQUIRE(_s == 0, "%s: " #codes " is a decoder's cache of %d code slots a position (ti_qwen3_kv_layout), not one slot a KV head", fn, _s); } while (0)
+
 // ---- the T-token forward (2 <= T <= 16) ---------------------------------------------
 // Input of a T-token projection: int8 codes (xq [T][K/4], xs [T][K/32]) or, with x set,
 // the f32 activation x [T][K] that the kernel RMS-normalises (weight nw, eps) and

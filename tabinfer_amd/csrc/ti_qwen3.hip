@@ -10,6 +10,7 @@
 #include "ti_internal.h"
 #include <string.h>
 #include <stdio.h>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -159,7 +160,12 @@ struct ti_qwen3 {
     int pos_hint = 0;            // the position last set from the host (set_pos, or a forward's end)
     int kvs = 0;                 // K/V code slots per cached position (ti_qwen3_kv_layout)
     std::vector<void*> allocs;
+    ti_qwen3* other = nullptr;   // the next one of live_models
 };
+
+// The decoders there are, for ti_padded_codes: a list through the models, so that it allocates nothing
+static std::mutex live_lock;
+static ti_qwen3* live_models = nullptr;
 
 // The decoder's K/V code rows carry one spare head slot per position when there are 4 or
 // more KV heads: a head's 128-byte slice then moves to the next slot of the row from one
@@ -323,6 +329,11 @@ extern "C" int ti_qwen3_create(ti_ctx* c, const ti_qwen3_config* cfg, ti_qwen3**
         if (e != hipSuccess) rc = ti_hip_fail(e, "ti_qwen3_create clear");
     }
     if (rc) { release(m); return rc; }
+    {
+        std::lock_guard<std::mutex> hold(live_lock);
+        m->other = live_models;
+        live_models = m;
+    }
     *out = m;
     return TI_OK;
 }
@@ -332,8 +343,27 @@ extern "C" int ti_qwen3_destroy(ti_ctx* c, ti_qwen3* m) {
     if (!m) return TI_OK;
     TI_REQUIRE(!c->capturing, "ti_qwen3_destroy: not during graph capture");
     TI_HIP(hipStreamSynchronize(c->stream));
+    {                                                          // looked up, not looked into: it may be gone
+        std::lock_guard<std::mutex> hold(live_lock);
+        ti_qwen3** p = &live_models;
+        while (*p && *p != m) p = &(*p)->other;
+        TI_REQUIRE(*p, "ti_qwen3_destroy: no such decoder");
+        *p = m->other;
+    }
     release(m);
     return TI_OK;
+}
+
+int ti_padded_codes(const void* p) {
+    std::lock_guard<std::mutex> hold(live_lock);
+    for (const ti_qwen3* m = live_models; m; m = m->other) {
+        if (m->kvs == m->cfg.n_kv_heads) continue;
+        const size_t bytes = (size_t)m->cfg.max_ctx * m->kvs * m->cfg.head_dim;
+        for (const Layer& y : m->L)
+            for (const uint32_t* codes : {y.kq, y.vq})
+                if ((uintptr_t)p - (uintptr_t)codes < bytes) return m->kvs;
+    }
+    return 0;
 }
 
 // Tensor names follow the Hugging Face checkpoint (models/qwen3.js:3470, 3945-4049).
