@@ -11,12 +11,13 @@
 // across workgroups would cost a launch a digit (about 5 us each). 1024 threads: of an earlier version for 4097 and
 // 16384 slots 512 took 20.1 and 28.1 us where 1024 took 17.2 and 22.2, and 256 29.3 and 54.3 (more keys a thread, in turn).
 #include "ti_dev.h"
+#include "ti_evict.h"
 #include "ti_span.h"
 
 namespace {
 
 constexpr int SEL = 1024;       // threads of a head's workgroup
-constexpr int FORMED = 2048;    // up to so many slots it forms their keys itself, see k_evict_keys
+constexpr int FORMED = TI_EVICT_FORMED;     // see k_evict_keys
 
 struct EvictArgs {
     uint8_t* kq;
@@ -328,18 +329,14 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
                sinks, recent, keep);
     TI_REQUIRE(next >= n - known, "ti_kv_evict_q8: %d slots without a known position before position %d", n - known, next);
     const int kept = keep < n ? keep : n;
-    const int room = kept < n - kept ? kept : n - kept;      // moves of a head, at most
-    const int words = (kept + 63) / 64;
-    // scratch: the slots that stay, the moves' counts, the moves, the keys of many slots
     const bool single = n - kept == 1, many = n > FORMED;
-    const long need = 2L * nKv * words + nKv + 2L * nKv * room + (many ? (long)nKv * n : 0);
-    TI_REQUIRE(need <= (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch", n, room);
-    uint64_t* stays = reinterpret_cast<uint64_t*>(c->attn_po);
-    int32_t* count = reinterpret_cast<int32_t*>(stays + (size_t)nKv * words);
-    int32_t* moves = count + nKv;
-    EvictArgs a = {reinterpret_cast<uint8_t*>(kq), ks, reinterpret_cast<uint8_t*>(vq), vs, mass, where, mass_out, where_out, moves, count,
-                   reinterpret_cast<uint32_t*>(moves + 2 * (size_t)nKv * room), stays, n, known, kept, sinks,
-                   recent > next ? 0 : next - recent, next, nKv, hd, room, words};
+    const TiEvictScratch at(n, kept, nKv);
+    const int room = at.room;
+    TI_REQUIRE(at.fits(), "ti_kv_evict_q8: %d slots and %d moves a head exceed the scratch", n, room);
+    int32_t* scratch = reinterpret_cast<int32_t*>(c->attn_po);
+    EvictArgs a = {reinterpret_cast<uint8_t*>(kq), ks, reinterpret_cast<uint8_t*>(vq), vs, mass, where, mass_out, where_out,
+                   scratch + at.moves, scratch + at.count, reinterpret_cast<uint32_t*>(scratch + at.keys), reinterpret_cast<uint64_t*>(scratch),
+                   n, known, kept, sinks, recent > next ? 0 : next - recent, next, nKv, hd, room, at.words};
     if (room == 0) {
         k_evict_none<<<(unsigned)(((long)n * nKv + 255) / 256), 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_evict_none");

@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include "ti_host.h"
+#include "ti_limits.h"
 
 // ---- host-side error plumbing (ti_fail, TI_REQUIRE: ti_host.h) -----------------
 int ti_hip_fail(hipError_t e, const char* what);
@@ -50,14 +51,9 @@ struct ti_graph {
 };
 
 // Scratch capacities (elements). Activation rows up to 65536 wide, up to 256
-// tokens for the batched path; split-KV partials for (query rows x splits) <= 512 x 512.
+// tokens for the batched path; the attention's: ti_limits.h.
 #define TI_ACT_CAP 65536
 #define TI_ACT_TMAX 256
-#define TI_ATTN_HEADS_MAX 64
-#define TI_ATTN_ROWS_MAX 4096     // T * nHq of one attention call (a 256-token prefill of 16 heads)
-#define TI_ATTN_SPLITS_MAX 512
-#define TI_ATTN_ROWSPLITS (512 * 512)   // (T * nHq) x splits of one call: the partials' capacity
-#define TI_ATTN_HD_MAX 128
 #define TI_AMAX_PARTS 1024
 #define TI_MOE_P_MAX 8192
 #define TI_MOE_E_MAX 256
