@@ -38,9 +38,8 @@ extern "C" int ti_attn_window_q8(ti_ctx* c, const float* qr, const uint32_t* kq,
     TI_REQUIRE(pos0 >= 0 && pos0 <= TI_POS_END - T && sinks >= 0, "ti_attn_window_q8: bad positions (T=%d pos0=%d sinks=%d)", T, pos0, sinks);
     TI_REQUIRE((long)T * nHq <= 0x7fffffffL / 256, "ti_attn_window_q8: %d x %d query rows in one call", T, nHq);
     if (few_rows(T, nHq / nKv)) {
-        const long keys = window < 0 ? (long)pos0 + T : ti_min((long)pos0 + T, (long)window + sinks + T);
         const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
-                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, keys, nullptr, nullptr, 0};
+                               TiPages{nullptr, 0, 0, 0}, nullptr, 1, T, pos0, nHq, nKv, window, sinks, 0, nullptr, nullptr, 0};
         return ti_token_attn_launch(c, p, hd);
     }
     const TiWindowAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
@@ -78,7 +77,7 @@ extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, c
     const uint8_t *k8 = reinterpret_cast<const uint8_t*>(kq), *v8 = reinterpret_cast<const uint8_t*>(vq);
     if (T > 1) return ti_mass_attn_launch(c, TiWindowAttn{qr, k8, ks, v8, vs, out, T, pos0, nHq, nKv, -1, 0}, hd, mass);
     // the scores go to the upper half of the partials' scratch
-    const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, pos0 + 1L, mass,
+    const TiTokenAttn t = {qr, k8, ks, v8, vs, out, TiPages{nullptr, 0, 0, 0}, nullptr, 1, 1, pos0, nHq, nKv, -1, 0, 0, mass,
                            c->attn_po + MASS_SCORES, (pos0 + 32L) / 32 * 32};
     return ti_token_attn_launch(c, t, hd);
 }

@@ -16,8 +16,8 @@
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
 //    P times the V scale of (key, group) in f32, as three bf16, exactly; V through the transposing LDS read.
 //  - The waves' (m, l, O) meet in LDS; the workgroups' partials in k_token_merge.
-//  - Bound by the stream where the keys are many (32 ragged sequences of 8 heads of 128 dims, 211 MB: 49.6 + 4.8 us, 4.2
-//    TB/s with the merge where a copy reaches 4.9), else by its round trips (length, table, rows) and the second launch: 4100
+//  - Bound by the stream where the keys are many (32 ragged sequences of 8 heads of 128 dims, 211 MB: 49.6 + 4.8 us: 4.3
+//    TB/s, 3.9 with the merge), else by its round trips (length, table, rows) and the second launch: 4100
 //    keys 8.3 + 4.2 us, one sequence of 8191 over pages 11.6 + 4.4.
 //  - A row that sees nothing has m = -inf; one that sees only scores of -inf has the finite floor, and gives NaN as the formula does.
 #include "ti_dev.h"

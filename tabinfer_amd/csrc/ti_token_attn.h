@@ -15,7 +15,7 @@ struct TiTokenAttn {
     TiPages pg;
     const int32_t* lens;                     // keys of each sequence (pages); else the one sequence's queries are at pos0 ..
     int B, T, pos0, nHq, nKv, window, sinks;
-    long max_keys;                           // keys that a sequence's queries can see, at most
+    long max_keys;                           // of a sequence over pages: keys that its query can see, at most
     float* mass;                             // of one token of one sequence: mass[j nKv + h] (+)= the weights of key j, or nullptr
     float* scores;                           // [nHq][sstride] room for its scores in log2
     long sstride;
