@@ -83,8 +83,9 @@ __global__ __launch_bounds__(256) void k_evict_keys(EvictArgs a) {
     a.keys[(size_t)h * a.n + i] = order_key(a, slot_pos(a, i, h), a.mass[x]);
 }
 
-// A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 32 every key stays in a register, more slots
-// go through in chunks, read again for each digit; no more registers than the slots need (4097 slots 11.6 us with 8, 15.2
+// A workgroup a head. Slot i = 1024 k + tid of a chunk of 1024 x KPT; up to KPT = 16 every key stays in a register, more slots
+// go through in chunks of 16, read again for each digit (32 keys a thread spill: 17000 slots to 4096 42.4 us against 34.6 in chunks, 32000
+// to 8000 46.8 / 34.8, 100000 to 25000 171 / 121); no more registers than the slots need (4097 slots 11.6 us with 8, 15.2
 // with 16). The keep-th largest key by a radix select of 11, 11 and 10 bits: a histogram in LDS, its bins added
 // up from the top, and only the keys with the digits so far go on; done as soon
 // as all of these are kept (16384 slots of 8 heads to 4096: 22 us, all three digits' passes, to 20). Lanes of a wave that all have one digit count as one, so
@@ -352,8 +353,7 @@ extern "C" int ti_kv_evict_q8(ti_ctx* c, uint32_t* kq, float* ks, uint32_t* vq, 
     else if (single) k_evict_one<true><<<nKv, SEL, 0, c->stream>>>(a, placed);
     else if (n <= FORMED) k_evict_pick<FORMED / SEL, true><<<nKv, SEL, 0, c->stream>>>(a);
     else if (n <= 8 * SEL) k_evict_pick<8, false><<<nKv, SEL, 0, c->stream>>>(a);
-    else if (n <= 16 * SEL) k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
-    else k_evict_pick<32, false><<<nKv, SEL, 0, c->stream>>>(a);
+    else k_evict_pick<16, false><<<nKv, SEL, 0, c->stream>>>(a);
     TI_LAUNCHED("k_evict_pick");
     if (single && placed) return TI_OK;
     const int per_head = (room + 15) / 16, sblocks = placed ? 0 : (int)(((long)kept * nKv + 255) / 256);
