@@ -487,7 +487,10 @@ int ti_attn_causal_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const fl
 /* ---- a bounded and a shared int8 KV cache ------------------------------------------------
  * No reference counterparts: the reference keeps the whole of one conversation in one buffer. The codes have one slot
  * a KV head and position, as ti_kv_write_q8 and ti_attn_prep_q8 write them. The cache of a ti_qwen3 of four and more KV heads
- * has a spare slot (ti_qwen3_kv_layout); these calls refuse it, and the decoder's own steps make none of them. */
+ * has a spare slot (ti_qwen3_kv_layout); these calls refuse it, and the decoder's own steps make none of them.
+ * Positions that are arguments (pos0; an eviction's n, known and next) are the host's: a captured call replays with those
+ * of its capture. The paged calls read theirs on the device: a captured step of one conversation is one of B = 1
+ * over a table of its own. */
 /* Attention under a sliding window with sinks: query t (position p = pos0 + t) sees the keys j <= p with
  * j > p - window or j < sinks; window < 0 is no window (ti_attn_causal_q8's keys), window = 0 leaves the sinks
  * alone. A query that sees nothing gives zeros. qr/out are [T][nHq][hd], the cache is the contiguous one of

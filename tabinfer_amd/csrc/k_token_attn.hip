@@ -678,8 +678,10 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     const int rows = tile_rows(hd, true) >= a.R ? tile_rows(hd, true) : 16;
     a.RT = (a.R + rows - 1) / rows;
     static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS, "the sequences' slots fit the scratch");
-    // four heads of a position together where their number allows it: more of each 1 KB row at a time (32 ragged sequences of
-    // 8 heads, 211 MB, one head a wave of 1 / 2 / 4: 72 / 61 / 56 us)
+    // four heads of a position together where their number allows it: more of each 1 KB row at a time, though one head a workgroup
+    // would join four blocks in LDS. Kernel + merge of 8 heads of 128 dims, a head a wave of 1 / 4: 32 ragged sequences (211 MB) 71.2 + 4.8 /
+    // 50.0 + 4.9 us, one token of 4100 keys 9.5 + 4.0 / 8.8 + 4.0, of 8191 in pages of 16 13.3 + 3.9 / 12.2 + 4.2, with the weights added up
+    // 8.2 + 4.5 / 7.4 + 5.2; 8 windowed sequences of 64 dims 18.3 + 3.9 / 13.7 + 3.9
     a.HW = p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
     a.BW = WAVES / a.HW;
     // the workgroups that the CUs hold at once (three; two of those with a column a row); as many as there are sequences,
