@@ -419,7 +419,8 @@ int ti_qwen3_kv(ti_qwen3* m, int layer, uint32_t** kq, float** ks, uint32_t** vq
  * reference's. Codes: [max_ctx][slots][head_dim] int8, where *slots >= n_kv_heads; the
  * decoder keeps one spare head slot per position (with 4 or more KV heads), so that a
  * head's slice does not sit at the same offset of every row (no reference counterpart:
- * the reference's cache is its own buffer). Head h of position p is slot h. */
+ * the reference's cache is its own buffer). Head h of position p is slot h. The stand-alone calls on a cache
+ * (ti_kv_write_q8, ti_attn_prep_q8, ti_attn_*_q8, ...) take codes without a spare slot. */
 int ti_qwen3_kv_layout(const ti_qwen3* m, int* slots);
 /* kvQuantWrite (models/qwen3.js:2180-2216) into the decoder's own cache of `layer`: rows
  * [pos, pos+T) from the roped K rows kr and the V rows v ([T][n_kv_heads*head_dim] f32,
