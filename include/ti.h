@@ -529,6 +529,19 @@ int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const flo
                      const uint32_t* vq, const float* vs, const int32_t* table, const int32_t* lens,
                      float* out, int B, int nHq, int nKv, int hd, int page, int pages, int width,
                      int window, int sinks);
+/* attnPrepQ8 (ti_attn_prep_q8) for T rows of any sequences, into the pages: row t of q ([T] rows of nHq heads) normed (qn_w, f16;
+ * NULL: not) and rotated at rot[t] (rot NULL: at pos[t]) into row t of qr ([T][nHq][hd]), whether its place exists or not; row t of k
+ * likewise (kn_w) and of v as it is, quantized into position pos[t] of sequence seq[t]. The operations are ti_attn_prep_q8's in its order, the
+ * angles rot * theta^(-2i/hd) of 64 bits. table, seq, pos, places that do not exist and rows of one place as
+ * ti_kv_write_paged_q8's; rot is any number: after an eviction a token's slot is not its position. ldq floats from one row of q to
+ * the next, ldkv of k and of v (0: dense; multiples of 4, at least a row's heads): q, k and v may be parts of one projection's rows. nHq 0:
+ * K and V alone, q and qr NULL. qr is q itself (dense rows) or does not overlap it. nHq and nKv <= 64; theta >= 1; q, k, v, qr, kq and
+ * vq 16-byte, the norms' weights 8-byte aligned; T times the (nHq + 2 nKv) hd / 1024 of a row, rounded up, < 2^24. */
+int ti_attn_prep_paged_q8(ti_ctx* ctx, const float* q, const float* k, const float* v, const uint16_t* qn_w,
+                          const uint16_t* kn_w, float* qr, uint32_t* kq, float* ks, uint32_t* vq, float* vs,
+                          const int32_t* table, const int32_t* seq, const int32_t* pos, const int32_t* rot, int T, int B,
+                          int nHq, int nKv, int hd, int page, int pages, int width, int ldq, int ldkv, float theta,
+                          float eps);
 /* ti_attn_causal_q8 that also adds up the attention each key receives: mass[j*nKv + h] += the softmax weights of key j
  * summed over the T queries and the nHq/nKv query heads of KV head h. The slots pos0 .. pos0+T-1, the call's own
  * tokens, are set instead (no earlier query saw them), so a mass buffer needs no clearing. pos0 is a slot of the

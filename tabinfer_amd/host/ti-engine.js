@@ -198,6 +198,12 @@ function createEngine({ device = 0 } = {}) {
     attnPagedQ8(qrBuf, kv, table, lensBuf, oBuf, nHq, nKv, hd, window = -1, sinks = 0) {
       TI.attn_paged_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, table.buf, lensBuf, oBuf, table.B, nHq, nKv, hd, kv.page, kv.pages, table.width, window, sinks);
     },
+    // rows of q, k and v of any sequences: norm, rotation (at rotBuf's positions, or posBuf's), k and v into the pages;
+    // ldq / ldkv: floats a row where q, k and v are parts of wider rows
+    attnPrepPagedQ8(qBuf, kBuf, vBuf, qwBuf, kwBuf, qrBuf, kv, table, seqBuf, posBuf, rotBuf, T, nHq, nKv, hd, theta, eps, ldq = 0, ldkv = 0) {
+      TI.attn_prep_paged_q8(ctx, U(qBuf), kBuf, vBuf, U(qwBuf), U(kwBuf), U(qrBuf), kv.kq, kv.ks, kv.vq, kv.vs, table.buf, U(seqBuf), posBuf, U(rotBuf),
+        T, table.B, nHq, nKv, hd, kv.page, kv.pages, table.width, ldq, ldkv, theta, eps);
+    },
     attnMassQ8(qrBuf, kv, oBuf, massBuf, T, pos0, nHq, nKv, hd) {
       TI.attn_mass_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, oBuf, massBuf, T, pos0, nHq, nKv, hd);
     },
