@@ -176,6 +176,14 @@ int ti_argmax(ti_ctx* ctx, const float* logits, int N, uint32_t* tok_hist, int o
  * place; ti_argmax of the result samples softmax(logits / temp). `seed` is the already
  * advanced seed of this step (the reference advances _rngSeed before each call). */
 int ti_gumbel_noise(ti_ctx* ctx, float* logits, int N, uint32_t seed, float temp);
+/* Log probabilities under T rows of N logits, ld apart (0: N), in one pass (no reference counterpart). lp[t] =
+ * log softmax(row t)[ids[t]]; -inf where ids[t] is outside [0, N). May be NULL: entropy[t] = -sum p log p of the row, in nats; rank[t] = 1 + the
+ * number of logits above the token's (0 for an id outside). top_ids / top_lp [T][top] (NULL for top = 0): the likeliest tokens, larger
+ * logits first, equal ones by the lower index (not ti_argmax's order, and without its bound of -3e38), and their log probabilities. A logit of -inf
+ * has no probability and counts as a candidate, after all others. A NaN is no candidate and makes the row's lp, entropy and top_lp NaN; so does
+ * +inf, and a row of nothing but -inf. Missing candidates: id -1, log probability -inf. T <= 131072, top <= 64 and <= N. */
+int ti_logprobs(ti_ctx* ctx, const float* logits, const int32_t* ids, float* lp, float* entropy, int32_t* rank,
+                int32_t* top_ids, float* top_lp, int T, int N, int ld, int top);
 /* embedGather (models/qwen3.js:1663-1676): y[t] = f32(emb[ids[id_off+t]]), t < T. */
 int ti_embed(ti_ctx* ctx, const int32_t* ids, const uint16_t* emb, float* y, int T, int H, int id_off, int vocab);
 

@@ -66,6 +66,7 @@ SIGS = {
     "ti_rmsnorm_gateup_silu_q4": [_p, _p, _p, _f, _p, _p, _p, _p, _p, _i, _i, _p, _p],
     "ti_rmsnorm_lm_head_argmax": [_p, _p, _p, _f, _p, _p, _p, _i, _i, _p, _i],
     "ti_argmax": [_p, _p, _i, _p, _i],
+    "ti_logprobs": [_p] * 8 + [_i] * 4,
     "ti_gumbel_noise": [_p, _p, _i, C.c_uint32, _f],
     "ti_embed": [_p, _p, _p, _p, _i, _i, _i, _i],
     "ti_attn_step_q8": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _f, _i, _p, _p],

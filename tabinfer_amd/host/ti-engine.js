@@ -178,6 +178,10 @@ function createEngine({ device = 0 } = {}) {
       TI.rope_qk(ctx, xBuf, U(wBuf), outBuf, T, nH, hd, pos0, theta, eps);
     },
     argmaxKernel(logitsBuf, outBuf, N, outPos) { TI.argmax(ctx, logitsBuf, N, outBuf, outPos); },          // :2681
+    // out: {lp, entropy, rank, topIds, topLp}, all but lp optional
+    logprobs(logitsBuf, idsBuf, out, T, N, top = 0, ld = 0) {
+      TI.logprobs(ctx, logitsBuf, idsBuf, out.lp, U(out.entropy), U(out.rank), U(out.topIds), U(out.topLp), T, N, ld, top);
+    },
     embedGather(idsBuf, embRec, yBuf, T, H, idOff) {                                                       // :1663
       TI.embed(ctx, idsBuf, embRec.buf, yBuf, T, H, idOff | 0, embRec.vocab);
     },
