@@ -60,6 +60,7 @@ SIGS = {
     "ti_gemv_q4_q8": [_p, _p, _p, _p, _p, _p, _i, _i, _i],
     "ti_gemv_q4_f32": [_p, _p, _p, _p, _p, _i, _i, _i],
     "ti_gateup_silu_q4": [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i],
+    "ti_lora_add": [_p] * 7 + [_i] * 8,
     "ti_linear_q4": [_p, _p, _p, _p, _p, _i, _i, _i, _i],
     "ti_group_dots_q4_q8": [_p, _p, _p, _p, _i, _i],
     "ti_rmsnorm_gemv_q4": [_p, _p, _p, _f, _i, _i, _p, _p, _p, _p, _p, _p],

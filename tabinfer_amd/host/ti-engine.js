@@ -178,6 +178,11 @@ function createEngine({ device = 0 } = {}) {
       TI.rope_qk(ctx, xBuf, U(wBuf), outBuf, T, nH, hd, pos0, theta, eps);
     },
     argmaxKernel(logitsBuf, outBuf, N, outPos) { TI.argmax(ctx, logitsBuf, N, outBuf, outPos); },          // :2681
+    // low-rank adapters beside a projection and log probabilities (no reference counterparts). adapters: {a, b, scale, n, r, K, N, bf16}
+    loraAdd(xBuf, idxBuf, adapters, yBuf, T, ldx = 0, ldy = 0) {
+      const { a, b, scale, n, r, K, N, bf16 } = adapters;
+      TI.lora_add(ctx, xBuf, idxBuf, a, b, scale, yBuf, T, K, N, r, n, ldx, ldy, b01(bf16));
+    },
     // out: {lp, entropy, rank, topIds, topLp}, all but lp optional
     logprobs(logitsBuf, idsBuf, out, T, N, top = 0, ld = 0) {
       TI.logprobs(ctx, logitsBuf, idsBuf, out.lp, U(out.entropy), U(out.rank), U(out.topIds), U(out.topLp), T, N, ld, top);
