@@ -557,6 +557,17 @@ int ti_attn_prep_paged_q8(ti_ctx* ctx, const float* q, const float* k, const flo
                           const int32_t* table, const int32_t* seq, const int32_t* pos, const int32_t* rot, int T, int B,
                           int nHq, int nKv, int hd, int page, int pages, int width, int ldq, int ldkv, float theta,
                           float eps);
+/* ti_attn_paged_q8 without a window for sequences in groups that share their first positions (a system prompt, samples of one
+ * prompt), which are read once a group. Group g of P holds the sequences starts[g] .. starts[g+1] - 1 (starts: P + 1 device numbers,
+ * not falling, of [0, B]); its positions 0 .. shared[g] - 1 are looked up in the table's row of its first sequence, the others in each sequence's
+ * own. lens[b] counts all of a sequence's keys; a sequence shorter than what its group shares sees the first of them. Sequences of
+ * no group, or alone in theirs, share nothing. starts and shared are read on the device, as table and lens. P <= B <= 2048;
+ * B (nHq + G nKv) + 16 nKv min(P, B/2) and room for the workgroups' partials within 262144 rows (G = nHq/nKv; 512 sequences of 16
+ * heads over 8 in any groups are); out must not overlap qr. */
+int ti_attn_shared_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks, const uint32_t* vq,
+                      const float* vs, const int32_t* table, const int32_t* lens, const int32_t* starts,
+                      const int32_t* shared, float* out, int B, int P, int nHq, int nKv, int hd, int page, int pages,
+                      int width);
 /* ti_attn_causal_q8 that also adds up the attention each key receives: mass[j*nKv + h] += the softmax weights of key j
  * summed over the T queries and the nHq/nKv query heads of KV head h. The slots pos0 .. pos0+T-1, the call's own
  * tokens, are set instead (no earlier query saw them), so a mass buffer needs no clearing. pos0 is a slot of the

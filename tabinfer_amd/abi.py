@@ -113,6 +113,7 @@ SIGS = {
     "ti_kv_read_paged_q8": [_p] * 10 + [_i] * 7,
     "ti_attn_paged_q8": [_p] * 9 + [_i] * 9,
     "ti_attn_prep_paged_q8": [_p] * 15 + [_i] * 10 + [_f] * 2,
+    "ti_attn_shared_q8": [_p] * 11 + [_i] * 8,
     "ti_attn_mass_q8": [_p] * 8 + [_i] * 5,
     "ti_kv_evict_q8": [_p] * 9 + [_i] * 8,
 }

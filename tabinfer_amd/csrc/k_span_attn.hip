@@ -64,6 +64,22 @@ extern "C" int ti_attn_paged_q8(ti_ctx* c, const float* qr, const uint32_t* kq, 
     return ti_token_attn_launch(c, p, hd);
 }
 
+extern "C" int ti_attn_shared_q8(ti_ctx* c, const float* qr, const uint32_t* kq, const float* ks, const uint32_t* vq, const float* vs,
+                                 const int32_t* table, const int32_t* lens, const int32_t* starts, const int32_t* shared, float* out, int B,
+                                 int P, int nHq, int nKv, int hd, int page, int pages, int width) {
+    TI_CHECK_CTX(c);
+    const int rc = check_attn("ti_attn_shared_q8", qr, kq, ks, vq, vs, out, B, nHq, nKv, hd);
+    if (rc) return rc;
+    TI_REQUIRE(table && lens && starts && shared, "ti_attn_shared_q8: null table, lengths or groups");
+    TI_REQUIRE(B <= TI_TOKEN_SEQS && P > 0 && P <= B, "ti_attn_shared_q8: %d sequences > %d, or %d groups of them", B, TI_TOKEN_SEQS, P);
+    TI_REQUIRE(ti_pow2(page) && pages > 0 && width > 0 && (long)page * width <= TI_POS_END,
+               "ti_attn_shared_q8: bad pages (length %d, a power of two; %d of them; table width %d)", page, pages, width);
+    const TiTokenAttn p = {qr, reinterpret_cast<const uint8_t*>(kq), ks, reinterpret_cast<const uint8_t*>(vq), vs, out,
+                           TiPages{table, ti_log2(page), pages, width}, lens, B, 1, 0, nHq, nKv, -1, 0, (long)page * width, nullptr, nullptr, 0,
+                           starts, shared, P};
+    return ti_group_attn_launch(c, p, hd);
+}
+
 extern "C" int ti_attn_mass_q8(ti_ctx* c, const float* qr, const uint32_t* kq, const float* ks, const uint32_t* vq, const float* vs,
                                float* out, float* mass, int T, int pos0, int nHq, int nKv, int hd) {
     TI_CHECK_CTX(c);

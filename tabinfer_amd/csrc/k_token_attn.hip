@@ -36,6 +36,10 @@ constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr float FLOOR = -3.402823466e38f;
 constexpr float PSCALE = 0x1p-24f;           // of every weight in P V: 127 x a V scale x thousands of keys stays in f32's range
 
+// Which keys a launch is about: a contiguous cache's; pages'; of sequences in groups that share their first positions, each
+// sequence's own, or the groups' shared ones, for all rows of a group
+enum Keys { LINE, PAGES, OWN, SHARED };
+
 struct TokArgs {
     TiTokenAttn p;
     float* po;                               // [slot][nKv][T G][HD] partials, (m, l) of each
@@ -43,6 +47,9 @@ struct TokArgs {
     int32_t* meta;                           // [B][2]: a sequence's first slot and their number
     int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups of HW KV heads, at most
     int HW, BW;                              // a workgroup's waves: HW KV heads x BW blocks
+    float *spo, *spml;                       // the merge of groups: the same of the shared positions, [slot][nKv][tile's rows][HD]
+    int32_t* smeta;                          // [ti_group_tile][2]
+    int srows, sslots;                       // rows of their tiles; slots
 };
 
 // Blocks that hold the keys [0, first) and [low, end): [0, sb) and [wb, sb + ... )
@@ -59,22 +66,37 @@ __host__ __device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
     return b;
 }
 
-template <bool PAGED>
-__device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // position of the sequence's last query
-    if (!PAGED) return a.p.pos0 + a.p.T - 1;
-    return ti_last_pos(a.p.lens[b], (long)a.p.pg.width << a.p.pg.shift);
+__device__ __forceinline__ int page_end(const TokArgs& a, int len) {    // position behind a sequence's last that there can be
+    return ti_last_pos(len, (long)a.p.pg.width << a.p.pg.shift) + 1;
 }
-template <bool PAGED>
-__device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int last) {   // the keys that any of its queries sees
+template <Keys KEYS>
+__device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // position of the sequence's last query, or of a group's last shared key
+    if (KEYS == LINE) return a.p.pos0 + a.p.T - 1;
+    return page_end(a, KEYS == SHARED ? a.p.shared[b] : a.p.lens[b]) - 1;
+}
+template <Keys KEYS>
+__device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int b, int last) {   // the keys that any of its queries sees
+    if (KEYS == SHARED) return TiSpan{0, 0, last + 1};
+    if (KEYS == OWN) return TiSpan{0, ti_min(ti_group_base(a.p.starts, a.p.shared, a.p.P, a.p.B, b), last + 1), last + 1};
     TiSpan s = ti_span(last - (a.p.T - 1), a.p.window, a.p.sinks);
     s.end = last + 1;
     return s;
 }
 // blocks of a sequence; one (of nothing) where no key is visible, so that every sequence has a slot
-template <bool PAGED>
+template <Keys KEYS>
 __device__ __forceinline__ int seq_blocks(const TokArgs& a, int b) {
-    const int last = seq_last<PAGED>(a, b);
-    return last < 0 ? 1 : ti_max(1, blocks_of(seq_span<PAGED>(a, last)).n);
+    const int last = seq_last<KEYS>(a, b);
+    return last < 0 ? 1 : ti_max(1, blocks_of(seq_span<KEYS>(a, b, last)).n);
+}
+// a group's row tiles: none where there is nothing to share
+__device__ __forceinline__ int group_tiles(const TokArgs& a, int g) {
+    return (ti_group_members(a.p.starts, a.p.B, g).count * a.G + a.srows - 1) / a.srows;
+}
+template <Keys KEYS>
+__device__ __forceinline__ long unit_blocks(const TokArgs& a, int b) {  // of a sequence, or of all of a group's tiles
+    if (KEYS != SHARED) return seq_blocks<KEYS>(a, b);
+    const int tiles = group_tiles(a, b);
+    return tiles ? (long)tiles * seq_blocks<KEYS>(a, b) : 0;
 }
 
 // sum of the threads before this one, and of all of the workgroup
@@ -109,17 +131,18 @@ __device__ __forceinline__ long uniform(long v) {
 struct Run {
     long chunk, left;                        // blocks of every workgroup's run; of this one, still to do
     long start;
-    int b, block;
+    int b, block, tile;                      // groups: of b's row tiles, this one
 };
 // blocks of a run: an equal share, but a block for each of the BW waves of a head where the sequences have as many
 __host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs, int BW) {
     return ti_max((total + wgs - 1) / wgs, ti_min((long)BW, (total + B - 1) / B));
 }
-template <bool PAGED>
+template <Keys KEYS>
 __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, int* s_b) {
-    const int B = a.p.B, tid = threadIdx.x;
-    if (B == 1) {
-        const long n = seq_blocks<PAGED>(a, 0);
+    const int B = KEYS == SHARED ? a.p.P : a.p.B, tid = threadIdx.x;
+    r.tile = 0;
+    if (KEYS != SHARED && B == 1) {
+        const long n = seq_blocks<KEYS>(a, 0);
         r.chunk = run_chunk(n, 1, a.wgs, a.BW);
         r.b = 0;
         r.start = 0;
@@ -130,14 +153,14 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     // a thread: the sequences [tid per, tid per + per)
     const int per = (B + THREADS - 1) / THREADS, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
-    for (int b = b0; b < b1; b++) mine += seq_blocks<PAGED>(a, b);
+    for (int b = b0; b < b1; b++) mine += unit_blocks<KEYS>(a, b);
     long at = wg_scan(mine, s4, total);
     total = uniform(total);
     r.chunk = run_chunk(total, B, a.wgs, a.BW);
     const long g0 = w * r.chunk;
     if (g0 >= at && g0 < at + mine) {
         for (int b = b0; b < b1; b++) {
-            const int n = seq_blocks<PAGED>(a, b);
+            const long n = unit_blocks<KEYS>(a, b);
             if (g0 < at + n) {
                 *s_b = b;
                 *s_at = at;
@@ -151,6 +174,11 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     r.left = ti_min(r.chunk, total - g0);
     r.b = __builtin_amdgcn_readfirstlane(*s_b);
     r.start = uniform(*s_at);
+    if (KEYS == SHARED) {
+        const int n = seq_blocks<KEYS>(a, r.b);
+        r.tile = (int)((g0 - r.start) / n);
+        r.start += (long)r.tile * n;
+    }
     r.block = (int)(g0 - r.start);
     return true;
 }
@@ -212,8 +240,9 @@ __device__ __forceinline__ float slot_sum(float v) {
     return v;
 }
 
-template <int HD, bool PAGED, bool COLS>
+template <int HD, Keys KEYS, bool COLS>
 __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a) {
+    constexpr bool PAGED = KEYS != LINE;
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
@@ -223,13 +252,14 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the waves of a workgroup read HW heads of the same positions together: rows of a position lie side by side
     const int groups = a.p.nKv / a.HW, hr = blockIdx.x % (groups * a.RT), w = blockIdx.x / (groups * a.RT);
-    const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs, rt = hr / groups;
+    const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs;
+    int rt = hr / groups, R = a.R;
     Run run;
-    if (!find_run<PAGED>(a, w, run, L.s4, &L.at, &L.b)) return;        // workgroup-uniform
+    if (!find_run<KEYS>(a, w, run, L.s4, &L.at, &L.b)) return;         // workgroup-uniform
     const int r16 = lane & 15, j = lane >> 4;
 
     const int slot = r16 / ROWS, grp = ti_min(slot, NG - 1), tr = r16 % ROWS;   // this lane's column: row of the tile, group
-    const int rg = ti_min(rt * ROWS + tr, a.R - 1), t = rg / a.G, h = rg % a.G;
+    int rg = ti_min(rt * ROWS + tr, R - 1), t = rg / a.G, h = rg % a.G;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
     const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
@@ -248,22 +278,42 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
 
     for (;;) {
         // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
-        const int last = seq_last<PAGED>(a, run.b);
-        const TiSpan span = seq_span<PAGED>(a, last);
+        const int last = seq_last<KEYS>(a, run.b);
+        const TiSpan span = seq_span<KEYS>(a, run.b, last);
+        int tiles = 1, q0 = run.b * a.p.T, seq = run.b;        // of queries and table, the first row
+        if constexpr (KEYS == SHARED) {                        // rows: the group's sequences x query heads of a KV head
+            const TiMembers mb = ti_group_members(a.p.starts, a.p.B, run.b);
+            tiles = (mb.count * a.G + ROWS - 1) / ROWS;
+            q0 = seq = mb.first;
+            rt = run.tile;
+            R = mb.count * a.G;
+            rg = ti_min(rt * ROWS + tr, R - 1);
+            t = rg / a.G;
+            h = rg % a.G;
+        }
         Blocks bl = blocks_of(span);
         if (last < 0) bl.n = 0;
         const int nb = ti_max(1, bl.n);
         const int c0 = run.block, part = (int)ti_min((long)(nb - c0), run.left), c1 = ti_min(bl.n, c0 + part);
-        const int pos = last - (a.p.T - 1) + t;
-        const int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
+        int pos = last - (a.p.T - 1) + t;
+        int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
         // what every row of the tile sees: [full_low, full_end)
-        const int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
+        int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
+        if constexpr (KEYS == OWN) low = full_low = span.low;
+        if constexpr (KEYS == SHARED) {                        // a sequence may be shorter than what its group shares
+            pos = ti_min(last, page_end(a, a.p.lens[q0 + t]) - 1);
+            low = full_low = 0;
+            full_end = pos + 1;
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) full_end = ti_min(full_end, ti_xor(full_end, x));
+            full_end = __builtin_amdgcn_readfirstlane(full_end);
+        }
         // the query's loads before the keys': they come back first
         v4f_u qv[NQ][2];
         const int qc = j + 4 * (slot / 2);                     // COLS: the lane's 16 dims of the 64 that its column's group is in
         auto q_dim = [&](int x) { return COLS ? 16 * ti_min(qc, PC - 1) + 8 * x : 32 * x + 8 * j; };
         {
-            const float* q = a.p.qr + ((size_t)(run.b * a.p.T + t) * a.p.nHq + hk * a.G + h) * HD;
+            const float* q = a.p.qr + ((size_t)(q0 + t) * a.p.nHq + hk * a.G + h) * HD;
 #pragma unroll
             for (int x = 0; x < NQ; x++)
 #pragma unroll
@@ -276,7 +326,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
         auto fetch_page = [&](int i) -> int {
             if constexpr (!PAGED) return 0;
             const int k = ti_min((bl.at(i) * BLK + (lane & 31)) >> a.p.pg.shift, a.p.pg.width - 1);
-            return a.p.pg.table[(size_t)run.b * a.p.pg.width + k];
+            return a.p.pg.table[(size_t)seq * a.p.pg.width + k];
         };
         auto check_page = [&](int i, int id) -> int {
             const int key = bl.at(i) * BLK + (lane & 31);
@@ -436,7 +486,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                     seen |= ok ? 1u << e : 0u;
                 }
             }
-            if (a.p.mass && slot == 0 && rt * ROWS + tr < a.R) {
+            if (KEYS == LINE && a.p.mass && slot == 0 && rt * ROWS + tr < R) {
                 float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
                 *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
                 *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
@@ -525,7 +575,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
         for (int d = 0; d < HD / 16; d++)
             if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
         __syncthreads();
-        const int nr = ti_min(ROWS, a.R - rt * ROWS);
+        const int nr = ti_min(ROWS, R - rt * ROWS);
         for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
             const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, r = q % nr;
             float M = L.m[hh][r];
@@ -539,7 +589,8 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                 for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
                 y = fmaf(L.l[k][r], f, y);
             }
-            const size_t at = ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
+            const size_t at = KEYS == SHARED ? ((size_t)(w + ti_group_tile(q0, run.b, rt, a.G, ROWS)) * a.p.nKv + hk0 + hh) * ROWS + r
+                                             : ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
             *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
             if (d == 0) {
                 a.pml[2 * at] = M;
@@ -547,14 +598,20 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
             }
         }
         if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
-            a.meta[2 * run.b] = w + run.b;
-            a.meta[2 * run.b + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
+            const int u = KEYS == SHARED ? ti_group_tile(q0, run.b, rt, a.G, ROWS) : run.b;
+            a.meta[2 * u] = w + u;
+            a.meta[2 * u + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
         }
         run.left -= part;
         if (run.left <= 0) return;
-        run.b++;
         run.start += nb;
         run.block = 0;
+        if (++run.tile >= tiles) {
+            run.tile = 0;
+            run.b++;
+            if constexpr (KEYS == SHARED)
+                while (run.b < a.p.P - 1 && !group_tiles(a, run.b)) run.b++;
+        }
         __syncthreads();                                   // the parts are read
     }
 }
@@ -593,7 +650,7 @@ __device__ __forceinline__ void token_mass(const TokArgs& a, int ns, int part, i
 // A workgroup a (sequence, token, head) and DW of its dims: the slots' partials into the output row, each group of threads
 // those of its own slots with every load in flight at once. DW = 32 where whole rows leave CUs idle (16 rows of 128
 // dims: 4.1 us, whole rows 5.4)
-template <int HD, int DW>
+template <int HD, int DW, bool GROUPS>
 __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
     constexpr int D4 = DW / 4, SG = 256 / D4, UN = 8;
     __shared__ float s_m[SG], s_l[SG];
@@ -603,8 +660,23 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
     if (row >= rows) return token_mass(a, ns1, (row - rows) * gridDim.y + blockIdx.y, (gridDim.x - rows) * gridDim.y);
     const int hq = row % a.p.nHq, t = (row / a.p.nHq) % a.p.T, b = row / (a.p.nHq * a.p.T);
     const int hk = hq / a.G, r = t * a.G + hq % a.G;
-    const int s0 = ns1 ? 0 : a.meta[2 * b], ns = ns1 ? ns1 : a.meta[2 * b + 1];
+    const int s0 = ns1 ? 0 : a.meta[2 * b];
+    int ns = ns1 ? ns1 : a.meta[2 * b + 1];
     const size_t step = (size_t)a.p.nKv * a.R, base = (size_t)s0 * step + (size_t)hk * a.R + r;
+    // the group's slots behind the sequence's own
+    const int own = ns, g = GROUPS ? ti_group_of(a.p.starts, a.p.shared, a.p.P, a.p.B, b) : -1;
+    size_t sbase = 0;
+    const size_t sstep = (size_t)a.p.nKv * a.srows;
+    if (GROUPS && g >= 0) {
+        const int first = ti_group_members(a.p.starts, a.p.B, g).first, row_s = (b - first) * a.G + r;
+        const int u = ti_group_tile(first, g, row_s / a.srows, a.G, a.srows);
+        // groups that are out of order may have left numbers that do not belong together: none outside the scratch is followed
+        const int us = a.smeta[2 * u], un = a.smeta[2 * u + 1];
+        if (us >= 0 && un > 0 && us < a.sslots && un <= a.sslots - us) {
+            sbase = (size_t)us * sstep + (size_t)hk * a.srows + row_s % a.srows;
+            ns += un;
+        }
+    }
     float m = -INFINITY, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i0 = sg; i0 < ns && (256 % D4 == 0 || sg < SG); i0 += UN * SG) {
@@ -612,10 +684,13 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
         float mi[UN], li[UN];
 #pragma unroll
         for (int k = 0; k < UN; k++) {
-            const size_t at = base + (size_t)ti_min(i0 + k * SG, ns - 1) * step;
-            mi[k] = a.pml[2 * at];
-            li[k] = a.pml[2 * at + 1];
-            x[k] = *reinterpret_cast<const v4f*>(a.po + at * HD + d0 + 4 * d);
+            const int sl = ti_min(i0 + k * SG, ns - 1);
+            const bool shared = GROUPS && sl >= own;
+            const size_t at = shared ? sbase + (size_t)(sl - own) * sstep : base + (size_t)sl * step;
+            const float *ml = shared ? a.spml : a.pml, *po = shared ? a.spo : a.po;
+            mi[k] = ml[2 * at];
+            li[k] = ml[2 * at + 1];
+            x[k] = *reinterpret_cast<const v4f*>(po + at * HD + d0 + 4 * d);
         }
         float mn = m;
 #pragma unroll
@@ -653,22 +728,31 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
     a.p.out[(size_t)row * HD + d0 + tid] = M == -INFINITY ? 0.0f : v / (127.0f * PSCALE * Lt);
 }
 
-template <int HD, bool PAGED>
-void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
-    const unsigned grid = (unsigned)(wgs * a.RT * (a.p.nKv / a.HW));
-    if (HD == 32 || a.R <= tile_rows(HD, true)) k_token_attn<HD, PAGED, true><<<grid, THREADS, 0, c->stream>>>(a);
-    else if constexpr (HD > 32) k_token_attn<HD, PAGED, false><<<grid, THREADS, 0, c->stream>>>(a);
+template <int HD, Keys KEYS>
+void launch_attn(ti_ctx* c, const TokArgs& a, unsigned grid, bool cols) {
+    if (HD == 32 || cols) k_token_attn<HD, KEYS, true><<<grid, THREADS, 0, c->stream>>>(a);
+    else if constexpr (HD > 32) k_token_attn<HD, KEYS, false><<<grid, THREADS, 0, c->stream>>>(a);
+}
+template <int HD, bool GROUPS>
+void launch_merge(ti_ctx* c, const TokArgs& a, int ns1) {
     const int rows = a.p.B * a.p.T * a.p.nHq;
     // the weights' workgroups: two a CU at most, since each forms every head's sum
     const long n = a.p.mass ? ti_min(((a.p.pos0 + 1L) * a.p.nKv + 255) / 256, 2L * c->cus) : 0;
-    if (HD == 32 || rows >= c->cus) k_token_merge<HD, HD><<<rows + n, 256, 0, c->stream>>>(a, ns1);
-    else if constexpr (HD > 32) k_token_merge<HD, 32><<<dim3(rows + (n + HD / 32 - 1) / (HD / 32), HD / 32), 256, 0, c->stream>>>(a, ns1);
+    if (HD == 32 || rows >= c->cus) k_token_merge<HD, HD, GROUPS><<<rows + n, 256, 0, c->stream>>>(a, ns1);
+    else if constexpr (HD > 32) k_token_merge<HD, 32, GROUPS><<<dim3(rows + (n + HD / 32 - 1) / (HD / 32), HD / 32), 256, 0, c->stream>>>(a, ns1);
 }
+template <int HD, Keys KEYS>
+void launch(ti_ctx* c, const TokArgs& a, long wgs, int ns1) {
+    launch_attn<HD, KEYS>(c, a, (unsigned)(wgs * a.RT * (a.p.nKv / a.HW)), a.R <= tile_rows(HD, true));
+    launch_merge<HD, false>(c, a, ns1);
+}
+
+int heads_together(int nKv) { return nKv % 4 == 0 ? 4 : nKv % 2 == 0 ? 2 : 1; }
 
 }  // namespace
 
 int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
-    TokArgs a;
+    TokArgs a = {};
     a.p = p;
     a.po = c->attn_po;
     a.pml = c->attn_ml;
@@ -682,7 +766,7 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     // would join four blocks in LDS. Kernel + merge of 8 heads of 128 dims, a head a wave of 1 / 4: 32 ragged sequences (211 MB) 71.2 + 4.8 /
     // 50.0 + 4.9 us, one token of 4100 keys 9.5 + 4.0 / 8.8 + 4.0, of 8191 in pages of 16 13.3 + 3.9 / 12.2 + 4.2, with the weights added up
     // 8.2 + 4.5 / 7.4 + 5.2; 8 windowed sequences of 64 dims 18.3 + 3.9 / 13.7 + 3.9
-    a.HW = p.nKv % 4 == 0 ? 4 : p.nKv % 2 == 0 ? 2 : 1;
+    a.HW = heads_together(p.nKv);
     a.BW = WAVES / a.HW;
     // the workgroups that the CUs hold at once (three; two of those with a column a row); as many as there are sequences,
     // if that is more; as far as the partials' slots (one for each workgroup and one for each sequence) fit: half of the
@@ -704,9 +788,58 @@ int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
         const long most = p.max_keys / BLK + 3;            // blocks of a sequence, at most (three ragged ends)
         wgs = ti_min(wgs, p.B * most);
     }
-#define TOK(HD_) if (hd == HD_) { if (paged) launch<HD_, true>(c, a, wgs, ns1); else launch<HD_, false>(c, a, wgs, ns1); }
+#define TOK(HD_) if (hd == HD_) { if (paged) launch<HD_, PAGES>(c, a, wgs, ns1); else launch<HD_, LINE>(c, a, wgs, ns1); }
     TOK(128) TOK(96) TOK(64) TOK(32)
 #undef TOK
+    TI_LAUNCHED("k_token_attn");
+    return TI_OK;
+}
+
+// Groups' shared positions for all rows of the group, then each sequence's own, each as above, and one merge of both. The scratch: the
+// own partials' slots (one for each workgroup and sequence), behind them the shared ones' (one for each workgroup and place of a tile).
+int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
+    TokArgs a = {};
+    a.p = p;
+    a.G = p.nHq / p.nKv;
+    a.R = a.G;
+    const int crows = tile_rows(hd, true);
+    const int rows = crows >= a.R ? crows : 16;
+    a.RT = (a.R + rows - 1) / rows;
+    a.HW = heads_together(p.nKv);
+    a.BW = WAVES / a.HW;
+    a.srows = 16;
+    const int heads = p.nKv / a.HW, held = a.R <= crows ? 3 : 2;
+    const long places = ti_group_tile(p.B, p.P, 0, a.G, a.srows);
+    const long fixed = (long)p.B * p.nHq + places * p.nKv * a.srows;
+    long wgs = ti_max(((long)held * c->cus + heads * a.RT - 1) / (heads * a.RT), (long)p.B), swgs = (2L * c->cus + heads - 1) / heads;
+    const long room = TI_ATTN_ROWSPLITS - fixed;
+    wgs = ti_min(wgs, room / 2 / p.nHq);
+    swgs = ti_min(swgs, room / 2 / (p.nKv * a.srows));
+    TI_REQUIRE(wgs > 0 && swgs > 0, "ti_attn_shared_q8: %d sequences of %d heads in %d groups exceed the scratch", p.B, p.nHq, p.P);
+    const long most = p.max_keys / BLK + 3;
+    a.po = c->attn_po;
+    a.pml = c->attn_ml;
+    const size_t behind = (size_t)(wgs + p.B) * p.nHq;
+    a.spo = a.po + behind * hd;
+    a.spml = a.pml + 2 * behind;
+    a.meta = reinterpret_cast<int32_t*>(c->tg_part);
+    a.smeta = a.meta + 2 * p.B;
+    static_assert(TI_TG_SPLIT_BLOCKS * 2 * 256 >= 2 * TI_TOKEN_SEQS + 2 * (TI_TOKEN_SEQS * TI_ATTN_HEADS_MAX / 16 + TI_TOKEN_SEQS + 1), "the slots' numbers fit the scratch");
+    TokArgs s = a;
+    s.po = a.spo;
+    s.pml = a.spml;
+    s.meta = a.smeta;
+    s.wgs = (int)swgs;
+    a.wgs = (int)wgs;
+    a.sslots = s.sslots = (int)(swgs + places);
+    wgs = ti_min(wgs, p.B * most);
+    swgs = ti_min(swgs, places * most);
+#define GROUP(HD_) if (hd == HD_) { \
+        launch_attn<HD_, SHARED>(c, s, (unsigned)(swgs * heads), false); \
+        launch_attn<HD_, OWN>(c, a, (unsigned)(wgs * a.RT * heads), a.R <= crows); \
+        launch_merge<HD_, true>(c, a, 0); }
+    GROUP(128) GROUP(96) GROUP(64) GROUP(32)
+#undef GROUP
     TI_LAUNCHED("k_token_attn");
     return TI_OK;
 }

@@ -45,6 +45,38 @@ struct TiPages {
 };
 // Position of a sequence's last query: of `len` keys, taken as at most `most` of them; -1 where there is none, whatever the length
 TI_HD inline int ti_last_pos(int len, long most) { return len <= 0 ? -1 : (int)ti_min((long)len, most) - 1; }
+
+// Groups of sequences that share their first positions: group g holds the sequences [starts[g], starts[g + 1]) of B. One of a single
+// sequence shares nothing: it counts as empty. Whatever `starts` holds, members are of [0, B).
+struct TiMembers {
+    int first, count;
+};
+TI_HD inline TiMembers ti_group_members(const int32_t* starts, int B, int g) {
+    const int lo = ti_max(0, ti_min((int)starts[g], B)), n = ti_max(lo, ti_min((int)starts[g + 1], B)) - lo;
+    return TiMembers{lo, n > 1 ? n : 0};
+}
+// The group of sequence b, with something to share: -1 for none
+TI_HD inline int ti_group_of(const int32_t* starts, const int32_t* shared, int P, int B, int b) {
+    int lo = 0, hi = P;                      // the first group that begins behind b is in [lo, hi]
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (starts[mid] <= b) lo = mid + 1;
+        else hi = mid;
+    }
+    const int g = lo - 1;
+    if (g < 0 || b >= starts[g + 1] || shared[g] <= 0) return -1;
+    return ti_group_members(starts, B, g).count ? g : -1;
+}
+TI_HD inline int ti_group_base(const int32_t* starts, const int32_t* shared, int P, int B, int b) {   // positions that b shares
+    const int g = ti_group_of(starts, shared, P, B, b);
+    return g < 0 ? 0 : (int)shared[g];
+}
+// A number for tile `tile` of `rows` rows of group g, whose first sequence is `first` and whose sequences have G rows each: larger for
+// later tiles and later groups (a group of n G rows has at most one tile more than n G / rows, and takes one number more: groups with
+// something to share are at least two sequences apart). Below ti_group_tile(B, P, 0, G, rows) for those of P groups.
+TI_HD inline int ti_group_tile(int first, int g, int tile, int G, int rows) {
+    return (int)((long)first * G / rows) + ti_min(g, first / 2) + tile;
+}
 inline bool ti_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
 inline int ti_log2(int v) { return 31 - __builtin_clz((unsigned)v); }
 static inline bool ti_al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

@@ -19,5 +19,8 @@ struct TiTokenAttn {
     float* mass;                             // of one token of one sequence: mass[j nKv + h] (+)= the weights of key j, or nullptr
     float* scores;                           // [nHq][sstride] room for its scores in log2
     long sstride;
+    const int32_t *starts, *shared;          // groups of sequences (TiMembers), P of them, and the positions that each shares
+    int P;
 };
 int ti_token_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd);
+int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd);       // of one token a sequence, over pages, without a window

@@ -213,6 +213,10 @@ function createEngine({ device = 0 } = {}) {
       TI.attn_prep_paged_q8(ctx, U(qBuf), kBuf, vBuf, U(qwBuf), U(kwBuf), U(qrBuf), kv.kq, kv.ks, kv.vq, kv.vs, table.buf, U(seqBuf), posBuf, U(rotBuf),
         T, table.B, nHq, nKv, hd, kv.page, kv.pages, table.width, ldq, ldkv, theta, eps);
     },
+    // groups: {starts, shared, P}
+    attnSharedQ8(qrBuf, kv, table, lensBuf, groups, oBuf, nHq, nKv, hd) {
+      TI.attn_shared_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, table.buf, lensBuf, groups.starts, groups.shared, oBuf, table.B, groups.P, nHq, nKv, hd, kv.page, kv.pages, table.width);
+    },
     attnMassQ8(qrBuf, kv, oBuf, massBuf, T, pos0, nHq, nKv, hd) {
       TI.attn_mass_q8(ctx, qrBuf, kv.kq, kv.ks, kv.vq, kv.vs, oBuf, massBuf, T, pos0, nHq, nKv, hd);
     },

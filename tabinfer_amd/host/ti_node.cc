@@ -1569,6 +1569,7 @@ napi_value module_init(napi_env env, napi_value exports) {
         ENTRY("kv_read_paged_q8", ti_kv_read_paged_q8),
         ENTRY("attn_paged_q8", ti_attn_paged_q8),
         ENTRY("attn_prep_paged_q8", ti_attn_prep_paged_q8),
+        ENTRY("attn_shared_q8", ti_attn_shared_q8),
         ENTRY("lora_add", ti_lora_add),
         ENTRY("logprobs", ti_logprobs),
         ENTRY("attn_mass_q8", ti_attn_mass_q8),
