@@ -214,6 +214,10 @@ class DevBuf:
     def __int__(self):
         return self.ptr
 
+    @property
+    def _as_parameter_(self):
+        return self.ptr
+
     def free(self):
         if self.ptr:
             check(lib().ti_buf_free(self.ctx.h, self.ptr))
@@ -270,6 +274,10 @@ class Ctx:
     # ---- generic call ---------------------------------------------------------------
     def call(self, name, *args):
         fn = getattr(lib(), name)
+        try:                                    # ints, addresses and buffers go as they are
+            return check(fn(self.h, *args))
+        except C.ArgumentError:
+            pass
         conv = []
         for a in args:
             if isinstance(a, DevBuf):
