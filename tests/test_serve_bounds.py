@@ -30,7 +30,7 @@ REFUSED = {
     "ti_attn_shared_q8": (SHARED, [{i: None} for i in range(10)] + [{9: P}, {1: P + 8}, {3: P + 4}, {10: 0}, {10: 2049}, {11: 0}, {11: -1}, {11: 5}, {12: 3}, {12: 65, 13: 65}, {13: 0},
                           {14: 40}, {14: 160}, {15: 0}, {15: 12}, {16: 0}, {17: 0}, {17: 2 ** 27 + 1}, {10: 2048, 11: 2048, 12: 64, 13: 64}, {10: 2048, 11: 1, 12: 64, 13: 8}]),
     "ti_lora_add": (LORA, [{i: None} for i in range(6)] + [{0: P + 4}, {2: P + 8}, {3: P + 2}, {5: P}, {5: P + 64}, {6: 0}, {6: -1}, {7: 0}, {7: 40}, {8: 0}, {9: 0}, {9: 129}, {10: 0},
-                    {11: 60}, {11: 66}, {11: -64}, {12: 39}, {13: 2}, {13: -1}, {6: 2 ** 20 + 1, 5: Q * 64}, {6: 2 ** 19, 9: 128, 5: Q * 64}]),
+                    {11: 60}, {11: 66}, {11: -64}, {12: 39}, {13: 2}, {13: -1}, {6: 2 ** 18 + 1, 5: Q * 64}]),
     "ti_logprobs": (LP, [{i: None} for i in (0, 1, 2, 5, 6)] + [{7: 0}, {7: -1}, {7: 2 ** 17 + 1}, {8: 0}, {8: -5}, {8: IMAX}, {9: 99}, {9: -1}, {10: -1}, {10: 65}, {8: 4, 10: 5}]),
 }
 
