@@ -6,11 +6,13 @@
 // s' = a s, u' = a (u + (m - m') s), a = e^(m - m'); lanes, waves and workgroups are joined by the same rule in a fixed order.
 //
 // The likeliest: a value and its index are one 64-bit key (the float's bits in an order of whole numbers, then the inverted index: the lower
-// index wins), so that no two are equal. A wave takes 1024 elements at a time, in registers. Where fewer than `top` lanes hold something
-// above its last kept key, what is above it goes to a list in LDS; where as many do, as always at first, the limit is raised to the top-th
-// largest of the lanes' maxima, found bit by bit with ballots: no more than `top` lanes then hold anything to list, so that the list's room,
-// 16 keys a lane, is bounded whatever the values are. List and kept keys are ranked by counting. So all chunks but a wave's first
-// cost a comparison and little more.
+// index wins), so that no two are equal. A wave takes 1024 elements at a time, in registers. Where `top` lanes hold something above its
+// limit, as always at first, the limit is raised to the top-th largest of the lanes' maxima, found bit by bit with ballots; what is above it
+// goes to a list in LDS, of at most `top` lanes and so 16 top keys a chunk, whatever the values are. Where it has grown to more than 64 keys, and
+// at the end, the list is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
+// cost little more than a comparison. A workgroup sorts once, what is above the largest of its waves' limits.
+//
+// Long rows are cut into parts. Of up to 128 rows the workgroup that ends last joins a row's parts, of more a second launch does.
 #include "ti_dev.h"
 #include "ti_span.h"
 
@@ -20,6 +22,7 @@ typedef float v4f_u __attribute__((ext_vector_type(4), aligned(4)));   // rows s
 
 constexpr int EPT = 16, CHUNK = 64 * EPT, WAVES = 4, STEP = WAVES * CHUNK;     // elements of a lane, a wave's chunk, a workgroup's
 constexpr int TOP_MAX = 64;                  // one lane a kept key
+constexpr int LONG = 64;                     // keys after which a list is sorted
 constexpr int SEGS_MAX = 64;                 // workgroups a row: one lane each where they are joined
 constexpr int ROWS_MAX = 1 << 17;
 constexpr float LOW = -3.402823466e38f;
@@ -32,6 +35,7 @@ struct LpArgs {
     float* top_lp;
     float4* part;                            // [row][segs] (m, s, u, number of logits above the token's)
     uint64_t* keys;                          // [row][segs][top], from large to small, 0 behind the last
+    uint32_t* arrived;                       // a line a row, 0 between launches; or nullptr: a second launch joins the parts
     long ld;
     int T, N, top, segs, per;                // a row is cut into `segs` parts of `per` steps
 };
@@ -53,34 +57,59 @@ __device__ __forceinline__ Sum joined(const Sum& a, const Sum& b) {
     return {m, a.s * ea + b.s * eb, ea * (a.u + da * a.s) + eb * (b.u + db * b.s)};
 }
 __device__ __forceinline__ Sum wave_joined(Sum a) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = joined(a, Sum{ti_xor(a.m, o), ti_xor(a.s, o), ti_xor(a.u, o)});
-    return a;
+    // the maximum first, so that every lane turns its own to it once; the offsets spelled out, as ti_wave_sum's
+    const float m = ti_wave_max(a.m), d = down_to(a.m - m), e = expf(d);
+    return {m, ti_wave_sum(a.s * e), ti_wave_sum(e * (a.u + d * a.s))};
 }
 
-// a wave's keys: kept ones from large to small, 0 behind the last, and a list
-struct Kept {
-    uint64_t *now, *next, *list;
-};
-// `n` listed keys into the kept ones
-__device__ __forceinline__ void keep(Kept& k, int n, int top) {
+// ---- 64 keys, a lane each, from large to small ---------------------------------------------------------------------
+__device__ __forceinline__ uint64_t key_xor(uint64_t k, int o) {
+    return (uint64_t)ti_xor((uint32_t)(k >> 32), o) << 32 | ti_xor((uint32_t)k, o);
+}
+// lanes O apart: the one without bit O takes the larger key where `down`, the smaller elsewhere
+template <int O>
+__device__ __forceinline__ uint64_t exchange(uint64_t k, bool down) {
+    const uint64_t other = key_xor(k, O);
+    const bool first = (threadIdx.x & O) == 0;
+    return (other > k) == (first == down) ? other : k;
+}
+// a sequence that rises and falls once (in every 2 O lanes), sorted
+template <int O>
+__device__ __forceinline__ uint64_t merged(uint64_t k, bool down) {
+    k = exchange<O>(k, down);
+    if constexpr (O > 1) k = merged<O / 2>(k, down);
+    return k;
+}
+template <int O>
+__device__ __forceinline__ uint64_t sorted(uint64_t k) {   // in every 2 O lanes, down and up in turn
+    if constexpr (O > 1) k = sorted<O / 2>(k);
+    return merged<O>(k, (threadIdx.x & 63 & 2 * O) == 0);
+}
+// the 64 largest of two sorted 64, the second from small to large
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t up) { return merged<32>(a > up ? a : up, true); }
+// 64 keys in any order into the kept ones
+__device__ __forceinline__ uint64_t taken(uint64_t kept, uint64_t k) {
+    k = merged<32>(sorted<16>(k), false);                  // from small to large
+    return larger(kept, k);
+}
+// the first keys that are kept: n of them, in the lowest lanes
+__device__ __forceinline__ uint64_t taken_first(uint64_t k, int n) {
+    k = sorted<8>(k);
+    if (n > 16) {
+        k = merged<16>(k, (threadIdx.x & 32) == 0);
+        if (n > 32) k = merged<32>(k, true);
+    }
+    return k;
+}
+// a wave's list into its kept keys
+__device__ __forceinline__ uint64_t taken(uint64_t kept, const uint64_t* list, int n) {
     const int lane = threadIdx.x & 63;
     ti_wave_lds_fence();
-    if (lane < top) k.next[lane] = 0;
+    for (int j = 0; j < n; j += 64) kept = taken(kept, j + lane < n ? list[j + lane] : 0ull);
     ti_wave_lds_fence();
-    for (int j = lane; j < n + top; j += 64) {
-        const uint64_t key = j < top ? k.now[j] : k.list[j - top];
-        if (key == 0) continue;
-        int rank = 0;
-        for (int i = 0; i < top; i++) rank += k.now[i] > key;
-        for (int i = 0; i < n; i++) rank += k.list[i] > key;
-        if (rank < top) k.next[rank] = key;
-    }
-    ti_wave_lds_fence();
-    uint64_t* t = k.now;
-    k.now = k.next;
-    k.next = t;
+    return kept;
 }
+__device__ __forceinline__ uint32_t value_at(uint64_t kept, int i) { return __builtin_amdgcn_readlane((uint32_t)(kept >> 32), i); }
 
 // what a row's numbers come to, and its likeliest tokens' (key of lane i the i-th)
 __device__ __forceinline__ void finish(const LpArgs& a, int t, const Sum& r, int above, uint64_t key) {
@@ -100,11 +129,58 @@ __device__ __forceinline__ void finish(const LpArgs& a, int t, const Sum& r, int
     }
 }
 
+// The m-th largest value that 64 lanes hold, m <= 64 (0 where fewer hold one); `held`: lanes that reach it. Bit by bit with ballots
+__device__ __forceinline__ uint32_t value_of_rank(uint32_t v, int m, int& held) {
+    uint32_t limit = 0;
+    held = 65;
+    for (uint32_t bit = 0x80000000u; bit && held > m; bit >>= 1) {
+        const int n = __builtin_popcountll(__ballot(v >= (limit | bit)));
+        if (n >= m) {
+            limit |= bit;
+            held = n;
+        }
+    }
+    return limit;
+}
+
+// A row's parts, by a workgroup: their numbers, a lane of the first wave each, and their keys, 64 at a time. (Only those above what the parts' j-th
+// keys show to be unwanted, in a list: 48 rows with 20 tokens 26.1 us against 23.2, one row 12.9 against 13.6.) PUB: other workgroups of
+// this launch wrote them
+template <bool PUB>
+__device__ __forceinline__ void join_parts(const LpArgs& a, int t, uint64_t (*s_waves)[64]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = a.segs * a.top;
+    const bool has = lane < a.segs;
+    const float* q = reinterpret_cast<const float*>(a.part + (size_t)t * a.segs + ti_min(lane, a.segs - 1));
+    const uint64_t* keys = a.keys + (size_t)t * n;
+    auto number = [&](int i) { return PUB ? ti_pub_load(q + i) : q[i]; };
+    const float m = number(0), sum = number(1), u = number(2), above = number(3);
+    auto load = [&](int j) {
+        const uint64_t* k = keys + ti_min(j + lane, n - 1);
+        const uint64_t key = PUB ? ti_pub_load(k) : *k;
+        return j + lane < n ? key : 0ull;
+    };
+    uint64_t kept = 0;
+    if (64 * wave < n) kept = taken_first(load(64 * wave), ti_min(64, n - 64 * wave));
+    for (int j = 64 * (wave + WAVES); j < n; j += 64 * WAVES) kept = taken(kept, load(j));
+    if (n > 64) {
+        if (wave > 0) s_waves[wave - 1][63 - lane] = kept;
+        __syncthreads();
+    }
+    if (wave != 0) return;
+    if (n > 64)
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; w++) kept = larger(kept, s_waves[w][lane]);
+    const Sum r = wave_joined(has ? Sum{m, sum, u} : Sum{LOW, 0.0f, 0.0f});
+    finish(a, t, r, ti_wave_sum_i(has ? __float_as_int(above) : 0), kept);
+}
+
 template <bool TOP>
 __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
     extern __shared__ __align__(16) uint64_t s_keys[];
     __shared__ Sum s_sum[WAVES];
-    __shared__ int s_above[WAVES];
+    __shared__ int s_above[WAVES], s_all, s_last;
+    __shared__ uint32_t s_limit[WAVES];
+    __shared__ uint64_t s_waves[2 * WAVES][64];            // the waves' lists and kept keys; later three waves' parts
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = blockIdx.x / a.segs, seg = blockIdx.x % a.segs, top = a.top;
     const float* x = a.x + t * a.ld;
@@ -112,15 +188,10 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
     const float xi = id >= 0 && id < a.N ? x[id] : INFINITY;
     const long begin = (long)seg * a.per * STEP;
     const int end = (int)ti_min((long)a.N, begin + (long)a.per * STEP);
-    Kept kept;
-    if constexpr (TOP) {
-        kept.now = s_keys + wave * (EPT + 2) * top;
-        kept.next = kept.now + top;
-        kept.list = kept.next + top;
-        if (lane < top) kept.now[lane] = 0;
-        ti_wave_lds_fence();
-    }
-    uint32_t last = 0;                                     // the kept keys' last value: what comes later has to be larger
+    uint64_t* list = s_keys + wave * (EPT * top + LONG);   // what a chunk adds at most, behind what is there
+    uint64_t kept = 0;
+    int listed = 0;
+    uint32_t last = 0;                                     // a value that `top` keys so far reach: what comes later has to be larger
     Sum r = {LOW, 0.0f, 0.0f};
     int above = 0;
     auto load = [&](long at, float (&v)[EPT]) {
@@ -149,9 +220,10 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
 #pragma unroll
             for (int i = 0; i < EPT; i++) v[i] = 256 * (i / 4) + i % 4 < in ? v[i] : -INFINITY;
         }
-        float m = r.m;
+        float most = v[0];
 #pragma unroll
-        for (int i = 0; i < EPT; i++) m = fmaxf(m, v[i]);
+        for (int i = 1; i < EPT; i++) most = fmaxf(most, v[i]);
+        const float m = fmaxf(r.m, most);
         const float d = down_to(r.m - m), f = expf(d);
         r.u = f * (r.u + d * r.s);
         r.s = f * r.s;
@@ -164,22 +236,46 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
             above += v[i] > xi;
         }
         if constexpr (TOP) {
+            const uint64_t lanes = __ballot(last == 0 || most > value_of(last));
+            if (lanes == 0) continue;
+            if (last != 0 && __builtin_popcountll(lanes) < top) {
+                const float least = value_of(last);
+#pragma unroll
+                for (int i = 0; i < EPT; i++) {
+                    const bool take = v[i] > least;        // no NaN, nothing behind the row's end
+                    const uint64_t who = __ballot(take);
+                    if (who == 0) continue;
+                    if (take) list[listed + __builtin_popcountll(who & ((1ull << lane) - 1))] = key_of(ordered(v[i]), (uint32_t)(at + 256 * (i / 4) + 4 * lane + i % 4));
+                    listed += __builtin_popcountll(who);
+                }
+                if (listed > LONG) {
+                    kept = taken(kept, list, listed);
+                    listed = 0;
+                    last = max(last, value_at(kept, top - 1));
+                }
+                continue;
+            }
             uint32_t u[EPT], mine = 0;
 #pragma unroll
             for (int i = 0; i < EPT; i++) {
                 u[i] = 256 * (i / 4) + i % 4 < in ? ordered(v[i]) : 0u;
                 mine = max(mine, u[i]);
             }
-            if (!__any(mine > last)) continue;
             uint32_t limit = last, place = 0xffffffffu;    // listed: above the limit, or at it up to this place in the chunk
             bool ties = false;
             if (__builtin_popcountll(__ballot(mine > last)) >= top) {
                 limit = 0;
-                for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-                    if (__builtin_popcountll(__ballot(mine >= (limit | bit))) >= top) limit |= bit;
+                int held = 65;                             // lanes at or above the limit
+                for (uint32_t bit = 0x80000000u; bit && held > top; bit >>= 1) {
+                    const int n = __builtin_popcountll(__ballot(mine >= (limit | bit)));
+                    if (n >= top) {
+                        limit |= bit;
+                        held = n;
+                    }
+                }
                 ties = true;
                 const int more = __builtin_popcountll(__ballot(mine > limit));
-                if (__builtin_popcountll(__ballot(mine >= limit)) > top) {
+                if (held > top) {
                     // lanes whose maxima are equal: those whose first is at the lowest places
                     uint32_t first = 0xffffffffu;
 #pragma unroll
@@ -191,17 +287,20 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
                         if (more + __builtin_popcountll(__ballot(first < (place | bit))) < top) place |= bit;
                 }
             }
-            int n = 0;
 #pragma unroll
             for (int i = 0; i < EPT; i++) {
                 const uint32_t p = 256 * (i / 4) + 4 * lane + i % 4;
                 const bool take = u[i] > limit || (ties && u[i] == limit && p <= place);
                 const uint64_t who = __ballot(take);
-                if (take) kept.list[n + __builtin_popcountll(who & ((1ull << lane) - 1))] = key_of(u[i], (uint32_t)(at + p));
-                n += __builtin_popcountll(who);
+                if (take) list[listed + __builtin_popcountll(who & ((1ull << lane) - 1))] = key_of(u[i], (uint32_t)(at + p));
+                listed += __builtin_popcountll(who);
             }
-            keep(kept, n, top);
-            last = (uint32_t)(kept.now[top - 1] >> 32);
+            last = limit;
+            if (listed > LONG) {
+                kept = taken(kept, list, listed);
+                listed = 0;
+                last = max(last, value_at(kept, top - 1));
+            }
         }
     }
     r = wave_joined(r);
@@ -209,65 +308,65 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
     if (lane == 0) {
         s_sum[wave] = r;
         s_above[wave] = above;
+        s_limit[wave] = last;
+        if (wave == 0) s_all = 0;
     }
     __syncthreads();
     r = joined(joined(s_sum[0], s_sum[1]), joined(s_sum[2], s_sum[3]));
     above = (s_above[0] + s_above[1]) + (s_above[2] + s_above[3]);
     uint64_t key = 0;
     if constexpr (TOP) {
-        // the waves' kept keys, ranked into the first wave's list
-        const int tid = threadIdx.x;
-        uint64_t* out = s_keys + WAVES * (EPT + 2) * top;
-        uint64_t* all = out + top;
-        if (tid < top) out[tid] = 0;
-        if (lane < top) all[wave * top + lane] = kept.now[lane];
-        __syncthreads();
-        if (tid < 4 * top && all[tid]) {
-            int rank = 0;
-            for (int i = 0; i < 4 * top; i++) rank += all[i] > all[tid];
-            if (rank < top) out[rank] = all[tid];
+        // what reaches the largest of the waves' limits, in any order
+        const uint32_t limit = max(max(s_limit[0], s_limit[1]), max(s_limit[2], s_limit[3]));
+        uint64_t* all = &s_waves[0][0];
+        ti_wave_lds_fence();
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint64_t k = half ? lane < top ? kept : 0ull : lane < listed ? list[lane] : 0ull;
+            const bool take = k && (uint32_t)(k >> 32) >= limit;
+            const uint64_t who = __ballot(take);
+            if (who == 0) continue;
+            int first = 0;
+            if (lane == 0) first = __hip_atomic_fetch_add(&s_all, __builtin_popcountll(who), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            first = __builtin_amdgcn_readfirstlane(first);
+            if (take) all[first + __builtin_popcountll(who & ((1ull << lane) - 1))] = k;
         }
         __syncthreads();
-        if (lane < top) key = out[lane];
+        if (wave == 0) {
+            const int n = s_all;
+            key = taken_first(lane < n ? all[lane] : 0ull, n);
+            if (n > 64) key = taken(key, all + 64, n - 64);
+            key = lane < top ? key : 0;
+        }
     }
-    if (wave != 0) return;
-    if (a.segs == 1) return finish(a, t, r, above, key);
+    if (a.segs == 1) {
+        if (wave == 0) finish(a, t, r, above, key);
+        return;
+    }
     const size_t p = (size_t)t * a.segs + seg;
-    if (lane == 0) a.part[p] = make_float4(r.m, r.s, r.u, __int_as_float(above));
-    if (TOP && lane < top) a.keys[p * top + lane] = key;
+    float* q = reinterpret_cast<float*>(a.part + p);
+    if (!a.arrived) {
+        if (wave != 0) return;
+        if (lane == 0) *reinterpret_cast<float4*>(q) = make_float4(r.m, r.s, r.u, __int_as_float(above));
+        if (TOP && lane < top) a.keys[p * top + lane] = key;
+        return;
+    }
+    if (wave == 0) {
+        const float number = lane == 0 ? r.m : lane == 1 ? r.s : lane == 2 ? r.u : __int_as_float(above);
+        if (lane < 4) ti_pub_store(q + lane, number);
+        if (TOP && lane < top) ti_pub_store(a.keys + p * top + lane, key);
+        ti_stores_done();
+        if (lane == 0) s_last = ti_arrive(a.arrived + t * TI_SYNC_LOGPROBS_STRIDE) == (uint32_t)(a.segs - 1);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) ti_pub_store(a.arrived + t * TI_SYNC_LOGPROBS_STRIDE, 0u);
+    join_parts<true>(a, t, s_waves);
 }
 
-// A wave a row: its parts' numbers, a lane each, and of their keys the largest of the heads, `top` times
 __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
-    const int lane = threadIdx.x & 63, t = blockIdx.x * WAVES + (threadIdx.x >> 6);
-    if (t >= a.T) return;                                  // wave-uniform
-    const bool has = lane < a.segs;
-    const size_t p = (size_t)t * a.segs + ti_min(lane, a.segs - 1);
-    const float4 q = a.part[p];
-    const Sum r = wave_joined(has ? Sum{q.x, q.y, q.z} : Sum{LOW, 0.0f, 0.0f});
-    const int above = ti_wave_sum_i(has ? __float_as_int(q.w) : 0);
-    uint64_t key = 0;
-    if (a.top) {
-        const uint64_t* mine = a.keys + p * a.top;
-        uint64_t head = has ? mine[0] : 0, after = has && a.top > 1 ? mine[1] : 0;
-        int at = 1;
-        for (int i = 0; i < a.top; i++) {
-            uint64_t best = head;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const uint64_t other = (uint64_t)ti_xor((uint32_t)(best >> 32), o) << 32 | ti_xor((uint32_t)best, o);
-                best = other > best ? other : best;
-            }
-            if (best == 0) break;
-            if (lane == i) key = best;
-            if (head == best) {
-                head = after;
-                at++;
-                after = at < a.top ? mine[at] : 0;
-            }
-        }
-    }
-    finish(a, t, r, above, key);
+    __shared__ uint64_t s_waves[WAVES - 1][64];
+    join_parts<false>(a, blockIdx.x, s_waves);
 }
 
 }  // namespace
@@ -280,22 +379,24 @@ extern "C" int ti_logprobs(ti_ctx* c, const float* logits, const int32_t* ids, f
     TI_REQUIRE(top >= 0 && top <= TOP_MAX && top <= N, "ti_logprobs: top = %d of %d logits, at most %d", top, N, TOP_MAX);
     TI_REQUIRE(top == 0 || (top_ids && top_lp), "ti_logprobs: null buffer for the likeliest tokens");
     TI_REQUIRE(ld == 0 || ld >= N, "ti_logprobs: rows of %d logits, %d apart", N, ld);
-    LpArgs a = {logits, ids, lp, entropy, rank, top_ids, top_lp, nullptr, nullptr, ld ? ld : N, T, N, top, 1, 0};
-    // four workgroups a CU where the rows are long enough, each of whole steps
+    LpArgs a = {logits, ids, lp, entropy, rank, top_ids, top_lp, nullptr, nullptr, nullptr, ld ? ld : N, T, N, top, 1, 0};
+    // workgroups of whole steps until every CU has four, or two where tokens are kept, which costs most in a wave's first chunk
+    // (400 rows with 20 tokens 62.2 us, with four a CU 64.7; 1000 rows of 30000 with 5 37.0 / 45.1; 48 rows with 20 23.7 / 23.0)
     const long steps = ((long)N + STEP - 1) / STEP;
-    const long segs = ti_max(1L, ti_min(ti_min((long)SEGS_MAX, steps), (4L * c->cus + T - 1) / T));
+    const long segs = ti_max(1L, ti_min(ti_min((long)SEGS_MAX, steps), ((top ? 2L : 4L) * c->cus + T - 1) / T));
     a.per = (int)((steps + segs - 1) / segs);
     a.segs = (int)((steps + a.per - 1) / a.per);
     // fewer than T + 4 CUs of them
     static_assert((ROWS_MAX + 4L * 4096) * (16 + 8 * TOP_MAX) <= 4L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "the parts fit the scratch");
     a.part = reinterpret_cast<float4*>(c->attn_po);
     a.keys = reinterpret_cast<uint64_t*>(a.part + (size_t)T * a.segs);
+    if (T <= TI_LOGPROBS_ROWS) a.arrived = c->sync + TI_SYNC_LOGPROBS;
     const unsigned grid = (unsigned)(T * a.segs);
-    if (top) k_logprobs<true><<<grid, 256, (WAVES * (EPT + 2) + 5) * top * 8, c->stream>>>(a);
+    if (top) k_logprobs<true><<<grid, 256, WAVES * (EPT * top + LONG) * 8, c->stream>>>(a);
     else k_logprobs<false><<<grid, 256, 0, c->stream>>>(a);
     TI_LAUNCHED("k_logprobs");
-    if (a.segs > 1) {
-        k_logprobs_join<<<(T + WAVES - 1) / WAVES, 256, 0, c->stream>>>(a);
+    if (a.segs > 1 && !a.arrived) {
+        k_logprobs_join<<<T, 256, 0, c->stream>>>(a);
         TI_LAUNCHED("k_logprobs_join");
     }
     return TI_OK;

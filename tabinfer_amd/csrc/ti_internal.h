@@ -57,12 +57,15 @@ struct ti_graph {
 #define TI_AMAX_PARTS 1024
 #define TI_MOE_P_MAX 8192
 #define TI_MOE_E_MAX 256
-#define TI_SYNC_WORDS (TI_SYNC_ATTN + TI_ATTN_COUNTERS * TI_SYNC_ATTN_STRIDE)
+#define TI_SYNC_WORDS (TI_SYNC_LOGPROBS + TI_LOGPROBS_ROWS * TI_SYNC_LOGPROBS_STRIDE)
 #define TI_SYNC_LMHEAD 0          // lm_head argmax
 #define TI_SYNC_BONSAI 1          // Bonsai attention merge: the head workgroups' arrivals
 #define TI_SYNC_ATTN 1024         // fused attention: one counter per KV head (up to 64), each on its
 #define TI_SYNC_ATTN_STRIDE 64    //   own 256-byte line (atomics on one line serialise at the memory side)
 #define TI_ATTN_COUNTERS 64
+#define TI_SYNC_LOGPROBS (TI_SYNC_ATTN + TI_ATTN_COUNTERS * TI_SYNC_ATTN_STRIDE)
+#define TI_SYNC_LOGPROBS_STRIDE 64   // log probabilities: the parts of a row that have ended, a line a row
+#define TI_LOGPROBS_ROWS 128
 #define TI_SYNC_TGEMM 512         // split-K T-token projections: one counter per 16-row block
 #define TI_TG_SPLIT_BLOCKS 128    // (blocks of one split-K launch, at most)
 #define TI_SYNC_DUMMY 256         // 256 words never written: a valid read target for unused inputs

@@ -83,10 +83,11 @@ def test_ties_go_to_the_lower_index(ctx, top):
     check(run(ctx, x, ids, top), x, ids, top)
 
 
-def test_masked_and_not_finite(ctx):
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_masked_and_not_finite(ctx, top):
     """-inf and the type's lowest value as masks, rows of nothing else, NaN, +inf; too few candidates; ids that are none."""
     rng = np.random.default_rng(5)
-    N, top = 9000, 20
+    N = 9000
     x = rng.standard_normal((12, N)).astype(np.float32)
     x[0, rng.random(N) < 0.99] = -np.inf
     x[1] = -np.inf
