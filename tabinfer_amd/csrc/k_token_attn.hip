@@ -47,6 +47,7 @@ struct TokArgs {
     int32_t* meta;                           // [B][2]: a sequence's first slot and their number
     int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups of HW KV heads, at most
     int HW, BW;                              // a workgroup's waves: HW KV heads x BW blocks
+    int many;                                // groups: the workgroups where runs are long
     float *spo, *spml;                       // the merge of groups: the same of the shared positions, [slot][nKv][tile's rows][HD]
     int32_t* smeta;                          // [ti_group_tile][2]
     int srows, sslots;                       // rows of their tiles; slots
@@ -69,6 +70,17 @@ __host__ __device__ __forceinline__ Blocks blocks_of(const TiSpan& s) {
 __device__ __forceinline__ int page_end(const TokArgs& a, int len) {    // position behind a sequence's last that there can be
     return ti_last_pos(len, (long)a.p.pg.width << a.p.pg.shift) + 1;
 }
+// ti_group_of, in one round trip where the groups fit a wave's lanes: every lane a start. All lanes of the wave take part, b may differ
+__device__ __forceinline__ TiGroup group_of(const TokArgs& a, int b) {
+    if (a.p.P > 63) return ti_group_of(a.p.starts, a.p.shared, a.p.P, a.p.B, b);
+    const int lane = threadIdx.x & 63;
+    const int start = lane <= a.p.P ? a.p.starts[lane] : 0x7fffffff, sh = lane < a.p.P ? a.p.shared[lane] : 0;
+    int n = 0;
+    for (int i = 0; i < a.p.P; i++) n += __builtin_amdgcn_readlane(start, i) <= b;
+    const int g = ti_max(n - 1, 0);
+    const TiGroup at = ti_group_at(g, __shfl(start, g), __shfl(start, g + 1), __shfl(sh, g), a.p.B, b);
+    return n ? at : TiGroup{-1, 0, 0};
+}
 template <Keys KEYS>
 __device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // position of the sequence's last query, or of a group's last shared key
     if (KEYS == LINE) return a.p.pos0 + a.p.T - 1;
@@ -77,7 +89,7 @@ __device__ __forceinline__ int seq_last(const TokArgs& a, int b) {      // posit
 template <Keys KEYS>
 __device__ __forceinline__ TiSpan seq_span(const TokArgs& a, int b, int last) {   // the keys that any of its queries sees
     if (KEYS == SHARED) return TiSpan{0, 0, last + 1};
-    if (KEYS == OWN) return TiSpan{0, ti_min(ti_group_base(a.p.starts, a.p.shared, a.p.P, a.p.B, b), last + 1), last + 1};
+    if (KEYS == OWN) return TiSpan{0, ti_min(group_of(a, b).shared, last + 1), last + 1};
     TiSpan s = ti_span(last - (a.p.T - 1), a.p.window, a.p.sinks);
     s.end = last + 1;
     return s;
@@ -132,38 +144,90 @@ struct Run {
     long chunk, left;                        // blocks of every workgroup's run; of this one, still to do
     long start;
     int b, block, tile;                      // groups: of b's row tiles, this one
+    int last, base;                          // of sequence b, where `known`: its last position, and the first that is its own
+    bool known;
 };
+// a / b of numbers that are rarely as large as 64 bits, whose division takes four times as long
+__host__ __device__ __forceinline__ long quotient(long a, long b) {
+    return (a | b) >> 31 ? a / b : (long)((uint32_t)a / (uint32_t)b);
+}
 // blocks of a run: an equal share, but a block for each of the BW waves of a head where the sequences have as many
 __host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs, int BW) {
-    return ti_max((total + wgs - 1) / wgs, ti_min((long)BW, (total + B - 1) / B));
+    return ti_max(quotient(total + wgs - 1, wgs), ti_min((long)BW, quotient(total + B - 1, B)));
 }
+// Groups: how many workgroups share the blocks: one a CU, two where a wave of one would have more than 12 blocks. A second
+// hides the first one's loads and waits, but doubles the partials and its operands, which short runs feel (32 sequences of 16 heads over 8
+// behind 8192 shared keys 34.7 us with one, 38.5 with two; 16384 48.3 / 52.7; 32768 76.0 / 71.9; 128 sequences of 32768 241 / 182)
+constexpr int LONG_RUN = 12;
 template <Keys KEYS>
-__device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, int* s_b) {
+__device__ __forceinline__ int run_wgs(const TokArgs& a, long total) {
+    return KEYS == SHARED && total > (long)LONG_RUN * a.BW * a.wgs ? a.many : a.wgs;
+}
+struct RunLds {
+    long s4[WAVES], at;
+    int b, last, base;
+};
+template <Keys KEYS>
+__device__ bool find_run(const TokArgs& a, int w, Run& r, RunLds& s) {
     const int B = KEYS == SHARED ? a.p.P : a.p.B, tid = threadIdx.x;
     r.tile = 0;
-    if (KEYS != SHARED && B == 1) {
-        const long n = seq_blocks<KEYS>(a, 0);
-        r.chunk = run_chunk(n, 1, a.wgs, a.BW);
+    r.known = false;
+    if (B == 1) {
+        const int nb = seq_blocks<KEYS>(a, 0);
+        const long n = KEYS == SHARED ? unit_blocks<KEYS>(a, 0) : nb;
+        r.chunk = run_chunk(n, 1, run_wgs<KEYS>(a, n), a.BW);
         r.b = 0;
-        r.start = 0;
-        r.block = (int)ti_min(w * r.chunk, n);
-        r.left = ti_min(r.chunk, n - r.block);
+        const long g0 = ti_min(w * r.chunk, n);
+        r.left = ti_min(r.chunk, n - g0);
+        if (KEYS == SHARED) r.tile = (int)quotient(g0, nb);
+        r.start = (long)r.tile * nb;
+        r.block = (int)(g0 - r.start);
         return r.left > 0;
     }
     // a thread: the sequences [tid per, tid per + per)
     const int per = (B + THREADS - 1) / THREADS, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
-    for (int b = b0; b < b1; b++) mine += unit_blocks<KEYS>(a, b);
-    long at = wg_scan(mine, s4, total);
+    int last = -1, base = 0;
+    if (KEYS == OWN) {                       // every lane takes part in the look-up of groups
+        for (int i = 0; i < per; i++) {
+            const int b = ti_min(tid * per + i, B - 1);
+            last = seq_last<KEYS>(a, b);
+            const TiSpan sp = seq_span<KEYS>(a, b, last);
+            base = sp.low;
+            if (tid * per + i < B) mine += last < 0 ? 1 : ti_max(1, blocks_of(sp).n);
+        }
+    } else {
+        for (int b = b0; b < b1; b++) mine += unit_blocks<KEYS>(a, b);
+    }
+    long at = wg_scan(mine, s.s4, total);
     total = uniform(total);
-    r.chunk = run_chunk(total, B, a.wgs, a.BW);
+    r.chunk = run_chunk(total, B, run_wgs<KEYS>(a, total), a.BW);
     const long g0 = w * r.chunk;
-    if (g0 >= at && g0 < at + mine) {
+    if (KEYS == OWN && per > 1) {
+        for (int i = 0; i < per; i++) {
+            const int b = ti_min(tid * per + i, B - 1), l = seq_last<KEYS>(a, b);
+            const TiSpan sp = seq_span<KEYS>(a, b, l);
+            const int n = tid * per + i < B ? l < 0 ? 1 : ti_max(1, blocks_of(sp).n) : 0;
+            if (g0 >= at && g0 < at + n) {
+                s.b = b;
+                s.at = at;
+                s.last = l;
+                s.base = sp.low;
+            }
+            at += n;
+        }
+    } else if (g0 >= at && g0 < at + mine) {
+        if (KEYS == OWN) {
+            s.b = b0;
+            s.at = at;
+            s.last = last;
+            s.base = base;
+        } else
         for (int b = b0; b < b1; b++) {
             const long n = unit_blocks<KEYS>(a, b);
             if (g0 < at + n) {
-                *s_b = b;
-                *s_at = at;
+                s.b = b;
+                s.at = at;
                 break;
             }
             at += n;
@@ -172,12 +236,17 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
     __syncthreads();
     if (g0 >= total) return false;
     r.left = ti_min(r.chunk, total - g0);
-    r.b = __builtin_amdgcn_readfirstlane(*s_b);
-    r.start = uniform(*s_at);
+    r.b = __builtin_amdgcn_readfirstlane(s.b);
+    r.start = uniform(s.at);
     if (KEYS == SHARED) {
         const int n = seq_blocks<KEYS>(a, r.b);
-        r.tile = (int)((g0 - r.start) / n);
+        r.tile = (int)quotient(g0 - r.start, n);
         r.start += (long)r.tile * n;
+    }
+    if (KEYS == OWN) {
+        r.known = true;
+        r.last = __builtin_amdgcn_readfirstlane(s.last);
+        r.base = __builtin_amdgcn_readfirstlane(s.base);
     }
     r.block = (int)(g0 - r.start);
     return true;
@@ -189,7 +258,11 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, long* s4, long* s_at, 
 constexpr int tile_slots(int hd, bool cols) { return !cols || hd == 32 ? 1 : hd == 64 ? 2 : 4; }
 constexpr int tile_rows(int hd, bool cols) { return 16 / tile_slots(hd, cols); }
 
-template <int HD, bool COLS>
+// Row tiles of a wave: two for groups, whose blocks are then read and widened once for 32 rows, the queries' operands in LDS
+constexpr int wave_tiles(Keys keys, bool cols) { return keys == SHARED && !cols ? 2 : 1; }
+constexpr int group_rows(int hd) { return hd == 32 ? 16 : 32; }
+
+template <int HD, bool COLS, int TR>
 struct TokLds {
     static constexpr int NG = HD / 32;
     // a block as its loads write it: rows of HD bytes one behind the other, their 16-byte pieces permuted (piece_slot)
@@ -201,9 +274,10 @@ struct TokLds {
         Wave w[WAVES];
         float o[WAVES][tile_rows(HD, COLS)][HD];
     };
+    ti_h8 q[TR > 1 ? TR : 0][NG][2][64];
+    float fr[TR][16];
     float m[WAVES][16], l[WAVES][16];
-    long s4[WAVES], at;
-    int b;
+    RunLds run;
 };
 
 // Where piece c of a key's row lies: both operand reads, 16 keys' piece and 8 keys' 16 bytes, without bank conflicts (rows of
@@ -241,25 +315,26 @@ __device__ __forceinline__ float slot_sum(float v) {
 }
 
 template <int HD, Keys KEYS, bool COLS>
-__global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a) {
+__device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned block, TokLds<HD, COLS, wave_tiles(KEYS, COLS)>& L) {
     constexpr bool PAGED = KEYS != LINE;
+    constexpr int TR = wave_tiles(KEYS, COLS);
     constexpr int NG = HD / 32, PC = HD / 16, NL = HD / 32;            // 16-byte pieces a row; loads a lane a block
     constexpr int SL = (BLK * NG + 63) / 64;                           // scale loads a lane
     constexpr int SLOTS = tile_slots(HD, COLS), ROWS = tile_rows(HD, COLS);
     constexpr int NQ = COLS ? 2 : NG, NU = HD > 64 ? 2 : 1;            // Q operands; COLS: of NU x 64 dims, a column's own
-    __shared__ __align__(16) TokLds<HD, COLS> L;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the waves of a workgroup read HW heads of the same positions together: rows of a position lie side by side
-    const int groups = a.p.nKv / a.HW, hr = blockIdx.x % (groups * a.RT), w = blockIdx.x / (groups * a.RT);
+    const int groups = a.p.nKv / a.HW, hr = block % (groups * a.RT), w = block / (groups * a.RT);
     const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs;
     int rt = hr / groups, R = a.R;
     Run run;
-    if (!find_run<KEYS>(a, w, run, L.s4, &L.at, &L.b)) return;         // workgroup-uniform
+    if (!find_run<KEYS>(a, w, run, L.run)) return;                     // workgroup-uniform
     const int r16 = lane & 15, j = lane >> 4;
 
     const int slot = r16 / ROWS, grp = ti_min(slot, NG - 1), tr = r16 % ROWS;   // this lane's column: row of the tile, group
     int rg = ti_min(rt * ROWS + tr, R - 1), t = rg / a.G, h = rg % a.G;
+    const int qt = TR > 1 ? wave % TR : 0;                                      // tile whose queries this wave takes
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     // the transposing read's rows: lanes 2 rr, 2 rr + 1 of 16 address key 4 j + rr (rr < 4) or 16 + 4 j + rr - 4
     const int rr = r16 >> 1, vrow = rr < 4 ? 4 * j + rr : 12 + 4 * j + rr;
@@ -278,35 +353,43 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
 
     for (;;) {
         // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
-        const int last = seq_last<KEYS>(a, run.b);
-        const TiSpan span = seq_span<KEYS>(a, run.b, last);
+        const int last = KEYS == OWN && run.known ? run.last : seq_last<KEYS>(a, run.b);
+        const TiSpan span = KEYS == OWN && run.known ? TiSpan{0, run.base, last + 1} : seq_span<KEYS>(a, run.b, last);
+        run.known = false;
         int tiles = 1, q0 = run.b * a.p.T, seq = run.b;        // of queries and table, the first row
         if constexpr (KEYS == SHARED) {                        // rows: the group's sequences x query heads of a KV head
             const TiMembers mb = ti_group_members(a.p.starts, a.p.B, run.b);
-            tiles = (mb.count * a.G + ROWS - 1) / ROWS;
+            tiles = (mb.count * a.G + TR * ROWS - 1) / (TR * ROWS);
             q0 = seq = mb.first;
             rt = run.tile;
             R = mb.count * a.G;
-            rg = ti_min(rt * ROWS + tr, R - 1);
+            rg = ti_min((rt * TR + qt) * ROWS + tr, R - 1);
             t = rg / a.G;
             h = rg % a.G;
         }
+        const bool two = TR > 1 && R - rt * TR * ROWS > ROWS;   // the second tile holds rows
         Blocks bl = blocks_of(span);
         if (last < 0) bl.n = 0;
         const int nb = ti_max(1, bl.n);
         const int c0 = run.block, part = (int)ti_min((long)(nb - c0), run.left), c1 = ti_min(bl.n, c0 + part);
-        int pos = last - (a.p.T - 1) + t;
-        int low = a.p.window < 0 || a.p.window > pos ? 0 : pos + 1 - a.p.window;
+        int pos[TR];
+        pos[0] = last - (a.p.T - 1) + t;
+        int low = a.p.window < 0 || a.p.window > pos[0] ? 0 : pos[0] + 1 - a.p.window;
         // what every row of the tile sees: [full_low, full_end)
         int full_low = a.p.window < 0 || a.p.window > last ? 0 : last + 1 - a.p.window, full_end = last - (a.p.T - 1) + 1;
         if constexpr (KEYS == OWN) low = full_low = span.low;
         if constexpr (KEYS == SHARED) {                        // a sequence may be shorter than what its group shares
-            pos = ti_min(last, page_end(a, a.p.lens[q0 + t]) - 1);
             low = full_low = 0;
-            full_end = pos + 1;
+            full_end = last + 1;
 #pragma unroll
-            for (int x = 1; x < 16; x <<= 1) full_end = ti_min(full_end, ti_xor(full_end, x));
-            full_end = __builtin_amdgcn_readfirstlane(full_end);
+            for (int r = 0; r < TR; r++) {
+                pos[r] = ti_min(last, page_end(a, a.p.lens[q0 + ti_min((rt * TR + r) * ROWS + tr, R - 1) / a.G]) - 1);
+                full_end = ti_min(full_end, pos[r] + 1);
+            }
+            full_end = ti_min(full_end, ti_xor(full_end, 1));
+            full_end = ti_min(full_end, ti_xor(full_end, 2));
+            full_end = ti_min(full_end, ti_xor(full_end, 4));
+            full_end = __builtin_amdgcn_readfirstlane(ti_min(full_end, ti_xor(full_end, 8)));
         }
         // the query's loads before the keys': they come back first
         v4f_u qv[NQ][2];
@@ -399,7 +482,8 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
         // ---- Q operand: the lane's row, dims 32 g + 8 j.. (COLS: dims 16 j.. of 64, those of other groups than the column's
         // as zeros), scaled by 2^k so that the row's largest element is below 16
         ti_h8 qh[NQ], ql[NQ];
-        float fr = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
+        float fr[TR];
+        fr[0] = 1.44269504088896341f / (127.0f * sqrtf((float)HD));
         {
             float mx = 0.0f;
 #pragma unroll
@@ -413,7 +497,7 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
             if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
             const int k = ti_min(4 - ex, 100);
             const float up = ldexpf(1.0f, k);
-            fr = fr * ldexpf(1.0f, -k);
+            fr[0] = fr[0] * ldexpf(1.0f, -k);
 #pragma unroll
             for (int x = 0; x < NQ; x++) {
                 const bool mine = !COLS || (qc < PC && qc / 2 == slot);
@@ -427,22 +511,42 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
             }
         }
 
-        v4f o[HD / 16];
+        if constexpr (TR > 1) {                                // every wave needs all tiles'; waves of a tile write half of its groups each
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++) o[d] = zero;
-        float m = -INFINITY, l = 0.0f;
+            for (int g = 0; g < NG; g++)
+                if (g % (WAVES / TR) == wave / TR) {
+                    L.q[qt][g][0][lane] = qh[g];
+                    L.q[qt][g][1][lane] = ql[g];
+                }
+            if (wave < TR && j == 0) L.fr[qt][r16] = fr[0];
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < TR; r++) fr[r] = L.fr[r][r16];
+        }
+        v4f o[TR][HD / 16];
+        float m[TR], l[TR];
+#pragma unroll
+        for (int r = 0; r < TR; r++) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++) o[r][d] = zero;
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+        }
 
+        // the blocks, for the first NT of the row tiles
+        auto pass = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
         for (; i < c1; i += a.BW) {
             __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): the block is there
             ti_wave_lds_fence();
             const int k0 = bl.at(i) * BLK;
             const uint32_t there = (uint32_t)__ballot(page >= 0);
 
-            float s[8];
+            float s[NT][8];
 #pragma unroll
             for (int b = 0; b < 2; b++) {
-                v4f acc = zero;
                 if constexpr (COLS) {
+                    v4f acc = zero;
 #pragma unroll
                     for (int u = 0; u < NU; u++) {
                         const int key = 16 * b + r16;
@@ -457,91 +561,117 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                     }
                     const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * grp + 16 * b + 4 * j]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[e] = slot_sum<SLOTS>(acc[e] * sc[e]);
-                } else
+                    for (int e = 0; e < 4; e++) s[0][4 * b + e] = slot_sum<SLOTS>(acc[e] * sc[e]);
+                } else {
+                    v4f acc[NT];
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const int key = 16 * b + r16;
-                    const uint2 kw = *reinterpret_cast<const uint2*>(&W.k[key * HD + 16 * piece_slot<HD>(key, 2 * g + j / 2) + 8 * (j & 1)]);
-                    const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
-                    const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * g + 16 * b + 4 * j]);
-                    v4f d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
+                    for (int r = 0; r < NT; r++) acc[r] = zero;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[e] = fmaf(d[e], sc[e], acc[e]);
+                    for (int g = 0; g < NG; g++) {
+                        const int key = 16 * b + r16;
+                        const uint2 kw = *reinterpret_cast<const uint2*>(&W.k[key * HD + 16 * piece_slot<HD>(key, 2 * g + j / 2) + 8 * (j & 1)]);
+                        const ti_h8 kf = ti_i8x8_h8(kw.x, kw.y);
+                        const v4f sc = *reinterpret_cast<const v4f*>(&W.ks[BLK * g + 16 * b + 4 * j]);
+#pragma unroll
+                        for (int r = 0; r < NT; r++) {
+                            v4f d;
+                            if constexpr (TR > 1) {
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, L.q[r][g][0][lane], zero, 0, 0, 0);
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, L.q[r][g][1][lane], d, 0, 0, 0);
+                            } else {
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero, 0, 0, 0);
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], d, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[r][e] = fmaf(d[e], sc[e], acc[r][e]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < NT; r++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[r][4 * b + e] = acc[r][e];
                 }
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * b + e] = acc[e];
             }
-            // which of the lane's keys its row sees
-            uint32_t seen = 0xffu;
+            // which of the lane's keys its rows see
+            uint32_t seen[NT];
             const bool whole = there == 0xffffffffu && k0 + BLK <= full_end && (k0 >= full_low || k0 + BLK <= a.p.sinks);
+#pragma unroll
+            for (int r = 0; r < NT; r++) seen[r] = 0xffu;
             if (!whole) {                                      // wave-uniform
                 asm volatile("");                              // a branch: not computed where every key is seen
-                seen = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int kl = 16 * (e >> 2) + 4 * j + (e & 3), key = k0 + kl;
-                    const bool ok = ((there >> kl) & 1u) & (key <= pos) & ((key >= low) | (key < a.p.sinks));
-                    seen |= ok ? 1u << e : 0u;
+                for (int r = 0; r < NT; r++) {
+                    seen[r] = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int kl = 16 * (e >> 2) + 4 * j + (e & 3), key = k0 + kl;
+                        const bool ok = ((there >> kl) & 1u) & (key <= pos[r]) & ((key >= low) | (key < a.p.sinks));
+                        seen[r] |= ok ? 1u << e : 0u;
+                    }
                 }
             }
             if (KEYS == LINE && a.p.mass && slot == 0 && rt * ROWS + tr < R) {
                 float* sp = a.p.scores + (size_t)(hk * a.G + rg) * a.p.sstride + k0 + 4 * j;
-                *reinterpret_cast<v4f*>(sp) = v4f{s[0], s[1], s[2], s[3]} * fr;
-                *reinterpret_cast<v4f*>(sp + 16) = v4f{s[4], s[5], s[6], s[7]} * fr;
+                *reinterpret_cast<v4f*>(sp) = v4f{s[0][0], s[0][1], s[0][2], s[0][3]} * fr[0];
+                *reinterpret_cast<v4f*>(sp + 16) = v4f{s[0][4], s[0][5], s[0][6], s[0][7]} * fr[0];
             }
-            // the largest of the lane's scores, in log2; what a row sees is never below the floor
-            float tm = FLOOR;
-            if (!whole) {
-                tm = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen >> e & 1u ? fmaxf(s[e], FLOOR) : -INFINITY);
-                tm = tm > -INFINITY ? fmaxf(tm * fr, FLOOR) : -INFINITY;
-            } else {
+            for (int r = 0; r < NT; r++) {
+                // the largest of the lane's scores, in log2; what a row sees is never below the floor
+                float tm = FLOOR;
+                if (!whole) {
+                    tm = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[e]);
-                tm = fmaxf(tm * fr, FLOOR);
+                    for (int e = 0; e < 8; e++) tm = fmaxf(tm, seen[r] >> e & 1u ? fmaxf(s[r][e], FLOOR) : -INFINITY);
+                    tm = tm > -INFINITY ? fmaxf(tm * fr[r], FLOOR) : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) tm = fmaxf(tm, s[r][e]);
+                    tm = fmaxf(tm * fr[r], FLOOR);
+                }
+                // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
+                if (__any(tm > m[r] + 6.0f)) {
+                    tm = fmaxf(tm, ti_xor(tm, 16));
+                    tm = fmaxf(tm, ti_xor(tm, 32));
+                    const bool bump = tm > m[r] + 6.0f;
+                    const float mn = bump ? tm : m[r];
+                    const float alpha = bump ? __builtin_amdgcn_exp2f(m[r] - mn) : 1.0f;
+                    l[r] = l[r] * alpha;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; d++) o[r][d] = o[r][d] * alpha;
+                    m[r] = mn;
+                }
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[r][e], fr[r], -m[r]));
+                    if (!whole) p = seen[r] >> e & 1u ? p : 0.0f;
+                    sum += p;
+                    s[r][e] = p * PSCALE;
+                }
+                l[r] += sum;
             }
-            // the reference maximum moves when it is exceeded by more than 2^6 (weights up to 64): o is rescaled rarely
-            if (__any(tm > m + 6.0f)) {
-                tm = fmaxf(tm, ti_xor(tm, 16));
-                tm = fmaxf(tm, ti_xor(tm, 32));
-                const bool bump = tm > m + 6.0f;
-                const float mn = bump ? tm : m;
-                const float alpha = bump ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-                l = l * alpha;
-#pragma unroll
-                for (int d = 0; d < HD / 16; d++) o[d] = o[d] * alpha;
-                m = mn;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float p = __builtin_amdgcn_exp2f(fmaf(s[e], fr, -m));
-                if (!whole) p = seen >> e & 1u ? p : 0.0f;
-                sum += p;
-                s[e] = p * PSCALE;
-            }
-            l += sum;
-            ti_b8 pb[3];
+            ti_b8 pb[NT][3];
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 if constexpr (COLS) TI_ISSUE_FENCE();          // a group's operands at a time: registers for three waves a SIMD
                 if (!COLS || g == 0) {
                     const v4f v0 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 4 * j]);
                     const v4f v1 = *reinterpret_cast<const v4f*>(&W.vs[BLK * (COLS ? grp : g) + 16 + 4 * j]);
-                    float x[8];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[e] = s[e] * v0[e];
-                        x[4 + e] = s[4 + e] * v1[e];
-                    }
-                    if (!whole) {                              // the scale of a key that the row does not see may be NaN
+                    for (int r = 0; r < NT; r++) {
+                        float x[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = seen >> e & 1u ? x[e] : 0.0f;
+                        for (int e = 0; e < 4; e++) {
+                            x[e] = s[r][e] * v0[e];
+                            x[4 + e] = s[r][4 + e] * v1[e];
+                        }
+                        if (!whole) {                          // the scale of a key that the row does not see may be NaN
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = seen[r] >> e & 1u ? x[e] : 0.0f;
+                        }
+                        ti_bf16x3(x, pb[r]);
                     }
-                    ti_bf16x3(x, pb);
                 }
 #pragma unroll
                 for (int d = 2 * g; d < 2 * g + 2; d++) {      // COLS: of these 16 dims, the columns of group g hold the output
@@ -550,7 +680,10 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                     const uint2 lo = ti_i8x4_b4((uint32_t)vb.x), hi = ti_i8x4_b4((uint32_t)vb.y);
                     const ti_b8 vv = __builtin_bit_cast(ti_b8, make_uint4(lo.x, lo.y, hi.x, hi.y));
 #pragma unroll
-                    for (int e = 2; e >= 0; e--) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[e], o[d], 0, 0, 0);
+                    for (int r = 0; r < NT; r++) {
+#pragma unroll
+                        for (int e = 2; e >= 0; e--) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pb[r][e], o[r][d], 0, 0, 0);
+                    }
                 }
             }
             // the next block into the place of this one, which has been read
@@ -562,45 +695,54 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
                 load(i + a.BW, page);
             }
         }
+        };
+        if constexpr (TR > 1) {
+            if (two) pass(std::integral_constant<int, 2>{});
+            else pass(std::integral_constant<int, 1>{});
+        } else pass(std::integral_constant<int, 1>{});
 
         // ---- the waves' parts into the workgroup's partial
-        l += ti_xor(l, 16);
-        l += ti_xor(l, 32);
-        __syncthreads();                                       // the tiles are read
-        if (j == 0 && slot == 0) {
-            L.m[wave][tr] = m;
-            L.l[wave][tr] = l;
-        }
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++)
-            if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[d];
-        __syncthreads();
-        const int nr = ti_min(ROWS, R - rt * ROWS);
-        for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
-            const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, r = q % nr;
-            float M = L.m[hh][r];
-            for (int k = hh + a.HW; k < WAVES; k += a.HW) M = fmaxf(M, L.m[k][r]);
-            v4f x = zero;
-            float y = 0.0f;
-            for (int k = hh; k < WAVES; k += a.HW) {
-                const float mk = L.m[k][r], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
-                const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][r][4 * d]);
-#pragma unroll
-                for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
-                y = fmaf(L.l[k][r], f, y);
+        for (int r = 0; r < TR; r++) {
+            if (r > 0 && !two) continue;
+            l[r] += ti_xor(l[r], 16);
+            l[r] += ti_xor(l[r], 32);
+            __syncthreads();                                   // the blocks, or the tile before, are read
+            if (j == 0 && slot == 0) {
+                L.m[wave][tr] = m[r];
+                L.l[wave][tr] = l[r];
             }
-            const size_t at = KEYS == SHARED ? ((size_t)(w + ti_group_tile(q0, run.b, rt, a.G, ROWS)) * a.p.nKv + hk0 + hh) * ROWS + r
-                                             : ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + r;
-            *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
-            if (d == 0) {
-                a.pml[2 * at] = M;
-                a.pml[2 * at + 1] = y;
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+                if (!COLS || slot == d / 2) *reinterpret_cast<v4f*>(&L.o[wave][tr][16 * d + 4 * j]) = o[r][d];
+            __syncthreads();
+            const int nr = ti_min(ROWS, R - (rt * TR + r) * ROWS);
+            for (int e = tid; e < a.HW * nr * (HD / 4); e += THREADS) {
+                const int q = e / (HD / 4), d = e % (HD / 4), hh = q / nr, rr = q % nr;
+                float M = L.m[hh][rr];
+                for (int k = hh + a.HW; k < WAVES; k += a.HW) M = fmaxf(M, L.m[k][rr]);
+                v4f x = zero;
+                float y = 0.0f;
+                for (int k = hh; k < WAVES; k += a.HW) {
+                    const float mk = L.m[k][rr], f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+                    const v4f ok = *reinterpret_cast<const v4f*>(&L.o[k][rr][4 * d]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
+                    y = fmaf(L.l[k][rr], f, y);
+                }
+                const size_t at = KEYS == SHARED ? ((size_t)(w + ti_group_tile(q0, run.b, rt, a.G, TR * ROWS)) * a.p.nKv + hk0 + hh) * (TR * ROWS) + ROWS * r + rr
+                                                 : ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + rr;
+                *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
+                if (d == 0) {
+                    a.pml[2 * at] = M;
+                    a.pml[2 * at + 1] = y;
+                }
             }
         }
         if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
-            const int u = KEYS == SHARED ? ti_group_tile(q0, run.b, rt, a.G, ROWS) : run.b;
+            const int u = KEYS == SHARED ? ti_group_tile(q0, run.b, rt, a.G, TR * ROWS) : run.b;
             a.meta[2 * u] = w + u;
-            a.meta[2 * u + 1] = (int)((run.start + nb - 1) / run.chunk) - w + 1;
+            a.meta[2 * u + 1] = (int)quotient(run.start + nb - 1, run.chunk) - w + 1;
         }
         run.left -= part;
         if (run.left <= 0) return;
@@ -614,6 +756,25 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
         }
         __syncthreads();                                   // the parts are read
     }
+}
+
+template <int HD, Keys KEYS, bool COLS>
+__global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a) {
+    __shared__ __align__(16) TokLds<HD, COLS, wave_tiles(KEYS, COLS)> L;
+    token_attn<HD, KEYS, COLS>(a, blockIdx.x, L);
+}
+
+// Groups: the first `nshared` workgroups and those behind `nown` more take the positions that groups share, the others each
+// sequence's own. Those of long runs come last: where there are none they end at once, and nothing waits for them
+template <int HD, bool COLS>
+__global__ __launch_bounds__(THREADS, 2) void k_group_attn(TokArgs own, TokArgs shared, unsigned nshared, unsigned nown) {
+    __shared__ __align__(16) union {
+        TokLds<HD, COLS, 1> own;
+        TokLds<HD, HD == 32, wave_tiles(SHARED, HD == 32)> shared;
+    } L;
+    const unsigned i = blockIdx.x;
+    if (i - nshared < nown) token_attn<HD, OWN, COLS>(own, i - nshared, L.own);
+    else token_attn<HD, SHARED, HD == 32>(shared, i < nshared ? i : i - nown, L.shared);
 }
 
 // The weights that each key received, by the merge's workgroups behind the rows' own (part of parts): every head's (max, sum)
@@ -664,12 +825,14 @@ __global__ __launch_bounds__(256) void k_token_merge(TokArgs a, int ns1) {
     int ns = ns1 ? ns1 : a.meta[2 * b + 1];
     const size_t step = (size_t)a.p.nKv * a.R, base = (size_t)s0 * step + (size_t)hk * a.R + r;
     // the group's slots behind the sequence's own
-    const int own = ns, g = GROUPS ? ti_group_of(a.p.starts, a.p.shared, a.p.P, a.p.B, b) : -1;
+    const int own = ns;
+    TiGroup gr = {-1, 0, 0};
+    if constexpr (GROUPS) gr = group_of(a, b);
     size_t sbase = 0;
     const size_t sstep = (size_t)a.p.nKv * a.srows;
-    if (GROUPS && g >= 0) {
-        const int first = ti_group_members(a.p.starts, a.p.B, g).first, row_s = (b - first) * a.G + r;
-        const int u = ti_group_tile(first, g, row_s / a.srows, a.G, a.srows);
+    if (GROUPS && gr.g >= 0) {
+        const int row_s = (b - gr.first) * a.G + r;
+        const int u = ti_group_tile(gr.first, gr.g, row_s / a.srows, a.G, a.srows);
         // groups that are out of order may have left numbers that do not belong together: none outside the scratch is followed
         const int us = a.smeta[2 * u], un = a.smeta[2 * u + 1];
         if (us >= 0 && un > 0 && us < a.sslots && un <= a.sslots - us) {
@@ -807,15 +970,16 @@ int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     a.RT = (a.R + rows - 1) / rows;
     a.HW = heads_together(p.nKv);
     a.BW = WAVES / a.HW;
-    a.srows = 16;
-    const int heads = p.nKv / a.HW, held = a.R <= crows ? 3 : 2;
+    a.srows = group_rows(hd);
+    const int heads = p.nKv / a.HW;
     const long places = ti_group_tile(p.B, p.P, 0, a.G, a.srows);
     const long fixed = (long)p.B * p.nHq + places * p.nKv * a.srows;
-    long wgs = ti_max(((long)held * c->cus + heads * a.RT - 1) / (heads * a.RT), (long)p.B), swgs = (2L * c->cus + heads - 1) / heads;
+    // two workgroups a CU; of the shared keys' a workgroup's waves take blocks of one head, for whose rows they share the operands, and join in LDS
+    long wgs = ti_max((2L * c->cus + heads * a.RT - 1) / (heads * a.RT), (long)p.B), many = (2L * c->cus + p.nKv - 1) / p.nKv;
     const long room = TI_ATTN_ROWSPLITS - fixed;
     wgs = ti_min(wgs, room / 2 / p.nHq);
-    swgs = ti_min(swgs, room / 2 / (p.nKv * a.srows));
-    TI_REQUIRE(wgs > 0 && swgs > 0, "ti_attn_shared_q8: %d sequences of %d heads in %d groups exceed the scratch", p.B, p.nHq, p.P);
+    many = ti_min(many, room / 2 / (p.nKv * a.srows));
+    TI_REQUIRE(wgs > 0 && many > 0, "ti_attn_shared_q8: %d sequences of %d heads in %d groups exceed the scratch", p.B, p.nHq, p.P);
     const long most = p.max_keys / BLK + 3;
     a.po = c->attn_po;
     a.pml = c->attn_ml;
@@ -829,17 +993,22 @@ int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     s.po = a.spo;
     s.pml = a.spml;
     s.meta = a.smeta;
-    s.wgs = (int)swgs;
+    s.many = (int)many;
+    s.wgs = (int)((many + 1) / 2);
+    s.HW = 1;
+    s.BW = WAVES;
+    s.RT = 1;
     a.wgs = (int)wgs;
-    a.sslots = s.sslots = (int)(swgs + places);
+    a.sslots = s.sslots = (int)(many + places);
     wgs = ti_min(wgs, p.B * most);
-    swgs = ti_min(swgs, places * most);
+    many = ti_min(many, places * most);
+    const unsigned ns = (unsigned)(ti_min(many, (long)s.wgs) * p.nKv), no = (unsigned)(wgs * a.RT * heads), grid = (unsigned)(many * p.nKv) + no;
 #define GROUP(HD_) if (hd == HD_) { \
-        launch_attn<HD_, SHARED>(c, s, (unsigned)(swgs * heads), false); \
-        launch_attn<HD_, OWN>(c, a, (unsigned)(wgs * a.RT * heads), a.R <= crows); \
+        if (HD_ == 32 || a.R <= crows) k_group_attn<HD_, true><<<grid, THREADS, 0, c->stream>>>(a, s, ns, no); \
+        else if constexpr (HD_ > 32) k_group_attn<HD_, false><<<grid, THREADS, 0, c->stream>>>(a, s, ns, no); \
         launch_merge<HD_, true>(c, a, 0); }
     GROUP(128) GROUP(96) GROUP(64) GROUP(32)
 #undef GROUP
-    TI_LAUNCHED("k_token_attn");
+    TI_LAUNCHED("k_group_attn");
     return TI_OK;
 }

@@ -55,8 +55,16 @@ TI_HD inline TiMembers ti_group_members(const int32_t* starts, int B, int g) {
     const int lo = ti_max(0, ti_min((int)starts[g], B)), n = ti_max(lo, ti_min((int)starts[g + 1], B)) - lo;
     return TiMembers{lo, n > 1 ? n : 0};
 }
-// The group of sequence b, with something to share: -1 for none
-TI_HD inline int ti_group_of(const int32_t* starts, const int32_t* shared, int P, int B, int b) {
+// The group of sequence b, with something to share, and what that is: -1 and 0 for none
+struct TiGroup {
+    int g, first, shared;
+};
+TI_HD inline TiGroup ti_group_at(int g, int s0, int s1, int shared, int B, int b) {   // group g = [s0, s1), if b is in it
+    const int32_t s[2] = {s0, s1};
+    const TiMembers m = ti_group_members(s, B, 0);
+    return b < s0 || b >= s1 || shared <= 0 || m.count == 0 ? TiGroup{-1, 0, 0} : TiGroup{g, m.first, shared};
+}
+TI_HD inline TiGroup ti_group_of(const int32_t* starts, const int32_t* shared, int P, int B, int b) {
     int lo = 0, hi = P;                      // the first group that begins behind b is in [lo, hi]
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -64,12 +72,7 @@ TI_HD inline int ti_group_of(const int32_t* starts, const int32_t* shared, int P
         else hi = mid;
     }
     const int g = lo - 1;
-    if (g < 0 || b >= starts[g + 1] || shared[g] <= 0) return -1;
-    return ti_group_members(starts, B, g).count ? g : -1;
-}
-TI_HD inline int ti_group_base(const int32_t* starts, const int32_t* shared, int P, int B, int b) {   // positions that b shares
-    const int g = ti_group_of(starts, shared, P, B, b);
-    return g < 0 ? 0 : (int)shared[g];
+    return g < 0 ? TiGroup{-1, 0, 0} : ti_group_at(g, starts[g], starts[g + 1], shared[g], B, b);
 }
 // A number for tile `tile` of `rows` rows of group g, whose first sequence is `first` and whose sequences have G rows each: larger for
 // later tiles and later groups (a group of n G rows has at most one tile more than n G / rows, and takes one number more: groups with

@@ -52,8 +52,8 @@ def test_bad_arguments_are_refused(name):
 
 SRC = r"""
 #include "ti_span.h"
-extern "C" int group_of(const int32_t* starts, const int32_t* shared, int P, int B, int b) { return ti_group_of(starts, shared, P, B, b); }
-extern "C" int base(const int32_t* starts, const int32_t* shared, int P, int B, int b) { return ti_group_base(starts, shared, P, B, b); }
+extern "C" int group_of(const int32_t* starts, const int32_t* shared, int P, int B, int b) { return ti_group_of(starts, shared, P, B, b).g; }
+extern "C" int base(const int32_t* starts, const int32_t* shared, int P, int B, int b) { return ti_group_of(starts, shared, P, B, b).shared; }
 extern "C" int first(const int32_t* starts, int B, int g) { return ti_group_members(starts, B, g).first; }
 extern "C" int count(const int32_t* starts, int B, int g) { return ti_group_members(starts, B, g).count; }
 extern "C" int number(int first, int g, int tile, int G, int rows) { return ti_group_tile(first, g, tile, G, rows); }
