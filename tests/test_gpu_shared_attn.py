@@ -113,6 +113,13 @@ def test_groups(ctx, starts, shared, lens, page, nHq, nKv, hd):
             assert not got[b].any()
 
 
+@pytest.mark.parametrize("starts,shared,lens,page,nHq,nKv,hd", [
+    ([0, 96], [2080], [2081 + i % 50 for i in range(96)], 32, 32, 16, 32), ([0, 12, 24], [8200, 5000], [8201 + 7 * i for i in range(12)] + [5001] * 12, 64, 64, 16, 64)])
+def test_runs_long_enough_for_two_workgroups_a_cu(ctx, starts, shared, lens, page, nHq, nKv, hd):
+    rng = np.random.default_rng(hd)
+    check(ctx, rng, starts, shared, lens, page, nHq, nKv, hd)
+
+
 @pytest.mark.parametrize("page", [1, 16, 64])
 def test_bad_pages_are_not_there(ctx, page):
     """Ids outside the pool in shared places and a sequence's own; lengths and shared lengths past the table."""
