@@ -33,6 +33,7 @@ typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int BLK = 32;                      // keys of a wave's block
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
+constexpr int XCDS = TI_XCDS;
 constexpr float FLOOR = -3.402823466e38f;
 constexpr float PSCALE = 0x1p-24f;           // of every weight in P V: 127 x a V scale x thousands of keys stays in f32's range
 
@@ -47,7 +48,7 @@ struct TokArgs {
     int32_t* meta;                           // [B][2]: a sequence's first slot and their number
     int G, R, RT, wgs;                       // R = T G rows a KV head in RT tiles; wgs: workgroups of HW KV heads, at most
     int HW, BW;                              // a workgroup's waves: HW KV heads x BW blocks
-    int many;                                // groups: the workgroups where runs are long
+    int many;                                // shared keys: the workgroups where runs are long
     float *spo, *spml;                       // the merge of groups: the same of the shared positions, [slot][nKv][tile's rows][HD]
     int32_t* smeta;                          // [ti_group_tile][2]
     int srows, sslots;                       // rows of their tiles; slots
@@ -104,13 +105,6 @@ __device__ __forceinline__ int seq_blocks(const TokArgs& a, int b) {
 __device__ __forceinline__ int group_tiles(const TokArgs& a, int g) {
     return (ti_group_members(a.p.starts, a.p.B, g).count * a.G + a.srows - 1) / a.srows;
 }
-template <Keys KEYS>
-__device__ __forceinline__ long unit_blocks(const TokArgs& a, int b) {  // of a sequence, or of all of a group's tiles
-    if (KEYS != SHARED) return seq_blocks<KEYS>(a, b);
-    const int tiles = group_tiles(a, b);
-    return tiles ? (long)tiles * seq_blocks<KEYS>(a, b) : 0;
-}
-
 // sum of the threads before this one, and of all of the workgroup
 __device__ __forceinline__ long wg_scan(long v, long* s4, long& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -139,92 +133,121 @@ __device__ __forceinline__ long uniform(long v) {
     return (long)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 
-// The run of blocks of a workgroup, in sequence b from its block `block` (at block `start` of all) on
+// The run of blocks of a workgroup, in sequence b from its block `block` (at block `start` of all) on. Of groups' keys a run is in one
+// row tile of one group, or in one sequence, and slots are the runs' own: a second part would begin with the same chain of loads as
+// the first (six groups 37.7 us, 33.4 so)
 struct Run {
     long chunk, left;                        // blocks of every workgroup's run; of this one, still to do
     long start;
-    int b, block, tile;                      // groups: of b's row tiles, this one
-    int last, base;                          // of sequence b, where `known`: its last position, and the first that is its own
-    bool known;
+    int b, block, tile, parts;               // groups: of b's row tiles, this one; runs of a tile or sequence
+    int last, base;                          // groups: of b, its last position, and the first that is its own
 };
-// a / b of numbers that are rarely as large as 64 bits, whose division takes four times as long
-__host__ __device__ __forceinline__ long quotient(long a, long b) {
-    return (a | b) >> 31 ? a / b : (long)((uint32_t)a / (uint32_t)b);
-}
 // blocks of a run: an equal share, but a block for each of the BW waves of a head where the sequences have as many
 __host__ __device__ __forceinline__ long run_chunk(long total, int B, int wgs, int BW) {
-    return ti_max(quotient(total + wgs - 1, wgs), ti_min((long)BW, quotient(total + B - 1, B)));
-}
-// Groups: how many workgroups share the blocks: one a CU, two where a wave of one would have more than 12 blocks. A second
-// hides the first one's loads and waits, but doubles the partials and its operands, which short runs feel (32 sequences of 16 heads over 8
-// behind 8192 shared keys 34.7 us with one, 38.5 with two; 16384 48.3 / 52.7; 32768 76.0 / 71.9; 128 sequences of 32768 241 / 182)
-constexpr int LONG_RUN = 12;
-template <Keys KEYS>
-__device__ __forceinline__ int run_wgs(const TokArgs& a, long total) {
-    return KEYS == SHARED && total > (long)LONG_RUN * a.BW * a.wgs ? a.many : a.wgs;
+    return ti_max(ti_quotient(total + wgs - 1, wgs), ti_min((long)BW, ti_quotient(total + B - 1, B)));
 }
 struct RunLds {
-    long s4[WAVES], at;
-    int b, last, base;
+    long s4[WAVES], t4[WAVES], at;
+    int b, last, base, nb, parts;
+};
+// a sequence's own blocks, or a group's shared ones and row tiles
+struct Unit {
+    int last, base, nb, tiles;
 };
 template <Keys KEYS>
-__device__ bool find_run(const TokArgs& a, int w, Run& r, RunLds& s) {
+__device__ __forceinline__ Unit unit_of(const TokArgs& a, int b) {        // all lanes of the wave
+    Unit u;
+    u.last = seq_last<KEYS>(a, b);
+    const TiSpan sp = seq_span<KEYS>(a, b, u.last);
+    u.base = sp.low;
+    u.nb = u.last < 0 ? 1 : ti_max(1, blocks_of(sp).n);
+    u.tiles = KEYS == OWN ? 1 : u.last < 0 ? 0 : group_tiles(a, b);
+    return u;
+}
+__device__ __forceinline__ int parts_of(const TokArgs& a, long total, const Unit& u) {
+    return ti_group_parts(total, u.nb, u.tiles, a.wgs, a.many, a.BW);
+}
+template <Keys KEYS>
+__device__ bool find_part(const TokArgs& a, int w, Run& r, RunLds& s) {
     const int B = KEYS == SHARED ? a.p.P : a.p.B, tid = threadIdx.x;
-    r.tile = 0;
-    r.known = false;
+    long at = 0;
+    int nb;
     if (B == 1) {
-        const int nb = seq_blocks<KEYS>(a, 0);
-        const long n = KEYS == SHARED ? unit_blocks<KEYS>(a, 0) : nb;
-        r.chunk = run_chunk(n, 1, run_wgs<KEYS>(a, n), a.BW);
+        const Unit u = unit_of<KEYS>(a, 0);
+        r.parts = parts_of(a, (long)u.nb * u.tiles, u);
+        if (w >= u.tiles * r.parts) return false;
         r.b = 0;
-        const long g0 = ti_min(w * r.chunk, n);
-        r.left = ti_min(r.chunk, n - g0);
-        if (KEYS == SHARED) r.tile = (int)quotient(g0, nb);
-        r.start = (long)r.tile * nb;
-        r.block = (int)(g0 - r.start);
+        r.last = u.last;
+        r.base = u.base;
+        nb = u.nb;
+    } else {
+        // a thread: the units [tid per, tid per + per)
+        const int per = (B + THREADS - 1) / THREADS;
+        const Unit u0 = unit_of<KEYS>(a, ti_min(tid * per, B - 1));
+        long mine = tid * per < B ? (long)u0.nb * u0.tiles : 0, total;
+        for (int i = 1; i < per; i++) {
+            const Unit u = unit_of<KEYS>(a, ti_min(tid * per + i, B - 1));
+            mine += tid * per + i < B ? (long)u.nb * u.tiles : 0;
+        }
+        wg_scan(mine, s.s4, total);
+        const long blocks = uniform(total);
+        auto runs = [&](const Unit& u, int i) { return tid * per + i < B ? (long)u.tiles * parts_of(a, blocks, u) : 0; };
+        mine = runs(u0, 0);
+        for (int i = 1; i < per; i++) mine += runs(unit_of<KEYS>(a, ti_min(tid * per + i, B - 1)), i);
+        at = wg_scan(mine, s.t4, total);
+        for (int i = 0; i < per; i++) {
+            const Unit u = i ? unit_of<KEYS>(a, ti_min(tid * per + i, B - 1)) : u0;
+            const long n = runs(u, i);
+            if (w >= at && w < at + n) {
+                s.b = tid * per + i;
+                s.at = at;
+                s.last = u.last;
+                s.base = u.base;
+                s.nb = u.nb;
+                s.parts = parts_of(a, blocks, u);
+            }
+            at += n;
+        }
+        __syncthreads();
+        if (w >= uniform(total)) return false;
+        r.b = __builtin_amdgcn_readfirstlane(s.b);
+        r.last = __builtin_amdgcn_readfirstlane(s.last);
+        r.base = __builtin_amdgcn_readfirstlane(s.base);
+        nb = __builtin_amdgcn_readfirstlane(s.nb);
+        r.parts = __builtin_amdgcn_readfirstlane(s.parts);
+        at = uniform(s.at);
+    }
+    const int i = (int)(w - at);
+    r.tile = (int)ti_quotient(i, r.parts);
+    const long part = i - (long)r.tile * r.parts;
+    r.block = (int)ti_quotient(part * nb, r.parts);
+    r.left = ti_quotient((part + 1) * nb, r.parts) - r.block;
+    return true;
+}
+template <Keys KEYS>
+__device__ bool find_run(const TokArgs& a, int w, Run& r, RunLds& s) {
+    if constexpr (KEYS == OWN || KEYS == SHARED) return find_part<KEYS>(a, w, r, s);
+    const int B = a.p.B, tid = threadIdx.x;
+    if (B == 1) {
+        const long n = seq_blocks<KEYS>(a, 0);
+        r.chunk = run_chunk(n, 1, a.wgs, a.BW);
+        r.b = 0;
+        r.start = 0;
+        r.block = (int)ti_min(w * r.chunk, n);
+        r.left = ti_min(r.chunk, n - r.block);
         return r.left > 0;
     }
     // a thread: the sequences [tid per, tid per + per)
     const int per = (B + THREADS - 1) / THREADS, b0 = ti_min(B, tid * per), b1 = ti_min(B, b0 + per);
     long mine = 0, total;
-    int last = -1, base = 0;
-    if (KEYS == OWN) {                       // every lane takes part in the look-up of groups
-        for (int i = 0; i < per; i++) {
-            const int b = ti_min(tid * per + i, B - 1);
-            last = seq_last<KEYS>(a, b);
-            const TiSpan sp = seq_span<KEYS>(a, b, last);
-            base = sp.low;
-            if (tid * per + i < B) mine += last < 0 ? 1 : ti_max(1, blocks_of(sp).n);
-        }
-    } else {
-        for (int b = b0; b < b1; b++) mine += unit_blocks<KEYS>(a, b);
-    }
+    for (int b = b0; b < b1; b++) mine += seq_blocks<KEYS>(a, b);
     long at = wg_scan(mine, s.s4, total);
     total = uniform(total);
-    r.chunk = run_chunk(total, B, run_wgs<KEYS>(a, total), a.BW);
+    r.chunk = run_chunk(total, B, a.wgs, a.BW);
     const long g0 = w * r.chunk;
-    if (KEYS == OWN && per > 1) {
-        for (int i = 0; i < per; i++) {
-            const int b = ti_min(tid * per + i, B - 1), l = seq_last<KEYS>(a, b);
-            const TiSpan sp = seq_span<KEYS>(a, b, l);
-            const int n = tid * per + i < B ? l < 0 ? 1 : ti_max(1, blocks_of(sp).n) : 0;
-            if (g0 >= at && g0 < at + n) {
-                s.b = b;
-                s.at = at;
-                s.last = l;
-                s.base = sp.low;
-            }
-            at += n;
-        }
-    } else if (g0 >= at && g0 < at + mine) {
-        if (KEYS == OWN) {
-            s.b = b0;
-            s.at = at;
-            s.last = last;
-            s.base = base;
-        } else
+    if (g0 >= at && g0 < at + mine) {
         for (int b = b0; b < b1; b++) {
-            const long n = unit_blocks<KEYS>(a, b);
+            const int n = seq_blocks<KEYS>(a, b);
             if (g0 < at + n) {
                 s.b = b;
                 s.at = at;
@@ -238,16 +261,6 @@ __device__ bool find_run(const TokArgs& a, int w, Run& r, RunLds& s) {
     r.left = ti_min(r.chunk, total - g0);
     r.b = __builtin_amdgcn_readfirstlane(s.b);
     r.start = uniform(s.at);
-    if (KEYS == SHARED) {
-        const int n = seq_blocks<KEYS>(a, r.b);
-        r.tile = (int)quotient(g0 - r.start, n);
-        r.start += (long)r.tile * n;
-    }
-    if (KEYS == OWN) {
-        r.known = true;
-        r.last = __builtin_amdgcn_readfirstlane(s.last);
-        r.base = __builtin_amdgcn_readfirstlane(s.base);
-    }
     r.block = (int)(g0 - r.start);
     return true;
 }
@@ -293,8 +306,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* base, int
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
 }
 // a lane's 16 bytes (streamed) or 4 (scales: neighbouring heads share their cache lines) to LDS, lane after lane
+template <bool AGAIN>   // not streamed: other tiles read it again (32 sequences behind 8192 shared keys 34.1 / 32.4 us, six groups 31.5 / 29.2)
 __device__ __forceinline__ void run_to_lds16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t lane_off, int off) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, lane_off, off, 0, 2);
+    if (AGAIN) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, lane_off, off, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, lane_off, off, 0, 2);
 }
 __device__ __forceinline__ void run_to_lds4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t lane_off) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 4, lane_off, 0, 0, 0);
@@ -325,7 +340,14 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the waves of a workgroup read HW heads of the same positions together: rows of a position lie side by side
-    const int groups = a.p.nKv / a.HW, hr = block % (groups * a.RT), w = block / (groups * a.RT);
+    const int groups = a.p.nKv / a.HW;
+    int hr = block % (groups * a.RT), w = block / (groups * a.RT);
+    // all heads of a run on one XCD, whose L2 then reads a line of scales once (six groups 33.3 us, a head an XCD; 31.5)
+    if constexpr (KEYS == OWN || KEYS == SHARED) {
+        const int i = block / XCDS, n = groups * a.RT;
+        hr = i % n;
+        w = i / n * XCDS + block % XCDS;
+    }
     const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs;
     int rt = hr / groups, R = a.R;
     Run run;
@@ -353,13 +375,12 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
 
     for (;;) {
         // ---- this workgroup's part of sequence run.b: blocks [c0, c1)
-        const int last = KEYS == OWN && run.known ? run.last : seq_last<KEYS>(a, run.b);
-        const TiSpan span = KEYS == OWN && run.known ? TiSpan{0, run.base, last + 1} : seq_span<KEYS>(a, run.b, last);
-        run.known = false;
-        int tiles = 1, q0 = run.b * a.p.T, seq = run.b;        // of queries and table, the first row
+        constexpr bool GROUPS = KEYS == OWN || KEYS == SHARED;
+        const int last = GROUPS ? run.last : seq_last<KEYS>(a, run.b);
+        const TiSpan span = GROUPS ? TiSpan{0, run.base, last + 1} : seq_span<KEYS>(a, run.b, last);
+        int q0 = run.b * a.p.T, seq = run.b;                   // of queries and table, the first row
         if constexpr (KEYS == SHARED) {                        // rows: the group's sequences x query heads of a KV head
             const TiMembers mb = ti_group_members(a.p.starts, a.p.B, run.b);
-            tiles = (mb.count * a.G + TR * ROWS - 1) / (TR * ROWS);
             q0 = seq = mb.first;
             rt = run.tile;
             R = mb.count * a.G;
@@ -445,8 +466,8 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
                 const __amdgpu_buffer_rsrc_t rks = resource(a.p.ks + row * NG, scales), rvs = resource(a.p.vs + row * NG, scales);
 #pragma unroll
                 for (int p = 0; p < NL; p++) {
-                    run_to_lds16(rk, &W.k[1024 * p], po[p % PF], p / PF * far);
-                    run_to_lds16(rv, &W.v[1024 * p], po[p % PF], p / PF * far);
+                    run_to_lds16<KEYS >= OWN>(rk, &W.k[1024 * p], po[p % PF], p / PF * far);
+                    run_to_lds16<KEYS >= OWN>(rv, &W.v[1024 * p], po[p % PF], p / PF * far);
                 }
 #pragma unroll
                 for (int p = 0; p < SL; p++) {
@@ -730,8 +751,8 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
                     for (int c = 0; c < 4; c++) x[c] = fmaf(ok[c], f, x[c]);
                     y = fmaf(L.l[k][rr], f, y);
                 }
-                const size_t at = KEYS == SHARED ? ((size_t)(w + ti_group_tile(q0, run.b, rt, a.G, TR * ROWS)) * a.p.nKv + hk0 + hh) * (TR * ROWS) + ROWS * r + rr
-                                                 : ((size_t)(w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + rr;
+                const size_t at = KEYS == SHARED ? ((size_t)w * a.p.nKv + hk0 + hh) * (TR * ROWS) + ROWS * r + rr
+                                                 : ((size_t)(GROUPS ? w : w + run.b) * a.p.nKv + hk0 + hh) * a.R + rt * ROWS + rr;
                 *reinterpret_cast<v4f*>(a.po + at * HD + 4 * d) = x;
                 if (d == 0) {
                     a.pml[2 * at] = M;
@@ -739,21 +760,23 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
                 }
             }
         }
+        if constexpr (GROUPS) {
+            if (c0 == 0 && hk0 == 0 && (KEYS == SHARED || rt == 0) && tid == 0) {   // the tile's or sequence's slots, for the merge
+                const int u = KEYS == SHARED ? ti_group_tile(q0, run.b, rt, a.G, TR * ROWS) : run.b;
+                a.meta[2 * u] = w;
+                a.meta[2 * u + 1] = run.parts;
+            }
+            return;
+        }
         if (PAGED && c0 == 0 && hr == 0 && tid == 0) {          // the sequence's slots, for the merge
-            const int u = KEYS == SHARED ? ti_group_tile(q0, run.b, rt, a.G, TR * ROWS) : run.b;
-            a.meta[2 * u] = w + u;
-            a.meta[2 * u + 1] = (int)quotient(run.start + nb - 1, run.chunk) - w + 1;
+            a.meta[2 * run.b] = w + run.b;
+            a.meta[2 * run.b + 1] = (int)ti_quotient(run.start + nb - 1, run.chunk) - w + 1;
         }
         run.left -= part;
         if (run.left <= 0) return;
+        run.b++;
         run.start += nb;
         run.block = 0;
-        if (++run.tile >= tiles) {
-            run.tile = 0;
-            run.b++;
-            if constexpr (KEYS == SHARED)
-                while (run.b < a.p.P - 1 && !group_tiles(a, run.b)) run.b++;
-        }
         __syncthreads();                                   // the parts are read
     }
 }
@@ -764,17 +787,15 @@ __global__ __launch_bounds__(THREADS, COLS ? 3 : 2) void k_token_attn(TokArgs a)
     token_attn<HD, KEYS, COLS>(a, blockIdx.x, L);
 }
 
-// Groups: the first `nshared` workgroups and those behind `nown` more take the positions that groups share, the others each
-// sequence's own. Those of long runs come last: where there are none they end at once, and nothing waits for them
+// Groups: the first `nshared` workgroups take the positions that groups share, the others each sequence's own
 template <int HD, bool COLS>
-__global__ __launch_bounds__(THREADS, 2) void k_group_attn(TokArgs own, TokArgs shared, unsigned nshared, unsigned nown) {
+__global__ __launch_bounds__(THREADS, 2) void k_group_attn(TokArgs own, TokArgs shared, unsigned nshared) {
     __shared__ __align__(16) union {
         TokLds<HD, COLS, 1> own;
         TokLds<HD, HD == 32, wave_tiles(SHARED, HD == 32)> shared;
     } L;
-    const unsigned i = blockIdx.x;
-    if (i - nshared < nown) token_attn<HD, OWN, COLS>(own, i - nshared, L.own);
-    else token_attn<HD, SHARED, HD == 32>(shared, i < nshared ? i : i - nown, L.shared);
+    if (blockIdx.x < nshared) token_attn<HD, SHARED, HD == 32>(shared, blockIdx.x, L.shared);
+    else token_attn<HD, OWN, COLS>(own, blockIdx.x - nshared, L.own);
 }
 
 // The weights that each key received, by the merge's workgroups behind the rows' own (part of parts): every head's (max, sum)
@@ -993,6 +1014,7 @@ int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     s.po = a.spo;
     s.pml = a.spml;
     s.meta = a.smeta;
+    a.many = (int)wgs;
     s.many = (int)many;
     s.wgs = (int)((many + 1) / 2);
     s.HW = 1;
@@ -1000,12 +1022,12 @@ int ti_group_attn_launch(ti_ctx* c, const TiTokenAttn& p, int hd) {
     s.RT = 1;
     a.wgs = (int)wgs;
     a.sslots = s.sslots = (int)(many + places);
-    wgs = ti_min(wgs, p.B * most);
-    many = ti_min(many, places * most);
-    const unsigned ns = (unsigned)(ti_min(many, (long)s.wgs) * p.nKv), no = (unsigned)(wgs * a.RT * heads), grid = (unsigned)(many * p.nKv) + no;
+    // a run more for every sequence and tile, which its last one may leave short
+    const unsigned ns = (unsigned)((ti_min(many + places, places * most) + XCDS - 1) / XCDS * XCDS * p.nKv);
+    const unsigned grid = ns + (unsigned)((ti_min(wgs + p.B, p.B * most) + XCDS - 1) / XCDS * XCDS * a.RT * heads);
 #define GROUP(HD_) if (hd == HD_) { \
-        if (HD_ == 32 || a.R <= crows) k_group_attn<HD_, true><<<grid, THREADS, 0, c->stream>>>(a, s, ns, no); \
-        else if constexpr (HD_ > 32) k_group_attn<HD_, false><<<grid, THREADS, 0, c->stream>>>(a, s, ns, no); \
+        if (HD_ == 32 || a.R <= crows) k_group_attn<HD_, true><<<grid, THREADS, 0, c->stream>>>(a, s, ns); \
+        else if constexpr (HD_ > 32) k_group_attn<HD_, false><<<grid, THREADS, 0, c->stream>>>(a, s, ns); \
         launch_merge<HD_, true>(c, a, 0); }
     GROUP(128) GROUP(96) GROUP(64) GROUP(32)
 #undef GROUP

@@ -80,6 +80,23 @@ TI_HD inline TiGroup ti_group_of(const int32_t* starts, const int32_t* shared, i
 TI_HD inline int ti_group_tile(int first, int g, int tile, int G, int rows) {
     return (int)((long)first * G / rows) + ti_min(g, first / 2) + tile;
 }
+// a / b of numbers that are rarely as large as 64 bits, whose division takes four times as long
+TI_HD inline long ti_quotient(long a, long b) { return (a | b) >> 31 ? a / b : (long)((uint32_t)a / (uint32_t)b); }
+// Into how many runs a tile's or sequence's nb blocks are cut, where all units of `tiles` tiles each have `total` together: its share
+// of wgs workgroups, of a block for each of a run's BW waves at least. `many` (2 wgs or one less) instead where a wave would have more than
+// 8 blocks: a second workgroup a CU hides the first one's loads and waits, but doubles the partials and the operands, which short runs feel (32
+// sequences of 16 heads over 8 behind 8192 shared keys 33.8 us with one, 38.5 with two; 16384 47.3 / 45.6; 32768 71.0 / 62.2; 128 sequences of
+// 32768 241 / 172). Of several tiles a multiple of the XCDs, so that a part's workgroups are on one XCD for all of them and its keys come
+// into that L2 once (48 sequences of three tiles behind 12288 keys 63.0 us, 47.3 so). All units' runs are many plus their tiles at most: rounding
+// up concerns units of nine runs and more, eight times as many in all as there are such tiles, and makes them 16/9 as many
+constexpr int TI_XCDS = 8, TI_LONG_RUN = 8;
+TI_HD inline int ti_group_parts(long total, int nb, int tiles, int wgs, int many, int BW) {
+    const bool more = many > wgs && total > (long)TI_LONG_RUN * BW * wgs;
+    const int n = more ? many : wgs;
+    const long chunk = ti_max(ti_quotient(total + n - 1, n), (long)BW);
+    const int parts = (int)ti_quotient(nb + chunk - 1, chunk);
+    return tiles < 2 || parts <= TI_XCDS ? parts : (more ? parts : parts + TI_XCDS - 1) / TI_XCDS * TI_XCDS;
+}
 inline bool ti_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
 inline int ti_log2(int v) { return 31 - __builtin_clz((unsigned)v); }
 static inline bool ti_al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

@@ -56,6 +56,7 @@ extern "C" int group_of(const int32_t* starts, const int32_t* shared, int P, int
 extern "C" int base(const int32_t* starts, const int32_t* shared, int P, int B, int b) { return ti_group_of(starts, shared, P, B, b).shared; }
 extern "C" int first(const int32_t* starts, int B, int g) { return ti_group_members(starts, B, g).first; }
 extern "C" int count(const int32_t* starts, int B, int g) { return ti_group_members(starts, B, g).count; }
+extern "C" int parts(long total, int nb, int tiles, int wgs, int many, int BW) { return ti_group_parts(total, nb, tiles, wgs, many, BW); }
 extern "C" int number(int first, int g, int tile, int G, int rows) { return ti_group_tile(first, g, tile, G, rows); }
 """
 
@@ -133,3 +134,24 @@ def test_the_adapters_bound_sees_a_lost_piece(K):
         assert np.linalg.norm(got - want) > norm, bits
     got, _, _ = ref.lora(x.astype(np.float32).astype(np.float64), y, [0], a, b, np.ones(1))
     assert np.linalg.norm(got - want) < norm
+
+
+def test_runs_of_groups_fit_their_slots(host):
+    """Every tile has a run, none more than blocks; all of them have no more than the slots that a call keeps: many, and one a tile."""
+    rng = np.random.default_rng(6)
+    host.parts.argtypes = [C.c_long] + [C.c_int] * 5
+    most = 0.0
+    for _ in range(20000):
+        units = int(rng.integers(1, 12))
+        nb, tiles = np.rint(2.0 ** rng.uniform(0, 22 if rng.random() < 0.1 else 9, units)).astype(int), np.rint(2.0 ** rng.uniform(0, rng.integers(1, 6), units)).astype(int)
+        many = int(np.rint(2.0 ** rng.uniform(0, 10)))
+        wgs, BW = (many + 1) // 2, 4
+        if rng.random() < 0.2:                             # sequences' own keys: always one tile
+            wgs, tiles, BW = many, np.ones_like(tiles), int(rng.choice([1, 2, 4]))
+        total = int((nb * tiles).sum())
+        n = [host.parts(total, int(b), int(t), wgs, many, BW) for b, t in zip(nb, tiles)]
+        assert all(1 <= p <= b for p, b in zip(n, nb))
+        runs = sum(p * int(t) for p, t in zip(n, tiles))
+        assert runs <= many + tiles.sum()
+        most = max(most, runs / (many + tiles.sum()))
+    assert most > 0.9
