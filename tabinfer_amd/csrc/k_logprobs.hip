@@ -12,6 +12,9 @@
 // at the end, the list is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
 // cost little more than a comparison. A workgroup sorts once, what is above the largest of its waves' limits.
 //
+// Bound by the stream where rows are many (400 rows of 151936 logits, 243 MB, 42.1 + 4.8 us: 5.2 TB/s), with tokens kept by each wave's first chunk and
+// the sorts (48 rows with 20 tokens, 29 MB, 23.8 us; without tokens 10.1), in one row by the chain from its first load to the join (with five tokens 10.0).
+//
 // Long rows are cut into parts. Of up to 128 rows the workgroup that ends last joins a row's parts, of more a second launch does.
 #include "ti_dev.h"
 #include "ti_span.h"

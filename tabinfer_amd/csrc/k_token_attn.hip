@@ -16,6 +16,13 @@
 //    lane's scores are those of one row: they are the B operand of O^T = V^T P^T as they stand.
 //    P times the V scale of (key, group) in f32, as three bf16, exactly; V through the transposing LDS read.
 //  - The waves' (m, l, O) meet in LDS; the workgroups' partials in k_token_merge.
+//  - Groups that share their first positions (ti_attn_shared_q8): softmax over the shared keys and a sequence's own are two partials of the
+//    same row, joined as all are. One launch has workgroups of both: the shared keys' take two tiles of 16 rows of a group (row = sequence x query
+//    head) at a time, so that a block is read and widened once for 32 rows, with four waves on one head's blocks and the queries' operands
+//    in LDS; a sequence's own keys go as above. 32 sequences of 16 heads over 8 behind 8192 shared keys, 500 and fewer of their own (32 MB):
+//    28.4 + 6.0 us, of which the shared keys take about 16; four samples of 1024 10.5 + 4.4; six groups of up to 8 x 6000 24.6 + 6.7. A CU's
+//    SIMDs issue VALU instructions in half of their cycles (a weight times its V scale, split for every group, is half of those), the rest is waits
+//    for LDS and for keys, four waves a CU having none to cover them.
 //  - Bound by the stream where the keys are many (32 ragged sequences of 8 heads of 128 dims, 211 MB: 49.6 + 4.8 us: 4.3
 //    TB/s, 3.9 with the merge), else by its round trips (length, table, rows) and the second launch: 4100
 //    keys 8.3 + 4.2 us, one sequence of 8191 over pages 11.6 + 4.4.
