@@ -550,7 +550,7 @@ int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const flo
  * angles rot * theta^(-2i/hd) of 64 bits. table, seq, pos, places that do not exist and rows of one place as
  * ti_kv_write_paged_q8's; rot is any number: after an eviction a token's slot is not its position. ldq floats from one row of q to
  * the next, ldkv of k and of v (0: dense; multiples of 4, at least a row's heads): q, k and v may be parts of one projection's rows. nHq 0:
- * K and V alone, q and qr NULL. qr is q itself (dense rows) or does not overlap it. nHq and nKv <= 64; theta >= 1; q, k, v, qr, kq and
+ * K and V alone, q and qr NULL. qr is q itself (dense rows) or does not overlap it, nor k or v. nHq and nKv <= 64; theta >= 1; q, k, v, qr, kq and
  * vq 16-byte, the norms' weights 8-byte aligned; T times the (nHq + 2 nKv) hd / 1024 of a row, rounded up, < 2^24. */
 int ti_attn_prep_paged_q8(ti_ctx* ctx, const float* q, const float* k, const float* v, const uint16_t* qn_w,
                           const uint16_t* kn_w, float* qr, uint32_t* kq, float* ks, uint32_t* vq, float* vs,

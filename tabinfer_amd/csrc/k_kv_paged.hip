@@ -277,6 +277,8 @@ extern "C" int ti_attn_prep_paged_q8(ti_ctx* c, const float* q, const float* k, 
     if (nHq) {
         const uintptr_t q0 = (uintptr_t)q, r0 = (uintptr_t)qr, q1 = q0 + 4 * ((T - 1) * (size_t)a.ldq + nHq * hd), r1 = r0 + 4 * (size_t)T * nHq * hd;
         TI_REQUIRE((q0 == r0 && a.ldq == nHq * hd) || q1 <= r0 || r1 <= q0, "%s: qr is q itself, with dense rows, or does not overlap it", fn);
+        const size_t kv = 4 * ((T - 1) * (size_t)a.ldkv + nKv * hd);
+        for (const float* p : {k, v}) TI_REQUIRE((uintptr_t)p + kv <= r0 || r1 <= (uintptr_t)p, "%s: qr overlaps k or v", fn);
     }
     TI_REQUIRE_DENSE(fn, kq);
     TI_REQUIRE_DENSE(fn, vq);

@@ -356,6 +356,7 @@ __device__ __forceinline__ void token_attn(const TokArgs& a, const unsigned bloc
         w = i / n * XCDS + block % XCDS;
     }
     const int hs = wave % a.HW, bw = wave / a.HW, hk0 = hr % groups * a.HW, hk = hk0 + hs;
+    if (KEYS == SHARED && w >= a.sslots) return;           // groups that overlap may have more runs than there are slots
     int rt = hr / groups, R = a.R;
     Run run;
     if (!find_run<KEYS>(a, w, run, L.run)) return;                     // workgroup-uniform

@@ -24,7 +24,7 @@ LORA = [P, P, P, P, P, Q, 3, 64, 40, 8, 2, 0, 0, 1]
 LP = [P, P, P, P, P, P, P, 3, 100, 0, 5]
 REFUSED = {
     "ti_attn_prep_paged_q8": (PREP, [{i: None} for i in (0, 1, 2, 5, 6, 7, 8, 9, 12)] + [{0: P + 4}, {1: P + 8}, {2: P + 4}, {3: P + 2}, {4: P + 4}, {5: Q + 8}, {6: P + 4}, {8: P + 8},
-                              {5: P + 16}, {5: P, 22: 512}, {14: 0}, {14: -1}, {15: 0}, {16: -1}, {16: 65}, {17: 0}, {17: 65}, {18: 0}, {18: 48}, {18: 160}, {19: 0}, {19: 12}, {20: 0},
+                              {5: P + 16}, {5: P, 22: 512}, {1: Q}, {2: Q + 2032}, {14: 0}, {14: -1}, {15: 0}, {16: -1}, {16: 65}, {17: 0}, {17: 65}, {18: 0}, {18: 48}, {18: 160}, {19: 0}, {19: 12}, {20: 0},
                               {21: 0}, {11: None, 14: 5, 15: 4}, {22: 255}, {22: 252}, {22: -4}, {23: 130}, {23: 124}, {24: 0.5}, {24: 0.0}, {24: -1.0}, {24: NAN}, {24: INF},
                               {14: 2 ** 24, 15: 2 ** 24}, {19: 2 ** 20, 21: 2 ** 11}]),
     "ti_attn_shared_q8": (SHARED, [{i: None} for i in range(10)] + [{9: P}, {1: P + 8}, {3: P + 4}, {10: 0}, {10: 2049}, {11: 0}, {11: -1}, {11: 5}, {12: 3}, {12: 65, 13: 65}, {13: 0},
