@@ -1,9 +1,10 @@
 // k_logprobs.hip — log probabilities of given tokens under rows of logits, the rows' entropy and their likeliest tokens, in one pass over
 // the logits. The reference has no counterpart: its sampler keeps an index (models/qwen3.js:2624-2740).
 //
-// With M the row's maximum, S = sum e^(x - M) and U = sum e^(x - M) (x - M): log p(x) = (x - M) - ln S and the entropy
-// ln S - U / S, two terms of one sign. A lane keeps (m, s, u) of its own elements and turns them to a new maximum by
-// s' = a s, u' = a (u + (m - m') s), a = e^(m - m'); lanes, waves and workgroups are joined by the same rule in a fixed order.
+// With M the row's maximum, C the number of elements equal to it, S = sum e^(x - M) of the others and U = sum e^(x - M) (x - M): log p(x) =
+// (x - M) - ln (C + S) and the entropy ln (C + S) - U / (C + S), two terms of one sign. C and S apart, so that the logarithm is that of 1 + (C - 1 + S)
+// and a token that is nearly certain keeps its digits. A lane keeps (m, c, s, u) of its own elements and turns them to a larger maximum by
+// s' = a (s + c), c' = 0, u' = a (u + (m - m') (s + c)), a = e^(m - m'); lanes, waves and workgroups are joined by the same rule in a fixed order.
 //
 // The likeliest: a value and its index are one 64-bit key (the float's bits in an order of whole numbers, then the inverted index: the lower
 // index wins), so that no two are equal. A wave takes 1024 elements at a time, in registers. Where `top` lanes hold something above its
@@ -30,13 +31,15 @@ constexpr int SEGS_MAX = 64;                 // workgroups a row: one lane each 
 constexpr int ROWS_MAX = 1 << 17;
 constexpr float LOW = -3.402823466e38f;
 
+constexpr int PART = 8;                      // floats a part
+
 struct LpArgs {
     const float* x;
     const int32_t* ids;
     float *lp, *ent;
     int32_t *rank, *top_ids;
     float* top_lp;
-    float4* part;                            // [row][segs] (m, s, u, number of logits above the token's)
+    float* part;                             // [row][segs][PART] (m, s, u, c, number of logits above the token's)
     uint64_t* keys;                          // [row][segs][top], from large to small, 0 behind the last
     uint32_t* arrived;                       // a line a row, 0 between launches; or nullptr: a second launch joins the parts
     long ld;
@@ -52,17 +55,24 @@ __device__ __forceinline__ uint64_t key_of(uint32_t u, uint32_t index) { return 
 
 struct Sum {
     float m, s, u;
+    int c;
 };
 __device__ __forceinline__ float down_to(float d) { return d < -150.0f ? -150.0f : d; }      // e^-150 is 0; NaN stays
-__device__ __forceinline__ Sum joined(const Sum& a, const Sum& b) {
-    const float m = fmaxf(a.m, b.m), da = down_to(a.m - m), db = down_to(b.m - m);
-    const float ea = expf(da), eb = expf(db);
-    return {m, a.s * ea + b.s * eb, ea * (a.u + da * a.s) + eb * (b.u + db * b.s)};
+// a, at the maximum m of its own or a larger one
+__device__ __forceinline__ Sum turned(const Sum& a, float m) {
+    const float d = down_to(a.m - m), e = expf(d), all = a.s + (float)a.c;
+    const bool same = d == 0.0f;
+    return {m, same ? a.s : all * e, e * (a.u + d * all), same ? a.c : 0};
 }
-__device__ __forceinline__ Sum wave_joined(Sum a) {
+__device__ __forceinline__ Sum joined(const Sum& a, const Sum& b) {
+    const float m = fmaxf(a.m, b.m);
+    const Sum x = turned(a, m), y = turned(b, m);
+    return {m, x.s + y.s, x.u + y.u, x.c + y.c};
+}
+__device__ __forceinline__ Sum wave_joined(const Sum& a) {
     // the maximum first, so that every lane turns its own to it once; the offsets spelled out, as ti_wave_sum's
-    const float m = ti_wave_max(a.m), d = down_to(a.m - m), e = expf(d);
-    return {m, ti_wave_sum(a.s * e), ti_wave_sum(e * (a.u + d * a.s))};
+    const Sum x = turned(a, ti_wave_max(a.m));
+    return {x.m, ti_wave_sum(x.s), ti_wave_sum(x.u), ti_wave_sum_i(x.c)};
 }
 
 // ---- 64 keys, a lane each, from large to small ---------------------------------------------------------------------
@@ -117,12 +127,12 @@ __device__ __forceinline__ uint32_t value_at(uint64_t kept, int i) { return __bu
 // what a row's numbers come to, and its likeliest tokens' (key of lane i the i-th)
 __device__ __forceinline__ void finish(const LpArgs& a, int t, const Sum& r, int above, uint64_t key) {
     const int lane = threadIdx.x & 63;
-    const float ln = logf(r.s);
+    const float ln = log1pf((float)(r.c - 1) + r.s);
     if (lane == 0) {
         const int id = a.ids[t];
         const bool there = id >= 0 && id < a.N;
         a.lp[t] = there ? (a.x[t * a.ld + id] - r.m) - ln : -INFINITY;
-        if (a.ent) a.ent[t] = ln - r.u / r.s;
+        if (a.ent) a.ent[t] = ln - r.u / ((float)r.c + r.s);
         if (a.rank) a.rank[t] = there ? above + 1 : 0;
     }
     if (lane < a.top) {
@@ -153,10 +163,10 @@ template <bool PUB>
 __device__ __forceinline__ void join_parts(const LpArgs& a, int t, uint64_t (*s_waves)[64]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = a.segs * a.top;
     const bool has = lane < a.segs;
-    const float* q = reinterpret_cast<const float*>(a.part + (size_t)t * a.segs + ti_min(lane, a.segs - 1));
+    const float* q = a.part + ((size_t)t * a.segs + ti_min(lane, a.segs - 1)) * PART;
     const uint64_t* keys = a.keys + (size_t)t * n;
     auto number = [&](int i) { return PUB ? ti_pub_load(q + i) : q[i]; };
-    const float m = number(0), sum = number(1), u = number(2), above = number(3);
+    const float m = number(0), sum = number(1), u = number(2), c = number(3), above = number(4);
     auto load = [&](int j) {
         const uint64_t* k = keys + ti_min(j + lane, n - 1);
         const uint64_t key = PUB ? ti_pub_load(k) : *k;
@@ -173,7 +183,7 @@ __device__ __forceinline__ void join_parts(const LpArgs& a, int t, uint64_t (*s_
     if (n > 64)
 #pragma unroll
         for (int w = 0; w < WAVES - 1; w++) kept = larger(kept, s_waves[w][lane]);
-    const Sum r = wave_joined(has ? Sum{m, sum, u} : Sum{LOW, 0.0f, 0.0f});
+    const Sum r = wave_joined(has ? Sum{m, sum, u, __float_as_int(c)} : Sum{LOW, 0.0f, 0.0f, 0});
     finish(a, t, r, ti_wave_sum_i(has ? __float_as_int(above) : 0), kept);
 }
 
@@ -195,7 +205,7 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
     uint64_t kept = 0;
     int listed = 0;
     uint32_t last = 0;                                     // a value that `top` keys so far reach: what comes later has to be larger
-    Sum r = {LOW, 0.0f, 0.0f};
+    Sum r = {LOW, 0.0f, 0.0f, 0};
     int above = 0;
     auto load = [&](long at, float (&v)[EPT]) {
         const long i0 = at + 4 * lane;
@@ -227,14 +237,12 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
 #pragma unroll
         for (int i = 1; i < EPT; i++) most = fmaxf(most, v[i]);
         const float m = fmaxf(r.m, most);
-        const float d = down_to(r.m - m), f = expf(d);
-        r.u = f * (r.u + d * r.s);
-        r.s = f * r.s;
-        r.m = m;
+        r = turned(r, m);
 #pragma unroll
         for (int i = 0; i < EPT; i++) {
             const float z = down_to(v[i] - m), e = __builtin_amdgcn_exp2f(z * 1.44269504088896341f);
-            r.s += e;
+            r.s += z == 0.0f ? 0.0f : e;
+            r.c += z == 0.0f;
             r.u = fmaf(e, z, r.u);
             above += v[i] > xi;
         }
@@ -347,16 +355,19 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
         return;
     }
     const size_t p = (size_t)t * a.segs + seg;
-    float* q = reinterpret_cast<float*>(a.part + p);
+    float* q = a.part + p * PART;
     if (!a.arrived) {
         if (wave != 0) return;
-        if (lane == 0) *reinterpret_cast<float4*>(q) = make_float4(r.m, r.s, r.u, __int_as_float(above));
+        if (lane == 0) {
+            *reinterpret_cast<float4*>(q) = make_float4(r.m, r.s, r.u, __int_as_float(r.c));
+            q[4] = __int_as_float(above);
+        }
         if (TOP && lane < top) a.keys[p * top + lane] = key;
         return;
     }
     if (wave == 0) {
-        const float number = lane == 0 ? r.m : lane == 1 ? r.s : lane == 2 ? r.u : __int_as_float(above);
-        if (lane < 4) ti_pub_store(q + lane, number);
+        const float number = lane == 0 ? r.m : lane == 1 ? r.s : lane == 2 ? r.u : __int_as_float(lane == 3 ? r.c : above);
+        if (lane < 5) ti_pub_store(q + lane, number);
         if (TOP && lane < top) ti_pub_store(a.keys + p * top + lane, key);
         ti_stores_done();
         if (lane == 0) s_last = ti_arrive(a.arrived + t * TI_SYNC_LOGPROBS_STRIDE) == (uint32_t)(a.segs - 1);
@@ -390,9 +401,9 @@ extern "C" int ti_logprobs(ti_ctx* c, const float* logits, const int32_t* ids, f
     a.per = (int)((steps + segs - 1) / segs);
     a.segs = (int)((steps + a.per - 1) / a.per);
     // fewer than T + 4 CUs of them
-    static_assert((ROWS_MAX + 4L * 4096) * (16 + 8 * TOP_MAX) <= 4L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "the parts fit the scratch");
-    a.part = reinterpret_cast<float4*>(c->attn_po);
-    a.keys = reinterpret_cast<uint64_t*>(a.part + (size_t)T * a.segs);
+    static_assert((ROWS_MAX + 4L * 4096) * (4 * PART + 8 * TOP_MAX) <= 4L * TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX, "the parts fit the scratch");
+    a.part = c->attn_po;
+    a.keys = reinterpret_cast<uint64_t*>(a.part + (size_t)T * a.segs * PART);
     if (T <= TI_LOGPROBS_ROWS) a.arrived = c->sync + TI_SYNC_LOGPROBS;
     const unsigned grid = (unsigned)(T * a.segs);
     if (top) k_logprobs<true><<<grid, 256, WAVES * (EPT * top + LONG) * 8, c->stream>>>(a);

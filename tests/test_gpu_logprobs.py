@@ -168,3 +168,34 @@ def test_captured_call_follows_logits_and_ids(ctx):
     ctx.graph_destroy(g)
     for b in [dx, di] + outs:
         b.free()
+
+
+@pytest.mark.parametrize("T", [127, 128, 129])
+def test_rows_joined_by_their_last_workgroup_or_a_second_launch(ctx, T):
+    """Two calls one behind the other on the same scratch; the second's rows as if it were alone."""
+    rng = np.random.default_rng(T)
+    for N, top in ((9001, 5), (20000, 64)):
+        x = (2.5 * rng.standard_normal((T, N))).astype(np.float32)
+        ids = rng.integers(0, N, T).astype(np.int32)
+        check(run(ctx, x, ids, top), x, ids, top)
+
+
+@pytest.mark.parametrize("T,N,top,far", [(1, 100, 5, 9.0), (4, 5000, 0, 12.0), (3, 151936, 20, 25.0), (200, 9001, 3, 18.0), (2, 3000, 1, 40.0)])
+def test_near_certainty(ctx, T, N, top, far):
+    """One token has almost all of the probability: its log probability and the row's entropy keep their digits. With s the others' sum of e^d, d
+    their distances: ln S = log1p(s), s off by (N / 256 + 58) U of itself and 3 U of the sum of e^d |d|; the entropy's sum of e^d |d| likewise, by d^2 more."""
+    rng = np.random.default_rng(N)
+    x = (2 * rng.standard_normal((T, N))).astype(np.float32)
+    ids = rng.integers(0, N, T).astype(np.int32)
+    x[np.arange(T), ids] = x.max(1) + np.float32(far)
+    got = run(ctx, x, ids, top)
+    for t in range(T):
+        d = np.delete(x[t].astype(np.float64) - x[t].max().astype(np.float64), ids[t])
+        e = np.exp(d)
+        s, sd, sdd = e.sum(), (e * -d).sum(), (e * d * d).sum()
+        lp, ent = -np.log1p(s), np.log1p(s) + sd / (1 + s)
+        tl = ((N / 256 + 58) * s + 3 * sd) * ref.U + 4 * ref.U * -lp + 2.0 ** -140
+        te = tl + ((N / 256 + 62) * sd + 3 * sdd) * ref.U + 4 * ref.U * ent + 2.0 ** -140
+        assert got["rank"][t] == 1 and abs(got["lp"][t] - lp) <= tl and abs(got["ent"][t] - ent) <= te, (t, got["lp"][t], lp, got["ent"][t], ent)
+        if top:
+            assert got["top_ids"][t, 0] == ids[t] and abs(got["top_lp"][t, 0] - lp) <= tl
