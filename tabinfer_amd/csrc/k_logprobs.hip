@@ -240,10 +240,10 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
         r = turned(r, m);
 #pragma unroll
         for (int i = 0; i < EPT; i++) {
-            const float z = down_to(v[i] - m), e = __builtin_amdgcn_exp2f(z * 1.44269504088896341f);
+            const float z = v[i] - m, e = __builtin_amdgcn_exp2f(z * 1.44269504088896341f);
             r.s += z == 0.0f ? 0.0f : e;
             r.c += z == 0.0f;
-            r.u = fmaf(e, z, r.u);
+            r.u = fmaf(e, fmaxf(z, -150.0f), r.u);         // e^-150 is 0; a NaN is in s
             above += v[i] > xi;
         }
         if constexpr (TOP) {
