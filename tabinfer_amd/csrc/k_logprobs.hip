@@ -9,8 +9,8 @@
 // The likeliest: a value and its index are one 64-bit key (the float's bits in an order of whole numbers, then the inverted index: the lower
 // index wins), so that no two are equal. A wave takes 1024 elements at a time, in registers. Where `top` lanes hold something above its
 // limit, as always at first, the limit is raised to the top-th largest of the lanes' maxima, found bit by bit with ballots; what is above it
-// goes to a list in LDS, of at most `top` lanes and so 16 top keys a chunk, whatever the values are. Where it has grown to more than 64 keys, and
-// at the end, the list is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
+// goes to a list in LDS, of at most `top` lanes and so 16 top keys a chunk, whatever the values are. (The first limit is that of all of the
+// workgroup's waves together.) Where the list has grown to more than 64 keys, and at the end, it is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
 // cost little more than a comparison. A workgroup sorts once, what is above the largest of its waves' limits.
 //
 // Bound by the stream where rows are many (400 rows of 151936 logits, 243 MB, 42.1 + 4.8 us: 5.2 TB/s), with tokens kept by each wave's first chunk and
@@ -142,18 +142,34 @@ __device__ __forceinline__ void finish(const LpArgs& a, int t, const Sum& r, int
     }
 }
 
-// The m-th largest value that 64 lanes hold, m <= 64 (0 where fewer hold one); `held`: lanes that reach it. Bit by bit with ballots
-__device__ __forceinline__ uint32_t value_of_rank(uint32_t v, int m, int& held) {
-    uint32_t limit = 0;
-    held = 65;
-    for (uint32_t bit = 0x80000000u; bit && held > m; bit >>= 1) {
-        const int n = __builtin_popcountll(__ballot(v >= (limit | bit)));
-        if (n >= m) {
-            limit |= bit;
+// What `top` lanes of a workgroup's first step reach, of the upper 16 bits of a value: every wave then lists a fourth of what a limit of its own
+// would let through. 0 (every wave finds its own) where that is no number, or zero, below which there is no other next to it; or where more of this
+// wave's lanes reach it than its list has room for. 48 rows with 5 tokens 20.2 us (each wave with a limit of its own 22.3), with 20 20.8 (24.3), with 64
+// 28.8 (36.0), 1000 rows of 30000 with 5 35.9 (41.6); one row with 10 12.8 (11.9), with 64 22.9 (30.2)
+__device__ __forceinline__ uint32_t first_limit(const float (&v)[EPT], long there, int top, uint32_t* s_most) {
+    const int lane = threadIdx.x & 63, in = (int)ti_max(-256L, ti_min((long)CHUNK, there)) - 4 * lane;
+    uint32_t most = 0, reach = 0;
+    if (there > 0) {
+#pragma unroll
+        for (int i = 0; i < EPT; i++) most = max(most, 256 * (i / 4) + i % 4 < in ? ordered(v[i]) : 0u);
+    }
+    s_most[threadIdx.x] = most;
+    __syncthreads();
+    uint32_t w[WAVES];
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) w[k] = s_most[64 * k + lane];
+    int held = 64 * WAVES + 1;
+    for (uint32_t bit = 0x80000000u; bit > 0x8000u && held > top; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) n += __builtin_popcountll(__ballot(w[k] >= (reach | bit)));
+        if (n >= top) {
+            reach |= bit;
             held = n;
         }
     }
-    return limit;
+    const bool fits = __builtin_popcountll(__ballot(most >= reach)) <= top;
+    return fits && reach > ordered(-INFINITY) && reach != ordered(0.0f) ? reach : 0u;
 }
 
 // A row's parts, by a workgroup: their numbers, a lane of the first wave each, and their keys, 64 at a time. (Only those above what the parts' j-th
@@ -223,11 +239,15 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
     };
     float v[EPT], next[EPT];
     long at = begin + wave * CHUNK;
-    if (at < end) load(at, next);
-    for (; at < end; at += STEP) {
+    if (at < end) load(at, v);
+    if (at + STEP < end) load(at + STEP, next);
+    if constexpr (TOP) last = first_limit(v, end - at, top, reinterpret_cast<uint32_t*>(&s_waves[0][0]));
+    for (bool begun = false; at < end; at += STEP, begun = true) {
+        if (begun) {
 #pragma unroll
-        for (int i = 0; i < EPT; i++) v[i] = next[i];
-        if (at + STEP < end) load(at + STEP, next);
+            for (int i = 0; i < EPT; i++) v[i] = next[i];
+            if (at + STEP < end) load(at + STEP, next);
+        }
         const int in = (int)ti_min((long)CHUNK, end - at) - 4 * lane;       // of the lane's elements, those at 256 (i / 4) + i % 4 below it
         if (at + CHUNK > end) {
 #pragma unroll
@@ -247,10 +267,10 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
             above += v[i] > xi;
         }
         if constexpr (TOP) {
-            const uint64_t lanes = __ballot(last == 0 || most > value_of(last));
+            const float least = value_of(begun ? last : last - 1);               // what reaches the first step's limit counts in it
+            const uint64_t lanes = __ballot(last == 0 || most > least);
             if (lanes == 0) continue;
-            if (last != 0 && __builtin_popcountll(lanes) < top) {
-                const float least = value_of(last);
+            if (last != 0 && (!begun || __builtin_popcountll(lanes) < top)) {
 #pragma unroll
                 for (int i = 0; i < EPT; i++) {
                     const bool take = v[i] > least;        // no NaN, nothing behind the row's end

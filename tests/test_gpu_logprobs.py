@@ -199,3 +199,32 @@ def test_near_certainty(ctx, T, N, top, far):
         assert got["rank"][t] == 1 and abs(got["lp"][t] - lp) <= tl and abs(got["ent"][t] - ent) <= te, (t, got["lp"][t], lp, got["ent"][t], ent)
         if top:
             assert got["top_ids"][t, 0] == ids[t] and abs(got["top_lp"][t, 0] - lp) <= tl
+
+
+@pytest.mark.parametrize("top", [15, 16, 20, 64])
+@pytest.mark.parametrize("kind", ["few values", "zeros", "signed zeros", "mostly masked", "lowest", "one lane's", "large behind", "not numbers"])
+def test_limits_of_a_first_step(ctx, kind, top):
+    """Values that tie, that are next to no other, that lie in few lanes, in the first 4096 elements and behind them."""
+    rng = np.random.default_rng(top)
+    for T, N in ((2, 4096), (3, 4097), (2, 30011), (300, 9001)):
+        x = rng.standard_normal((T, N)).astype(np.float32)
+        if kind == "few values":
+            x = np.round(x)
+        elif kind == "zeros":
+            x = np.minimum(x, 0)
+        elif kind == "signed zeros":
+            x = np.where(x > 0, np.copysign(np.float32(0), rng.standard_normal((T, N)).astype(np.float32)), x)
+        elif kind == "mostly masked":
+            x[rng.random((T, N)) > 30 / N] = -np.inf
+        elif kind == "lowest":
+            x[rng.random((T, N)) > 30 / N] = LOW
+        elif kind == "one lane's":
+            x[:, 4 * 7:4 * 7 + 4] += 100                   # of the first wave: more than its share
+            x[:, 256 + 4 * 7:256 + 4 * 7 + 4] += 100
+            x[:, :1024] += 5
+        elif kind == "large behind":
+            x[:, N - 40:] += np.arange(40, dtype=np.float32)
+        else:
+            x[rng.random((T, N)) > 0.5] = np.nan
+        ids = rng.integers(0, N, T).astype(np.int32)
+        check(run(ctx, x, ids, top), x, ids, top)
