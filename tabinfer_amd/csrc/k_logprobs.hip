@@ -173,7 +173,7 @@ __device__ __forceinline__ uint32_t first_limit(const float (&v)[EPT], long ther
 }
 
 // A row's parts, by a workgroup: their numbers, a lane of the first wave each, and their keys, 64 at a time. (Only those above what the parts' j-th
-// keys show to be unwanted, in a list: 48 rows with 20 tokens 26.1 us against 23.2, one row 12.9 against 13.6.) PUB: other workgroups of
+// keys show to be unwanted, in a list: 48 rows with 20 tokens took 2.9 us more, one row 0.7 less.) PUB: other workgroups of
 // this launch wrote them
 template <bool PUB>
 __device__ __forceinline__ void join_parts(const LpArgs& a, int t, uint64_t (*s_waves)[64]) {
@@ -415,7 +415,7 @@ extern "C" int ti_logprobs(ti_ctx* c, const float* logits, const int32_t* ids, f
     TI_REQUIRE(ld == 0 || ld >= N, "ti_logprobs: rows of %d logits, %d apart", N, ld);
     LpArgs a = {logits, ids, lp, entropy, rank, top_ids, top_lp, nullptr, nullptr, nullptr, ld ? ld : N, T, N, top, 1, 0};
     // workgroups of whole steps until every CU has four, or two where tokens are kept, which costs most in a wave's first chunk
-    // (400 rows with 20 tokens 62.2 us, with four a CU 64.7; 1000 rows of 30000 with 5 37.0 / 45.1; 48 rows with 20 23.7 / 23.0)
+    // (400 rows with 20 tokens 67.7 us, with four a CU 71.8; 1000 rows of 30000 with 5 36.8 / 41.1; 48 rows with 20 21.0 / 21.5)
     const long steps = ((long)N + STEP - 1) / STEP;
     const long segs = ti_max(1L, ti_min(ti_min((long)SEGS_MAX, steps), ((top ? 2L : 4L) * c->cus + T - 1) / T));
     a.per = (int)((steps + segs - 1) / segs);
