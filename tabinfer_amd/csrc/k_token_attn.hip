@@ -20,7 +20,7 @@
 //    same row, joined as all are. One launch has workgroups of both: the shared keys' take two tiles of 16 rows of a group (row = sequence x query
 //    head) at a time, so that a block is read and widened once for 32 rows, with four waves on one head's blocks and the queries' operands
 //    in LDS; a sequence's own keys go as above. 32 sequences of 16 heads over 8 behind 8192 shared keys, 500 and fewer of their own (32 MB):
-//    28.4 + 6.0 us, of which the shared keys take about 16; four samples of 1024 10.5 + 4.4; six groups of up to 8 x 6000 24.6 + 6.7. A CU's
+//    28.0 + 6.0 us, of which the shared keys take about 16; four samples of 1024 10.6 + 4.4; six groups of up to 8 x 6000 24.6 + 6.8. A CU's
 //    SIMDs issue VALU instructions in half of their cycles (a weight times its V scale, split for every group, is half of those), the rest is waits
 //    for LDS and for keys, four waves a CU having none to cover them.
 //  - Bound by the stream where the keys are many (32 ragged sequences of 8 heads of 128 dims, 211 MB: 49.6 + 4.8 us: 4.3
