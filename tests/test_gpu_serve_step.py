@@ -218,3 +218,34 @@ def test_javascript_launchers(ctx, tmp_path):
         same(name, buf, buf.nbytes)
     same("only", out[0], B * 4)
     assert "top" in open(os.path.join(d, "refused.out")).read()
+
+
+def test_two_contexts_at_once(ctx):
+    """Steps of two batches on two contexts' streams, neither waiting for the other: the bits of each alone."""
+    rng = np.random.default_rng(8)
+    other = abi.Ctx(0)
+    steps, alone, outs = [], [], []
+    for c, B, starts, shared in ((ctx, 8, [0, 4, 7], [37, 90]), (other, 5, [0, 5, 5], [60, 9])):
+        st = Step(c, rng, B, 2)
+        lens = rng.integers(91, 180, B).astype(np.int32)
+        table = np.arange(B * st.width, dtype=np.int32).reshape(B, st.width)
+        new = dict(x=rng.standard_normal((B, st.H)).astype(np.float32), idx=rng.integers(-1, st.n, B), ids=rng.integers(0, st.V, B), pos=lens - 1, rot=lens - 1, lens=lens, starts=starts,
+                   shared=shared, table=table)
+        for name, a in new.items():
+            c.write(st.ins[name], np.ascontiguousarray(a, np.float32 if name == "x" else np.int32))
+        rows = st.pages * st.page * st.nKv
+        for b, a in zip(st.pool, (rng.integers(-127, 128, rows * st.hd).astype(np.int8), rng.uniform(0.5, 2, rows * st.hd // 32).astype(np.float32)) * 2):
+            c.write(b, a)
+        u = st.outs()
+        st.run(u)
+        alone.append({k: c.download(b, np.uint32, b.nbytes // 4) for k, b in u.items()})
+        steps.append(st)
+        outs.append([st.outs() for _ in range(10)])
+    for i in range(10):
+        for st, o in zip(steps, outs):
+            st.run(o[i])
+    for st, o, want in zip(steps, outs, alone):
+        for u in o:
+            for k, b in u.items():
+                assert np.array_equal(st.ctx.download(b, np.uint32, b.nbytes // 4), want[k]), k
+    other.close()
