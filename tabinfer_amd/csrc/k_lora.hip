@@ -11,6 +11,7 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int RANK_MAX = 128;
+constexpr int DIM_MAX = 1 << 30;            // of K and N: 32-bit indices step past them, by columns and rounding of all parts, or by stages loaded ahead
 constexpr long ROWS_MAX = 1 << 18, SCRATCH = (long)TI_ATTN_ROWSPLITS * TI_ATTN_HD_MAX;
 static_assert(ROWS_MAX * RANK_MAX <= SCRATCH, "h of every row fits the scratch");
 
@@ -512,7 +513,7 @@ extern "C" int ti_lora_add(ti_ctx* c, const float* x, const int32_t* idx, const 
     TI_REQUIRE(g.ldx >= K && g.ldx % 4 == 0 && g.ldy >= N, "ti_lora_add: rows of %ld and %ld floats, of K = %d and N = %d; x's in multiples of 4", g.ldx, g.ldy, K, N);
     TI_REQUIRE(ti_al16(x) && ti_al16(a) && ti_al16(b), "ti_lora_add: x, a and b must be 16-byte aligned");
     TI_REQUIRE((long)T <= ROWS_MAX, "ti_lora_add: %d rows in one call", T);
-    TI_REQUIRE(K <= TI_POS_END && N <= TI_POS_END, "ti_lora_add: K = %d, N = %d", K, N);
+    TI_REQUIRE(K <= DIM_MAX && N <= DIM_MAX, "ti_lora_add: K = %d, N = %d, at most %d", K, N, DIM_MAX);
     const uintptr_t x0 = (uintptr_t)x, y0 = (uintptr_t)y, x1 = x0 + 4 * ((T - 1) * (size_t)g.ldx + K), y1 = y0 + 4 * ((T - 1) * (size_t)g.ldy + N);
     TI_REQUIRE(x1 <= y0 || y1 <= x0, "ti_lora_add: x and y overlap");
     if ((long)T * r > FEW) {
