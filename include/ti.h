@@ -142,8 +142,10 @@ int ti_linear_q4(ti_ctx* ctx, const float* x, const uint32_t* pack, const uint16
 /* Low-rank adapters of many requests beside a projection that they share (no reference counterpart): y[t] += scale[i] * B_i (A_i x[t])
  * with i = idx[t], for T rows; rows whose idx is outside [0, n) are left as they are. a [n][r][K] and b [n][N][r] are f16, or bf16
  * with bf16 = 1 (smaller ranks: rows of zeros); x [T] rows of K f32, ldx apart (0: K; a multiple of 4), y [T] rows of N, ldy apart
- * (0: N). Weights are taken as they are, activations to 2^-22 and better, sums are f32. K % 32 == 0, K and N <= 2^30, r <= 128, T <= 2^18;
- * x, a and b 16-byte aligned; y does not overlap x (from the first row to the last, with what lies between). */
+ * (0: N). Weights are taken as they are, sums are f32. Activations count as f32 up to T r = 8192; of more rows (the matrix cores) exactly too beside
+ * bf16 weights, beside f16 ones to 2^-22 of themselves or 2^-39 of the largest of their row's 32 (from a multiple of 32 on), A x likewise
+ * under its row's largest: where single channels are 2^17 above their neighbours, bf16 weights or calls of fewer rows keep those. K % 32 == 0, K and
+ * N <= 2^30, r <= 128, T <= 2^18; x, a and b 16-byte aligned; y does not overlap x (from the first row to the last, with what lies between). */
 int ti_lora_add(ti_ctx* ctx, const float* x, const int32_t* idx, const uint16_t* a, const uint16_t* b, const float* scale,
                 float* y, int T, int K, int N, int r, int n, int ldx, int ldy, int bf16);
 /* Integer per-(row, group) dots of gemvDP4 (debug/parity: exact int32). */
