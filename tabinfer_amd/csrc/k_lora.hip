@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * FWAVES) void k_lora_few(LoraArgs a) {
 // 1500 rows of rank 64, 6144 to 2048, bf16: 14.4 us (37 MB of x, 2.6 TB/s; bound by splitting x into operands between the stages' barriers) and 10.7 (25 MB
 // of y in and out, 2.3 TB/s, behind the sums of h's parts that each workgroup forms first).
 
-// 8 f32 of a row as MFMA operands of the weights' type: f16, scaled by `up`, as hi + lo; bf16, as three
+// 8 f32 of a row as MFMA operands of the weights' type: f16, scaled by `up`, as hi + lo; bf16, as three. An infinity's other pieces are NaN
 template <bool BF16> struct Pieces;
 template <> struct Pieces<false> {
     ti_h8 p[2];
@@ -264,6 +264,24 @@ __device__ __forceinline__ int row_exponent(float mx) {
 
 constexpr int PROWS = 32, RW = PROWS / 16, DWAVES = 8, PWAVES = 4, SPLITS = 4;
 constexpr int KC = 128, XP = KC / 4, WP = KC / 8;          // K of a stage; 16-byte pieces of its rows of x and of A
+
+template <bool BF16>
+__device__ __forceinline__ float one(uint16_t w) { return BF16 ? __uint_as_float((uint32_t)w << 16) : ti_h2f(w); }
+// Ranks j0 .. j0 + 3 of a row's h over K's [k0, k1), element by element: where the pieces came to NaN, as they do beside an infinity, whose other
+// pieces have no value
+template <bool BF16>
+__device__ __forceinline__ v4f sums(const LoraArgs& a, const uint16_t* w, int row, int j0, int k0, int k1) {
+    v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = k0; k < k1; k++) {
+        const float x = a.x[row * a.ldx + k];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint16_t u = w[(size_t)ti_min(j0 + e, a.r - 1) * a.K + k];
+            h[e] = fmaf(one<BF16>(u), x, h[e]);
+        }
+    }
+    return h;
+}
 
 // A workgroup: 32 rows, a part of K in stages of 128, read in whole lines and put into LDS, pieces permuted so that 16 rows' are in different
 // banks; three stages are on their way. A wave takes 16 rows and one 32-step of each stage, so that a value of x is split once.
@@ -375,7 +393,9 @@ __global__ __launch_bounds__(64 * DWAVES, 1) void k_lora_down(LoraArgs a) {
             v4f h = zero;
 #pragma unroll
             for (int s = 0; s < DWAVES / RW; s++) h += L.part[RW * s + qq][k][l];
-            *reinterpret_cast<v4f*>(a.h + ((size_t)split * a.T + row0 + t) * a.rp + 16 * k + 4 * (l >> 4)) = h;
+            const int j0 = 16 * k + 4 * (l >> 4);
+            if (__builtin_expect(__builtin_isunordered(h[0] + h[1], h[2] + h[3]), 0)) h = sums<BF16>(a, w, row0 + t, j0, KC * g0, ti_min(a.K, KC * g1));
+            *reinterpret_cast<v4f*>(a.h + ((size_t)split * a.T + row0 + t) * a.rp + j0) = h;
         }
         __syncthreads();
     }
@@ -433,6 +453,7 @@ __global__ __launch_bounds__(64 * PWAVES) void k_lora_up(LoraArgs a) {
     __syncthreads();
     Pieces<BF16> hp[RW][RS];
     float down[RW][4];
+    uint32_t infinite = 0;                                 // rows whose h holds an infinity
 #pragma unroll
     for (int q = 0; q < RW; q++) {
         float v[RS][8], mx = 0.0f;
@@ -443,6 +464,8 @@ __global__ __launch_bounds__(64 * PWAVES) void k_lora_up(LoraArgs a) {
                 v[s][e] = s_h[16 * q + m16][32 * s + 8 * j + e];
                 mx = fmaxf(mx, fabsf(v[s][e]));
             }
+        const uint64_t some = __ballot(mx == INFINITY);
+        infinite |= (uint32_t)((some | some >> 16 | some >> 32 | some >> 48) & 0xffff) << (16 * q);
         const int ex = row_exponent<BF16>(mx);
         const float up = ldexpf(1.0f, ex);
 #pragma unroll
@@ -450,6 +473,7 @@ __global__ __launch_bounds__(64 * PWAVES) void k_lora_up(LoraArgs a) {
 #pragma unroll
         for (int s = 0; s < RS; s++) hp[q][s].set(v[s], up);
     }
+    ad.rows &= ~infinite;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     for (bool first = true;; first = false) {
         for (int t = t0; t < t1; t += NB * PWAVES) {
@@ -469,8 +493,22 @@ __global__ __launch_bounds__(64 * PWAVES) void k_lora_up(LoraArgs a) {
                 }
             }
         }
-        if (!ad.next(a.slots, slot)) return;
+        if (!ad.next(a.slots, slot)) break;
+        ad.rows &= ~infinite;
     }
+    if (infinite == 0) return;                             // workgroup-uniform
+    // those rows element by element, by all waves
+    Adapters<PROWS> all(a, row0, Adapters<PROWS>::fetch(a, row0));
+    while (all.next(a.slots, slot))
+        for (uint32_t left = all.rows & infinite; left; left &= left - 1) {
+            const int t = __builtin_ctz(left);
+            for (int n = 16 * part * per + tid; n < ti_min(a.N, 16 * (part + 1) * per); n += 64 * PWAVES) {
+                const uint16_t* b = a.b + ((size_t)all.id * a.N + n) * a.r;
+                float d = 0.0f;
+                for (int k = 0; k < a.r; k++) d = fmaf(one<BF16>(b[k]), s_h[t][k], d);
+                a.y[(row0 + t) * a.ldy + n] += d;
+            }
+        }
 }
 
 template <bool BF16, bool VEC>

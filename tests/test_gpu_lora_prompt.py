@@ -189,3 +189,41 @@ def test_repeats_and_replays_bit_for_bit(ctx, bf16):
     ctx.graph_destroy(g)
     for v in (da, db, ds, dx, di, y1, y2):
         v.free()
+
+
+def plain(x, y, idx, a64, b64, scale):
+    """The formula as it stands in 64 bits, infinities and NaN included (no library product, which may add zeros times infinity of its own)."""
+    want = y.astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        for t, i in enumerate(idx):
+            h = (a64[i] * x[t].astype(np.float64)).sum(-1) * float(scale[i])
+            want[t] += (b64[i] * h).sum(-1)
+    return want
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,K,r", [(30, 320, 1), (30, 544, 16), (8300, 64, 1), (530, 544, 16), (130, 2080, 66)])
+def test_infinite_activations_give_what_the_formula_does(ctx, T, K, r, bf16):
+    """However many rows a call has: infinities of the weights' signs, NaN where two of them meet, beside elements of any size."""
+    rng = np.random.default_rng(7)
+    N, n = 21, 3
+    x, y = rng.standard_normal((T, K)).astype(np.float32), rng.standard_normal((T, N)).astype(np.float32)
+    (a, _), (b, _) = weights(rng, (n, r, K), K ** -0.5, bf16), weights(rng, (n, N, r), 0.05, bf16)
+    if r > 1:                                              # adapters 0 and 1 of one sign each, so that infinities do not cancel
+        a[0], b[0], a[1], b[1] = a[0] & 0x7FFF, b[0] & 0x7FFF, a[1] & 0x7FFF, b[1] | 0x8000
+    f = (lambda v: (v.astype(np.uint32) << 16).view(np.float32).astype(np.float64)) if bf16 else (lambda v: v.view(np.float16).astype(np.float64))
+    a64, b64 = f(a), f(b)
+    scale = np.array([0.5, 1.5, -2.0], np.float32)
+    idx = rng.integers(0, n, T).astype(np.int32)
+    hit = rng.random(T) < 0.5
+    for t in np.flatnonzero(hit):
+        at = rng.choice(K, int(rng.integers(1, 3)), replace=False)
+        x[t, rng.integers(0, K, 5)] = 10.0 ** rng.uniform(-30, 30, 5) * rng.choice([-1, 1], 5)
+        x[t, at] = np.inf * rng.choice([1, 1, 1, -1], len(at))
+    got, want = run(ctx, x, y, idx, a, b, scale, N, bf16), plain(x, y, idx, a64, b64, scale)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    for s in (np.inf, -np.inf):
+        assert np.any(want == s) and np.array_equal(got == s, want == s)
+    fine = ~hit
+    _, _, tol = ref.lora(*f64(x[fine], y[fine]), idx[fine], a64, b64, *f64(scale))
+    assert np.all(np.abs(got[fine] - want[fine]) <= tol)
