@@ -549,7 +549,7 @@ int ti_attn_paged_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const flo
 /* attnPrepQ8 (ti_attn_prep_q8) for T rows of any sequences, into the pages: row t of q ([T] rows of nHq heads) normed (qn_w, f16;
  * NULL: not) and rotated at rot[t] (rot NULL: at pos[t]) into row t of qr ([T][nHq][hd]), whether its place exists or not; row t of k
  * likewise (kn_w) and of v as it is, quantized into position pos[t] of sequence seq[t]. The operations are ti_attn_prep_q8's in its order, the
- * angles rot * theta^(-2i/hd) of 64 bits. table, seq, pos, places that do not exist and rows of one place as
+ * angles rot * theta^(-2i/hd) of 64 bits, whose last bits may differ (seen from position 10^4 on). table, seq, pos, places that do not exist and rows of one place as
  * ti_kv_write_paged_q8's; rot is any number: after an eviction a token's slot is not its position. ldq floats from one row of q to
  * the next, ldkv of k and of v (0: dense; multiples of 4, at least a row's heads): q, k and v may be parts of one projection's rows. nHq 0:
  * K and V alone, q and qr NULL. qr is q itself (dense rows) or does not overlap it, nor k or v. nHq and nKv <= 64; theta >= 1; q, k, v, qr, kq and
