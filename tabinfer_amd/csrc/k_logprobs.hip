@@ -8,8 +8,8 @@
 //
 // The likeliest: a value and its index are one 64-bit key (the float's bits in an order of whole numbers, then the inverted index: the lower
 // index wins), so that no two are equal. A wave takes 1024 elements at a time, in registers. Where `top` lanes hold something above its
-// limit, as always at first, the limit is raised to the top-th largest of the lanes' maxima, found bit by bit with ballots; what is above it
-// goes to a list in LDS, of at most `top` lanes and so 16 top keys a chunk, whatever the values are. (The first limit is that of all of the
+// limit, as always at first, the limit is raised to the top-th largest of the lanes' maxima, or to the first bits of it that no other lane reaches,
+// found bit by bit with ballots; it never falls. What is above it goes to a list in LDS, of at most `top` lanes and so 16 top keys a chunk, whatever the values are. (The first limit is that of all of the
 // workgroup's waves together.) Where the list has grown to more than 64 keys, and at the end, it is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
 // cost little more than a comparison. A workgroup sorts once, what is above the largest of its waves' limits.
 //
@@ -305,7 +305,9 @@ __global__ __launch_bounds__(256) void k_logprobs(LpArgs a) {
                         held = n;
                     }
                 }
-                ties = true;
+                // a prefix that just `top` lanes reach may be below what was the limit before
+                ties = limit > last;
+                limit = max(limit, last);
                 const int more = __builtin_popcountll(__ballot(mine > limit));
                 if (held > top) {
                     // lanes whose maxima are equal: those whose first is at the lowest places

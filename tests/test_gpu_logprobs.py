@@ -228,3 +228,17 @@ def test_limits_of_a_first_step(ctx, kind, top):
             x[rng.random((T, N)) > 0.5] = np.nan
         ids = rng.integers(0, N, T).astype(np.int32)
         check(run(ctx, x, ids, top), x, ids, top)
+
+
+@pytest.mark.parametrize("top", [3, 20, 40])
+def test_later_chunks_whose_few_lanes_are_far_above_the_others(ctx, top):
+    """Just `top` lanes of every later chunk exceed the limit, by far more than what lies between it and the others, rising or all alike."""
+    rng = np.random.default_rng(top)
+    T, N = 4, 60000
+    x = rng.uniform(0, 1.9, (T, N)).astype(np.float32)
+    for t in range(T):
+        x[t, 4 * rng.permutation(1024)[:4 * 64]] = 5
+        for c in range(4, N // 1024):
+            x[t, c * 1024 + 4 * rng.permutation(64)[:top] + rng.integers(0, 4, top)] = 6 + 0.01 * c * (t % 2) + 0.001 * rng.integers(0, 3, top) * (t // 2)
+    ids = rng.integers(0, N, T).astype(np.int32)
+    check(run(ctx, x, ids, top), x, ids, top)
