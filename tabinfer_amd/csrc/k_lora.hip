@@ -268,7 +268,7 @@ constexpr int KC = 128, XP = KC / 4, WP = KC / 8;          // K of a stage; 16-b
 template <bool BF16>
 __device__ __forceinline__ float one(uint16_t w) { return BF16 ? __uint_as_float((uint32_t)w << 16) : ti_h2f(w); }
 // Ranks j0 .. j0 + 3 of a row's h over K's [k0, k1), element by element: where the pieces came to NaN, as they do beside an infinity, whose other
-// pieces have no value
+// pieces have no value. 1500 rows of rank 64, 6144 to 2048: one such row 0.15 ms a call, all of them 0.4 (NaN) to 0.95 (infinities)
 template <bool BF16>
 __device__ __forceinline__ v4f sums(const LoraArgs& a, const uint16_t* w, int row, int j0, int k0, int k1) {
     v4f h = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -555,7 +555,9 @@ extern "C" int ti_lora_add(ti_ctx* c, const float* x, const int32_t* idx, const 
     const uintptr_t x0 = (uintptr_t)x, y0 = (uintptr_t)y, x1 = x0 + 4 * ((T - 1) * (size_t)g.ldx + K), y1 = y0 + 4 * ((T - 1) * (size_t)g.ldy + N);
     TI_REQUIRE(x1 <= y0 || y1 <= x0, "ti_lora_add: x and y overlap");
     if ((long)T * r > FEW) {
-        // K and N in parts until two workgroups a CU are there; a tile's adapters dealt out as long as those with none are no more than that again
+        // K and N in parts until two workgroups a CU are there. A tile's adapters are dealt out to as many workgroups as make four a CU, since how
+        // many it has is known on the device alone; those dealt none end behind three stages' loads of x (1500 rows of four
+        // requests: about 200 of 940 have one)
         const long tiles = (T + PROWS - 1) / PROWS, want = ti_max(1L, 2L * c->cus / tiles);
         g.h = c->attn_po;
         g.splits = (int)ti_max(1L, ti_min(ti_min(want, (long)K / (4 * KC)), ti_min((long)SPLITS, SCRATCH / ((long)T * g.rp))));
