@@ -565,7 +565,8 @@ int ti_attn_prep_paged_q8(ti_ctx* ctx, const float* q, const float* k, const flo
  * own. lens[b] counts all of a sequence's keys; a sequence shorter than what its group shares sees the first of them. Sequences of
  * no group, or alone in theirs, share nothing. starts and shared are read on the device, as table and lens. P <= B <= 2048;
  * 2 B nHq + 32 nKv min(P, B/2) (hd 32: 16 nKv) and room for the workgroups' partials within 262144 rows (512 sequences of 16
- * heads over 8 in any groups are); out must not overlap qr. */
+ * heads over 8 in any groups are); out must not overlap qr. Below about 1000 shared positions, and of pairs below 16000, ti_attn_paged_q8 with the
+ * shared pages in every row of the table is faster. */
 int ti_attn_shared_q8(ti_ctx* ctx, const float* qr, const uint32_t* kq, const float* ks, const uint32_t* vq,
                       const float* vs, const int32_t* table, const int32_t* lens, const int32_t* starts,
                       const int32_t* shared, float* out, int B, int P, int nHq, int nKv, int hd, int page, int pages,
