@@ -13,7 +13,7 @@
 // workgroup's waves together.) Where the list has grown to more than 64 keys, and at the end, it is sorted into the 64 largest that the wave keeps, a lane each, by exchanges between lanes; so all chunks but a wave's first
 // cost little more than a comparison. A workgroup sorts once, what is above the largest of its waves' limits.
 //
-// Bound by the stream where rows are many (400 rows of 151936 logits, 243 MB, 44.2 + 4.8 us: 5.0 TB/s), with tokens kept by the listing of candidates, a
+// Bound by the stream where rows are many (400 rows of 151936 logits, 243 MB, 43.4 + 4.7 us: 5.0 TB/s), with tokens kept by the listing of candidates, a
 // ballot an element, and the sorts (48 rows with 20 tokens, 29 MB, 21.3 us; without tokens 12), in one row by the chain from its first load to the join (with
 // five tokens 10.3).
 //

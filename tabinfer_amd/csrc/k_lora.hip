@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * FWAVES) void k_lora_few(LoraArgs a) {
 // Both products on the matrix cores, weights exact, f32 activations as two f16 (f16 weights: each row scaled by a power of two, an
 // element off by 2^-22 of itself or 2^-39 of the largest) or three bf16 (bf16 weights: exactly), sums in f32. 32 rows a workgroup; an adapter
 // multiplies all of its tile's rows, and what is another's is zero or not kept. Two launches: h in parts of K, then its sums times B.
-// 1500 rows of rank 64, 6144 to 2048, bf16: 14.4 us (37 MB of x, 2.6 TB/s; bound by splitting x into operands between the stages' barriers) and 10.7 (25 MB
+// 1500 rows of rank 64, 6144 to 2048, bf16: 13.9 us (37 MB of x, 2.7 TB/s; bound by splitting x into operands between the stages' barriers) and 10.8 (25 MB
 // of y in and out, 2.3 TB/s, behind the sums of h's parts that each workgroup forms first).
 
 // 8 f32 of a row as MFMA operands of the weights' type: f16, scaled by `up`, as hi + lo; bf16, as three. An infinity's other pieces are NaN
